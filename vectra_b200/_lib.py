@@ -79,6 +79,8 @@ def _load():
     lib.vectra_rbf_launch_count.restype = ctypes.c_uint64
     lib.vectra_rbf_build_info.argtypes = []
     lib.vectra_rbf_build_info.restype = ctypes.c_char_p
+    lib.vectra_block_strerror.argtypes = [ctypes.c_int]
+    lib.vectra_block_strerror.restype = ctypes.c_char_p
     return lib
 
 

@@ -1,10 +1,10 @@
 """Builds the two shared libraries of vectra_b200, in-tree.
 
-* libvectra_rbf.so: the CUDA kernels and the C ABI (include/vectra_rbf.h
-  and include/vectra_scan.h),
+* libvectra_rbf.so: the CUDA kernels and the C ABI (include/vectra_rbf.h,
+  include/vectra_scan.h and include/vectra_block.h),
   compiled by nvcc for sm_100a only. No torch dependency.
-* _vectra_rbf_torch.so: the PyTorch binding that registers the CUDA kernel
-  of vectra::rbf_attention; links libvectra_rbf.so through $ORIGIN.
+* _vectra_rbf_torch.so: the PyTorch binding that registers
+  vectra::rbf_attention and the vectra_b200:: operators; links libvectra_rbf.so through $ORIGIN.
 
     python vectra_b200/build.py [--force] [--verbose]
 
@@ -32,7 +32,9 @@ LIB = os.path.join(PKG, 'libvectra_rbf.so')
 TORCH_EXT = os.path.join(PKG, '_vectra_rbf_torch.so')
 
 CU_SOURCES = ['capi.cu', 'rbf_generic.cu', 'rbf_decode.cu', 'rbf_tc.cu',
-              'rbf_small.cu', 'rbf_small_tc.cu', 'tma_maps.cu', 'scan.cu']
+              'rbf_small.cu', 'rbf_small_tc.cu', 'tma_maps.cu', 'scan.cu',
+              'block_capi.cu', 'block_grad.cu', 'gemm_generic.cu',
+              'gemm_select.cu', 'qk_norm_rope.cu']
 ARCH = ['-gencode', 'arch=compute_100a,code=sm_100a']
 
 
@@ -121,8 +123,9 @@ def build_library(force=False, verbose=False, extra_flags=(), lib_path=LIB,
 
 def build_torch_extension(force=False, verbose=False):
     """Compiles the PyTorch binding against the installed torch: the
-    operator's registration and CUDA launcher (torch_ext.cpp) and its CPU
-    implementation (rbf_cpu.cpp, parallel over planes with ATen's OpenMP
+    operator's registration and CUDA launcher (torch_ext.cpp), the
+    transformer-block operators' (block_ext.cpp) and the CPU implementation
+    of attention (rbf_cpu.cpp, parallel over planes with ATen's OpenMP
     thread pool, so it is compiled with -fopenmp and linked against the
     libgomp that torch itself loads)."""
     import torch  # pylint: disable=import-outside-toplevel
@@ -130,7 +133,9 @@ def build_torch_extension(force=False, verbose=False):
 
     src = os.path.join(CSRC, 'torch_ext.cpp')
     cpu_src = os.path.join(CSRC, 'rbf_cpu.cpp')
-    if not (force or _stale(TORCH_EXT, [src, cpu_src, LIB] + _headers())):
+    block_src = os.path.join(CSRC, 'block_ext.cpp')
+    sources = [src, cpu_src, block_src]
+    if not (force or _stale(TORCH_EXT, sources + [LIB] + _headers())):
         return TORCH_EXT
     abi = int(torch._C._GLIBCXX_USE_CXX11_ABI)  # pylint: disable=protected-access
     includes = cpp_extension.include_paths(device_type='cuda')
@@ -142,10 +147,20 @@ def build_torch_extension(force=False, verbose=False):
         common += ['-isystem', inc]
     os.makedirs(BUILD, exist_ok=True)
     cpu_obj = os.path.join(BUILD, 'rbf_cpu.o')
-    _run(['g++', '-c', '-O3', '-fopenmp'] + common + [cpu_src, '-o', cpu_obj],
-         verbose)
-    cmd = ['g++', '-shared', '-O2'] + common + [src, cpu_obj, '-o', TORCH_EXT,
-                                                '-L', PKG, '-lvectra_rbf']
+    ext_obj = os.path.join(BUILD, 'torch_ext.o')
+    block_obj = os.path.join(BUILD, 'block_ext.o')
+    headers = [h for h in _headers() if h.endswith('.h')]
+    jobs = [['g++', '-c', '-O3', '-fopenmp'] + common +
+            [cpu_src, '-o', cpu_obj],
+            ['g++', '-c', '-O2'] + common + [src, '-o', ext_obj],
+            ['g++', '-c', '-O2'] + common + [block_src, '-o', block_obj]]
+    jobs = [job for job in jobs
+            if force or _stale(job[-1], [job[-3]] + headers)]
+    if jobs:
+        with concurrent.futures.ThreadPoolExecutor(len(jobs)) as pool:
+            list(pool.map(lambda c: _run(c, verbose), jobs))
+    cmd = ['g++', '-shared', ext_obj, cpu_obj, block_obj, '-o', TORCH_EXT,
+           '-L', PKG, '-lvectra_rbf']
     for libdir in cpp_extension.library_paths(device_type='cuda'):
         cmd += ['-L', libdir]
     cmd += ['-lc10', '-lc10_cuda', '-ltorch', '-ltorch_cpu', '-ltorch_cuda',

@@ -1,0 +1,267 @@
+// block_common.cuh: activations, problem descriptions and the workspace of
+// the transformer-block operators (include/vectra_block.h).
+//
+// Every matrix product of these operators is one GemmProblem,
+//   acc[m, n] = sum over segments s, k of a[s](m, k) b[s](n, k),
+// followed by an epilogue on acc in float32. Operands are [rows][reduction]
+// views with two strides, so a forward product (x W^T), an input gradient
+// (dz W) and a weight gradient (dz^T x) differ only in strides.
+#pragma once
+
+#include <initializer_list>
+#include <type_traits>
+
+#include "rbf_common.cuh"
+#include "vectra_block.h"
+
+namespace vectra {
+
+// ---------------------------------------------------------------------------
+// Activations. kExact: CUDA's expf / erff / tanhf, for float32 tensors.
+// Otherwise forms on ex2.approx and rcp.approx whose error (below 1e-6
+// absolute) is far under the rounding of the 16-bit results.
+// ---------------------------------------------------------------------------
+__device__ __forceinline__ float fast_rcp(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+template <bool kExact>
+__device__ __forceinline__ float sigmoid_f(float z) {
+  if constexpr (kExact) return 1.f / (1.f + expf(-z));
+  return fast_rcp(1.f + fast_exp2(-kLog2e * z));
+}
+
+constexpr float kGeluTanhC = 0.7978845608028654f;  // sqrt(2 / pi)
+constexpr float kGeluTanhA = 0.044715f;
+
+// Phi(z) = erfc(-z / sqrt 2) / 2, and exp(-z^2 / 2) on the way: Abramowitz
+// and Stegun 7.1.26, erfc(x) = (a1 t + ... + a5 t^5) exp(-x^2) with
+// t = 1 / (1 + p x) for x >= 0 (absolute error 1.5e-7).
+__device__ __forceinline__ float phi_fast(float z, float* e_out) {
+  const float x = fabsf(z) * 0.70710678f;
+  const float t = fast_rcp(fmaf(0.3275911f, x, 1.f));
+  float p = fmaf(1.061405429f, t, -1.453152027f);
+  p = fmaf(p, t, 1.421413741f);
+  p = fmaf(p, t, -0.284496736f);
+  p = fmaf(p, t, 0.254829592f);
+  const float e = fast_exp2(-kLog2e * x * x);
+  *e_out = e;
+  const float half = 0.5f * p * t * e;  // erfc(|z| / sqrt 2) / 2
+  return z < 0.f ? half : 1.f - half;
+}
+
+template <bool kExact, int ACT>
+__device__ __forceinline__ float act_fwd(float z) {
+  if constexpr (ACT == VECTRA_ACT_RELU) {
+    return z > 0.f || z != z ? z : 0.f;  // NaN stays NaN
+  } else if constexpr (ACT == VECTRA_ACT_SILU) {
+    if constexpr (kExact) return z / (1.f + expf(-z));
+    return z * sigmoid_f<false>(z);
+  } else if constexpr (ACT == VECTRA_ACT_GELU) {
+    if constexpr (kExact) return 0.5f * z * (1.f + erff(z * 0.70710678118f));
+    float e;
+    return z * phi_fast(z, &e);
+  } else if constexpr (ACT == VECTRA_ACT_GELU_TANH) {
+    const float u = kGeluTanhC * fmaf(kGeluTanhA * z * z, z, z);
+    if constexpr (kExact) return 0.5f * z * (1.f + tanhf(u));
+    // (1 + tanh u) / 2 = sigmoid(2 u)
+    return z * sigmoid_f<false>(2.f * u);
+  } else {
+    return z;
+  }
+}
+
+// act(z) and act'(z) together (the backward of a gated layer needs both).
+template <bool kExact, int ACT>
+__device__ __forceinline__ float act_grad(float z, float* value) {
+  if constexpr (ACT == VECTRA_ACT_RELU) {
+    *value = z > 0.f || z != z ? z : 0.f;
+    return z > 0.f ? 1.f : 0.f;
+  } else if constexpr (ACT == VECTRA_ACT_SILU) {
+    const float s = sigmoid_f<kExact>(z);
+    *value = z * s;
+    return s * (1.f + z * (1.f - s));
+  } else if constexpr (ACT == VECTRA_ACT_GELU) {
+    float phi, e;
+    if constexpr (kExact) {
+      phi = 0.5f * (1.f + erff(z * 0.70710678118f));
+      e = expf(-0.5f * z * z);
+    } else {
+      phi = phi_fast(z, &e);
+    }
+    *value = z * phi;
+    return phi + z * 0.3989422804f * e;
+  } else if constexpr (ACT == VECTRA_ACT_GELU_TANH) {
+    // Past |z| = 100 the sigmoid is exactly 0 or 1; the clamp keeps z^3 and
+    // the product 0 * z^2 finite.
+    const float c = fminf(fmaxf(z, -100.f), 100.f);
+    const float u = kGeluTanhC * fmaf(kGeluTanhA * c * c, c, c);
+    const float s = sigmoid_f<kExact>(2.f * u);
+    *value = z * s;
+    const float du = kGeluTanhC * fmaf(3.f * kGeluTanhA * c, c, 1.f);
+    return s + 2.f * c * s * (1.f - s) * du;
+  } else {
+    *value = z;
+    return 1.f;
+  }
+}
+
+// Calls f with the activation as a compile-time constant.
+template <typename F>
+cudaError_t with_activation(int act, F&& f) {
+  switch (act) {
+    case VECTRA_ACT_RELU:
+      return f(std::integral_constant<int, VECTRA_ACT_RELU>{});
+    case VECTRA_ACT_GELU:
+      return f(std::integral_constant<int, VECTRA_ACT_GELU>{});
+    case VECTRA_ACT_GELU_TANH:
+      return f(std::integral_constant<int, VECTRA_ACT_GELU_TANH>{});
+    case VECTRA_ACT_SILU:
+      return f(std::integral_constant<int, VECTRA_ACT_SILU>{});
+    default:
+      return f(std::integral_constant<int, VECTRA_ACT_NONE>{});
+  }
+}
+
+// Calls f with a null pointer of the element type.
+template <typename F>
+cudaError_t with_dtype(int dtype, F&& f) {
+  if (dtype == VECTRA_F32) return f(static_cast<float*>(nullptr));
+  if (dtype == VECTRA_F16) return f(static_cast<__half*>(nullptr));
+  return f(static_cast<__nv_bfloat16*>(nullptr));
+}
+
+// ---------------------------------------------------------------------------
+// Matrix products.
+// ---------------------------------------------------------------------------
+// A view of [rows][K], K the reduced dimension; strides in elements.
+struct MatView {
+  const void* p = nullptr;
+  int64_t sr = 0, sk = 0;
+};
+
+// What happens to acc[m, n].
+enum GemmEpilogue {
+  kEpiStore = 0,   // out = acc
+  kEpiLinear = 1,  // z = acc + bias; pre = z; out = act(z) + residual
+  kEpiGated = 2    // g = acc + bias, u = acc2 + bias2; out = act(g) * u
+};
+
+struct GemmProblem {
+  int32_t dtype = VECTRA_F32;
+  int32_t epilogue = kEpiStore;
+  int32_t act = VECTRA_ACT_NONE;
+  int32_t segments = 1;  // products summed: 1 or 2 (kEpiGated: 1)
+  int64_t M = 0, N = 0, K = 0;  // every segment reduces over K
+  MatView a[2], b[2];    // kEpiGated: b[0] gate, b[1] up, both with a[0]
+  const void* bias[2] = {nullptr, nullptr};
+  int64_t bias_stride[2] = {0, 0};
+  const void* res = nullptr;
+  int64_t res_sm = 0, res_sn = 0;
+  void* out = nullptr;
+  int64_t out_ld = 0;
+  void* pre = nullptr;   // kEpiLinear: z in dtype
+  int64_t pre_ld = 0;
+  float* gate = nullptr;  // kEpiGated: g and u
+  float* up = nullptr;
+  int64_t gate_ld = 0, up_ld = 0;
+  unsigned int* err = nullptr;
+};
+
+// Bump allocator over the caller's workspace. With no base it only counts,
+// so one function both sizes a call and runs it.
+struct Workspace {
+  char* base = nullptr;
+  size_t size = 0;
+  size_t used = 0;
+  bool dry = true;
+  bool overflow = false;
+  void* take(size_t bytes) {
+    const size_t at = used;
+    used += (bytes + 255) / 256 * 256;
+    if (dry) return nullptr;
+    if (used > size) {
+      overflow = true;
+      return nullptr;
+    }
+    return base + at;
+  }
+};
+
+// Runs (or, when ws.dry, sizes) one product; picks the kernel.
+cudaError_t run_gemm(const GemmProblem& p, Workspace& ws, cudaStream_t stream);
+
+// gemm_generic.cu: any strides, any type. `split` > 1 cuts the reduction
+// into that many parts, whose sums go to `partial` ([split][M][N], twice
+// that for kEpiGated) for launch_split_finish.
+cudaError_t launch_gemm_generic(const GemmProblem& p, int split,
+                                float* partial, cudaStream_t stream);
+// Adds the parts in order and applies the epilogue.
+cudaError_t launch_split_finish(const GemmProblem& p, int split,
+                                const float* partial, cudaStream_t stream);
+
+// block_grad.cu: elementwise parts of the backward passes.
+struct GradProblem {
+  int32_t dtype = VECTRA_F32;
+  int32_t act = VECTRA_ACT_NONE;
+  bool gated = false;
+  int64_t M = 0, N = 0;
+  const void* dy = nullptr;
+  int64_t dy_sm = 0, dy_sn = 0;
+  const void* pre = nullptr;  // linear: z [M, pre_ld]
+  int64_t pre_ld = 0;
+  const float* gate = nullptr;  // gated: g and u
+  const float* up = nullptr;
+  int64_t gate_ld = 0, up_ld = 0;
+  void* dz = nullptr;   // linear: dz; gated: dg; null: only the sums
+  void* dz2 = nullptr;  // gated: du
+  int64_t dz_ld = 0;
+  void* db = nullptr;   // column sums in dtype; null: not wanted
+  void* db2 = nullptr;
+};
+cudaError_t run_grad(const GradProblem& p, Workspace& ws, cudaStream_t stream);
+
+// qk_norm_rope.cu
+struct QkSide {
+  const void* x = nullptr;
+  int64_t sx[4] = {0, 0, 0, 0};
+  void* out = nullptr;       // forward: the result; backward: dx
+  int64_t so[4] = {0, 0, 0, 0};
+  const void* dy = nullptr;  // backward
+  int64_t sy[4] = {0, 0, 0, 0};
+  const void* w = nullptr;
+  int64_t sw = 0;
+  void* dw = nullptr;        // backward, [D] in the weight's type
+  int64_t sdw = 0;
+  int32_t w_dtype = VECTRA_F32;
+  int32_t H = 0;
+};
+struct QkProblem {
+  QkSide side[2];  // queries, keys
+  int32_t dtype = VECTRA_F32;
+  int32_t interleaved = 0;
+  int64_t B = 0, N = 0;
+  int32_t D = 0, R2 = 0;
+  int64_t P = 0;
+  const float* cos = nullptr;
+  const float* sin = nullptr;
+  int64_t cos_ld = 0, sin_ld = 0;
+  const void* pos = nullptr;
+  int32_t pos_bytes = 8;
+  int64_t pos_sb = 0, pos_sn = 0;
+  float eps = 0.f;
+};
+cudaError_t launch_qk_forward(const QkProblem& p, cudaStream_t stream);
+cudaError_t run_qk_backward(const QkProblem& p, Workspace& ws,
+                            cudaStream_t stream);
+
+// Largest size of one dimension: indices of a whole tile past it still fit
+// 32 bits.
+constexpr int64_t kMaxSize = (int64_t(1) << 31) - 256;
+
+// Adds to the library's launch counter (capi.cu).
+void count_launches(int n);
+
+}  // namespace vectra

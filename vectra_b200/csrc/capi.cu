@@ -11,6 +11,7 @@
 #include <cstdio>
 #include <mutex>
 
+#include "block_common.cuh"
 #include "rbf_common.cuh"
 
 namespace vectra {
@@ -163,6 +164,10 @@ int select(const RbfProblem& p, uint32_t flags) {
 
 
 }  // namespace
+
+void count_launches(int n) {
+  g_launches.fetch_add(uint64_t(n), std::memory_order_relaxed);
+}
 
 int device_sm_count() {
   const int dev = current_device();

@@ -211,6 +211,25 @@ def test_linear_sizes(device, dtype, size):
                  rand(m, n) if n % 2 == 0 else None, act, rand(m, n))
 
 
+# Enough tiles for every launch shape: wide results, long and short
+# reductions, ragged edges, weight gradients over many rows.
+LARGE = [(2570, 192, 2056), (5001, 72, 1032), (1030, 2304, 600),
+         (257, 1100, 5000), (20000, 64, 72), (700, 520, 1304)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('size', LARGE)
+def test_large_products(dtype, size):
+    m, k, n = size
+    rand = Rand(m + k + n, 'cuda', dtype)
+    check_linear(rand(m, k), rand(n, k, scale=k**-0.5), rand(n), rand(m, n),
+                 'gelu', rand(m, n))
+    check_gated(rand(m, k), rand(n, k, scale=k**-0.5),
+                rand(n, k, scale=k**-0.5), rand(n), rand(n), 'silu',
+                rand(m, n))
+
+
 @pytest.mark.parametrize('device', DEVICES)
 @pytest.mark.parametrize('dtype', TYPES)
 @pytest.mark.parametrize('act', ACTS)

@@ -75,6 +75,10 @@ int check_common(const vectra_tensor& x, const vectra_tensor& w,
   return VECTRA_OK;
 }
 
+// Rows of the gradients in the workspace start on 16-byte boundaries, which
+// the tensor-core products need.
+int64_t pad8(int64_t n) { return (n + 7) / 8 * 8; }
+
 // The operators' passes. Each runs twice: dry, to size the workspace, and
 // for real.
 int linear_forward(const vectra_linear_args& a, Workspace& ws,
@@ -110,11 +114,6 @@ int linear_forward(const vectra_linear_args& a, Workspace& ws,
   return to_status(run_gemm(p, ws, stream), ws);
 }
 
-// dx = sum of dz W over one or two (dz, W) pairs; dw = dz^T x.
-struct GradOperand {
-  MatView rows, cols;
-};
-
 int linear_backward(const vectra_linear_grad_args& a, Workspace& ws,
                     cudaStream_t stream) {
   VECTRA_TRY(check_common(a.x, a.weight, a.activation));
@@ -144,10 +143,10 @@ int linear_backward(const vectra_linear_grad_args& a, Workspace& ws,
     g.pre = act ? a.pre.data : nullptr;
     g.pre_ld = a.pre.stride[0];
     if (act && products) {
-      g.dz = ws.take(size_t(M) * N * es);
-      g.dz_ld = N;
-      dz_rows = {g.dz, N, 1};
-      dz_cols = {g.dz, 1, N};
+      g.dz_ld = pad8(N);
+      g.dz = ws.take(size_t(M) * g.dz_ld * es);
+      dz_rows = {g.dz, g.dz_ld, 1};
+      dz_cols = {g.dz, 1, g.dz_ld};
     }
     g.db = const_cast<void*>(a.dbias.data);
     VECTRA_TRY(to_status(run_grad(g, ws, stream), ws));
@@ -242,7 +241,7 @@ int gated_backward(const vectra_gated_grad_args& a, Workspace& ws,
     VECTRA_TRY(check_result(a.db_up, dt, {F}));
   }
   const size_t es = dt == VECTRA_F32 ? 4 : 2;
-  // dg and du side by side, [M][2 F].
+  // dg and du side by side, [M][2 pad8(F)].
   GradProblem g;
   g.dtype = dt;
   g.act = a.activation;
@@ -256,11 +255,12 @@ int gated_backward(const vectra_gated_grad_args& a, Workspace& ws,
   g.gate_ld = a.gate.stride[0];
   g.up = static_cast<const float*>(a.up.data);
   g.up_ld = a.up.stride[0];
-  char* d = static_cast<char*>(ws.take(size_t(M) * 2 * F * es));
-  char* d2 = d ? d + F * es : nullptr;
+  const int64_t ld = 2 * pad8(F);
+  char* d = static_cast<char*>(ws.take(size_t(M) * ld * es));
+  char* d2 = d ? d + ld / 2 * es : nullptr;
   g.dz = d;
   g.dz2 = d2;
-  g.dz_ld = 2 * F;
+  g.dz_ld = ld;
   g.db = const_cast<void*>(a.db_gate.data);
   g.db2 = const_cast<void*>(a.db_up.data);
   VECTRA_TRY(to_status(run_grad(g, ws, stream), ws));
@@ -272,8 +272,8 @@ int gated_backward(const vectra_gated_grad_args& a, Workspace& ws,
     p.N = K;
     p.K = F;
     p.segments = 2;
-    p.a[0] = {d, 2 * F, 1};
-    p.a[1] = {d2, 2 * F, 1};
+    p.a[0] = {d, ld, 1};
+    p.a[1] = {d2, ld, 1};
     p.b[0] = cols_of(a.w_gate);
     p.b[1] = cols_of(a.w_up);
     p.out = const_cast<void*>(a.dx.data);
@@ -287,7 +287,7 @@ int gated_backward(const vectra_gated_grad_args& a, Workspace& ws,
       p.M = F;
       p.N = K;
       p.K = M;
-      p.a[0] = {i ? d2 : d, 1, 2 * F};
+      p.a[0] = {i ? d2 : d, 1, ld};
       p.b[0] = cols_of(a.x);
       p.out = const_cast<void*>(out[i]->data);
       p.out_ld = out[i]->stride[0];

@@ -195,8 +195,7 @@ cudaError_t run_grad(const GradProblem& p, Workspace& ws,
                      cudaStream_t stream) {
   if (p.N == 0 || (p.M == 0 && p.db == nullptr)) return cudaSuccess;
   const size_t es = p.dtype == VECTRA_F32 ? 4 : 2;
-  // dz lies in the workspace (256-byte aligned, rows of N or 2 N elements),
-  // so N % 8 == 0 aligns it.
+  // dz lies in the workspace, whose rows are aligned.
   const bool vec = p.N % 8 == 0 && p.dy_sn == 1 &&
                    aligned(p.dy, p.dy_sm, es) &&
                    (!p.pre || aligned(p.pre, p.pre_ld, es)) &&

@@ -373,6 +373,12 @@ bool make_tile_map(CUtensorMap* map, const void* base, int dtype, int64_t B,
                    int64_t H, int64_t N, int64_t D, const int64_t* s,
                    int box_rows, int box_cols = 64);
 
+// A matrix of `outer` lines of `inner` contiguous bf16/f16 elements, `ld`
+// apart, as a 2-D map with a box of 64 elements by `box_lines` lines,
+// SWIZZLE_128B; elements outside read as zeros.
+bool make_line_map(CUtensorMap* map, const void* base, int dtype,
+                   int64_t inner, int64_t outer, int64_t ld, int box_lines);
+
 // Streaming-multiprocessor count of the current device (cached).
 int device_sm_count();
 

@@ -59,4 +59,25 @@ bool make_tile_map(CUtensorMap* map, const void* base, int dtype, int64_t B,
   return r == CUDA_SUCCESS;
 }
 
+bool make_line_map(CUtensorMap* map, const void* base, int dtype,
+                   int64_t inner, int64_t outer, int64_t ld, int box_lines) {
+  auto fn = encode_fn();
+  if (!fn) return false;
+  // The stride of a single line is never used; give it a valid value.
+  if (outer == 1) ld = (inner + 7) / 8 * 8;
+  cuuint64_t dims[2] = {cuuint64_t(inner), cuuint64_t(outer)};
+  cuuint64_t strides[1] = {cuuint64_t(ld) * 2};
+  cuuint32_t box[2] = {64, cuuint32_t(box_lines)};
+  cuuint32_t estr[2] = {1, 1};
+  const CUresult r = fn(map,
+                        dtype == VECTRA_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                             : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+                        2, const_cast<void*>(base), dims, strides, box, estr,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        CU_TENSOR_MAP_SWIZZLE_128B,
+                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS;
+}
+
 }  // namespace vectra

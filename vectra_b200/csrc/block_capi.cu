@@ -95,7 +95,11 @@ int linear_forward(const vectra_linear_args& a, Workspace& ws,
   if (M == 0 || N == 0) return VECTRA_OK;
   GemmProblem p;
   p.dtype = dt;
-  p.epilogue = kEpiLinear;
+  // A bare product needs no more than a store.
+  p.epilogue = present(a.bias) || present(a.residual) || present(a.pre) ||
+                       a.activation != VECTRA_ACT_NONE
+                   ? kEpiLinear
+                   : kEpiStore;
   p.act = a.activation;
   p.M = M;
   p.N = N;

@@ -16,6 +16,7 @@ TcShape tc_shape(const GemmProblem& p) {
   };
   TcShape s;
   if (p.M > 128 && tiles(256, 256) >= sms / 2) {
+    s.bn = 256;
     s.cg = 2;
     return s;
   }

@@ -8,10 +8,37 @@ namespace vectra {
 // A launch shape: tile columns (accumulator columns; a gated tile has half
 // as many outputs), CTAs per tile, and parts of the reduction.
 struct TcShape {
-  int bn = 256;  // 256, 128 or 64
-  int cg = 1;    // 2 only with bn = 256
+  int bn = 128;  // 64, 128, or with CTA pairs 256
+  int cg = 1;
   int split = 1;
 };
+
+constexpr int kTcRows = 128;  // rows of a tile per CTA
+constexpr int kTcStep = 64;   // reduction per stage: one 128-byte row
+
+struct TcArgs {
+  GemmProblem p;
+  float* partial;     // split > 1: [split][planes][M][N]
+  int tiles_m, tiles_n;
+  int steps_seg;      // stages of one segment
+  int steps;          // of all segments
+  int split;
+  int steps_part;     // steps of one part
+  int64_t units;      // tiles * split
+  uint8_t a_mn, b_mn;  // operand staged MN-major
+  uint8_t vec_out, vec_pre, vec_res, vec_f32;
+};
+
+// Epilogues of the kernels beyond GemmEpilogue: float32 sums of one part.
+enum { kEpiPartial = 3, kEpiGatedPartial = 4 };
+
+template <typename T>
+cudaError_t launch_tc_linear(int bn, int cg, const CUtensorMap* maps,
+                             const TcArgs& g, cudaStream_t stream);
+template <typename T>
+cudaError_t launch_tc_other(int epilogue, int bn, int cg,
+                            const CUtensorMap* maps, const TcArgs& g,
+                            cudaStream_t stream);
 
 // bf16 / f16 products with a non-empty reduction, in any layout.
 bool gemm_tc_supports(const GemmProblem& p);

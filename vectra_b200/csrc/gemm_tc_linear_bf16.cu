@@ -1,0 +1,10 @@
+// gemm_tc_linear_bf16.cu: tensor-core kernels, products with an epilogue, bf16.
+#include "gemm_tc_kernel.cuh"
+
+namespace vectra {
+
+template cudaError_t launch_tc_linear<__nv_bfloat16>(
+    int bn, int cg, const CUtensorMap* maps, const TcArgs& g,
+    cudaStream_t stream);
+
+}  // namespace vectra

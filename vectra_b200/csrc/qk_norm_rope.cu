@@ -160,27 +160,380 @@ __global__ void __launch_bounds__(kWarps * 32)
   }
 }
 
-// Adds the blocks' weight-gradient sums in order.
-__global__ void __launch_bounds__(256)
-    qk_weight_finish_kernel(const QkProblem p, const float* partial,
-                            int blocks) {
-  __shared__ float sums[8][32];
+// ---------------------------------------------------------------------------
+// The vector kernels: 16-byte loads and stores.
+//
+// A group of G lanes (the power of two from 1 to 32 that covers the vector's
+// chunk pairs) owns a head vector; each lane holds two 16-byte chunks of VE
+// elements, chosen so that no rotated pair spans lanes: chunks j and
+// j + R2 / VE when pairs are (i, i + R2), so both members sit at the same
+// place of the two chunks, and any two chunks when pairs are neighbours.
+// Unrotated chunks pair up behind them and turn by cos = 1, sin = 0. The
+// norm is a butterfly over the group. A group walks several heads of one
+// token, so the token's cosines and sines (which a vector would otherwise
+// re-read at twice its own size) are loaded once into registers, and the
+// heads' loads are issued kBatch at a time before any is used.
+// ---------------------------------------------------------------------------
+template <typename T>
+constexpr int kVec = 16 / int(sizeof(T));
+
+template <typename T>
+union Chunk {
+  uint4 u;
+  T e[kVec<T>];
+};
+
+struct QkVecArgs {
+  QkProblem p;
+  float* partial;
+  int heads_per_group;
+  int groups_per_token[2];  // of the queries, of the keys
+  int64_t groups[2];
+  int blocks[2];            // backward: blocks of each side
+};
+
+// The two chunks of lane j's slot; -1: none.
+__device__ __forceinline__ void slot_chunks(int j, int slots, int chunks,
+                                            int r_chunks, int interleaved,
+                                            int* c0, int* c1) {
+  if (interleaved) {
+    *c0 = j;
+    *c1 = j + slots;
+  } else if (j < r_chunks) {
+    *c0 = j;
+    *c1 = j + r_chunks;
+  } else {
+    *c0 = 2 * j;
+    *c1 = 2 * j + 1;
+  }
+  if (j >= slots || *c0 >= chunks) *c0 = -1;
+  if (j >= slots || *c1 >= chunks) *c1 = -1;
+}
+
+// VE cosines and sines of a slot. Pairs (i, i + R2): element e of both
+// chunks. Neighbours: pair e / 2 of chunk 0, then of chunk 1.
+template <typename T>
+struct Angles {
+  float c[kVec<T>], s[kVec<T>];
+};
+
+template <typename T, bool INTER>
+__device__ __forceinline__ void load_angles(const QkProblem& p, int64_t pos,
+                                            bool known, int c0, int c1,
+                                            Angles<T>* a) {
+  constexpr int VE = kVec<T>;
+#pragma unroll
+  for (int i = 0; i < VE; ++i) {
+    a->c[i] = 1.f;
+    a->s[i] = 0.f;
+  }
+  if (!known) return;
+  const float* cr = p.cos + pos * p.cos_ld;
+  const float* sr = p.sin + pos * p.sin_ld;
+  if constexpr (!INTER) {
+    if (c0 >= 0 && c0 * VE < p.R2) {
+#pragma unroll
+      for (int i = 0; i < VE; i += 4) {
+        *reinterpret_cast<float4*>(a->c + i) =
+            __ldg(reinterpret_cast<const float4*>(cr + c0 * VE + i));
+        *reinterpret_cast<float4*>(a->s + i) =
+            __ldg(reinterpret_cast<const float4*>(sr + c0 * VE + i));
+      }
+    }
+  } else {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int c = h ? c1 : c0;
+      if (c < 0 || c * VE >= 2 * p.R2) continue;
+#pragma unroll
+      for (int i = 0; i < VE / 2; i += 2) {
+        *reinterpret_cast<float2*>(a->c + h * (VE / 2) + i) =
+            __ldg(reinterpret_cast<const float2*>(cr + c * VE / 2 + i));
+        *reinterpret_cast<float2*>(a->s + h * (VE / 2) + i) =
+            __ldg(reinterpret_cast<const float2*>(sr + c * VE / 2 + i));
+      }
+    }
+  }
+}
+
+// Turns the slot's values by the angles (sign = 1) or back (sign = -1).
+template <typename T, bool INTER>
+__device__ __forceinline__ void turn(float* x, const Angles<T>& a,
+                                     float sign) {
+  constexpr int VE = kVec<T>;
+#pragma unroll
+  for (int i = 0; i < VE; ++i) {
+    // Half style: x[i] and x[VE + i]. Neighbours: x[2 i] and x[2 i + 1],
+    // which runs over both chunks.
+    float& u = INTER ? x[2 * i] : x[i];
+    float& v = INTER ? x[2 * i + 1] : x[VE + i];
+    const float s = sign * a.s[i];
+    const float nu = u * a.c[i] - v * s;
+    v = v * a.c[i] + u * s;
+    u = nu;
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void load_weight(const QkSide& s, int chunk,
+                                            float* w) {
+  constexpr int VE = kVec<T>;
+#pragma unroll
+  for (int i = 0; i < VE; ++i) w[i] = 1.f;
+  if (s.w == nullptr || chunk < 0) return;
+#pragma unroll
+  for (int i = 0; i < VE; ++i)
+    w[i] = load_any(s.w, s.w_dtype, int64_t(chunk * VE + i) * s.sw);
+}
+
+template <int G>
+__device__ __forceinline__ float group_sum(float x) {
+#pragma unroll
+  for (int o = G / 2; o > 0; o >>= 1)
+    x += __shfl_xor_sync(0xffffffffu, x, o);
+  return x;
+}
+
+template <typename T>
+__device__ __forceinline__ void unpack_chunk(const Chunk<T>& c, float* x) {
+#pragma unroll
+  for (int i = 0; i < kVec<T>; ++i) x[i] = to_f32(c.e[i]);
+}
+
+template <typename T>
+__device__ __forceinline__ void store_chunk(T* p, const float* x) {
+  Chunk<T> c;
+#pragma unroll
+  for (int i = 0; i < kVec<T>; ++i) c.e[i] = from_f32<T>(x[i]);
+  *reinterpret_cast<uint4*>(p) = c.u;
+}
+
+template <typename T, int G, bool INTER, int BATCH>
+__global__ void __launch_bounds__(kWarps * 32)
+    qk_vec_forward_kernel(const __grid_constant__ QkVecArgs a) {
+  constexpr int VE = kVec<T>;
+  const QkProblem& p = a.p;
   allow_dependents();
   grid_dependency_wait();
+  const int lane = threadIdx.x % 32, j = lane % G;
+  int64_t g = (int64_t(blockIdx.x) * kWarps + threadIdx.x / 32) * (32 / G) +
+              lane / G;
+  const int side = g >= a.groups[0];
+  if (side) g -= a.groups[0];
+  const QkSide& s = p.side[side];
+  const bool live = g < a.groups[side];
+  if (!live) g = 0;
+  const int per = a.groups_per_token[side];
+  const int64_t token = per > 0 ? g / per : 0;
+  const int h0 = per > 0 ? int(g - token * per) * a.heads_per_group : 0;
+  const int h1 = !live ? h0
+                       : (h0 + a.heads_per_group < s.H ? h0 + a.heads_per_group
+                                                       : s.H);
+  const int64_t b = token / p.N, n = token - b * p.N;
+  const int chunks = p.D / VE, slots = (chunks + 1) / 2;
+  int c0, c1;
+  slot_chunks(j, slots, chunks, p.R2 / VE, INTER, &c0, &c1);
+  const int64_t pos = live ? load_pos(p, b, n) : 0;
+  const bool known = pos >= 0 && pos < p.P;
+  const T* x = static_cast<const T*>(s.x) + b * s.sx[0] + n * s.sx[2];
+  T* out = static_cast<T*>(s.out) + b * s.so[0] + n * s.so[2];
+  Angles<T> ang;
+  float w[2 * VE];
+  const float inv_d = 1.f / float(p.D);
+  bool first = true;
+  // Groups of one warp may have different head counts: the butterflies need
+  // every lane, so the loop runs to the longest.
+  const int most = __reduce_max_sync(0xffffffffu, h1 - h0);
+  for (int hb = 0; hb < most; hb += BATCH) {
+    Chunk<T> raw[BATCH][2];
+#pragma unroll
+    for (int i = 0; i < BATCH; ++i) {
+      raw[i][0].u = raw[i][1].u = make_uint4(0, 0, 0, 0);
+      const int h = h0 + hb + i;
+      if (h < h1) {
+        if (c0 >= 0)
+          raw[i][0].u = __ldg(
+              reinterpret_cast<const uint4*>(x + h * s.sx[1] + c0 * VE));
+        if (c1 >= 0)
+          raw[i][1].u = __ldg(
+              reinterpret_cast<const uint4*>(x + h * s.sx[1] + c1 * VE));
+      }
+    }
+    if (first) {
+      load_angles<T, INTER>(p, pos, known, c0, c1, &ang);
+      load_weight<T>(s, c0, w);
+      load_weight<T>(s, c1, w + VE);
+      first = false;
+    }
+#pragma unroll
+    for (int i = 0; i < BATCH; ++i) {
+      float v[2 * VE];
+      unpack_chunk<T>(raw[i][0], v);
+      unpack_chunk<T>(raw[i][1], v + VE);
+      float ss = 0.f;
+#pragma unroll
+      for (int e = 0; e < 2 * VE; ++e) ss = fmaf(v[e], v[e], ss);
+      float r = rsqrtf(group_sum<G>(ss) * inv_d + p.eps);
+      if (!known) r = NAN;
+      const int h = h0 + hb + i;
+      if (h >= h1) continue;
+#pragma unroll
+      for (int e = 0; e < 2 * VE; ++e) v[e] *= r * w[e];
+      turn<T, INTER>(v, ang, 1.f);
+      if (c0 >= 0) store_chunk<T>(out + h * s.so[1] + c0 * VE, v);
+      if (c1 >= 0) store_chunk<T>(out + h * s.so[1] + c1 * VE, v + VE);
+    }
+  }
+}
+
+// Backward: blocks 0 .. blocks[0] - 1 walk the queries' groups, the others
+// the keys', so a lane's weight-gradient sums belong to one side.
+template <typename T, int G, bool INTER, int BATCH>
+__global__ void __launch_bounds__(kWarps * 32)
+    qk_vec_backward_kernel(const __grid_constant__ QkVecArgs a) {
+  constexpr int VE = kVec<T>;
+  __shared__ float sums[kWarps][G * 2 * VE];
+  const QkProblem& p = a.p;
+  allow_dependents();
+  grid_dependency_wait();
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, j = lane % G;
+  const int side = int(blockIdx.x) >= a.blocks[0];
+  const int block = int(blockIdx.x) - (side ? a.blocks[0] : 0);
+  const QkSide& s = p.side[side];
+  const int per = a.groups_per_token[side];
+  const int chunks = p.D / VE, slots = (chunks + 1) / 2;
+  int c0, c1;
+  slot_chunks(j, slots, chunks, p.R2 / VE, INTER, &c0, &c1);
+  float w[2 * VE], dw[2 * VE];
+  load_weight<T>(s, c0, w);
+  load_weight<T>(s, c1, w + VE);
+#pragma unroll
+  for (int e = 0; e < 2 * VE; ++e) dw[e] = 0.f;
+  const float inv_d = 1.f / float(p.D);
+  const int64_t step = int64_t(a.blocks[side]) * kWarps * (32 / G);
+  for (int64_t base = (int64_t(block) * kWarps + warp) * (32 / G);
+       base < a.groups[side]; base += step) {
+    int64_t g = base + lane / G;
+    const bool live = g < a.groups[side];
+    if (!live) g = 0;
+    const int64_t token = g / per;
+    const int h0 = int(g - token * per) * a.heads_per_group;
+    const int h1 = !live
+                       ? h0
+                       : (h0 + a.heads_per_group < s.H ? h0 + a.heads_per_group
+                                                       : s.H);
+    const int64_t b = token / p.N, n = token - b * p.N;
+    const int64_t pos = load_pos(p, b, n);
+    const bool known = pos >= 0 && pos < p.P;
+    Angles<T> ang;
+    load_angles<T, INTER>(p, pos, known, c0, c1, &ang);
+    const T* x = static_cast<const T*>(s.x) + b * s.sx[0] + n * s.sx[2];
+    const T* dy = static_cast<const T*>(s.dy) + b * s.sy[0] + n * s.sy[2];
+    T* out = static_cast<T*>(s.out) + b * s.so[0] + n * s.so[2];
+    const int most = __reduce_max_sync(0xffffffffu, h1 - h0);
+    for (int hb = 0; hb < most; hb += BATCH) {
+      Chunk<T> rx[BATCH][2], ry[BATCH][2];
+#pragma unroll
+      for (int i = 0; i < BATCH; ++i) {
+        const int h = h0 + hb + i;
+        rx[i][0].u = rx[i][1].u = ry[i][0].u = ry[i][1].u =
+            make_uint4(0, 0, 0, 0);
+        if (h < h1) {
+          if (c0 >= 0) {
+            rx[i][0].u = __ldg(
+                reinterpret_cast<const uint4*>(x + h * s.sx[1] + c0 * VE));
+            ry[i][0].u = __ldg(
+                reinterpret_cast<const uint4*>(dy + h * s.sy[1] + c0 * VE));
+          }
+          if (c1 >= 0) {
+            rx[i][1].u = __ldg(
+                reinterpret_cast<const uint4*>(x + h * s.sx[1] + c1 * VE));
+            ry[i][1].u = __ldg(
+                reinterpret_cast<const uint4*>(dy + h * s.sy[1] + c1 * VE));
+          }
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < BATCH; ++i) {
+        float v[2 * VE], d[2 * VE];
+        unpack_chunk<T>(rx[i][0], v);
+        unpack_chunk<T>(rx[i][1], v + VE);
+        unpack_chunk<T>(ry[i][0], d);
+        unpack_chunk<T>(ry[i][1], d + VE);
+        turn<T, INTER>(d, ang, -1.f);
+        float ss = 0.f, dot = 0.f;
+#pragma unroll
+        for (int e = 0; e < 2 * VE; ++e) {
+          ss = fmaf(v[e], v[e], ss);
+          dot = fmaf(d[e] * w[e], v[e], dot);
+        }
+        float r = rsqrtf(group_sum<G>(ss) * inv_d + p.eps);
+        const float c = group_sum<G>(dot) * r * r * inv_d;
+        const int h = h0 + hb + i;
+        if (h >= h1) continue;
+        if (!known) r = NAN;
+#pragma unroll
+        for (int e = 0; e < 2 * VE; ++e) {
+          dw[e] = fmaf(d[e] * v[e], r, dw[e]);
+          v[e] = r * (d[e] * w[e] - v[e] * c);
+        }
+        if (c0 >= 0) store_chunk<T>(out + h * s.so[1] + c0 * VE, v);
+        if (c1 >= 0) store_chunk<T>(out + h * s.so[1] + c1 * VE, v + VE);
+      }
+    }
+  }
+  if (s.dw == nullptr) return;
+  // The warp's groups, then the warps, in a fixed order.
+#pragma unroll
+  for (int e = 0; e < 2 * VE; ++e) {
+#pragma unroll
+    for (int o = 16; o >= G; o >>= 1)
+      dw[e] += __shfl_xor_sync(0xffffffffu, dw[e], o);
+    if (lane < G) sums[warp][j * 2 * VE + e] = dw[e];
+  }
+  __syncthreads();
+  float* part = a.partial + int64_t(blockIdx.x) * p.D;
+  for (int q = threadIdx.x; q < G * 2 * VE; q += kWarps * 32) {
+    int k0, k1;
+    slot_chunks(q / (2 * VE), slots, chunks, p.R2 / VE, INTER, &k0, &k1);
+    const int e = q % (2 * VE);
+    const int chunk = e < VE ? k0 : k1;
+    if (chunk < 0) continue;
+    float t = 0.f;
+#pragma unroll
+    for (int v = 0; v < kWarps; ++v) t += sums[v][q];
+    part[chunk * VE + e % VE] = t;
+  }
+}
+
+// Adds the blocks' weight-gradient sums in order: blocks first[i] ..
+// first[i] + count[i] - 1 hold side i.
+struct QkFinish {
+  QkProblem p;
+  const float* partial;
+  int first[2], count[2];
+};
+__global__ void __launch_bounds__(1024)
+    qk_weight_finish_kernel(const QkFinish f) {
+  __shared__ float sums[32][32];
+  allow_dependents();
+  grid_dependency_wait();
+  const QkProblem& p = f.p;
   const QkSide& s = p.side[blockIdx.y];
   if (s.dw == nullptr) return;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int d = blockIdx.x * 32 + lane;
-  const float* src = partial + int64_t(blockIdx.y) * blocks * p.D;
+  const float* src = f.partial + int64_t(f.first[blockIdx.y]) * p.D;
   float t = 0.f;
   if (d < p.D)
-    for (int c = warp; c < blocks; c += 8) t += src[int64_t(c) * p.D + d];
+    for (int c = warp; c < f.count[blockIdx.y]; c += 32)
+      t += src[int64_t(c) * p.D + d];
   sums[warp][lane] = t;
   __syncthreads();
   if (warp == 0 && d < p.D) {
     float total = 0.f;
 #pragma unroll
-    for (int w = 0; w < 8; ++w) total += sums[w][lane];
+    for (int w = 0; w < 32; ++w) total += sums[w][lane];
     const int64_t i = d * s.sdw;
     if (s.w_dtype == VECTRA_F32)
       static_cast<float*>(s.dw)[i] = total;
@@ -188,6 +541,78 @@ __global__ void __launch_bounds__(256)
       static_cast<__half*>(s.dw)[i] = from_f32<__half>(total);
     else
       static_cast<__nv_bfloat16*>(s.dw)[i] = from_f32<__nv_bfloat16>(total);
+  }
+}
+
+bool lines_ok(const void* p, const int64_t* s, const int64_t* sizes, int es) {
+  if (reinterpret_cast<uintptr_t>(p) & 15) return false;
+  for (int i = 0; i < 3; ++i)
+    if (sizes[i] > 1 && (s[i] * es) % 16 != 0) return false;
+  return sizes[3] <= 1 || s[3] == 1;
+}
+
+// Whether the vector kernels can run: whole 16-byte chunks everywhere, in
+// the tables too, and at most 32 chunk pairs.
+bool vec_ok(const QkProblem& p, bool backward) {
+  const int es = p.dtype == VECTRA_F32 ? 4 : 2;
+  const int ve = 16 / es;
+  if (p.D % ve || p.D / ve > 64) return false;
+  if ((p.interleaved ? 2 * p.R2 : p.R2) % ve) return false;
+  if (p.R2 > 0 && ((reinterpret_cast<uintptr_t>(p.cos) & 15) ||
+                   (reinterpret_cast<uintptr_t>(p.sin) & 15) ||
+                   p.cos_ld % 4 || p.sin_ld % 4))
+    return false;
+  for (const QkSide& s : p.side) {
+    const int64_t sizes[4] = {p.B, s.H, p.N, p.D};
+    if (p.B * p.N * s.H == 0) continue;
+    if (!lines_ok(s.x, s.sx, sizes, es) || !lines_ok(s.out, s.so, sizes, es))
+      return false;
+    if (backward && !lines_ok(s.dy, s.sy, sizes, es)) return false;
+  }
+  return true;
+}
+
+int lanes_of(const QkProblem& p) {
+  const int slots = (p.D / (p.dtype == VECTRA_F32 ? 4 : 8) + 1) / 2;
+  int g = 1;
+  while (g < slots) g *= 2;
+  return g;
+}
+
+// Heads per group: all the parallelism there is for small calls, else up to
+// eight, so that a token's angles are read once for eight vectors.
+QkVecArgs vec_args(const QkProblem& p, int g) {
+  QkVecArgs a{p, nullptr, 1, {0, 0}, {0, 0}, {0, 0}};
+  const int64_t vectors = p.B * p.N * (p.side[0].H + p.side[1].H);
+  const int64_t slots = int64_t(device_sm_count()) * 64 * (32 / g);
+  a.heads_per_group = vectors >= 8 * slots ? 8 : (vectors >= 4 * slots ? 4 : 1);
+  for (int i = 0; i < 2; ++i) {
+    a.groups_per_token[i] =
+        (p.side[i].H + a.heads_per_group - 1) / a.heads_per_group;
+    a.groups[i] = p.B * p.N * a.groups_per_token[i];
+  }
+  return a;
+}
+
+template <typename T, typename F>
+cudaError_t with_lanes(int g, bool interleaved, F&& f) {
+  auto inner = [&](auto lanes) {
+    return interleaved ? f(lanes, std::true_type{})
+                       : f(lanes, std::false_type{});
+  };
+  switch (g) {
+    case 1:
+      return inner(std::integral_constant<int, 1>{});
+    case 2:
+      return inner(std::integral_constant<int, 2>{});
+    case 4:
+      return inner(std::integral_constant<int, 4>{});
+    case 8:
+      return inner(std::integral_constant<int, 8>{});
+    case 16:
+      return inner(std::integral_constant<int, 16>{});
+    default:
+      return inner(std::integral_constant<int, 32>{});
   }
 }
 
@@ -203,12 +628,29 @@ int general_blocks(const QkProblem& p) {
 cudaError_t launch_qk_forward(const QkProblem& p, cudaStream_t stream) {
   if (p.B * p.N == 0 || p.D == 0 || p.side[0].H + p.side[1].H == 0)
     return cudaSuccess;
-  const QkArgs a{p, nullptr};
   const cudaError_t e = with_dtype(p.dtype, [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
-    return launch_pdl(qk_general_kernel<T, false>,
-                      dim3(unsigned(general_blocks(p)), 2), dim3(kWarps * 32),
-                      0, stream, a);
+    if (!vec_ok(p, false)) {
+      const QkArgs a{p, nullptr};
+      return launch_pdl(qk_general_kernel<T, false>,
+                        dim3(unsigned(general_blocks(p)), 2),
+                        dim3(kWarps * 32), 0, stream, a);
+    }
+    const int g = lanes_of(p);
+    const QkVecArgs a = vec_args(p, g);
+    const int64_t per_block = kWarps * (32 / g);
+    const int64_t blocks =
+        (a.groups[0] + a.groups[1] + per_block - 1) / per_block;
+    if (blocks > 0x7fffffff) return cudaErrorInvalidValue;
+    return with_lanes<T>(g, p.interleaved, [&](auto lanes, auto inter) {
+      constexpr int G = decltype(lanes)::value;
+      constexpr bool I = decltype(inter)::value;
+      return launch_pdl(a.heads_per_group == 1
+                            ? qk_vec_forward_kernel<T, G, I, 1>
+                            : qk_vec_forward_kernel<T, G, I, 4>,
+                        dim3(unsigned(blocks)), dim3(kWarps * 32), 0, stream,
+                        a);
+    });
   });
   if (e == cudaSuccess) count_launches(1);
   return e;
@@ -217,24 +659,60 @@ cudaError_t launch_qk_forward(const QkProblem& p, cudaStream_t stream) {
 cudaError_t run_qk_backward(const QkProblem& p, Workspace& ws,
                             cudaStream_t stream) {
   if (p.D == 0) return cudaSuccess;
-  const int blocks = general_blocks(p);
   const bool weights = p.side[0].dw || p.side[1].dw;
-  QkArgs a{p, nullptr};
+  const bool vec = vec_ok(p, true) && p.B * p.N > 0 && p.side[0].H > 0 &&
+                   p.side[1].H > 0;
+  const int g = lanes_of(p);
+  QkVecArgs a{};
+  QkFinish f{p, nullptr, {0, 0}, {0, 0}};
+  const int general = general_blocks(p);
+  if (vec) {
+    a = vec_args(p, g);
+    // Blocks of each side in proportion to its vectors, four per SM in all.
+    const int64_t per_block = kWarps * (32 / g);
+    const int64_t all = a.groups[0] + a.groups[1];
+    const int64_t most = int64_t(device_sm_count()) * 4;
+    for (int i = 0; i < 2; ++i) {
+      int64_t n = (a.groups[i] + per_block - 1) / per_block;
+      const int64_t share = (most * a.groups[i] + all - 1) / all;
+      if (n > share) n = share;
+      a.blocks[i] = int(n < 1 ? 1 : n);
+    }
+    f.count[0] = a.blocks[0];
+    f.first[1] = a.blocks[0];
+    f.count[1] = a.blocks[1];
+  } else {
+    f.count[0] = f.count[1] = f.first[1] = general;
+  }
+  const int blocks = f.count[0] + f.count[1];
+  float* partial = nullptr;
   if (weights)
-    a.partial = static_cast<float*>(
-        ws.take(size_t(2) * blocks * p.D * sizeof(float)));
+    partial = static_cast<float*>(
+        ws.take(size_t(blocks) * p.D * sizeof(float)));
   if (ws.dry || ws.overflow) return cudaSuccess;
+  f.partial = a.partial = partial;
   cudaError_t e = with_dtype(p.dtype, [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
-    return launch_pdl(qk_general_kernel<T, true>, dim3(unsigned(blocks), 2),
-                      dim3(kWarps * 32), 0, stream, a);
+    if (!vec) {
+      const QkArgs ga{p, partial};
+      return launch_pdl(qk_general_kernel<T, true>,
+                        dim3(unsigned(general), 2), dim3(kWarps * 32), 0,
+                        stream, ga);
+    }
+    return with_lanes<T>(g, p.interleaved, [&](auto lanes, auto inter) {
+      constexpr int G = decltype(lanes)::value;
+      constexpr bool I = decltype(inter)::value;
+      return launch_pdl(qk_vec_backward_kernel<T, G, I, 2>,
+                        dim3(unsigned(blocks)), dim3(kWarps * 32), 0, stream,
+                        a);
+    });
   });
   if (e != cudaSuccess) return e;
   count_launches(1);
   if (!weights) return cudaSuccess;
   e = launch_pdl(qk_weight_finish_kernel,
-                 dim3(unsigned((p.D + 31) / 32), 2), dim3(256), 0, stream, p,
-                 static_cast<const float*>(a.partial), blocks);
+                 dim3(unsigned((p.D + 31) / 32), 2), dim3(1024), 0, stream,
+                 f);
   if (e == cudaSuccess) count_launches(1);
   return e;
 }

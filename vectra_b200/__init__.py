@@ -4,8 +4,7 @@ Importing the package registers torch.ops.vectra.rbf_attention with its
 CUDA implementation (hand-written kernels in libvectra_rbf.so behind the C
 ABI of include/vectra_rbf.h) and the operators of a transformer block around
 it (`vectra_b200.block`, include/vectra_block.h). It raises ImportError if
-the libraries have
-not been built (`python vectra_b200/build.py`).
+the libraries have not been built (`python vectra_b200/build.py`).
 """
 
 from vectra_b200 import _lib

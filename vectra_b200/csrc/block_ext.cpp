@@ -22,6 +22,7 @@
 #include <optional>
 #include <string>
 #include <tuple>
+#include <utility>
 #include <vector>
 
 #include "vectra_block.h"
@@ -34,14 +35,14 @@ using OptTensor = std::optional<Tensor>;
 // ---------------------------------------------------------------------------
 // Shared checks.
 // ---------------------------------------------------------------------------
-int32_t activation_of(const std::string& name) {
+int32_t activation_of(c10::string_view name) {
   if (name == "none") return VECTRA_ACT_NONE;
   if (name == "relu") return VECTRA_ACT_RELU;
   if (name == "gelu") return VECTRA_ACT_GELU;
   if (name == "gelu_tanh") return VECTRA_ACT_GELU_TANH;
   if (name == "silu") return VECTRA_ACT_SILU;
   TORCH_CHECK_VALUE(false, "activation must be 'none', 'relu', 'gelu', "
-                           "'gelu_tanh' or 'silu', got '", name, "'");
+                           "'gelu_tanh' or 'silu', got '", std::string(name), "'");
 }
 
 bool io_dtype(at::ScalarType t) {
@@ -113,6 +114,37 @@ vectra_tensor describe(const Tensor& t) {
 
 vectra_tensor describe(const OptTensor& t) {
   return has(t) ? describe(*t) : vectra_tensor{};
+}
+
+// The same view as the ABI's description, without making a tensor of it;
+// where the leading dimensions do not allow one, `copy` keeps the copy.
+vectra_tensor describe_rows(const Tensor& t, Tensor* copy) {
+  const int64_t last = t.dim() - 1;
+  int64_t rows = 1, ld = 0;
+  bool regular = true;
+  for (int64_t i = last - 1; i >= 0; --i) {
+    if (t.size(i) != 1) {
+      if (rows == 1) {
+        ld = t.stride(i);
+      } else if (t.stride(i) != ld * rows) {
+        regular = false;
+      }
+    }
+    rows *= t.size(i);
+  }
+  if (!regular && rows > 0) {
+    *copy = as_rows(t);
+    return describe(*copy);
+  }
+  vectra_tensor d{};
+  d.data = t.data_ptr();
+  d.dtype = abi_dtype(t.scalar_type());
+  d.ndim = 2;
+  d.size[0] = rows;
+  d.size[1] = t.size(last);
+  d.stride[0] = rows > 1 ? ld : t.size(last);
+  d.stride[1] = t.stride(last);
+  return d;
 }
 
 [[noreturn]] void raise_status(const char* op, int status) {
@@ -202,33 +234,46 @@ void check_linear(const Tensor& x, const Tensor& w, const OptTensor& bias,
   }
 }
 
+Tensor linear_run(const Tensor& x, const Tensor& w, const OptTensor& bias,
+                  const OptTensor& residual, c10::string_view activation,
+                  Tensor* pre) {
+  check_linear(x, w, bias, residual);
+  c10::cuda::CUDAGuard guard(x.device());
+  const auto shape = with_last(x.sizes(), w.size(0));
+  Tensor y = at::empty(shape, x.options());
+  Tensor x_copy, res_copy;
+  vectra_linear_args a{};
+  a.activation = activation_of(activation);
+  a.x = describe_rows(x, &x_copy);
+  a.weight = describe(w);
+  a.bias = describe(bias);
+  if (has(residual)) a.residual = describe_rows(*residual, &res_copy);
+  a.y = describe_rows(y, nullptr);
+  if (pre != nullptr) {
+    *pre = at::empty(shape, x.options());
+    a.pre = describe_rows(*pre, nullptr);
+  }
+  call_with_workspace("linear", a, x, vectra_linear_forward_workspace_bytes,
+                      vectra_linear_forward);
+  return y;
+}
+
 std::tuple<Tensor, Tensor> linear_cuda(const Tensor& x, const Tensor& w,
                                        const OptTensor& bias,
                                        const OptTensor& residual,
                                        const std::string& activation,
                                        bool want_pre) {
-  check_linear(x, w, bias, residual);
-  c10::cuda::CUDAGuard guard(x.device());
-  const auto shape = with_last(x.sizes(), w.size(0));
-  Tensor y = at::empty(shape, x.options());
-  Tensor pre = at::empty(want_pre ? shape : std::vector<int64_t>{0},
-                         x.options());
-  const Tensor x2 = as_rows(x);
-  Tensor res2;
-  vectra_linear_args a{};
-  a.activation = activation_of(activation);
-  a.x = describe(x2);
-  a.weight = describe(w);
-  a.bias = describe(bias);
-  if (has(residual)) {
-    res2 = as_rows(*residual);
-    a.residual = describe(res2);
-  }
-  a.y = describe(as_rows(y));
-  if (want_pre) a.pre = describe(as_rows(pre));
-  call_with_workspace("linear", a, x, vectra_linear_forward_workspace_bytes,
-                      vectra_linear_forward);
+  Tensor pre;
+  Tensor y = linear_run(x, w, bias, residual, activation,
+                        want_pre ? &pre : nullptr);
+  if (!want_pre) pre = at::empty({0}, x.options());
   return {y, pre};
+}
+
+Tensor linear_only_cuda(const Tensor& x, const Tensor& w,
+                        const OptTensor& bias, const OptTensor& residual,
+                        c10::string_view activation) {
+  return linear_run(x, w, bias, residual, activation, nullptr);
 }
 
 std::tuple<Tensor, Tensor> linear_cpu(const Tensor& x, const Tensor& w,
@@ -270,8 +315,7 @@ Grads3 linear_backward_cuda(const Tensor& dy, const Tensor& x,
   const int32_t act = activation_of(activation);
   check_linear_grad(dy, x, w, pre, act);
   c10::cuda::CUDAGuard guard(x.device());
-  const Tensor x2 = as_rows(x), dy2 = as_rows(dy);
-  Tensor pre2;
+  Tensor x_copy, dy_copy, pre_copy;
   Tensor dx = at::empty(need_dx ? x.sizes().vec() : std::vector<int64_t>{0},
                         x.options());
   Tensor dw = need_dw ? at::empty(w.sizes(), x.options())
@@ -279,14 +323,14 @@ Grads3 linear_backward_cuda(const Tensor& dy, const Tensor& x,
   Tensor db = at::empty({need_db ? w.size(0) : 0}, x.options());
   vectra_linear_grad_args a{};
   a.activation = act;
-  a.dy = describe(dy2);
-  a.x = describe(x2);
+  a.dy = describe_rows(dy, &dy_copy);
+  a.x = describe_rows(x, &x_copy);
   a.weight = describe(w);
   if (act != VECTRA_ACT_NONE) {
-    pre2 = as_rows(pre.contiguous());
-    a.pre = describe(pre2);
+    pre_copy = pre.contiguous();
+    a.pre = describe_rows(pre_copy, nullptr);
   }
-  if (need_dx) a.dx = describe(as_rows(dx));
+  if (need_dx) a.dx = describe_rows(dx, nullptr);
   if (need_dw) a.dweight = describe(dw);
   if (need_db) a.dbias = describe(db);
   call_with_workspace("linear_backward", a, x,
@@ -332,35 +376,51 @@ void check_gated(const Tensor& x, const Tensor& wg, const Tensor& wu,
   }
 }
 
-Grads3 gated_cuda(const Tensor& x, const Tensor& wg, const Tensor& wu,
-                  const OptTensor& bg, const OptTensor& bu,
-                  const std::string& activation, bool want_pre) {
+Tensor gated_run(const Tensor& x, const Tensor& wg, const Tensor& wu,
+                 const OptTensor& bg, const OptTensor& bu,
+                 c10::string_view activation, Tensor* gate, Tensor* up) {
   check_gated(x, wg, wu, bg, bu);
   c10::cuda::CUDAGuard guard(x.device());
   const auto shape = with_last(x.sizes(), wg.size(0));
   Tensor h = at::empty(shape, x.options());
-  const std::vector<int64_t> pre =
-      want_pre ? shape : std::vector<int64_t>{0};
-  const auto f32_options = x.options().dtype(at::kFloat);
-  Tensor gate = at::empty(pre, f32_options);
-  Tensor up = at::empty(pre, f32_options);
-  const Tensor x2 = as_rows(x);
+  Tensor x_copy;
   vectra_gated_args a{};
   a.activation = activation_of(activation);
-  a.x = describe(x2);
+  a.x = describe_rows(x, &x_copy);
   a.w_gate = describe(wg);
   a.w_up = describe(wu);
   a.b_gate = describe(bg);
   a.b_up = describe(bu);
-  a.h = describe(as_rows(h));
-  if (want_pre) {
-    a.gate = describe(as_rows(gate));
-    a.up = describe(as_rows(up));
+  a.h = describe_rows(h, nullptr);
+  if (gate != nullptr) {
+    const auto f32_options = x.options().dtype(at::kFloat);
+    *gate = at::empty(shape, f32_options);
+    *up = at::empty(shape, f32_options);
+    a.gate = describe_rows(*gate, nullptr);
+    a.up = describe_rows(*up, nullptr);
   }
   call_with_workspace("gated_linear", a, x,
                       vectra_gated_linear_forward_workspace_bytes,
                       vectra_gated_linear_forward);
+  return h;
+}
+
+Grads3 gated_cuda(const Tensor& x, const Tensor& wg, const Tensor& wu,
+                  const OptTensor& bg, const OptTensor& bu,
+                  const std::string& activation, bool want_pre) {
+  Tensor gate, up;
+  Tensor h = gated_run(x, wg, wu, bg, bu, activation,
+                       want_pre ? &gate : nullptr, &up);
+  if (!want_pre)
+    for (Tensor* t : {&gate, &up})
+      *t = at::empty({0}, x.options().dtype(at::kFloat));
   return {h, gate, up};
+}
+
+Tensor gated_only_cuda(const Tensor& x, const Tensor& wg, const Tensor& wu,
+                       const OptTensor& bg, const OptTensor& bu,
+                       c10::string_view activation) {
+  return gated_run(x, wg, wu, bg, bu, activation, nullptr, nullptr);
 }
 
 Grads3 gated_cpu(const Tensor& x, const Tensor& wg, const Tensor& wu,
@@ -404,8 +464,8 @@ Grads5 gated_backward_cuda(const Tensor& dh, const Tensor& x,
                            bool need_dw, bool need_db) {
   check_gated_grad(dh, x, wg, wu, gate, up);
   c10::cuda::CUDAGuard guard(x.device());
-  const Tensor x2 = as_rows(x), dh2 = as_rows(dh);
-  const Tensor g2 = as_rows(gate.contiguous()), u2 = as_rows(up.contiguous());
+  Tensor x_copy, dh_copy;
+  const Tensor g = gate.contiguous(), u = up.contiguous();
   Tensor dx = at::empty(need_dx ? x.sizes().vec() : std::vector<int64_t>{0},
                         x.options());
   const auto weight = [&] {
@@ -418,13 +478,13 @@ Grads5 gated_backward_cuda(const Tensor& dh, const Tensor& x,
   Tensor dwg = weight(), dwu = weight(), dbg = bias(), dbu = bias();
   vectra_gated_grad_args a{};
   a.activation = activation_of(activation);
-  a.dh = describe(dh2);
-  a.x = describe(x2);
+  a.dh = describe_rows(dh, &dh_copy);
+  a.x = describe_rows(x, &x_copy);
   a.w_gate = describe(wg);
   a.w_up = describe(wu);
-  a.gate = describe(g2);
-  a.up = describe(u2);
-  if (need_dx) a.dx = describe(as_rows(dx));
+  a.gate = describe_rows(g, nullptr);
+  a.up = describe_rows(u, nullptr);
+  if (need_dx) a.dx = describe_rows(dx, nullptr);
   if (need_dw) {
     a.dw_gate = describe(dwg);
     a.dw_up = describe(dwu);
@@ -783,18 +843,40 @@ Grads4 call_qk_backward(const Tensor& dq, const Tensor& dk, const Tensor& q,
                  need_dw);
 }
 
-// One with_pre operator per layer holds the arithmetic; the plain entry
-// points are that without the extra results.
+// On CPU the plain entry points are the with_pre operators without the extra
+// results.
+Tensor linear_only_cpu(const Tensor& x, const Tensor& w, const OptTensor& bias,
+                    const OptTensor& residual, c10::string_view activation) {
+  return std::get<0>(linear_cpu(x, w, bias, residual,
+                                std::string(activation), false));
+}
+Tensor gated_only_cpu(const Tensor& x, const Tensor& wg, const Tensor& wu,
+                   const OptTensor& bg, const OptTensor& bu,
+                   c10::string_view activation) {
+  return std::get<0>(
+      gated_cpu(x, wg, wu, bg, bu, std::string(activation), false));
+}
+
+// The entry points below autograd.
 Tensor linear_below(const Tensor& x, const Tensor& w, const OptTensor& bias,
                     const OptTensor& residual, c10::string_view activation) {
-  return std::get<0>(call_linear(x, w, bias, residual,
-                                 std::string(activation), false));
+  static const auto op =
+      c10::Dispatcher::singleton()
+          .findSchemaOrThrow("vectra_b200::linear", "")
+          .typed<Tensor(const Tensor&, const Tensor&, const OptTensor&,
+                        const OptTensor&, c10::string_view)>();
+  return op.call(x, w, bias, residual, activation);
 }
 Tensor gated_below(const Tensor& x, const Tensor& wg, const Tensor& wu,
                    const OptTensor& bg, const OptTensor& bu,
                    c10::string_view activation) {
-  return std::get<0>(
-      call_gated(x, wg, wu, bg, bu, std::string(activation), false));
+  static const auto op =
+      c10::Dispatcher::singleton()
+          .findSchemaOrThrow("vectra_b200::gated_linear", "")
+          .typed<Tensor(const Tensor&, const Tensor&, const Tensor&,
+                        const OptTensor&, const OptTensor&,
+                        c10::string_view)>();
+  return op.call(x, wg, wu, bg, bu, activation);
 }
 
 using torch::autograd::AutogradContext;
@@ -1032,10 +1114,10 @@ TORCH_LIBRARY_FRAGMENT(vectra_b200, m) {
 }
 
 TORCH_LIBRARY_IMPL(vectra_b200, CUDA, m) {
-  m.impl("linear", &linear_below);
+  m.impl("linear", &linear_only_cuda);
   m.impl("linear_with_pre", &linear_impl<linear_cuda>);
   m.impl("linear_backward", &linear_backward_impl<linear_backward_cuda>);
-  m.impl("gated_linear", &gated_below);
+  m.impl("gated_linear", &gated_only_cuda);
   m.impl("gated_linear_with_pre", &gated_impl<gated_cuda>);
   m.impl("gated_linear_backward", &gated_backward_impl<gated_backward_cuda>);
   m.impl("qk_norm_rope", &qk_cuda);
@@ -1043,10 +1125,10 @@ TORCH_LIBRARY_IMPL(vectra_b200, CUDA, m) {
 }
 
 TORCH_LIBRARY_IMPL(vectra_b200, CPU, m) {
-  m.impl("linear", &linear_below);
+  m.impl("linear", &linear_only_cpu);
   m.impl("linear_with_pre", &linear_impl<linear_cpu>);
   m.impl("linear_backward", &linear_backward_impl<linear_backward_cpu>);
-  m.impl("gated_linear", &gated_below);
+  m.impl("gated_linear", &gated_only_cpu);
   m.impl("gated_linear_with_pre", &gated_impl<gated_cpu>);
   m.impl("gated_linear_backward", &gated_backward_impl<gated_backward_cpu>);
   m.impl("qk_norm_rope", &qk_cpu);

@@ -1,0 +1,172 @@
+// gemm_rows.cu: the products of a serving step, act(x W^T + b) + r or the
+// gated layer for a handful of rows of x (bf16 / f16).
+//
+// Bound by reading the weights once: 2 N K bytes against 2 M N K operations
+// with M <= 8. There is no reuse to stage for, so the weights go straight
+// from global memory into mma.sync operands: in m16n8k16 the weight rows are
+// the 16 rows, the tokens the 8 columns, and since a sum may run over the
+// reduction in any order, a lane's 16-byte load (eight neighbours of one
+// weight row) supplies its share of two MMAs when the token operand is read
+// with the same assignment.
+//
+// A block of 8 warps owns 16 weight rows; a gated layer's block 8 rows of
+// each weight, gate rows as MMA rows 0-7 and up rows as 8-15, so that both
+// factors of an output meet in it. The warps cut the reduction into eight
+// contiguous ranges, keep kDepth steps of 32 elements in flight each, and
+// are added in order through shared memory. Two blocks per SM keep 128 KB in
+// flight, which covers DRAM latency at full rate.
+#include "block_common.cuh"
+#include "gemm_rows.cuh"
+#include "mma_sync.cuh"
+
+namespace vectra {
+namespace {
+
+constexpr int kWarps = 8;
+constexpr int kTokens = 8;
+constexpr int kStep = 32;   // reduction per load of a lane quad
+constexpr int kDepth = 8;
+
+__device__ __forceinline__ uint4 load_stream(const void* p) {
+  uint4 v;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "l"(p));
+  return v;
+}
+
+template <bool kExact>
+__device__ __forceinline__ float act_any(float z, int act) {
+  switch (act) {
+    case VECTRA_ACT_RELU:
+      return act_fwd<kExact, VECTRA_ACT_RELU>(z);
+    case VECTRA_ACT_GELU:
+      return act_fwd<kExact, VECTRA_ACT_GELU>(z);
+    case VECTRA_ACT_GELU_TANH:
+      return act_fwd<kExact, VECTRA_ACT_GELU_TANH>(z);
+    case VECTRA_ACT_SILU:
+      return act_fwd<kExact, VECTRA_ACT_SILU>(z);
+    default:
+      return z;
+  }
+}
+
+template <typename T, bool GATED>
+__global__ void __launch_bounds__(kWarps * 32, 2)
+    gemm_rows_kernel(const __grid_constant__ GemmProblem p) {
+  constexpr int kCols = GATED ? 8 : 16;  // outputs per token of a block
+  __shared__ float sums[kWarps][kTokens][16 + 1];
+  allow_dependents();
+  grid_dependency_wait();
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int g = lane / 4, t = lane % 4;
+  const int64_t n0 = int64_t(blockIdx.x) * kCols;
+  // Contiguous ranges of whole 128-byte lines.
+  const int64_t steps = (p.K + kStep - 1) / kStep;
+  const int64_t per = ((steps + kWarps - 1) / kWarps + 1) / 2 * 2;
+  const int64_t s0 = warp * per;
+  const int64_t s1 = s0 + per < steps ? s0 + per : steps;
+
+  // MMA rows g and g + 8 of this lane.
+  const T* wp[2];
+  bool wok[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int64_t n = n0 + g + (GATED ? 0 : 8 * h);
+    const MatView& w = p.b[GATED ? h : 0];
+    wok[h] = n < p.N;
+    wp[h] = static_cast<const T*>(w.p) + (wok[h] ? n : 0) * w.sr + t * 8;
+  }
+  const bool xok = g < p.M;
+  const T* xp =
+      static_cast<const T*>(p.a[0].p) + (xok ? g : 0) * p.a[0].sr + t * 8;
+
+  float acc[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int64_t step = s0; step < s1; step += kDepth) {
+    uint4 w[kDepth][2], x[kDepth];
+#pragma unroll
+    for (int q = 0; q < kDepth; ++q) {
+      const int64_t k = (step + q) * kStep;
+      const bool in = step + q < s1 && k + t * 8 < p.K;
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        w[q][h] = in && wok[h] ? load_stream(wp[h] + k)
+                               : make_uint4(0, 0, 0, 0);
+      x[q] = in && xok ? __ldg(reinterpret_cast<const uint4*>(xp + k))
+                       : make_uint4(0, 0, 0, 0);
+    }
+#pragma unroll
+    for (int q = 0; q < kDepth; ++q) {
+      const uint4 &a = w[q][0], &b = w[q][1];
+      const uint32_t lo[4] = {a.x, b.x, a.y, b.y};
+      const uint32_t hi[4] = {a.z, b.z, a.w, b.w};
+      mma16816<T>(acc, lo, x[q].x, x[q].y);
+      mma16816<T>(acc, hi, x[q].z, x[q].w);
+    }
+  }
+#pragma unroll
+  for (int c = 0; c < 4; ++c)
+    sums[warp][2 * t + (c & 1)][g + 8 * (c >> 1)] = acc[c];
+  __syncthreads();
+  const int m = threadIdx.x / kCols, r = threadIdx.x % kCols;
+  const int64_t n = n0 + r;
+  if (m >= p.M || m >= kTokens || n >= p.N) return;
+  float z = 0.f, u = 0.f;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) {
+    z += sums[w][m][r];
+    if constexpr (GATED) u += sums[w][m][8 + r];
+  }
+  if (p.bias[0])
+    z += to_f32(static_cast<const T*>(p.bias[0])[n * p.bias_stride[0]]);
+  T* out = static_cast<T*>(p.out) + m * p.out_ld + n;
+  if constexpr (GATED) {
+    if (p.bias[1])
+      u += to_f32(static_cast<const T*>(p.bias[1])[n * p.bias_stride[1]]);
+    if (p.gate) {
+      p.gate[m * p.gate_ld + n] = z;
+      p.up[m * p.up_ld + n] = u;
+    }
+    *out = from_f32<T>(act_any<false>(z, p.act) * u);
+  } else {
+    if (p.pre) static_cast<T*>(p.pre)[m * p.pre_ld + n] = from_f32<T>(z);
+    float y = act_any<false>(z, p.act);
+    if (p.res)
+      y += to_f32(static_cast<const T*>(p.res)[m * p.res_sm + n * p.res_sn]);
+    *out = from_f32<T>(y);
+  }
+}
+
+bool line_view(const MatView& m, int64_t rows) {
+  return m.sk == 1 && (reinterpret_cast<uintptr_t>(m.p) & 15) == 0 &&
+         (rows <= 1 || m.sr % 8 == 0);
+}
+
+template <typename T, bool GATED>
+cudaError_t launch(const GemmProblem& p, cudaStream_t stream) {
+  const int64_t cols = GATED ? 8 : 16;
+  return launch_pdl(gemm_rows_kernel<T, GATED>,
+                    dim3(unsigned((p.N + cols - 1) / cols)),
+                    dim3(kWarps * 32), 0, stream, p);
+}
+
+}  // namespace
+
+bool gemm_rows_supports(const GemmProblem& p) {
+  if (p.dtype != VECTRA_BF16 && p.dtype != VECTRA_F16) return false;
+  if (p.M > kRowsMost || p.segments != 1 || p.K % 8 != 0 || p.K == 0)
+    return false;
+  return line_view(p.a[0], p.M) && line_view(p.b[0], p.N) &&
+         (p.epilogue != kEpiGated || line_view(p.b[1], p.N));
+}
+
+cudaError_t launch_gemm_rows(const GemmProblem& p, cudaStream_t stream) {
+  const bool gated = p.epilogue == kEpiGated;
+  if (p.dtype == VECTRA_BF16)
+    return gated ? launch<__nv_bfloat16, true>(p, stream)
+                 : launch<__nv_bfloat16, false>(p, stream);
+  return gated ? launch<__half, true>(p, stream)
+               : launch<__half, false>(p, stream);
+}
+
+}  // namespace vectra

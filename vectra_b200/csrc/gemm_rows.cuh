@@ -1,0 +1,14 @@
+// gemm_rows.cuh: interface of the few-row products (gemm_rows.cu).
+#pragma once
+
+#include "block_common.cuh"
+
+namespace vectra {
+
+constexpr int64_t kRowsMost = 8;  // rows of x
+
+// bf16 / f16, one product, 16-byte aligned rows along the reduction.
+bool gemm_rows_supports(const GemmProblem& p);
+cudaError_t launch_gemm_rows(const GemmProblem& p, cudaStream_t stream);
+
+}  // namespace vectra

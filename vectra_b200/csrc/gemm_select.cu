@@ -1,6 +1,7 @@
 // gemm_select.cu: which kernel computes a matrix product of the
 // transformer-block operators.
 #include "block_common.cuh"
+#include "gemm_rows.cuh"
 #include "gemm_tc.cuh"
 
 namespace vectra {
@@ -35,6 +36,12 @@ TcShape tc_shape(const GemmProblem& p) {
 cudaError_t run_gemm(const GemmProblem& p, Workspace& ws,
                      cudaStream_t stream) {
   if (p.M == 0 || p.N == 0) return cudaSuccess;
+  if (gemm_rows_supports(p)) {
+    if (ws.dry) return cudaSuccess;
+    const cudaError_t e = launch_gemm_rows(p, stream);
+    if (e == cudaSuccess) count_launches(1);
+    return e;
+  }
   if (gemm_tc_supports(p)) return run_gemm_tc(p, tc_shape(p), ws, stream);
   // Split the reduction when the output tiles leave SMs idle: enough parts
   // for one block per SM, at least 256 of the reduction each.

@@ -370,24 +370,28 @@ __device__ __forceinline__ void store_block_f32(uint8_t* stage, const float* v,
   }
 }
 
-// The residual's 32 x 32 block: global loads into registers (coalesced, to
-// be in flight before the accumulator is ready), then turned so that a lane
-// holds its row.
+// The residual's 32 x 32 block: asynchronous copies into the turning buffer
+// (coalesced, in flight while the accumulator is waited for and read), from
+// which a lane then takes its row.
 template <typename T>
-__device__ __forceinline__ void fetch_residual(uint4* raw,
+__device__ __forceinline__ void fetch_residual(uint8_t* stage,
                                                const GemmProblem& p,
                                                const RowBlock& rb,
                                                int64_t col, int lane) {
   const int r = lane / 4, c = (lane % 4) * 8;
   const T* q = static_cast<const T*>(p.res) + (rb.row0 + r) * p.res_sm + col +
                c;
+  const uint32_t dst = smem_addr(stage) + r * kStagePitch + c * 2;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    raw[i] = make_uint4(0, 0, 0, 0);
     if (r + 8 * i < rb.rows && col + c < p.N)
-      raw[i] = __ldg(reinterpret_cast<const uint4*>(q));
+      asm volatile("cp.async.ca.shared.global [%0], [%1], 16;" ::"r"(
+                       dst + i * 8 * kStagePitch),
+                   "l"(q)
+                   : "memory");
     q += 8 * p.res_sm;
   }
+  asm volatile("cp.async.commit_group;" ::: "memory");
 }
 
 template <typename T>
@@ -401,15 +405,11 @@ __device__ __forceinline__ float2 unpack2(uint32_t w) {
 
 template <typename T>
 __device__ __forceinline__ void add_residual(uint8_t* stage, float* v,
-                                             const uint4* raw, bool vec,
-                                             const GemmProblem& p,
+                                             bool vec, const GemmProblem& p,
                                              const RowBlock& rb, int64_t col,
                                              int lane) {
   if (vec) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      *reinterpret_cast<uint4*>(stage + (lane / 4 + 8 * i) * kStagePitch +
-                                (lane % 4) * 16) = raw[i];
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
   } else {
     const T* q = static_cast<const T*>(p.res) + rb.row0 * p.res_sm +
                  (col + lane) * p.res_sn;
@@ -482,13 +482,16 @@ __device__ __forceinline__ void epilogue_tile(const TcArgs& g, uint8_t* stage,
                    WARP_COLS, lane);
     __syncwarp();
   }
-  uint4 raw[4];
-  if constexpr (RES)
-    if (g.vec_res) fetch_residual<T>(raw, p, rb, tile_col, lane);
+  // With saved values in the same buffer the residual comes after them.
+  constexpr bool kEarly = RES && !PRE;
+  if constexpr (kEarly)
+    if (g.vec_res) fetch_residual<T>(stage, p, rb, tile_col, lane);
   if (!wait()) return;
 #pragma unroll 1
   for (int c0 = 0; c0 < WARP_COLS; c0 += 32) {
     const int64_t col = tile_col + c0;
+    if constexpr (kEarly)
+      if (g.vec_res && c0 > 0) fetch_residual<T>(stage, p, rb, col, lane);
     uint32_t r0[32];
     uint32_t r1[kGated ? 32 : 1];
     tmem_ld32u(acc + c0, r0);
@@ -520,13 +523,12 @@ __device__ __forceinline__ void epilogue_tile(const TcArgs& g, uint8_t* stage,
             zk[j] = pack2<T>(v[2 * j], v[2 * j + 1]);
           store_block<T>(stage, zk, static_cast<T*>(p.pre), p.pre_ld, rb,
                          col, p.N, g.vec_pre, lane);
+          if constexpr (RES)
+            if (g.vec_res) fetch_residual<T>(stage, p, rb, col, lane);
         }
         activate32<ACT>(v);
-        if constexpr (RES) {
-          add_residual<T>(stage, v, raw, g.vec_res, p, rb, col, lane);
-          if (g.vec_res && c0 + 32 < WARP_COLS)
-            fetch_residual<T>(raw, p, rb, col + 32, lane);
-        }
+        if constexpr (RES)
+          add_residual<T>(stage, v, g.vec_res, p, rb, col, lane);
       }
       if constexpr (EPI == kEpiGated) {
         float up[32];

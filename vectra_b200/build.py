@@ -33,10 +33,11 @@ TORCH_EXT = os.path.join(PKG, '_vectra_rbf_torch.so')
 
 CU_SOURCES = ['capi.cu', 'rbf_generic.cu', 'rbf_decode.cu', 'rbf_tc.cu',
               'rbf_small.cu', 'rbf_small_tc.cu', 'tma_maps.cu', 'scan.cu',
-              'block_capi.cu', 'block_grad.cu', 'gemm_generic.cu',
+              'block_capi.cu', 'block_grad.cu', 'gemm_finish.cu',
               'gemm_rows.cu', 'gemm_select.cu', 'gemm_tc.cu', 'gemm_tc_linear_bf16.cu',
               'gemm_tc_linear_f16.cu', 'gemm_tc_other_bf16.cu',
-              'gemm_tc_other_f16.cu', 'qk_norm_rope.cu']
+              'gemm_tc_other_f16.cu', 'gemm_tc_linear_f32.cu',
+              'gemm_tc_other_f32.cu', 'qk_norm_rope.cu']
 ARCH = ['-gencode', 'arch=compute_100a,code=sm_100a']
 
 

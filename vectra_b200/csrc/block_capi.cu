@@ -68,7 +68,7 @@ int check_common(const vectra_tensor& x, const vectra_tensor& w,
     return VECTRA_ERR_UNSUPPORTED;
   for (int i = 0; i < 2; ++i) {
     if (x.size[i] < 0 || w.size[i] < 0) return VECTRA_ERR_SHAPE;
-    // Sizes count blocks and tensor-map extents, which are 32-bit.
+    // Sizes count blocks and tensor-map lines, which are 32-bit.
     if (x.size[i] > kMaxSize || w.size[i] > kMaxSize)
       return VECTRA_ERR_UNSUPPORTED;
   }
@@ -487,7 +487,7 @@ const char* vectra_block_strerror(int status) {
              "int32 or int64)";
     case VECTRA_ERR_UNSUPPORTED:
       return "unsupported activation, a head width above 512, or a size "
-             "above 2^31 - 256";
+             "above 2^29 - 256";
     case VECTRA_ERR_LAYOUT:
       return "results and rotation tables need a unit inner stride and rows "
              "that do not overlap";

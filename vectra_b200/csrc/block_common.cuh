@@ -193,11 +193,8 @@ struct Workspace {
 // Runs (or, when ws.dry, sizes) one product; picks the kernel.
 cudaError_t run_gemm(const GemmProblem& p, Workspace& ws, cudaStream_t stream);
 
-// gemm_generic.cu: any strides, any type. `split` > 1 cuts the reduction
-// into that many parts, whose sums go to `partial` ([split][M][N], twice
-// that for kEpiGated) for launch_split_finish.
-cudaError_t launch_gemm_generic(const GemmProblem& p, int split,
-                                float* partial, cudaStream_t stream);
+// gemm_finish.cu: `partial` holds [split][M][N] float32 sums (for kEpiGated
+// [split][2][M][N]).
 // Adds the parts in order and applies the epilogue.
 cudaError_t launch_split_finish(const GemmProblem& p, int split,
                                 const float* partial, cudaStream_t stream);
@@ -257,9 +254,9 @@ cudaError_t launch_qk_forward(const QkProblem& p, cudaStream_t stream);
 cudaError_t run_qk_backward(const QkProblem& p, Workspace& ws,
                             cudaStream_t stream);
 
-// Largest size of one dimension: indices of a whole tile past it still fit
-// 32 bits.
-constexpr int64_t kMaxSize = (int64_t(1) << 31) - 256;
+// Largest size of one dimension: tensor-map coordinates are 32-bit, and
+// float32 operands keep three planes of lines in one map.
+constexpr int64_t kMaxSize = (int64_t(1) << 29) - 256;
 
 // Adds to the library's launch counter (capi.cu).
 void count_launches(int n);

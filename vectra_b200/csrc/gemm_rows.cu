@@ -1,5 +1,5 @@
 // gemm_rows.cu: the products of a serving step, act(x W^T + b) + r or the
-// gated layer for a handful of rows of x (bf16 / f16).
+// gated layer for up to eight rows of x.
 //
 // Bound by reading the weights once: 2 N K bytes against 2 M N K operations
 // with M <= 8. There is no reuse to stage for, so the weights go straight
@@ -48,6 +48,41 @@ __device__ __forceinline__ float act_any(float z, int act) {
       return act_fwd<kExact, VECTRA_ACT_SILU>(z);
     default:
       return z;
+  }
+}
+
+// The warps' sums, added in order, and the epilogue: one output per thread.
+template <typename T, bool GATED>
+__device__ __forceinline__ void finish_rows(
+    const GemmProblem& p, const float (*sums)[kTokens][16 + 1], int64_t n0) {
+  constexpr int kCols = GATED ? 8 : 16;
+  constexpr bool kExact = std::is_same<T, float>::value;
+  const int m = threadIdx.x / kCols, r = threadIdx.x % kCols;
+  const int64_t n = n0 + r;
+  if (m >= p.M || m >= kTokens || n >= p.N) return;
+  float z = 0.f, u = 0.f;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) {
+    z += sums[w][m][r];
+    if constexpr (GATED) u += sums[w][m][8 + r];
+  }
+  if (p.bias[0])
+    z += to_f32(static_cast<const T*>(p.bias[0])[n * p.bias_stride[0]]);
+  T* out = static_cast<T*>(p.out) + m * p.out_ld + n;
+  if constexpr (GATED) {
+    if (p.bias[1])
+      u += to_f32(static_cast<const T*>(p.bias[1])[n * p.bias_stride[1]]);
+    if (p.gate) {
+      p.gate[m * p.gate_ld + n] = z;
+      p.up[m * p.up_ld + n] = u;
+    }
+    *out = from_f32<T>(act_any<kExact>(z, p.act) * u);
+  } else {
+    if (p.pre) static_cast<T*>(p.pre)[m * p.pre_ld + n] = from_f32<T>(z);
+    float y = act_any<kExact>(z, p.act);
+    if (p.res)
+      y += to_f32(static_cast<const T*>(p.res)[m * p.res_sm + n * p.res_sn]);
+    *out = from_f32<T>(y);
   }
 }
 
@@ -108,65 +143,129 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
   for (int c = 0; c < 4; ++c)
     sums[warp][2 * t + (c & 1)][g + 8 * (c >> 1)] = acc[c];
   __syncthreads();
-  const int m = threadIdx.x / kCols, r = threadIdx.x % kCols;
-  const int64_t n = n0 + r;
-  if (m >= p.M || m >= kTokens || n >= p.N) return;
-  float z = 0.f, u = 0.f;
+  finish_rows<T, GATED>(p, sums, n0);
+}
+
+// The same for float32, on the FP32 pipe: a lane's 16 bytes are four
+// neighbours of a weight row, multiplied by the same four of every token and
+// added over the quad at the end.
+template <bool GATED, int TOKENS>
+__global__ void __launch_bounds__(kWarps * 32, 2)
+    gemm_rows_f32_kernel(const __grid_constant__ GemmProblem p) {
+  constexpr int kCols = GATED ? 8 : 16;
+  constexpr int kStep32 = 16, kDepth32 = 4;
+  __shared__ float sums[kWarps][kTokens][16 + 1];
+  allow_dependents();
+  grid_dependency_wait();
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int g = lane / 4, t = lane % 4;
+  const int64_t n0 = int64_t(blockIdx.x) * kCols;
+  const int64_t steps = (p.K + kStep32 - 1) / kStep32;
+  const int64_t per = ((steps + kWarps - 1) / kWarps + 1) / 2 * 2;
+  const int64_t s0 = warp * per;
+  const int64_t s1 = s0 + per < steps ? s0 + per : steps;
+  const float* wp[2];
+  bool wok[2];
 #pragma unroll
-  for (int w = 0; w < kWarps; ++w) {
-    z += sums[w][m][r];
-    if constexpr (GATED) u += sums[w][m][8 + r];
+  for (int h = 0; h < 2; ++h) {
+    const int64_t n = n0 + g + (GATED ? 0 : 8 * h);
+    const MatView& w = p.b[GATED ? h : 0];
+    wok[h] = n < p.N;
+    wp[h] = static_cast<const float*>(w.p) + (wok[h] ? n : 0) * w.sr + t * 4;
   }
-  if (p.bias[0])
-    z += to_f32(static_cast<const T*>(p.bias[0])[n * p.bias_stride[0]]);
-  T* out = static_cast<T*>(p.out) + m * p.out_ld + n;
-  if constexpr (GATED) {
-    if (p.bias[1])
-      u += to_f32(static_cast<const T*>(p.bias[1])[n * p.bias_stride[1]]);
-    if (p.gate) {
-      p.gate[m * p.gate_ld + n] = z;
-      p.up[m * p.up_ld + n] = u;
+  // Tokens past M repeat the last one; nothing of theirs is written.
+  const float* xp[TOKENS];
+#pragma unroll
+  for (int m = 0; m < TOKENS; ++m)
+    xp[m] = static_cast<const float*>(p.a[0].p) +
+            (m < p.M ? m : p.M - 1) * p.a[0].sr + t * 4;
+  float acc[2][TOKENS];
+#pragma unroll
+  for (int m = 0; m < TOKENS; ++m) acc[0][m] = acc[1][m] = 0.f;
+  for (int64_t step = s0; step < s1; step += kDepth32) {
+    union {
+      uint4 u;
+      float f[4];
+    } w[kDepth32][2];
+#pragma unroll
+    for (int q = 0; q < kDepth32; ++q) {
+      const int64_t k = (step + q) * kStep32;
+      const bool in = step + q < s1 && k + t * 4 < p.K;
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        w[q][h].u = in && wok[h] ? load_stream(wp[h] + k)
+                                 : make_uint4(0, 0, 0, 0);
     }
-    *out = from_f32<T>(act_any<false>(z, p.act) * u);
-  } else {
-    if (p.pre) static_cast<T*>(p.pre)[m * p.pre_ld + n] = from_f32<T>(z);
-    float y = act_any<false>(z, p.act);
-    if (p.res)
-      y += to_f32(static_cast<const T*>(p.res)[m * p.res_sm + n * p.res_sn]);
-    *out = from_f32<T>(y);
+#pragma unroll
+    for (int q = 0; q < kDepth32; ++q) {
+      const int64_t k = (step + q) * kStep32;
+      const bool in = step + q < s1 && k + t * 4 < p.K;
+      float4 x[TOKENS];
+#pragma unroll
+      for (int m = 0; m < TOKENS; ++m)
+        x[m] = in ? __ldg(reinterpret_cast<const float4*>(xp[m] + k))
+                  : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int m = 0; m < TOKENS; ++m)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          float v = acc[h][m];
+          v = fmaf(w[q][h].f[0], x[m].x, v);
+          v = fmaf(w[q][h].f[1], x[m].y, v);
+          v = fmaf(w[q][h].f[2], x[m].z, v);
+          acc[h][m] = fmaf(w[q][h].f[3], x[m].w, v);
+        }
+    }
   }
+#pragma unroll
+  for (int m = 0; m < TOKENS; ++m)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      float v = acc[h][m];
+      v += __shfl_xor_sync(0xffffffffu, v, 1);
+      v += __shfl_xor_sync(0xffffffffu, v, 2);
+      if (t == 0) sums[warp][m][g + 8 * h] = v;
+    }
+  __syncthreads();
+  finish_rows<float, GATED>(p, sums, n0);
 }
 
-bool line_view(const MatView& m, int64_t rows) {
+bool line_view(const MatView& m, int64_t rows, int64_t es) {
   return m.sk == 1 && (reinterpret_cast<uintptr_t>(m.p) & 15) == 0 &&
-         (rows <= 1 || m.sr % 8 == 0);
-}
-
-template <typename T, bool GATED>
-cudaError_t launch(const GemmProblem& p, cudaStream_t stream) {
-  const int64_t cols = GATED ? 8 : 16;
-  return launch_pdl(gemm_rows_kernel<T, GATED>,
-                    dim3(unsigned((p.N + cols - 1) / cols)),
-                    dim3(kWarps * 32), 0, stream, p);
+         (rows <= 1 || m.sr * es % 16 == 0);
 }
 
 }  // namespace
 
 bool gemm_rows_supports(const GemmProblem& p) {
-  if (p.dtype != VECTRA_BF16 && p.dtype != VECTRA_F16) return false;
-  if (p.M > kRowsMost || p.segments != 1 || p.K % 8 != 0 || p.K == 0)
-    return false;
-  return line_view(p.a[0], p.M) && line_view(p.b[0], p.N) &&
-         (p.epilogue != kEpiGated || line_view(p.b[1], p.N));
+  const int64_t es = p.dtype == VECTRA_F32 ? 4 : 2;
+  if (p.M > kRowsMost || p.segments != 1 || p.K * es % 16 != 0) return false;
+  return line_view(p.a[0], p.M, es) && line_view(p.b[0], p.N, es) &&
+         (p.epilogue != kEpiGated || line_view(p.b[1], p.N, es));
 }
 
 cudaError_t launch_gemm_rows(const GemmProblem& p, cudaStream_t stream) {
   const bool gated = p.epilogue == kEpiGated;
-  if (p.dtype == VECTRA_BF16)
-    return gated ? launch<__nv_bfloat16, true>(p, stream)
-                 : launch<__nv_bfloat16, false>(p, stream);
-  return gated ? launch<__half, true>(p, stream)
-               : launch<__half, false>(p, stream);
+  const int64_t cols = gated ? 8 : 16;
+  const dim3 grid(unsigned((p.N + cols - 1) / cols)), block(kWarps * 32);
+  auto run = [&](auto kernel) {
+    return launch_pdl(kernel, grid, block, 0, stream, p);
+  };
+  if (p.dtype == VECTRA_F32) {
+    if (p.M == 1)
+      return gated ? run(gemm_rows_f32_kernel<true, 1>)
+                   : run(gemm_rows_f32_kernel<false, 1>);
+    if (p.M <= 4)
+      return gated ? run(gemm_rows_f32_kernel<true, 4>)
+                   : run(gemm_rows_f32_kernel<false, 4>);
+    return gated ? run(gemm_rows_f32_kernel<true, 8>)
+                 : run(gemm_rows_f32_kernel<false, 8>);
+  }
+  if (p.dtype == VECTRA_F16)
+    return gated ? run(gemm_rows_kernel<__half, true>)
+                 : run(gemm_rows_kernel<__half, false>);
+  return gated ? run(gemm_rows_kernel<__nv_bfloat16, true>)
+               : run(gemm_rows_kernel<__nv_bfloat16, false>);
 }
 
 }  // namespace vectra

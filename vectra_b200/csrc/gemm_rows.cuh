@@ -7,7 +7,7 @@ namespace vectra {
 
 constexpr int64_t kRowsMost = 8;  // rows of x
 
-// bf16 / f16, one product, 16-byte aligned rows along the reduction.
+// One product, operands in 16-byte aligned rows along the reduction.
 bool gemm_rows_supports(const GemmProblem& p);
 cudaError_t launch_gemm_rows(const GemmProblem& p, cudaStream_t stream);
 

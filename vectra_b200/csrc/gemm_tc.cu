@@ -24,6 +24,72 @@ __global__ void __launch_bounds__(256)
   }
 }
 
+// Splits float32 into three bf16 planes: hi the nearest bf16, mid the
+// nearest to the rest, lo the rest's rest (exact: 8 + 8 + 8 bits). A value
+// that would round up to infinity is truncated instead; infinities and NaN
+// stand in hi alone.
+__device__ __forceinline__ void split3(float x, __nv_bfloat16* hi,
+                                       __nv_bfloat16* mid,
+                                       __nv_bfloat16* lo) {
+  __nv_bfloat16 h = __float2bfloat16_rn(x);
+  const bool finite = fabsf(x) <= 3.402823466e38f;
+  if (finite && fabsf(x) >= 3.39e38f) h = __float2bfloat16_rz(x);
+  const float r = finite ? x - __bfloat162float(h) : 0.f;
+  const __nv_bfloat16 m = __float2bfloat16_rn(r);
+  *hi = h;
+  *mid = m;
+  *lo = __float2bfloat16_rn(r - __bfloat162float(m));
+}
+
+// dst[plane][line][i], lines past `outer` zero; VEC elements per thread.
+template <int VEC>
+__global__ void __launch_bounds__(256)
+    split_planes_kernel(const float* src, int64_t s_outer, int64_t s_inner,
+                        __nv_bfloat16* dst, int64_t ld, int64_t outer,
+                        int64_t lines, int64_t inner) {
+  allow_dependents();
+  grid_dependency_wait();
+  const int64_t per_line = (inner + VEC - 1) / VEC;
+  const int64_t total = lines * per_line;
+  const int64_t plane = lines * ld;
+  const int64_t step = int64_t(gridDim.x) * blockDim.x;
+  for (int64_t e = int64_t(blockIdx.x) * blockDim.x + threadIdx.x; e < total;
+       e += step) {
+    const int64_t o = e / per_line, i = (e - o * per_line) * VEC;
+    union {
+      __nv_bfloat16 e[VEC];
+      uint4 u[VEC / 8 > 0 ? VEC / 8 : 1];
+    } q[3];
+    float x[VEC];
+    if constexpr (VEC == 8) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (o < outer)
+          f = __ldg(reinterpret_cast<const float4*>(src + o * s_outer + i) +
+                    h);
+        x[4 * h] = f.x;
+        x[4 * h + 1] = f.y;
+        x[4 * h + 2] = f.z;
+        x[4 * h + 3] = f.w;
+      }
+    } else {
+      x[0] = o < outer ? src[o * s_outer + i * s_inner] : 0.f;
+    }
+#pragma unroll
+    for (int v = 0; v < VEC; ++v)
+      split3(x[v], &q[0].e[v], &q[1].e[v], &q[2].e[v]);
+#pragma unroll
+    for (int s = 0; s < 3; ++s) {
+      __nv_bfloat16* d = dst + s * plane + o * ld + i;
+      if constexpr (VEC == 8)
+        *reinterpret_cast<uint4*>(d) = q[s].u[0];
+      else
+        *d = q[s].e[0];
+    }
+  }
+}
+
 bool aligned16(const void* p) {
   return (reinterpret_cast<uintptr_t>(p) & 15) == 0;
 }
@@ -31,8 +97,10 @@ bool aligned16(const void* p) {
 // An operand as the tensor maps see it.
 struct TmaOperand {
   const void* p;
-  bool mn;        // rows contiguous
-  int64_t ld;     // elements between lines of the other direction
+  bool mn;         // rows contiguous
+  int64_t ld;      // elements between lines of the other direction
+  int64_t lines;   // lines of one plane
+  int planes;
 };
 
 bool describable(const MatView& m, int64_t rows, int64_t k, bool mn) {
@@ -55,7 +123,7 @@ cudaError_t pack(const MatView& m, int64_t rows, int64_t k, bool mn,
   const int64_t outer = mn ? k : rows, inner = mn ? rows : k;
   const int64_t ld = (inner + 7) / 8 * 8;
   uint16_t* dst = static_cast<uint16_t*>(ws.take(size_t(outer) * ld * 2));
-  *out = {dst, mn, ld};
+  *out = {dst, mn, ld, outer, 1};
   if (ws.dry || ws.overflow) return cudaSuccess;
   const int64_t blocks = (outer * inner + 255) / 256;
   const int64_t most = int64_t(device_sm_count()) * 16;
@@ -67,25 +135,51 @@ cudaError_t pack(const MatView& m, int64_t rows, int64_t k, bool mn,
   return e;
 }
 
-}  // namespace
-
-bool gemm_tc_supports(const GemmProblem& p) {
-  return (p.dtype == VECTRA_BF16 || p.dtype == VECTRA_F16) && p.K > 0 &&
-         p.K < (int64_t(1) << 30);
+// float32 to planes. The lines of a reduction are padded with zeros to whole
+// stages: a stage that ran past one plane would read the next.
+cudaError_t split_planes(const MatView& m, int64_t rows, int64_t k, bool mn,
+                         Workspace& ws, TmaOperand* out,
+                         cudaStream_t stream) {
+  const int64_t outer = mn ? k : rows, inner = mn ? rows : k;
+  const int64_t lines =
+      mn ? (k + kTcStep - 1) / kTcStep * kTcStep : rows;
+  const int64_t ld = (inner + 7) / 8 * 8;
+  auto* dst = static_cast<__nv_bfloat16*>(
+      ws.take(size_t(3) * lines * ld * 2));
+  *out = {dst, mn, ld, lines, 3};
+  if (ws.dry || ws.overflow) return cudaSuccess;
+  const int64_t s_outer = mn ? m.sk : m.sr, s_inner = mn ? m.sr : m.sk;
+  const bool vec = inner % 8 == 0 && (s_inner == 1 || inner == 1) &&
+                   aligned16(m.p) && (outer <= 1 || s_outer % 4 == 0);
+  const int64_t blocks = (lines * (inner / (vec ? 8 : 1) + 1) + 255) / 256;
+  const int64_t most = int64_t(device_sm_count()) * 16;
+  const dim3 grid(unsigned(blocks < most ? blocks : most));
+  const float* src = static_cast<const float*>(m.p);
+  const cudaError_t e =
+      vec ? launch_pdl(split_planes_kernel<8>, grid, dim3(256), 0, stream,
+                       src, s_outer, s_inner, dst, ld, outer, lines, inner)
+          : launch_pdl(split_planes_kernel<1>, grid, dim3(256), 0, stream,
+                       src, s_outer, s_inner, dst, ld, outer, lines, inner);
+  if (e == cudaSuccess) count_launches(1);
+  return e;
 }
+
+}  // namespace
 
 cudaError_t run_gemm_tc(const GemmProblem& p, const TcShape& shape,
                         Workspace& ws, cudaStream_t stream) {
   const bool gated = p.epilogue == kEpiGated;
   const int tile_n = gated ? shape.bn / 2 : shape.bn;
-  if (tile_n < 64 || (shape.bn == 256) != (shape.cg == 2))
+  if (tile_n < 64 || (shape.bn == 256) != (shape.cg == 2) ||
+      (shape.cg == 2 && p.dtype == VECTRA_F32))
     return cudaErrorInvalidValue;
   TcArgs g{};
   g.p = p;
   g.tiles_m = int((p.M + kTcRows * shape.cg - 1) / (kTcRows * shape.cg));
   g.tiles_n = int((p.N + tile_n - 1) / tile_n);
   g.steps_seg = int((p.K + kTcStep - 1) / kTcStep);
-  g.steps = g.steps_seg * p.segments;
+  const bool f32 = p.dtype == VECTRA_F32;
+  g.steps = g.steps_seg * p.segments * (f32 ? 6 : 1);
   g.split = shape.split;
   g.steps_part = (g.steps + g.split - 1) / g.split;
   g.split = (g.steps + g.steps_part - 1) / g.steps_part;  // no empty parts
@@ -98,20 +192,33 @@ cudaError_t run_gemm_tc(const GemmProblem& p, const TcShape& shape,
     const MatView* v = side ? p.b : p.a;
     const int n = side ? n_b : n_a;
     const int64_t rows = side ? p.N : p.M;
-    int form = form_of(v[0], rows, p.K);
+    int form = f32 ? -1 : form_of(v[0], rows, p.K);
     if (form < 0) form = v[0].sr == 1 && v[0].sk != 1;
+    const bool mn = form == 1;
     for (int i = 0; i < n; ++i) {
-      if (describable(v[i], rows, p.K, form == 1)) {
-        op[2 * side + i] = {v[i].p, form == 1, form ? v[i].sk : v[i].sr};
-      } else {
-        const cudaError_t e =
-            pack(v[i], rows, p.K, form == 1, ws, &op[2 * side + i], stream);
-        if (e != cudaSuccess) return e;
-      }
+      TmaOperand* o = &op[2 * side + i];
+      cudaError_t e = cudaSuccess;
+      if (f32)
+        e = split_planes(v[i], rows, p.K, mn, ws, o, stream);
+      else if (describable(v[i], rows, p.K, mn))
+        *o = {v[i].p, mn, mn ? v[i].sk : v[i].sr, mn ? p.K : rows, 1};
+      else
+        e = pack(v[i], rows, p.K, mn, ws, o, stream);
+      if (e != cudaSuccess) return e;
     }
     if (n == 1) op[2 * side + 1] = op[2 * side];
-    (side ? g.b_mn : g.a_mn) = uint8_t(form == 1);
+    (side ? g.b_mn : g.a_mn) = uint8_t(mn);
   }
+  // hi, mid and lo are planes 0, 1 and 2.
+  constexpr int kPlanes[6][2] = {{2, 0}, {0, 2}, {1, 1},
+                                 {1, 0}, {0, 1}, {0, 0}};
+  for (int s = 0; s < p.segments; ++s)
+    for (int i = 0; i < (f32 ? 6 : 1); ++i) {
+      TcSegment& seg = g.seg[f32 ? i * p.segments + s : s];
+      seg.map = s;
+      seg.a_line = f32 ? int(kPlanes[i][0] * op[0].lines) : 0;
+      seg.b_line = f32 ? int(kPlanes[i][1] * op[2].lines) : 0;
+    }
   if (g.split > 1)
     g.partial = static_cast<float*>(ws.take(
         size_t(g.split) * (gated ? 2 : 1) * p.M * p.N * sizeof(float)));
@@ -120,10 +227,11 @@ cudaError_t run_gemm_tc(const GemmProblem& p, const TcShape& shape,
   const auto vec = [](const void* q, int64_t ld, int64_t es) {
     return uint8_t(aligned16(q) && (ld * es) % 16 == 0);
   };
-  const bool n8 = p.N % 8 == 0;
-  g.vec_out = n8 && vec(p.out, p.out_ld, 2);
-  g.vec_pre = n8 && vec(p.pre, p.pre_ld, 2);
-  g.vec_res = n8 && p.res_sn == 1 && vec(p.res, p.res_sm, 2);
+  const int64_t es = f32 ? 4 : 2;
+  const bool whole = p.N * es % 16 == 0;
+  g.vec_out = whole && vec(p.out, p.out_ld, es);
+  g.vec_pre = whole && vec(p.pre, p.pre_ld, es);
+  g.vec_res = whole && p.res_sn == 1 && vec(p.res, p.res_sm, es);
   g.vec_f32 = g.split > 1 ? p.N % 4 == 0
                           : p.N % 4 == 0 && vec(p.gate, p.gate_ld, 4) &&
                                 vec(p.up, p.up_ld, 4);
@@ -134,24 +242,21 @@ cudaError_t run_gemm_tc(const GemmProblem& p, const TcShape& shape,
   for (int i = 0; i < 4; ++i) {
     const int64_t rows = i < 2 ? p.M : p.N;
     const TmaOperand& o = op[i];
-    const int64_t inner = o.mn ? rows : p.K, outer = o.mn ? p.K : rows;
     const int box = o.mn ? kTcStep : (i < 2 ? kTcRows : b_rows);
-    if (!make_line_map(&maps[i], o.p, p.dtype, inner, outer, o.ld, box))
+    if (!make_line_map(&maps[i], o.p,
+                       p.dtype == VECTRA_F16 ? VECTRA_F16 : VECTRA_BF16,
+                       o.mn ? rows : p.K, o.lines * o.planes, o.ld, box))
       return cudaErrorInvalidValue;
   }
   const int epilogue =
       g.split == 1 ? p.epilogue : (gated ? kEpiGatedPartial : kEpiPartial);
-  const bool bf16 = p.dtype == VECTRA_BF16;
-  const cudaError_t e =
-      epilogue == kEpiLinear
-          ? (bf16 ? launch_tc_linear<__nv_bfloat16>(shape.bn, shape.cg, maps,
-                                                    g, stream)
-                  : launch_tc_linear<__half>(shape.bn, shape.cg, maps, g,
-                                             stream))
-          : (bf16 ? launch_tc_other<__nv_bfloat16>(epilogue, shape.bn,
-                                                   shape.cg, maps, g, stream)
-                  : launch_tc_other<__half>(epilogue, shape.bn, shape.cg,
-                                            maps, g, stream));
+  const cudaError_t e = with_dtype(p.dtype, [&](auto* t) {
+    using T = std::remove_pointer_t<decltype(t)>;
+    return epilogue == kEpiLinear
+               ? launch_tc_linear<T>(shape.bn, shape.cg, maps, g, stream)
+               : launch_tc_other<T>(epilogue, shape.bn, shape.cg, maps, g,
+                                    stream);
+  });
   if (e != cudaSuccess) return e;
   count_launches(1);
   if (g.split > 1) {

@@ -16,6 +16,13 @@ struct TcShape {
 constexpr int kTcRows = 128;  // rows of a tile per CTA
 constexpr int kTcStep = 64;   // reduction per stage: one 128-byte row
 
+// One product of the sum: which tensor maps (0 or 1), and where the operands'
+// lines start in them (float32 operands keep three planes in one map).
+struct TcSegment {
+  int32_t map, a_line, b_line;
+};
+constexpr int kMostSegments = 12;
+
 struct TcArgs {
   GemmProblem p;
   float* partial;     // split > 1: [split][planes][M][N]
@@ -27,6 +34,7 @@ struct TcArgs {
   int64_t units;      // tiles * split
   uint8_t a_mn, b_mn;  // operand staged MN-major
   uint8_t vec_out, vec_pre, vec_res, vec_f32;
+  TcSegment seg[kMostSegments];
 };
 
 // Epilogues of the kernels beyond GemmEpilogue: float32 sums of one part.
@@ -40,8 +48,7 @@ cudaError_t launch_tc_other(int epilogue, int bn, int cg,
                             const CUtensorMap* maps, const TcArgs& g,
                             cudaStream_t stream);
 
-// bf16 / f16 products with a non-empty reduction, in any layout.
-bool gemm_tc_supports(const GemmProblem& p);
+// Any type and layout; the reduction is not empty.
 cudaError_t run_gemm_tc(const GemmProblem& p, const TcShape& shape,
                         Workspace& ws, cudaStream_t stream);
 

@@ -27,6 +27,12 @@
 // one MMA makes both projections, and the epilogue finds both factors of an
 // output in its row.
 //
+// float32 tensors: each operand is first split into three bf16 planes, hi +
+// mid + lo, 24 bits in all, and the product is the sum of the six plane
+// products that matter (lo hi, hi lo, mid mid, mid hi, hi mid, hi hi, small
+// ones first), as further segments of the same reduction: 6 bf16 products
+// run at 3.5 times the FP32 pipe's rate.
+//
 // A reduction too long for its few tiles is cut into parts that write
 // float32 sums to the workspace; launch_split_finish adds them in order.
 // Every wait is bounded (error word and early exit).
@@ -97,6 +103,21 @@ __device__ __forceinline__ Unit unit_of(const TcArgs& a, int64_t u) {
   r.m = first + in % rows;
   r.n = in / rows;
   return r;
+}
+
+// float32: where the accumulation that starts at step `from` ends. The tensor
+// cores add into the accumulator rounding toward zero, so a long sum drifts
+// (by -2e-8 of itself for every 16 products: 1.4e-5 after 4,096 positive
+// ones). The five small plane products are too small for that to matter, but
+// of the last, hi hi, every 512 of the reduction is accumulated apart and
+// added by the epilogue, which rounds to nearest.
+constexpr int kChunkSteps = 8;
+__device__ __forceinline__ int chunk_end(const TcArgs& g, int from,
+                                         int last) {
+  const int small = g.steps / 6 * 5;  // steps before hi hi
+  const int at = from < small ? 0 : (from - small) / kChunkSteps;
+  const int end = small + (at + 1) * kChunkSteps;
+  return end < last ? end : last;
 }
 
 // ---------------------------------------------------------------------------
@@ -274,11 +295,11 @@ __device__ __forceinline__ void tie8(float* v) {
                  "+f"(v[5]), "+f"(v[6]), "+f"(v[7]));
 }
 
-template <int ACT>
-__device__ __forceinline__ void activate32(float* v) {
+template <int ACT, int N>
+__device__ __forceinline__ void activate(float* v) {
   if constexpr (ACT != VECTRA_ACT_NONE) {
 #pragma unroll
-    for (int j = 0; j < 32; j += 8) {
+    for (int j = 0; j < N; j += 8) {
       tie8(v + j);
 #pragma unroll
       for (int i = 0; i < 8; i += 2) activate2<ACT>(v[j + i], v[j + i + 1]);
@@ -332,42 +353,45 @@ __device__ __forceinline__ void store_block(uint8_t* stage, const uint32_t* pk,
   __syncwarp();
 }
 
-// The same for float32, 16 columns at a time.
+// The same for 16 columns of float32.
+__device__ __forceinline__ void store_half_f32(uint8_t* stage, const float* v,
+                                               float* out, int64_t ld,
+                                               const RowBlock& rb,
+                                               int64_t col, int64_t cols,
+                                               bool vec, int lane) {
+#pragma unroll
+  for (int c = 0; c < 4; ++c)
+    *reinterpret_cast<float4*>(stage + lane * kStagePitch + c * 16) =
+        make_float4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
+  __syncwarp();
+  if (vec) {
+    const int r = lane / 4, c = (lane % 4) * 4;
+    if (col + c < cols) {
+      float* q = out + (rb.row0 + r) * ld + col + c;
+      const uint8_t* s = stage + r * kStagePitch + c * 4;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (r + 8 * i < rb.rows)
+          *reinterpret_cast<float4*>(q) =
+              *reinterpret_cast<const float4*>(s + i * 8 * kStagePitch);
+        q += 8 * ld;
+      }
+    }
+  } else if (col + lane % 16 < cols) {
+    float* q = out + (rb.row0 + lane / 16) * ld + col + lane % 16;
+    for (int r = lane / 16; r < rb.rows; r += 2, q += 2 * ld)
+      *q =
+          reinterpret_cast<const float*>(stage + r * kStagePitch)[lane % 16];
+  }
+  __syncwarp();
+}
 __device__ __forceinline__ void store_block_f32(uint8_t* stage, const float* v,
                                                 float* out, int64_t ld,
                                                 const RowBlock& rb,
-                                                int64_t col0, int64_t cols,
+                                                int64_t col, int64_t cols,
                                                 bool vec, int lane) {
-#pragma unroll
-  for (int h = 0; h < 32; h += 16) {
-    const int64_t col = col0 + h;
-#pragma unroll
-    for (int c = 0; c < 4; ++c)
-      *reinterpret_cast<float4*>(stage + lane * kStagePitch + c * 16) =
-          make_float4(v[h + 4 * c], v[h + 4 * c + 1], v[h + 4 * c + 2],
-                      v[h + 4 * c + 3]);
-    __syncwarp();
-    if (vec) {
-      const int r = lane / 4, c = (lane % 4) * 4;
-      if (col + c < cols) {
-        float* q = out + (rb.row0 + r) * ld + col + c;
-        const uint8_t* s = stage + r * kStagePitch + c * 4;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          if (r + 8 * i < rb.rows)
-            *reinterpret_cast<float4*>(q) =
-                *reinterpret_cast<const float4*>(s + i * 8 * kStagePitch);
-          q += 8 * ld;
-        }
-      }
-    } else if (col + lane % 16 < cols) {
-      float* q = out + (rb.row0 + lane / 16) * ld + col + lane % 16;
-      for (int r = lane / 16; r < rb.rows; r += 2, q += 2 * ld)
-        *q = reinterpret_cast<const float*>(stage +
-                                            r * kStagePitch)[lane % 16];
-    }
-    __syncwarp();
-  }
+  store_half_f32(stage, v, out, ld, rb, col, cols, vec, lane);
+  store_half_f32(stage, v + 16, out, ld, rb, col + 16, cols, vec, lane);
 }
 
 // The residual's 32 x 32 block: asynchronous copies into the turning buffer
@@ -433,6 +457,63 @@ __device__ __forceinline__ void add_residual(uint8_t* stage, float* v,
   __syncwarp();
 }
 
+// Adds a float32 residual, 16 columns at a time.
+__device__ __forceinline__ void add_residual_f32(uint8_t* stage, float* v,
+                                                 bool vec,
+                                                 const GemmProblem& p,
+                                                 const RowBlock& rb,
+                                                 int64_t col0, int lane) {
+  const float* res = static_cast<const float*>(p.res);
+#pragma unroll
+  for (int h = 0; h < 32; h += 16) {
+    const int64_t col = col0 + h;
+    if (vec) {
+      const int r = lane / 4, c = (lane % 4) * 4;
+      const float* q = res + (rb.row0 + r) * p.res_sm + col + c;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (r + 8 * i < rb.rows && col + c < p.N)
+          *reinterpret_cast<float4*>(stage + (r + 8 * i) * kStagePitch +
+                                     c * 4) =
+              __ldg(reinterpret_cast<const float4*>(q));
+        q += 8 * p.res_sm;
+      }
+    } else if (col + lane % 16 < p.N) {
+      for (int r = lane / 16; r < rb.rows; r += 2)
+        reinterpret_cast<float*>(stage + r * kStagePitch)[lane % 16] =
+            res[(rb.row0 + r) * p.res_sm + (col + lane % 16) * p.res_sn];
+    }
+    __syncwarp();
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const float4 q = *reinterpret_cast<const float4*>(
+          stage + lane * kStagePitch + c * 16);
+      v[h + 4 * c] += q.x;
+      v[h + 4 * c + 1] += q.y;
+      v[h + 4 * c + 2] += q.z;
+      v[h + 4 * c + 3] += q.w;
+    }
+    __syncwarp();
+  }
+}
+
+// A block of 32 x 32 results (or saved values) in T.
+template <typename T>
+__device__ __forceinline__ void store_values(uint8_t* stage, const float* v,
+                                             T* out, int64_t ld,
+                                             const RowBlock& rb, int64_t col,
+                                             int64_t cols, bool vec,
+                                             int lane) {
+  if constexpr (std::is_same<T, float>::value) {
+    store_block_f32(stage, v, out, ld, rb, col, cols, vec, lane);
+  } else {
+    uint32_t pk[16];
+#pragma unroll
+    for (int j = 0; j < 16; ++j) pk[j] = pack2<T>(v[2 * j], v[2 * j + 1]);
+    store_block<T>(stage, pk, out, ld, rb, col, cols, vec, lane);
+  }
+}
+
 // Biases of a warp's columns, as floats in its shared memory; zeros without
 // a bias, so that the columns' loop needs no branch.
 template <typename T>
@@ -444,9 +525,10 @@ __device__ __forceinline__ void load_bias(float* dst, const void* bias,
                  ? to_f32(static_cast<const T*>(bias)[(col + c) * stride])
                  : 0.f;
 }
+template <int N>
 __device__ __forceinline__ void add_bias(float* v, const float* cols) {
 #pragma unroll
-  for (int j = 0; j < 32; j += 4) {
+  for (int j = 0; j < N; j += 4) {
     const float4 b = *reinterpret_cast<const float4*>(cols + j);
     v[j] += b.x;
     v[j + 1] += b.y;
@@ -455,17 +537,17 @@ __device__ __forceinline__ void add_bias(float* v, const float* cols) {
   }
 }
 
-// One tile of one epilogue warp: `acc` is the TMEM address of its rows and
-// first column, `cols` its bias values in shared memory (a gated layer's up
-// biases 64 behind). `wait` waits for the accumulator, `release` gives it
-// back after its last read. What a call does not need is compiled out: with
+// One tile of one epilogue warp: `cols` its bias values in shared memory (a
+// gated layer's up biases 64 behind). `wait` waits for the next accumulator
+// and gives the TMEM address of the warp's rows and first column, `release`
+// gives it back after the last read. What a call does not need is compiled out: with
 // the residual, the saved values and the partial sums behind run-time
 // branches the values were copied between registers at every join, 10
 // instructions for each result where the bare store takes 6.
 template <int EPI, int ACT, bool RES, bool PRE, typename T, int TILE_N,
           int WARP_COLS, typename Wait, typename Release>
 __device__ __forceinline__ void epilogue_tile(const TcArgs& g, uint8_t* stage,
-                                              float* cols, uint32_t acc,
+                                              float* cols, int chunks,
                                               const RowBlock& rb,
                                               int64_t tile_col, int part,
                                               int lane, Wait&& wait,
@@ -483,74 +565,146 @@ __device__ __forceinline__ void epilogue_tile(const TcArgs& g, uint8_t* stage,
     __syncwarp();
   }
   // With saved values in the same buffer the residual comes after them.
-  constexpr bool kEarly = RES && !PRE;
+  constexpr bool kF32 = std::is_same<T, float>::value;
+  constexpr bool kEarly = RES && !PRE && !kF32;
   if constexpr (kEarly)
     if (g.vec_res) fetch_residual<T>(stage, p, rb, tile_col, lane);
-  if (!wait()) return;
-#pragma unroll 1
-  for (int c0 = 0; c0 < WARP_COLS; c0 += 32) {
+  // 32 columns: `v` their sums, `up` a gated layer's second ones.
+  auto finish = [&](float* v, float* up, int c0) {
     const int64_t col = tile_col + c0;
-    if constexpr (kEarly)
-      if (g.vec_res && c0 > 0) fetch_residual<T>(stage, p, rb, col, lane);
-    uint32_t r0[32];
-    uint32_t r1[kGated ? 32 : 1];
-    tmem_ld32u(acc + c0, r0);
-    if constexpr (kGated) tmem_ld32u(acc + TILE_N + c0, r1);
-    tmem_wait_ld_tied(r0);
-    if constexpr (kGated) regs_tie32(r1);
-    if (c0 + 32 == WARP_COLS) release();
-    if (rb.rows <= 0 || col >= p.N) continue;
-    float v[32];
-#pragma unroll
-    for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r0[j]);
     if constexpr (kPartial) {
       const int64_t plane = p.M * p.N;
       float* q = g.partial + int64_t(part) * (kGated ? 2 : 1) * plane;
       store_block_f32(stage, v, q, p.N, rb, col, p.N, g.vec_f32, lane);
-      if constexpr (kGated) {
-#pragma unroll
-        for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r1[j]);
-        store_block_f32(stage, v, q + plane, p.N, rb, col, p.N, g.vec_f32,
+      if constexpr (kGated)
+        store_block_f32(stage, up, q + plane, p.N, rb, col, p.N, g.vec_f32,
                         lane);
-      }
     } else {
       if constexpr (EPI == kEpiLinear) {
-        add_bias(v, cols + c0);
+        add_bias<32>(v, cols + c0);
         if constexpr (PRE) {
-          uint32_t zk[16];
-#pragma unroll
-          for (int j = 0; j < 16; ++j)
-            zk[j] = pack2<T>(v[2 * j], v[2 * j + 1]);
-          store_block<T>(stage, zk, static_cast<T*>(p.pre), p.pre_ld, rb,
-                         col, p.N, g.vec_pre, lane);
-          if constexpr (RES)
+          store_values<T>(stage, v, static_cast<T*>(p.pre), p.pre_ld, rb,
+                          col, p.N, g.vec_pre, lane);
+          if constexpr (RES && !kF32)
             if (g.vec_res) fetch_residual<T>(stage, p, rb, col, lane);
         }
-        activate32<ACT>(v);
-        if constexpr (RES)
+        activate<ACT, 32>(v);
+        if constexpr (RES && kF32)
+          add_residual_f32(stage, v, g.vec_res, p, rb, col, lane);
+        else if constexpr (RES)
           add_residual<T>(stage, v, g.vec_res, p, rb, col, lane);
       }
       if constexpr (EPI == kEpiGated) {
-        float up[32];
-#pragma unroll
-        for (int j = 0; j < 32; ++j) up[j] = __uint_as_float(r1[j]);
-        add_bias(v, cols + c0);
-        add_bias(up, cols + 64 + c0);
+        add_bias<32>(v, cols + c0);
+        add_bias<32>(up, cols + 64 + c0);
         if constexpr (PRE) {
           store_block_f32(stage, v, p.gate, p.gate_ld, rb, col, p.N,
                           g.vec_f32, lane);
           store_block_f32(stage, up, p.up, p.up_ld, rb, col, p.N, g.vec_f32,
                           lane);
         }
-        activate32<ACT>(v);
+        activate<ACT, 32>(v);
 #pragma unroll
         for (int j = 0; j < 32; ++j) v[j] *= up[j];
       }
+      store_values<T>(stage, v, static_cast<T*>(p.out), p.out_ld, rb, col,
+                      p.N, g.vec_out, lane);
+    }
+  };
+  if constexpr (kF32) {
+    // The chunks of the reduction are added here, rounding to nearest (see
+    // chunk_end).
+    constexpr int kSums = kGated ? 2 * WARP_COLS : WARP_COLS;
+    float sum[kSums];
+    for (int chunk = 0; chunk < chunks; ++chunk) {
+      uint32_t acc = 0;
+      if (!wait(&acc)) return;
+#pragma unroll
+      for (int c = 0; c < kSums; c += 16) {
+        uint32_t r[16];
+        tmem_ld16u(acc + (c < WARP_COLS ? c : TILE_N + c - WARP_COLS), r);
+        tmem_wait_ld();
+        regs_tie16(r);
+#pragma unroll
+        for (int j = 0; j < 16; ++j)
+          sum[c + j] = chunk == 0 ? __uint_as_float(r[j])
+                                  : sum[c + j] + __uint_as_float(r[j]);
+      }
+      release();
+    }
+#pragma unroll
+    for (int c0 = 0; c0 < WARP_COLS; c0 += 32)
+      if (rb.rows > 0 && tile_col + c0 < p.N)
+        finish(sum + c0, sum + (kGated ? WARP_COLS + c0 : 0), c0);
+  } else if constexpr (EPI == kEpiGated) {
+    // Both factors of 16 columns at a time: 32 of each would not fit the 96
+    // registers beside the packed results.
+    uint32_t acc = 0;
+    if (!wait(&acc)) return;
+#pragma unroll 1
+    for (int c0 = 0; c0 < WARP_COLS; c0 += 32) {
+      const int64_t col = tile_col + c0;
+      const bool live = rb.rows > 0 && col < p.N;
       uint32_t pk[16];
 #pragma unroll
-      for (int j = 0; j < 16; ++j) pk[j] = pack2<T>(v[2 * j], v[2 * j + 1]);
-      store_block<T>(stage, pk, static_cast<T*>(p.out), p.out_ld, rb, col,
-                     p.N, g.vec_out, lane);
+      for (int h = 0; h < 32; h += 16) {
+        uint32_t r0[16], r1[16];
+        tmem_ld16u(acc + c0 + h, r0);
+        tmem_ld16u(acc + TILE_N + c0 + h, r1);
+        tmem_wait_ld();
+        regs_tie16(r0);
+        regs_tie16(r1);
+        if (c0 + h + 16 == WARP_COLS) release();
+        float v[16], up[16];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          v[j] = __uint_as_float(r0[j]);
+          up[j] = __uint_as_float(r1[j]);
+        }
+        add_bias<16>(v, cols + c0 + h);
+        add_bias<16>(up, cols + 64 + c0 + h);
+        if constexpr (PRE) {
+          if (live) {
+            store_half_f32(stage, v, p.gate, p.gate_ld, rb, col + h, p.N,
+                           g.vec_f32, lane);
+            store_half_f32(stage, up, p.up, p.up_ld, rb, col + h, p.N,
+                           g.vec_f32, lane);
+          }
+        }
+        activate<ACT, 16>(v);
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          pk[h / 2 + j] = pack2<T>(v[2 * j] * up[2 * j],
+                                   v[2 * j + 1] * up[2 * j + 1]);
+      }
+      if (live)
+        store_block<T>(stage, pk, static_cast<T*>(p.out), p.out_ld, rb, col,
+                       p.N, g.vec_out, lane);
+    }
+  } else {
+    uint32_t acc = 0;
+    if (!wait(&acc)) return;
+#pragma unroll 1
+    for (int c0 = 0; c0 < WARP_COLS; c0 += 32) {
+      if constexpr (kEarly)
+        if (g.vec_res && c0 > 0)
+          fetch_residual<T>(stage, p, rb, tile_col + c0, lane);
+      uint32_t r0[32];
+      uint32_t r1[kGated ? 32 : 1];
+      tmem_ld32u(acc + c0, r0);
+      if constexpr (kGated) tmem_ld32u(acc + TILE_N + c0, r1);
+      tmem_wait_ld_tied(r0);
+      if constexpr (kGated) regs_tie32(r1);
+      if (c0 + 32 == WARP_COLS) release();
+      if (rb.rows <= 0 || tile_col + c0 >= p.N) continue;
+      float v[32], up[32];
+#pragma unroll
+      for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r0[j]);
+      if constexpr (kGated) {
+#pragma unroll
+        for (int j = 0; j < 32; ++j) up[j] = __uint_as_float(r1[j]);
+      }
+      finish(v, up, c0);
     }
   }
 }
@@ -564,8 +718,10 @@ __global__ void __launch_bounds__(Cfg<BN, CG>::THREADS, 1)
                    const __grid_constant__ TcArgs g) {
   using C = Cfg<BN, CG>;
   constexpr bool kGated = EPI == kEpiGated || EPI == kEpiGatedPartial;
+  constexpr bool kF32 = std::is_same<T, float>::value;
   constexpr int kTileN = kGated ? BN / 2 : BN;  // output columns of a tile
-  constexpr int FMT = std::is_same<T, __nv_bfloat16>::value ? 1 : 0;
+  // Operand format: bf16 (also float32's planes) or f16.
+  constexpr int FMT = std::is_same<T, __half>::value ? 0 : 1;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -622,6 +778,9 @@ __global__ void __launch_bounds__(Cfg<BN, CG>::THREADS, 1)
         const int k_last = k_first + g.steps_part < g.steps
                                ? k_first + g.steps_part
                                : g.steps;
+        int seg_at = k_first / g.steps_seg;
+        int in_seg = k_first - seg_at * g.steps_seg;
+        TcSegment seg = g.seg[seg_at];
         for (int k = k_first; k < k_last; ++k) {
           ok = mbar_wait(bar_empty(s), phase ^ 1, p.err);
           if (!ok) break;
@@ -629,17 +788,21 @@ __global__ void __launch_bounds__(Cfg<BN, CG>::THREADS, 1)
           if (CG == 1 || rank == 0)
             mbar_arrive_expect_tx(full, C::STAGE * CG);
           if constexpr (CG == 2) full = map_cta(full, 0);
-          const int seg = k >= g.steps_seg ? 1 : 0;
-          const int k0 = (k - seg * g.steps_seg) * kTcStep;
+          if (in_seg == g.steps_seg) {
+            in_seg = 0;
+            seg = g.seg[++seg_at];
+          }
+          const int k0 = in_seg++ * kTcStep;
           const uint32_t sa = sbase + uint32_t(s) * C::STAGE;
           const uint32_t sb = sa + C::A_BYTES;
-          const CUtensorMap* ma = seg ? &ta1 : &ta0;
+          const CUtensorMap* ma = seg.map ? &ta1 : &ta0;
           if (g.a_mn) {
 #pragma unroll
             for (int i = 0; i < kTcRows / 64; ++i)
-              tma_load_2d<CG>(sa + i * 8192, ma, full, m0 + i * 64, k0);
+              tma_load_2d<CG>(sa + i * 8192, ma, full, m0 + i * 64,
+                              k0 + seg.a_line);
           } else {
-            tma_load_2d<CG>(sa, ma, full, k0, m0);
+            tma_load_2d<CG>(sa, ma, full, k0, m0 + seg.a_line);
           }
           // Rows of B: in a pair, half each. A gated tile's first half is
           // the gate weight's rows, its second half the up weight's.
@@ -647,17 +810,17 @@ __global__ void __launch_bounds__(Cfg<BN, CG>::THREADS, 1)
 #pragma unroll
           for (int h = 0; h < C::B_ROWS / kBoxRows; ++h) {
             const CUtensorMap* mb =
-                kGated ? ((CG == 2 ? int(rank) : h) ? &tb1 : &tb0)
-                       : (seg ? &tb1 : &tb0);
+                (kGated ? (CG == 2 ? int(rank) : h) : seg.map) ? &tb1 : &tb0;
             const int row =
                 kGated ? n0 : n0 + int(rank) * C::B_ROWS;
             const uint32_t dst = sb + h * kBoxRows * 128;
             if (g.b_mn) {
 #pragma unroll
               for (int i = 0; i < kBoxRows / 64; ++i)
-                tma_load_2d<CG>(dst + i * 8192, mb, full, row + i * 64, k0);
+                tma_load_2d<CG>(dst + i * 8192, mb, full, row + i * 64,
+                                k0 + seg.b_line);
             } else {
-              tma_load_2d<CG>(dst, mb, full, k0, row);
+              tma_load_2d<CG>(dst, mb, full, k0, row + seg.b_line);
             }
           }
           ++issued;
@@ -701,11 +864,13 @@ __global__ void __launch_bounds__(Cfg<BN, CG>::THREADS, 1)
         const int k_last = k_first + g.steps_part < g.steps
                                ? k_first + g.steps_part
                                : g.steps;
+        for (int from = k_first; from < k_last && ok;) {
+        const int to = kF32 ? chunk_end(g, from, k_last) : k_last;
         ok = mbar_wait(bar_acc_empty(buf), buf_phase ^ 1, p.err);
         if (!ok) break;
         tc_fence_after();
         const uint32_t d = tmem + uint32_t(buf * BN);
-        for (int k = k_first; k < k_last; ++k) {
+        for (int k = from; k < to; ++k) {
           ok = mbar_wait(bar_full(s), phase, p.err);
           if (!ok) break;
           tc_fence_after();
@@ -714,7 +879,7 @@ __global__ void __launch_bounds__(Cfg<BN, CG>::THREADS, 1)
 #pragma unroll
           for (int i = 0; i < kTcStep / 16; ++i)
             mma_f16<CG>(d, da + i * ka, db + i * kb, idesc,
-                        k > k_first || i > 0);
+                        k > from || i > 0);
           commit_all<CG>(bar_empty(s));
           if (++s == C::STAGES) {
             s = 0;
@@ -725,6 +890,8 @@ __global__ void __launch_bounds__(Cfg<BN, CG>::THREADS, 1)
         commit_all<CG>(bar_acc_full(buf));
         buf ^= 1;
         if (buf == 0) buf_phase ^= 1;
+        from = to;
+        }
       }
     }
   } else if (warp >= kCtrlWarps) {
@@ -735,62 +902,72 @@ __global__ void __launch_bounds__(Cfg<BN, CG>::THREADS, 1)
     uint8_t* stage = smem + C::OFF_EPI + w * kEpiWarpBytes;
     float* cols = reinterpret_cast<float*>(stage + 32 * kStagePitch);
     const uint32_t lanes = tmem + (uint32_t(quarter * 32) << 16);
-    int buf = 0;
-    uint32_t buf_phase = 0;
-    for (int64_t u = first; u < g.units && ok; u += stride) {
-      const Unit t = unit_of(g, u);
-      RowBlock rb;
-      rb.row0 = int64_t(t.m * CG + int(rank)) * kTcRows + quarter * 32;
-      const int64_t left = p.M - rb.row0;
-      rb.rows = int(left < 0 ? 0 : (left < 32 ? left : 32));
-      const int64_t tile_col = int64_t(t.n) * kTileN + share * kWarpCols;
-      const uint32_t acc = lanes + uint32_t(buf * BN + share * kWarpCols);
-      auto wait = [&] {
-        ok = mbar_wait(bar_acc_full(buf), buf_phase, p.err);
-        ok = __all_sync(0xffffffffu, ok);
-        if (ok) tc_fence_after();
-        return ok;
-      };
-      auto release = [&] {
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) {
-          if constexpr (CG == 1)
-            mbar_arrive(bar_acc_empty(buf));
-          else
-            mbar_arrive_cluster(map_cta(bar_acc_empty(buf), 0));
+    // One copy of the whole loop per activation: with the choice inside it,
+    // the copies' registers met again after every tile and spilled.
+    auto role = [&](auto act) {
+      int buf = 0;
+      uint32_t buf_phase = 0;
+      for (int64_t u = first; u < g.units && ok; u += stride) {
+        const Unit t = unit_of(g, u);
+        RowBlock rb;
+        rb.row0 = int64_t(t.m * CG + int(rank)) * kTcRows + quarter * 32;
+        const int64_t left = p.M - rb.row0;
+        rb.rows = int(left < 0 ? 0 : (left < 32 ? left : 32));
+        const int64_t tile_col = int64_t(t.n) * kTileN + share * kWarpCols;
+        int chunks = 1;
+        if constexpr (kF32) {
+          const int k_first = t.part * g.steps_part;
+          const int k_last = k_first + g.steps_part < g.steps
+                                 ? k_first + g.steps_part
+                                 : g.steps;
+          chunks = 0;
+          for (int k = k_first; k < k_last; k = chunk_end(g, k, k_last))
+            ++chunks;
         }
-      };
-      auto tile = [&](auto act) {
+        auto wait = [&](uint32_t* acc) {
+          ok = mbar_wait(bar_acc_full(buf), buf_phase, p.err);
+          ok = __all_sync(0xffffffffu, ok);
+          if (ok) tc_fence_after();
+          *acc = lanes + uint32_t(buf * BN + share * kWarpCols);
+          return ok;
+        };
+        auto release = [&] {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) {
+            if constexpr (CG == 1)
+              mbar_arrive(bar_acc_empty(buf));
+            else
+              mbar_arrive_cluster(map_cta(bar_acc_empty(buf), 0));
+          }
+          buf ^= 1;
+          if (buf == 0) buf_phase ^= 1;
+        };
         epilogue_tile<EPI, decltype(act)::value, RES, PRE, T, kTileN,
-                      kWarpCols>(g, stage, cols, acc, rb, tile_col, t.part,
-                                 lane, wait, release);
-      };
-      // One copy of the loop per activation, so that a tile runs through
-      // straight code.
-      if constexpr (EPI != kEpiLinear && EPI != kEpiGated) {
-        tile(std::integral_constant<int, VECTRA_ACT_NONE>{});
-      } else {
-        switch (p.act) {
-          case VECTRA_ACT_RELU:
-            tile(std::integral_constant<int, VECTRA_ACT_RELU>{});
-            break;
-          case VECTRA_ACT_GELU:
-            tile(std::integral_constant<int, VECTRA_ACT_GELU>{});
-            break;
-          case VECTRA_ACT_GELU_TANH:
-            tile(std::integral_constant<int, VECTRA_ACT_GELU_TANH>{});
-            break;
-          case VECTRA_ACT_SILU:
-            tile(std::integral_constant<int, VECTRA_ACT_SILU>{});
-            break;
-          default:
-            tile(std::integral_constant<int, VECTRA_ACT_NONE>{});
-            break;
-        }
+                      kWarpCols>(g, stage, cols, chunks, rb, tile_col,
+                                 t.part, lane, wait, release);
       }
-      buf ^= 1;
-      if (buf == 0) buf_phase ^= 1;
+    };
+    if constexpr (EPI != kEpiLinear && EPI != kEpiGated) {
+      role(std::integral_constant<int, VECTRA_ACT_NONE>{});
+    } else {
+      switch (p.act) {
+        case VECTRA_ACT_RELU:
+          role(std::integral_constant<int, VECTRA_ACT_RELU>{});
+          break;
+        case VECTRA_ACT_GELU:
+          role(std::integral_constant<int, VECTRA_ACT_GELU>{});
+          break;
+        case VECTRA_ACT_GELU_TANH:
+          role(std::integral_constant<int, VECTRA_ACT_GELU_TANH>{});
+          break;
+        case VECTRA_ACT_SILU:
+          role(std::integral_constant<int, VECTRA_ACT_SILU>{});
+          break;
+        default:
+          role(std::integral_constant<int, VECTRA_ACT_NONE>{});
+          break;
+      }
     }
   }
 
@@ -842,7 +1019,11 @@ cudaError_t launch_cfg(const CUtensorMap* maps, const TcArgs& g,
 template <int EPI, bool RES, bool PRE, typename T>
 cudaError_t launch_shape(int bn, int cg, const CUtensorMap* maps,
                          const TcArgs& g, cudaStream_t stream) {
-  if (cg == 2) return launch_cfg<EPI, RES, PRE, T, 256, 2>(maps, g, stream);
+  // float32 keeps its sums in registers across chunks: the pair's tile, with
+  // 96 registers a thread, has no room for them.
+  if constexpr (!std::is_same<T, float>::value)
+    if (cg == 2)
+      return launch_cfg<EPI, RES, PRE, T, 256, 2>(maps, g, stream);
   if constexpr (EPI != kEpiGated && EPI != kEpiGatedPartial)
     if (bn == 64) return launch_cfg<EPI, RES, PRE, T, 64, 1>(maps, g, stream);
   return launch_cfg<EPI, RES, PRE, T, 128, 1>(maps, g, stream);

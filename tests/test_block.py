@@ -787,6 +787,26 @@ def test_other_streams():
 
 
 @pytest.mark.gpu
+def test_from_a_fresh_thread():
+    """A thread without a current CUDA context: tensor maps still encode
+    (products here, and the long-sequence attention)."""
+    import threading
+    rand = Rand(73, 'cuda', torch.bfloat16)
+    x, w = rand(64, 512), rand(256, 512)
+    q = rand(1, 2, 256, 64)
+    scale = torch.full((1, 2, 1, 1), 0.05, device='cuda')
+    calls = [lambda: block.linear(x, w),
+             lambda: vectra_b200.rbf_attention(q, q, q, scale)]
+    for call in calls:
+        want, got = call(), []
+        torch.cuda.synchronize()
+        thread = threading.Thread(target=lambda c=call: got.append(c()))
+        thread.start()
+        thread.join()
+        assert len(got) == 1 and torch.equal(got[0], want)
+
+
+@pytest.mark.gpu
 def test_results_past_32_bit_offsets():
     """More than 2^31 result elements."""
     rand = Rand(67, 'cuda', torch.bfloat16)

@@ -184,10 +184,9 @@ def _gated_with_pre_fake(x, w_gate, w_up, b_gate, b_up, activation,
 def _gated_backward_fake(dh, x, w_gate, w_up, gate, up, activation, need_dx,
                          need_dw, need_db):
     del dh, w_up, gate, up, activation
-    weight = w_gate.shape if need_dw else (0,)
-    bias = (w_gate.shape[0] if need_db else 0,)
-    return (x.new_empty(x.shape if need_dx else (0,)), x.new_empty(weight),
-            x.new_empty(weight), x.new_empty(bias), x.new_empty(bias))
+    return (x.new_empty(x.shape if need_dx else (0,)),
+            x.new_empty((2, *w_gate.shape) if need_dw else (0,)),
+            x.new_empty((2, w_gate.shape[0]) if need_db else (0,)))
 
 
 @torch.library.register_fake('vectra_b200::qk_norm_rope')

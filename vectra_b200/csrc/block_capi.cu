@@ -287,8 +287,15 @@ int gated_backward(const vectra_gated_grad_args& a, Workspace& ws,
   }
   if (present(a.dw_gate) && F > 0 && K > 0) {
     const vectra_tensor* out[2] = {&a.dw_gate, &a.dw_up};
-    for (int i = 0; i < 2; ++i) {
-      p.M = F;
+    // Results that lie one behind the other, like dg and du, are one product
+    // of twice the rows: x is read once for both.
+    const bool joined =
+        F % 8 == 0 && a.dw_gate.stride[0] == a.dw_up.stride[0] &&
+        static_cast<const char*>(a.dw_gate.data) +
+                size_t(F) * a.dw_gate.stride[0] * es ==
+            static_cast<const char*>(a.dw_up.data);
+    for (int i = 0; i < (joined ? 1 : 2); ++i) {
+      p.M = joined ? 2 * F : F;
       p.N = K;
       p.K = M;
       p.a[0] = {i ? d2 : d, 1, ld};

@@ -440,8 +440,7 @@ Grads3 gated_cpu(const Tensor& x, const Tensor& wg, const Tensor& wu,
   return {h, g, u};
 }
 
-using Grads5 = std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor>;
-
+// Gradients of x, of both weights [2, F, K] and of both biases [2, F].
 void check_gated_grad(const Tensor& dh, const Tensor& x, const Tensor& wg,
                       const Tensor& wu, const Tensor& gate,
                       const Tensor& up) {
@@ -457,7 +456,7 @@ void check_gated_grad(const Tensor& dh, const Tensor& x, const Tensor& wg,
   }
 }
 
-Grads5 gated_backward_cuda(const Tensor& dh, const Tensor& x,
+Grads3 gated_backward_cuda(const Tensor& dh, const Tensor& x,
                            const Tensor& wg, const Tensor& wu,
                            const Tensor& gate, const Tensor& up,
                            const std::string& activation, bool need_dx,
@@ -468,14 +467,11 @@ Grads5 gated_backward_cuda(const Tensor& dh, const Tensor& x,
   const Tensor g = gate.contiguous(), u = up.contiguous();
   Tensor dx = at::empty(need_dx ? x.sizes().vec() : std::vector<int64_t>{0},
                         x.options());
-  const auto weight = [&] {
-    return need_dw ? at::empty(wg.sizes(), x.options())
-                   : at::empty({0}, x.options());
-  };
-  const auto bias = [&] {
-    return at::empty({need_db ? wg.size(0) : 0}, x.options());
-  };
-  Tensor dwg = weight(), dwu = weight(), dbg = bias(), dbu = bias();
+  const int64_t f = wg.size(0);
+  Tensor dw = need_dw ? at::empty({2, f, wg.size(1)}, x.options())
+                      : at::empty({0}, x.options());
+  Tensor db = need_db ? at::empty({2, f}, x.options())
+                      : at::empty({0}, x.options());
   vectra_gated_grad_args a{};
   a.activation = activation_of(activation);
   a.dh = describe_rows(dh, &dh_copy);
@@ -486,20 +482,20 @@ Grads5 gated_backward_cuda(const Tensor& dh, const Tensor& x,
   a.up = describe_rows(u, nullptr);
   if (need_dx) a.dx = describe_rows(dx, nullptr);
   if (need_dw) {
-    a.dw_gate = describe(dwg);
-    a.dw_up = describe(dwu);
+    a.dw_gate = describe(dw.select(0, 0));
+    a.dw_up = describe(dw.select(0, 1));
   }
   if (need_db) {
-    a.db_gate = describe(dbg);
-    a.db_up = describe(dbu);
+    a.db_gate = describe(db.select(0, 0));
+    a.db_up = describe(db.select(0, 1));
   }
   call_with_workspace("gated_linear_backward", a, x,
                       vectra_gated_linear_backward_workspace_bytes,
                       vectra_gated_linear_backward);
-  return {dx, dwg, dwu, dbg, dbu};
+  return {dx, dw, db};
 }
 
-Grads5 gated_backward_cpu(const Tensor& dh, const Tensor& x,
+Grads3 gated_backward_cpu(const Tensor& dh, const Tensor& x,
                           const Tensor& wg, const Tensor& wu,
                           const Tensor& gate, const Tensor& up,
                           const std::string& activation, bool need_dx,
@@ -515,11 +511,11 @@ Grads5 gated_backward_cpu(const Tensor& dh, const Tensor& x,
                             .reshape(x.sizes())
                       : none();
   const Tensor x2 = f32(as_rows(x));
-  Tensor dwg = need_dw ? at::matmul(dg.t(), x2).to(dt) : none();
-  Tensor dwu = need_dw ? at::matmul(du.t(), x2).to(dt) : none();
-  Tensor dbg = need_db ? dg.sum(0).to(dt) : none();
-  Tensor dbu = need_db ? du.sum(0).to(dt) : none();
-  return {dx, dwg, dwu, dbg, dbu};
+  Tensor dw = need_dw ? at::stack({at::matmul(dg.t(), x2),
+                                   at::matmul(du.t(), x2)}).to(dt)
+                      : none();
+  Tensor db = need_db ? at::stack({dg.sum(0), du.sum(0)}).to(dt) : none();
+  return {dx, dw, db};
 }
 
 // ---------------------------------------------------------------------------
@@ -797,7 +793,7 @@ Grads3 call_gated(const Tensor& x, const Tensor& wg, const Tensor& wu,
   return op.call(x, wg, wu, bg, bu, activation, want_pre);
 }
 
-Grads5 call_gated_backward(const Tensor& dh, const Tensor& x,
+Grads3 call_gated_backward(const Tensor& dh, const Tensor& x,
                            const Tensor& wg, const Tensor& wu,
                            const Tensor& gate, const Tensor& up,
                            const std::string& activation, bool need_dx,
@@ -805,7 +801,7 @@ Grads5 call_gated_backward(const Tensor& dh, const Tensor& x,
   static const auto op =
       c10::Dispatcher::singleton()
           .findSchemaOrThrow("vectra_b200::gated_linear_backward", "")
-          .typed<Grads5(const Tensor&, const Tensor&, const Tensor&,
+          .typed<Grads3(const Tensor&, const Tensor&, const Tensor&,
                         const Tensor&, const Tensor&, const Tensor&,
                         c10::string_view, bool, bool, bool)>();
   return op.call(dh, x, wg, wu, gate, up, activation, need_dx, need_dw,
@@ -890,6 +886,15 @@ OptTensor optional(const Tensor& t) {
   return t.defined() ? OptTensor(t) : OptTensor();
 }
 
+// Backward calls go straight to the kernels unless their results are to be
+// differentiated again, which the operators' own autograd entry refuses.
+struct BelowUnlessRecording {
+  std::optional<at::AutoDispatchBelowADInplaceOrView> below;
+  BelowUnlessRecording() {
+    if (!at::GradMode::is_enabled()) below.emplace();
+  }
+};
+
 struct LinearFunction : public Function<LinearFunction> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x,
                         const Tensor& w, const OptTensor& bias,
@@ -917,6 +922,7 @@ struct LinearFunction : public Function<LinearFunction> {
     variable_list out(5);
     if (!grads[0].defined()) return out;
     if (dx || dw || db) {
+      BelowUnlessRecording below;
       auto [gx, gw, gb] = call_linear_backward(
           grads[0], saved[0], saved[1], saved[2],
           ctx->saved_data["activation"].toStringRef(), dx, dw, db);
@@ -950,13 +956,16 @@ struct GatedFunction : public Function<GatedFunction> {
     const int64_t mask = ctx->saved_data["mask"].toInt();
     variable_list out(6);
     if (!grads[0].defined()) return out;
-    auto [dx, dwg, dwu, dbg, dbu] = call_gated_backward(
+    BelowUnlessRecording below;
+    auto [dx, dw, db] = call_gated_backward(
         grads[0], s[0], s[1], s[2], s[3], s[4],
         ctx->saved_data["activation"].toStringRef(), (mask & 1) != 0,
         (mask & 6) != 0, (mask & 24) != 0);
-    const Tensor got[5] = {dx, dwg, dwu, dbg, dbu};
-    for (int i = 0; i < 5; ++i)
-      if (mask >> i & 1) out[i] = got[i];
+    if (mask & 1) out[0] = dx;
+    for (int i = 0; i < 2; ++i) {
+      if (mask >> (1 + i) & 1) out[1 + i] = dw.select(0, i);
+      if (mask >> (3 + i) & 1) out[3 + i] = db.select(0, i);
+    }
     return out;
   }
 };
@@ -988,6 +997,7 @@ struct QkFunction : public Function<QkFunction> {
     const bool dkw = ctx->saved_data["dkw"].toBool();
     variable_list out(9);
     if (!grads[0].defined() && !grads[1].defined()) return out;
+    BelowUnlessRecording below;
     // A result that nothing used has no gradient: its share is zero.
     const Tensor gq =
         grads[0].defined() ? grads[0] : at::zeros_like(s[0]);
@@ -1066,7 +1076,7 @@ Grads3 gated_impl(const Tensor& x, const Tensor& wg, const Tensor& wu,
   return F(x, wg, wu, bg, bu, std::string(activation), want_pre);
 }
 template <auto F>
-Grads5 gated_backward_impl(const Tensor& dh, const Tensor& x,
+Grads3 gated_backward_impl(const Tensor& dh, const Tensor& x,
                            const Tensor& wg, const Tensor& wu,
                            const Tensor& gate, const Tensor& up,
                            c10::string_view activation, bool need_dx,
@@ -1099,8 +1109,7 @@ TORCH_LIBRARY_FRAGMENT(vectra_b200, m) {
   m.def(
       "gated_linear_backward(Tensor dh, Tensor x, Tensor w_gate, "
       "Tensor w_up, Tensor gate, Tensor up, str activation, bool need_dx, "
-      "bool need_dw, bool need_db) "
-      "-> (Tensor, Tensor, Tensor, Tensor, Tensor)");
+      "bool need_dw, bool need_db) -> (Tensor, Tensor, Tensor)");
   m.def(
       "qk_norm_rope(Tensor q, Tensor k, Tensor cos, Tensor sin, "
       "Tensor? q_weight=None, Tensor? k_weight=None, "

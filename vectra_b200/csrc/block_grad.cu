@@ -16,6 +16,7 @@ namespace vectra {
 namespace {
 
 constexpr int kWarps = 8;
+constexpr int kBlocksPerSm = 8;
 
 struct GradArgs {
   GradProblem p;
@@ -24,27 +25,25 @@ struct GradArgs {
   float* partial2;
 };
 
+// VEC elements as loaded, converted when used.
 template <typename T, int VEC>
-__device__ __forceinline__ void load_vec(const T* p, int64_t stride,
-                                         float* v) {
-  if constexpr (VEC == 1) {
-    v[0] = to_f32(*p);
-  } else {
-    (void)stride;
-    constexpr int kWords = VEC * int(sizeof(T)) / 16;
+struct Raw {
+  union {
+    uint4 u[VEC * sizeof(T) / 16 > 0 ? VEC * sizeof(T) / 16 : 1];
+    T e[VEC];
+  };
+  __device__ __forceinline__ Raw() {}
+  __device__ __forceinline__ void load(const T* p) {
+    if constexpr (VEC == 1) {
+      e[0] = *p;
+    } else {
 #pragma unroll
-    for (int w = 0; w < kWords; ++w) {
-      union {
-        uint4 u;
-        T e[16 / sizeof(T)];
-      } raw;
-      raw.u = *(reinterpret_cast<const uint4*>(p) + w);
-#pragma unroll
-      for (int i = 0; i < int(16 / sizeof(T)); ++i)
-        v[w * int(16 / sizeof(T)) + i] = to_f32(raw.e[i]);
+      for (int w = 0; w < int(VEC * sizeof(T) / 16); ++w)
+        u[w] = __ldg(reinterpret_cast<const uint4*>(p) + w);
     }
   }
-}
+  __device__ __forceinline__ float at(int i) const { return to_f32(e[i]); }
+};
 
 template <typename T, int VEC>
 __device__ __forceinline__ void store_vec(T* p, const float* v) {
@@ -71,6 +70,7 @@ __global__ void __launch_bounds__(kWarps * 32)
     grad_kernel(const GradArgs a) {
   constexpr bool kExact = std::is_same<T, float>::value;
   constexpr int kSides = GATED ? 2 : 1;
+  constexpr int kBatch = GATED ? 2 : 4;
   __shared__ float sums[kSides][kWarps][32 * VEC];
   const GradProblem& p = a.p;
   allow_dependents();
@@ -84,44 +84,47 @@ __global__ void __launch_bounds__(kWarps * 32)
 #pragma unroll
   for (int i = 0; i < VEC; ++i) sg[i] = su[i] = 0.f;
   if (n < p.N) {
-#pragma unroll 2
-    for (int64_t m = r0 + warp; m < r1; m += kWarps) {
-      float dy[VEC], d1[VEC], d2[VEC];
-      load_vec<T, VEC>(
-          static_cast<const T*>(p.dy) + m * p.dy_sm + n * p.dy_sn, 0, dy);
-      if constexpr (GATED) {
-        float g[VEC], u[VEC];
-        load_vec<float, VEC>(p.gate + m * p.gate_ld + n, 0, g);
-        load_vec<float, VEC>(p.up + m * p.up_ld + n, 0, u);
+    // kBatch rows' loads are issued before any of them is used.
+    for (int64_t m0 = r0 + warp; m0 < r1; m0 += kWarps * kBatch) {
+      Raw<T, VEC> dy[kBatch], z[GATED ? 1 : kBatch];
+      Raw<float, VEC> g[GATED ? kBatch : 1], u[GATED ? kBatch : 1];
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) {
+      for (int i = 0; i < kBatch; ++i) {
+        const int64_t m = m0 + i * kWarps;
+        if (m >= r1) break;
+        dy[i].load(static_cast<const T*>(p.dy) + m * p.dy_sm + n * p.dy_sn);
+        if constexpr (GATED) {
+          g[i].load(p.gate + m * p.gate_ld + n);
+          u[i].load(p.up + m * p.up_ld + n);
+        } else if constexpr (ACT != VECTRA_ACT_NONE) {
+          z[i].load(static_cast<const T*>(p.pre) + m * p.pre_ld + n);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) {
+        const int64_t m = m0 + i * kWarps;
+        if (m >= r1) break;
+        float d1[VEC], d2[VEC];
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+          const float d = dy[i].at(j);
           float value;
-          const float slope = act_grad<kExact, ACT>(g[i], &value);
-          d1[i] = dy[i] * u[i] * slope;
-          d2[i] = dy[i] * value;
-          sg[i] += d1[i];
-          su[i] += d2[i];
-        }
-        store_vec<T, VEC>(static_cast<T*>(p.dz) + m * p.dz_ld + n, d1);
-        store_vec<T, VEC>(static_cast<T*>(p.dz2) + m * p.dz_ld + n, d2);
-      } else {
-        if constexpr (ACT != VECTRA_ACT_NONE) {
-          float z[VEC];
-          load_vec<T, VEC>(static_cast<const T*>(p.pre) + m * p.pre_ld + n,
-                           0, z);
-#pragma unroll
-          for (int i = 0; i < VEC; ++i) {
-            float value;
-            d1[i] = dy[i] * act_grad<kExact, ACT>(z[i], &value);
+          if constexpr (GATED) {
+            const float slope = act_grad<kExact, ACT>(g[i].at(j), &value);
+            d1[j] = d * u[i].at(j) * slope;
+            d2[j] = d * value;
+            su[j] += d2[j];
+          } else if constexpr (ACT != VECTRA_ACT_NONE) {
+            d1[j] = d * act_grad<kExact, ACT>(z[i].at(j), &value);
+          } else {
+            d1[j] = d;
           }
-        } else {
-#pragma unroll
-          for (int i = 0; i < VEC; ++i) d1[i] = dy[i];
+          sg[j] += d1[j];
         }
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) sg[i] += d1[i];
-        if (p.dz)
+        if (GATED || p.dz)
           store_vec<T, VEC>(static_cast<T*>(p.dz) + m * p.dz_ld + n, d1);
+        if constexpr (GATED)
+          store_vec<T, VEC>(static_cast<T*>(p.dz2) + m * p.dz_ld + n, d2);
       }
     }
   }
@@ -201,10 +204,10 @@ cudaError_t run_grad(const GradProblem& p, Workspace& ws,
                    (!p.pre || aligned(p.pre, p.pre_ld, es)) &&
                    (!p.gate || (aligned(p.gate, p.gate_ld, 4) &&
                                 aligned(p.up, p.up_ld, 4)));
-  // Chunks: enough blocks for about four per SM, at least 16 rows each, and
+  // Chunks: enough blocks for kBlocksPerSm, at least 16 rows each, and
   // few enough that the chunk sums stay small beside the data.
   const int64_t cols = (p.N + (vec ? 255 : 31)) / (vec ? 256 : 32);
-  int64_t chunks = (int64_t(device_sm_count()) * 4 + cols - 1) / cols;
+  int64_t chunks = (int64_t(device_sm_count()) * kBlocksPerSm + cols - 1) / cols;
   const int64_t most = (p.M + 15) / 16;
   if (chunks > most) chunks = most;
   if (chunks > 4096) chunks = 4096;

@@ -7,29 +7,56 @@
 namespace vectra {
 namespace {
 
-// Tile shape and parts of a tensor-core product.
+// Tile shape and parts of a tensor-core product: the least estimated time
+// over the shapes, each with one part or as many as fill the SMs.
+//
+// A stage of 64 of the reduction takes a CTA about kStep microseconds: for
+// the pair's 256 x 256 tile the tensor cores bound it, for the narrow tiles
+// the 24 or 32 KB that it brings in. A tile's start and epilogue that nothing
+// overlaps take kTile. Parts write and re-read float32 sums and need a
+// second launch.
 TcShape tc_shape(const GemmProblem& p) {
-  const bool gated = p.epilogue == kEpiGated;
-  const int64_t sms = device_sm_count();
-  const int64_t n = gated ? 2 * p.N : p.N;
-  auto tiles = [&](int64_t rows, int64_t cols) {
-    return ((p.M + rows - 1) / rows) * ((n + cols - 1) / cols);
+  struct Option {
+    int bn, cg;
+    double step;
   };
-  TcShape s;
-  if (p.dtype != VECTRA_F32 && p.M > 128 && tiles(256, 256) >= sms / 2) {
-    s.bn = 256;
-    s.cg = 2;
-    return s;
-  }
-  s.bn = gated || tiles(128, 128) >= sms / 2 || p.K >= 4096 ? 128 : 64;
-  const int64_t t = tiles(128, s.bn);
+  constexpr Option kOptions[] = {
+      {256, 2, 0.28}, {128, 1, 0.25}, {64, 1, 0.19}};
+  constexpr double kTile = 2.0, kSecondLaunch = 2.5, kBytesPerUs = 5.0e6;
+  const bool gated = p.epilogue == kEpiGated;
+  const double sms = device_sm_count();
   const int64_t steps =
       (p.K + 63) / 64 * p.segments * (p.dtype == VECTRA_F32 ? 6 : 1);
-  int64_t split = sms / t;
-  if (split > steps / 8) split = steps / 8;
-  if (split > 32) split = 32;
-  s.split = int(split < 1 ? 1 : split);
-  return s;
+  TcShape best;
+  double least = 1e30;
+  for (const Option& o : kOptions) {
+    if (o.cg == 2 && (p.dtype == VECTRA_F32 || p.M <= 128)) continue;
+    if (gated && o.bn < 128) continue;
+    const int64_t cols = gated ? o.bn / 2 : o.bn;
+    const int64_t rows = int64_t(kTcRows) * o.cg;
+    const int64_t tiles =
+        ((p.M + rows - 1) / rows) * ((p.N + cols - 1) / cols);
+    const int64_t slots = int64_t(sms) / o.cg;
+    int64_t most = slots / tiles;
+    if (most > steps / 4) most = steps / 4;
+    if (most > 64) most = 64;
+    for (const int64_t split : {int64_t(1), most}) {
+      if (split < 1) continue;
+      const int64_t per = (steps + split - 1) / split;
+      const int64_t waves = (tiles * split + slots - 1) / slots;
+      double t = double(waves) * double(per) * o.step + kTile;
+      if (split > 1)
+        t += kSecondLaunch + 8.0 * double(split) * double(p.M) *
+                                 double(p.N) * (gated ? 2 : 1) / kBytesPerUs;
+      if (t < least) {
+        least = t;
+        best.bn = o.bn;
+        best.cg = o.cg;
+        best.split = int(split);
+      }
+    }
+  }
+  return best;
 }
 
 }  // namespace

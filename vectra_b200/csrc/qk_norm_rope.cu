@@ -190,6 +190,7 @@ struct QkVecArgs {
   int groups_per_token[2];  // of the queries, of the keys
   int64_t groups[2];
   int blocks[2];            // backward: blocks of each side
+  bool w_vec[2];            // weights in 16-byte pieces
 };
 
 // The two chunks of lane j's slot; -1: none.
@@ -274,16 +275,30 @@ __device__ __forceinline__ void turn(float* x, const Angles<T>& a,
   }
 }
 
+// One chunk's weights; `w_vec`: they can be read 16 bytes at a time.
 template <typename T>
-__device__ __forceinline__ void load_weight(const QkSide& s, int chunk,
-                                            float* w) {
+__device__ __forceinline__ void load_weight(const QkSide& s, bool w_vec,
+                                            int chunk, float* w) {
   constexpr int VE = kVec<T>;
 #pragma unroll
   for (int i = 0; i < VE; ++i) w[i] = 1.f;
   if (s.w == nullptr || chunk < 0) return;
+  if (w_vec && s.w_dtype == VECTRA_F32) {
 #pragma unroll
-  for (int i = 0; i < VE; ++i)
-    w[i] = load_any(s.w, s.w_dtype, int64_t(chunk * VE + i) * s.sw);
+    for (int i = 0; i < VE; i += 4)
+      *reinterpret_cast<float4*>(w + i) = __ldg(reinterpret_cast<const float4*>(
+          static_cast<const float*>(s.w) + chunk * VE + i));
+  } else if (w_vec) {
+    Chunk<T> c;
+    c.u = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(s.w) +
+                                               chunk * VE));
+#pragma unroll
+    for (int i = 0; i < VE; ++i) w[i] = to_f32(c.e[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < VE; ++i)
+      w[i] = load_any(s.w, s.w_dtype, int64_t(chunk * VE + i) * s.sw);
+  }
 }
 
 template <int G>
@@ -361,8 +376,8 @@ __global__ void __launch_bounds__(kWarps * 32)
     }
     if (first) {
       load_angles<T, INTER>(p, pos, known, c0, c1, &ang);
-      load_weight<T>(s, c0, w);
-      load_weight<T>(s, c1, w + VE);
+      load_weight<T>(s, a.w_vec[side], c0, w);
+      load_weight<T>(s, a.w_vec[side], c1, w + VE);
       first = false;
     }
 #pragma unroll
@@ -405,8 +420,8 @@ __global__ void __launch_bounds__(kWarps * 32)
   int c0, c1;
   slot_chunks(j, slots, chunks, p.R2 / VE, INTER, &c0, &c1);
   float w[2 * VE], dw[2 * VE];
-  load_weight<T>(s, c0, w);
-  load_weight<T>(s, c1, w + VE);
+  load_weight<T>(s, a.w_vec[side], c0, w);
+  load_weight<T>(s, a.w_vec[side], c1, w + VE);
 #pragma unroll
   for (int e = 0; e < 2 * VE; ++e) dw[e] = 0.f;
   const float inv_d = 1.f / float(p.D);
@@ -579,17 +594,23 @@ int lanes_of(const QkProblem& p) {
   return g;
 }
 
-// Heads per group: all the parallelism there is for small calls, else up to
-// eight, so that a token's angles are read once for eight vectors.
+// Heads per group: as many as still leave two groups for every lane group
+// that the SMs hold at eight warps each, up to 16, so that a token's angles
+// are read once for as many vectors as can be.
 QkVecArgs vec_args(const QkProblem& p, int g) {
-  QkVecArgs a{p, nullptr, 1, {0, 0}, {0, 0}, {0, 0}};
+  QkVecArgs a{};
+  a.p = p;
   const int64_t vectors = p.B * p.N * (p.side[0].H + p.side[1].H);
-  const int64_t slots = int64_t(device_sm_count()) * 64 * (32 / g);
-  a.heads_per_group = vectors >= 8 * slots ? 8 : (vectors >= 4 * slots ? 4 : 1);
+  const int64_t slots = int64_t(device_sm_count()) * 8 * (32 / g) * 2;
+  a.heads_per_group = 16;
+  while (a.heads_per_group > 1 && vectors / a.heads_per_group < slots)
+    a.heads_per_group /= 2;
   for (int i = 0; i < 2; ++i) {
     a.groups_per_token[i] =
         (p.side[i].H + a.heads_per_group - 1) / a.heads_per_group;
     a.groups[i] = p.B * p.N * a.groups_per_token[i];
+    a.w_vec[i] = (reinterpret_cast<uintptr_t>(p.side[i].w) & 15) == 0 &&
+                 (p.side[i].sw == 1 || p.D == 1);
   }
   return a;
 }

@@ -22,6 +22,17 @@ PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
   return fn;
 }
 
+// Encodes through `call`. A thread that has made no CUDA runtime call yet (an
+// autograd worker, a serving thread) has no current context, which the
+// encoder refuses: bind the device's and try once more.
+template <typename F>
+bool encode(F&& call) {
+  if (call() == CUDA_SUCCESS) return true;
+  int dev = 0;
+  return cudaGetDevice(&dev) == cudaSuccess &&
+         cudaSetDevice(dev) == cudaSuccess && call() == CUDA_SUCCESS;
+}
+
 }  // namespace
 
 bool tensor_maps_available() { return encode_fn() != nullptr; }
@@ -49,14 +60,15 @@ bool make_tile_map(CUtensorMap* map, const void* base, int dtype, int64_t B,
                                           : CU_TENSOR_MAP_SWIZZLE_32B);
   cuuint32_t box[4] = {cuuint32_t(box_cols), cuuint32_t(box_rows), 1, 1};
   cuuint32_t estr[4] = {1, 1, 1, 1};
-  const CUresult r = fn(map,
-                        dtype == VECTRA_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
-                                             : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
-                        4, const_cast<void*>(base), dims, strides, box, estr,
-                        CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
-                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  return r == CUDA_SUCCESS;
+  return encode([&] {
+    return fn(map,
+              dtype == VECTRA_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                   : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+              4, const_cast<void*>(base), dims, strides, box, estr,
+              CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+              CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  });
 }
 
 bool make_line_map(CUtensorMap* map, const void* base, int dtype,
@@ -69,15 +81,15 @@ bool make_line_map(CUtensorMap* map, const void* base, int dtype,
   cuuint64_t strides[1] = {cuuint64_t(ld) * 2};
   cuuint32_t box[2] = {64, cuuint32_t(box_lines)};
   cuuint32_t estr[2] = {1, 1};
-  const CUresult r = fn(map,
-                        dtype == VECTRA_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
-                                             : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
-                        2, const_cast<void*>(base), dims, strides, box, estr,
-                        CU_TENSOR_MAP_INTERLEAVE_NONE,
-                        CU_TENSOR_MAP_SWIZZLE_128B,
-                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  return r == CUDA_SUCCESS;
+  return encode([&] {
+    return fn(map,
+              dtype == VECTRA_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                   : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+              2, const_cast<void*>(base), dims, strides, box, estr,
+              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+              CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  });
 }
 
 }  // namespace vectra

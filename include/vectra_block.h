@@ -88,13 +88,23 @@ typedef struct {
   size_t workspace_bytes;
 } vectra_gated_args;
 
+/* With a reduction (K) up to this long, forming gate and up again in the
+ * backward pass takes no more time than writing and reading them (bf16 /
+ * f16; forward and elementwise backward of 66,560 x 256 -> 704 on a B200:
+ * 160 us against 207; of 16,384 x 1024 -> 2816: 275 against 274). The second
+ * limit holds when db_gate and db_up are wanted, whose sums cost the
+ * recomputing kernel more (209 against 212, 298 against 279). */
+#define VECTRA_GATED_RECOMPUTE_K 768
+#define VECTRA_GATED_RECOMPUTE_K_SUMS 256
+
 /* Gradients of the above for dh [M,F]: dg = dh * up * act'(gate), du = dh *
- * act(gate); dx = dg Wg + du Wu; dw_gate = dg^T x, dw_up = du^T x; db_gate
+ * act(gate), with gate and up as the forward saved them, or formed again
+ * from x, the weights and the biases when both are NULL; dx = dg Wg + du Wu; dw_gate = dg^T x, dw_up = du^T x; db_gate
  * and db_up the sums of dg and du over rows. Unwanted results: data NULL
  * (dw_gate and dw_up together, db_gate and db_up together). dw_up directly
  * behind dw_gate in memory saves a pass over x. */
 typedef struct {
-  vectra_tensor dh, x, w_gate, w_up, gate, up;
+  vectra_tensor dh, x, w_gate, w_up, b_gate, b_up, gate, up;
   vectra_tensor dx, dw_gate, dw_up, db_gate, db_up;
   int32_t activation;
   void* workspace;

@@ -346,6 +346,38 @@ def test_gated_empty(device, dtype, size):
 
 
 @pytest.mark.parametrize('device', DEVICES)
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('size', [(1, 64, 64), (7, 40, 33), (70, 96, 200),
+                                  (300, 264, 136), (40, 1100, 72)])
+def test_gated_backward_without_saved_values(device, dtype, size):
+    """The backward operator with gate and up saved, and formed again: the
+    same gradients but for the order of float32 sums (each is within half an
+    output rounding and the accumulation's error, so they differ by at most
+    two roundings of dz or of the result)."""
+    m, k, f = size
+    rand = Rand(19, device, dtype)
+    x, dh = rand(m, k), rand(m, f)
+    wg, wu = rand(f, k, scale=k**-0.5), rand(f, k, scale=k**-0.5)
+    bg, bu = rand(f), rand(f)
+    ops = torch.ops.vectra_b200
+    for act in ('silu', 'gelu', 'gelu_tanh', 'relu', 'none'):
+        _, gate, up = ops.gated_linear_with_pre(x, wg, wu, bg, bu, act, True)
+        none = gate.new_empty(0)
+        for sums in (True, False):
+            want = ops.gated_linear_backward(dh, x, wg, wu, bg, bu, gate, up,
+                                             act, True, True, sums)
+            got = ops.gated_linear_backward(dh, x, wg, wu, bg, bu, none,
+                                            none, act, True, True, sums)
+            # dz differs by one rounding where it lies between two values;
+            # a product sums those against factors of order 1.
+            for a, b, n in zip(got, want, (2 * f, m, m)):
+                assert a.shape == b.shape
+                scale = 16 * U[dtype] * math.sqrt(n) + 16 * U[dtype] * d(
+                    b).abs() + 1e-4
+                assert ((d(a) - d(b)).abs() <= scale).all()
+
+
+@pytest.mark.parametrize('device', DEVICES)
 def test_gated_only_wanted_gradients(device):
     rand = Rand(5, device, torch.float16)
     args = [rand(20, 64), rand(48, 64), rand(48, 64), rand(48), rand(48)]

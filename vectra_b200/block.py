@@ -181,9 +181,9 @@ def _gated_with_pre_fake(x, w_gate, w_up, b_gate, b_up, activation,
 
 
 @torch.library.register_fake('vectra_b200::gated_linear_backward')
-def _gated_backward_fake(dh, x, w_gate, w_up, gate, up, activation, need_dx,
-                         need_dw, need_db):
-    del dh, w_up, gate, up, activation
+def _gated_backward_fake(dh, x, w_gate, w_up, b_gate, b_up, gate, up,
+                         activation, need_dx, need_dw, need_db):
+    del dh, w_up, b_gate, b_up, gate, up, activation
     return (x.new_empty(x.shape if need_dx else (0,)),
             x.new_empty((2, *w_gate.shape) if need_dw else (0,)),
             x.new_empty((2, w_gate.shape[0]) if need_db else (0,)))

@@ -230,8 +230,13 @@ int gated_backward(const vectra_gated_grad_args& a, Workspace& ws,
   VECTRA_TRY(check(a.w_gate, dt, {F, K}));
   VECTRA_TRY(check(a.w_up, dt, {F, K}));
   VECTRA_TRY(check(a.dh, dt, {M, F}));
-  VECTRA_TRY(check_result(a.gate, VECTRA_F32, {M, F}));
-  VECTRA_TRY(check_result(a.up, VECTRA_F32, {M, F}));
+  if (present(a.gate) != present(a.up)) return VECTRA_ERR_NULL;
+  if (present(a.gate)) {
+    VECTRA_TRY(check_result(a.gate, VECTRA_F32, {M, F}));
+    VECTRA_TRY(check_result(a.up, VECTRA_F32, {M, F}));
+  }
+  if (present(a.b_gate)) VECTRA_TRY(check(a.b_gate, dt, {F}));
+  if (present(a.b_up)) VECTRA_TRY(check(a.b_up, dt, {F}));
   if (present(a.dx)) VECTRA_TRY(check_result(a.dx, dt, {M, K}));
   if (present(a.dw_gate) != present(a.dw_up) ||
       present(a.db_gate) != present(a.db_up))
@@ -246,28 +251,76 @@ int gated_backward(const vectra_gated_grad_args& a, Workspace& ws,
   }
   const size_t es = dt == VECTRA_F32 ? 4 : 2;
   // dg and du side by side, [M][2 pad8(F)].
-  GradProblem g;
-  g.dtype = dt;
-  g.act = a.activation;
-  g.gated = true;
-  g.M = M;
-  g.N = F;
-  g.dy = a.dh.data;
-  g.dy_sm = a.dh.stride[0];
-  g.dy_sn = a.dh.stride[1];
-  g.gate = static_cast<const float*>(a.gate.data);
-  g.gate_ld = a.gate.stride[0];
-  g.up = static_cast<const float*>(a.up.data);
-  g.up_ld = a.up.stride[0];
   const int64_t ld = 2 * pad8(F);
   char* d = static_cast<char*>(ws.take(size_t(M) * ld * es));
   char* d2 = d ? d + ld / 2 * es : nullptr;
-  g.dz = d;
-  g.dz2 = d2;
-  g.dz_ld = ld;
-  g.db = const_cast<void*>(a.db_gate.data);
-  g.db2 = const_cast<void*>(a.db_up.data);
-  VECTRA_TRY(to_status(run_grad(g, ws, stream), ws));
+  void* db = const_cast<void*>(a.db_gate.data);
+  void* db2 = const_cast<void*>(a.db_up.data);
+  // The layer's own product, for values that were not saved.
+  GemmProblem layer;
+  layer.dtype = dt;
+  layer.act = a.activation;
+  layer.M = M;
+  layer.N = F;
+  layer.K = K;
+  layer.a[0] = rows_of(a.x);
+  layer.b[0] = rows_of(a.w_gate);
+  layer.b[1] = rows_of(a.w_up);
+  layer.bias[0] = a.b_gate.data;
+  layer.bias_stride[0] = a.b_gate.stride[0];
+  layer.bias[1] = a.b_up.data;
+  layer.bias_stride[1] = a.b_up.stride[0];
+  const bool saved = present(a.gate) || M == 0 || F == 0;
+  if (!saved && dt != VECTRA_F32 && K > 0) {
+    const int64_t blocks = (M + 31) / 32;
+    layer.epilogue = kEpiGatedGrad;
+    layer.res = a.dh.data;
+    layer.res_sm = a.dh.stride[0];
+    layer.res_sn = a.dh.stride[1];
+    layer.out = d;
+    layer.pre = d2;
+    layer.out_ld = layer.pre_ld = ld;
+    if (db) {
+      layer.gate = static_cast<float*>(ws.take(size_t(blocks) * F * 4));
+      layer.up = static_cast<float*>(ws.take(size_t(blocks) * F * 4));
+    }
+    VECTRA_TRY(to_status(run_gemm(layer, ws, stream), ws));
+    if (db && !ws.dry)
+      VECTRA_TRY(to_status(
+          launch_column_finish(dt, layer.gate, layer.up, int(blocks), F, db,
+                               db2, stream), ws));
+  } else {
+    GradProblem g;
+    g.dtype = dt;
+    g.act = a.activation;
+    g.gated = true;
+    g.M = M;
+    g.N = F;
+    g.dy = a.dh.data;
+    g.dy_sm = a.dh.stride[0];
+    g.dy_sn = a.dh.stride[1];
+    g.gate = static_cast<const float*>(a.gate.data);
+    g.gate_ld = a.gate.stride[0];
+    g.up = static_cast<const float*>(a.up.data);
+    g.up_ld = a.up.stride[0];
+    if (!saved) {
+      layer.epilogue = kEpiGated;
+      layer.out = ws.take(size_t(M) * F * es);
+      layer.gate = static_cast<float*>(ws.take(size_t(M) * F * 4));
+      layer.up = static_cast<float*>(ws.take(size_t(M) * F * 4));
+      layer.out_ld = layer.gate_ld = layer.up_ld = F;
+      VECTRA_TRY(to_status(run_gemm(layer, ws, stream), ws));
+      g.gate = layer.gate;
+      g.up = layer.up;
+      g.gate_ld = g.up_ld = F;
+    }
+    g.dz = d;
+    g.dz2 = d2;
+    g.dz_ld = ld;
+    g.db = db;
+    g.db2 = db2;
+    VECTRA_TRY(to_status(run_grad(g, ws, stream), ws));
+  }
   GemmProblem p;
   p.dtype = dt;
   p.epilogue = kEpiStore;

@@ -146,7 +146,11 @@ struct MatView {
 enum GemmEpilogue {
   kEpiStore = 0,   // out = acc
   kEpiLinear = 1,  // z = acc + bias; pre = z; out = act(z) + residual
-  kEpiGated = 2    // g = acc + bias, u = acc2 + bias2; out = act(g) * u
+  kEpiGated = 2,   // g = acc + bias, u = acc2 + bias2; out = act(g) * u
+  // The backward of that without saved values (bf16 / f16): with g and u
+  // formed again and dh in `res`, out = dh u act'(g), pre = dh act(g), and
+  // their sums over blocks of 32 rows in gate and up ([blocks][N]).
+  kEpiGatedGrad = 3
 };
 
 struct GemmProblem {
@@ -155,7 +159,7 @@ struct GemmProblem {
   int32_t act = VECTRA_ACT_NONE;
   int32_t segments = 1;  // products summed: 1 or 2 (kEpiGated: 1)
   int64_t M = 0, N = 0, K = 0;  // every segment reduces over K
-  MatView a[2], b[2];    // kEpiGated: b[0] gate, b[1] up, both with a[0]
+  MatView a[2], b[2];    // gated: b[0] gate, b[1] up, both with a[0]
   const void* bias[2] = {nullptr, nullptr};
   int64_t bias_stride[2] = {0, 0};
   const void* res = nullptr;
@@ -219,6 +223,10 @@ struct GradProblem {
   void* db2 = nullptr;
 };
 cudaError_t run_grad(const GradProblem& p, Workspace& ws, cudaStream_t stream);
+// db = column sums of `partial` [chunks][N], in order; db2 likewise.
+cudaError_t launch_column_finish(int32_t dtype, const float* partial,
+                                 const float* partial2, int chunks, int64_t N,
+                                 void* db, void* db2, cudaStream_t stream);
 
 // qk_norm_rope.cu
 struct QkSide {

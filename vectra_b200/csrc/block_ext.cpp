@@ -441,13 +441,16 @@ Grads3 gated_cpu(const Tensor& x, const Tensor& wg, const Tensor& wu,
 }
 
 // Gradients of x, of both weights [2, F, K] and of both biases [2, F].
+// gate and up may both be empty: they are formed again.
 void check_gated_grad(const Tensor& dh, const Tensor& x, const Tensor& wg,
-                      const Tensor& wu, const Tensor& gate,
+                      const Tensor& wu, const OptTensor& bg,
+                      const OptTensor& bu, const Tensor& gate,
                       const Tensor& up) {
-  check_gated(x, wg, wu, std::nullopt, std::nullopt);
+  check_gated(x, wg, wu, bg, bu);
   check_like(dh, "dh", x);
   const auto shape = with_last(x.sizes(), wg.size(0));
   check_sizes(dh, "dh", shape);
+  if (gate.numel() == 0 && up.numel() == 0) return;
   for (const Tensor* t : {&gate, &up}) {
     check_sizes(*t, "gate and up", shape);
     TORCH_CHECK_VALUE(t->device() == x.device() &&
@@ -458,10 +461,11 @@ void check_gated_grad(const Tensor& dh, const Tensor& x, const Tensor& wg,
 
 Grads3 gated_backward_cuda(const Tensor& dh, const Tensor& x,
                            const Tensor& wg, const Tensor& wu,
+                           const OptTensor& bg, const OptTensor& bu,
                            const Tensor& gate, const Tensor& up,
                            const std::string& activation, bool need_dx,
                            bool need_dw, bool need_db) {
-  check_gated_grad(dh, x, wg, wu, gate, up);
+  check_gated_grad(dh, x, wg, wu, bg, bu, gate, up);
   c10::cuda::CUDAGuard guard(x.device());
   Tensor x_copy, dh_copy;
   const Tensor g = gate.contiguous(), u = up.contiguous();
@@ -478,8 +482,12 @@ Grads3 gated_backward_cuda(const Tensor& dh, const Tensor& x,
   a.x = describe_rows(x, &x_copy);
   a.w_gate = describe(wg);
   a.w_up = describe(wu);
-  a.gate = describe_rows(g, nullptr);
-  a.up = describe_rows(u, nullptr);
+  a.b_gate = describe(bg);
+  a.b_up = describe(bu);
+  if (g.numel()) {
+    a.gate = describe_rows(g, nullptr);
+    a.up = describe_rows(u, nullptr);
+  }
   if (need_dx) a.dx = describe_rows(dx, nullptr);
   if (need_dw) {
     a.dw_gate = describe(dw.select(0, 0));
@@ -497,13 +505,24 @@ Grads3 gated_backward_cuda(const Tensor& dh, const Tensor& x,
 
 Grads3 gated_backward_cpu(const Tensor& dh, const Tensor& x,
                           const Tensor& wg, const Tensor& wu,
+                          const OptTensor& bg, const OptTensor& bu,
                           const Tensor& gate, const Tensor& up,
                           const std::string& activation, bool need_dx,
                           bool need_dw, bool need_db) {
-  check_gated_grad(dh, x, wg, wu, gate, up);
+  check_gated_grad(dh, x, wg, wu, bg, bu, gate, up);
   const int32_t act = activation_of(activation);
   const auto dt = x.scalar_type();
-  const Tensor d = f32(as_rows(dh)), g = as_rows(gate), u = as_rows(up);
+  const Tensor d = f32(as_rows(dh));
+  Tensor g, u;
+  if (gate.numel() || d.numel() == 0) {
+    g = as_rows(gate).reshape(d.sizes());
+    u = as_rows(up).reshape(d.sizes());
+  } else {
+    g = at::matmul(f32(as_rows(x)), f32(wg).t());
+    u = at::matmul(f32(as_rows(x)), f32(wu).t());
+    if (has(bg)) g = g + f32(*bg);
+    if (has(bu)) u = u + f32(*bu);
+  }
   const Tensor dg = cpu_act_grad(d * u, g, act), du = d * cpu_act(g, act);
   const auto none = [&] { return at::empty({0}, x.options()); };
   Tensor dx = need_dx ? (at::matmul(dg, f32(wg)) + at::matmul(du, f32(wu)))
@@ -795,6 +814,7 @@ Grads3 call_gated(const Tensor& x, const Tensor& wg, const Tensor& wu,
 
 Grads3 call_gated_backward(const Tensor& dh, const Tensor& x,
                            const Tensor& wg, const Tensor& wu,
+                           const OptTensor& bg, const OptTensor& bu,
                            const Tensor& gate, const Tensor& up,
                            const std::string& activation, bool need_dx,
                            bool need_dw, bool need_db) {
@@ -802,10 +822,11 @@ Grads3 call_gated_backward(const Tensor& dh, const Tensor& x,
       c10::Dispatcher::singleton()
           .findSchemaOrThrow("vectra_b200::gated_linear_backward", "")
           .typed<Grads3(const Tensor&, const Tensor&, const Tensor&,
-                        const Tensor&, const Tensor&, const Tensor&,
-                        c10::string_view, bool, bool, bool)>();
-  return op.call(dh, x, wg, wu, gate, up, activation, need_dx, need_dw,
-                 need_db);
+                        const Tensor&, const OptTensor&, const OptTensor&,
+                        const Tensor&, const Tensor&, c10::string_view, bool,
+                        bool, bool)>();
+  return op.call(dh, x, wg, wu, bg, bu, gate, up, activation, need_dx,
+                 need_dw, need_db);
 }
 
 std::tuple<Tensor, Tensor> call_qk(const Tensor& q, const Tensor& k,
@@ -941,8 +962,14 @@ struct GatedFunction : public Function<GatedFunction> {
                         const OptTensor& bg, const OptTensor& bu,
                         const std::string& activation) {
     at::AutoDispatchBelowADInplaceOrView below;
-    auto [h, gate, up] = call_gated(x, wg, wu, bg, bu, activation, true);
-    ctx->save_for_backward({x, wg, wu, gate, up});
+    // Short reductions: the backward forms gate and up again.
+    const bool sums = wants_grad(bg) || wants_grad(bu);
+    const bool save = x.scalar_type() == at::kFloat ||
+                      wg.size(1) > (sums ? VECTRA_GATED_RECOMPUTE_K_SUMS
+                                         : VECTRA_GATED_RECOMPUTE_K);
+    auto [h, gate, up] = call_gated(x, wg, wu, bg, bu, activation, save);
+    ctx->save_for_backward({x, wg, wu, gate, up, bg.value_or(Tensor()),
+                            bu.value_or(Tensor())});
     ctx->saved_data["activation"] = activation;
     const bool needs[5] = {wants_grad(x), wants_grad(wg), wants_grad(wu),
                            wants_grad(bg), wants_grad(bu)};
@@ -958,8 +985,8 @@ struct GatedFunction : public Function<GatedFunction> {
     if (!grads[0].defined()) return out;
     BelowUnlessRecording below;
     auto [dx, dw, db] = call_gated_backward(
-        grads[0], s[0], s[1], s[2], s[3], s[4],
-        ctx->saved_data["activation"].toStringRef(), (mask & 1) != 0,
+        grads[0], s[0], s[1], s[2], optional(s[5]), optional(s[6]), s[3],
+        s[4], ctx->saved_data["activation"].toStringRef(), (mask & 1) != 0,
         (mask & 6) != 0, (mask & 24) != 0);
     if (mask & 1) out[0] = dx;
     for (int i = 0; i < 2; ++i) {
@@ -1078,11 +1105,12 @@ Grads3 gated_impl(const Tensor& x, const Tensor& wg, const Tensor& wu,
 template <auto F>
 Grads3 gated_backward_impl(const Tensor& dh, const Tensor& x,
                            const Tensor& wg, const Tensor& wu,
+                           const OptTensor& bg, const OptTensor& bu,
                            const Tensor& gate, const Tensor& up,
                            c10::string_view activation, bool need_dx,
                            bool need_dw, bool need_db) {
-  return F(dh, x, wg, wu, gate, up, std::string(activation), need_dx,
-           need_dw, need_db);
+  return F(dh, x, wg, wu, bg, bu, gate, up, std::string(activation),
+           need_dx, need_dw, need_db);
 }
 
 }  // namespace
@@ -1108,8 +1136,9 @@ TORCH_LIBRARY_FRAGMENT(vectra_b200, m) {
       "-> (Tensor, Tensor, Tensor)");
   m.def(
       "gated_linear_backward(Tensor dh, Tensor x, Tensor w_gate, "
-      "Tensor w_up, Tensor gate, Tensor up, str activation, bool need_dx, "
-      "bool need_dw, bool need_db) -> (Tensor, Tensor, Tensor)");
+      "Tensor w_up, Tensor? b_gate, Tensor? b_up, Tensor gate, Tensor up, "
+      "str activation, bool need_dx, bool need_dw, bool need_db) "
+      "-> (Tensor, Tensor, Tensor)");
   m.def(
       "qk_norm_rope(Tensor q, Tensor k, Tensor cos, Tensor sin, "
       "Tensor? q_weight=None, Tensor? k_weight=None, "

@@ -148,13 +148,13 @@ __global__ void __launch_bounds__(kWarps * 32)
   }
 }
 
-// Adds the chunks' sums: one warp per 32 columns would leave the chunks
-// serial, so 8 warps share them and are joined in shared memory.
+// Adds the chunks' sums: 32 warps share the chunks of 32 columns and are
+// joined in shared memory.
 template <typename T>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(1024)
     colsum_finish_kernel(const float* partial, const float* partial2,
                          int chunks, int64_t N, T* out, T* out2) {
-  __shared__ float sums[8][32];
+  __shared__ float sums[32][32];
   allow_dependents();
   grid_dependency_wait();
   const float* src = blockIdx.y ? partial2 : partial;
@@ -162,14 +162,16 @@ __global__ void __launch_bounds__(256)
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int64_t n = int64_t(blockIdx.x) * 32 + lane;
   float t = 0.f;
-  if (n < N)
-    for (int c = warp; c < chunks; c += 8) t += src[c * N + n];
+  if (n < N) {
+#pragma unroll 4
+    for (int c = warp; c < chunks; c += 32) t += __ldg(src + c * N + n);
+  }
   sums[warp][lane] = t;
   __syncthreads();
   if (warp == 0 && n < N) {
     float total = 0.f;
 #pragma unroll
-    for (int w = 0; w < 8; ++w) total += sums[w][lane];
+    for (int w = 0; w < 32; ++w) total += sums[w][lane];
     dst[n] = from_f32<T>(total);
   }
 }
@@ -228,14 +230,19 @@ cudaError_t run_grad(const GradProblem& p, Workspace& ws,
   if (e != cudaSuccess) return e;
   count_launches(1);
   if (!p.db) return cudaSuccess;
-  e = with_dtype(p.dtype, [&](auto* t) {
+  return launch_column_finish(p.dtype, a.partial, a.partial2, int(chunks),
+                              p.N, p.db, p.db2, stream);
+}
+
+cudaError_t launch_column_finish(int32_t dtype, const float* partial,
+                                 const float* partial2, int chunks, int64_t N,
+                                 void* db, void* db2, cudaStream_t stream) {
+  const cudaError_t e = with_dtype(dtype, [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
     return launch_pdl(colsum_finish_kernel<T>,
-                      dim3(unsigned((p.N + 31) / 32), p.gated ? 2 : 1),
-                      dim3(256), 0, stream,
-                      static_cast<const float*>(a.partial),
-                      static_cast<const float*>(a.partial2), int(chunks),
-                      p.N, static_cast<T*>(p.db), static_cast<T*>(p.db2));
+                      dim3(unsigned((N + 31) / 32), db2 ? 2 : 1), dim3(1024),
+                      0, stream, partial, partial2, chunks, N,
+                      static_cast<T*>(db), static_cast<T*>(db2));
   });
   if (e == cudaSuccess) count_launches(1);
   return e;

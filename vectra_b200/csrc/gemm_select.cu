@@ -23,7 +23,8 @@ TcShape tc_shape(const GemmProblem& p) {
   constexpr Option kOptions[] = {
       {256, 2, 0.28}, {128, 1, 0.25}, {64, 1, 0.19}};
   constexpr double kTile = 2.0, kSecondLaunch = 2.5, kBytesPerUs = 5.0e6;
-  const bool gated = p.epilogue == kEpiGated;
+  const bool gated =
+      p.epilogue == kEpiGated || p.epilogue == kEpiGatedGrad;
   const double sms = device_sm_count();
   const int64_t steps =
       (p.K + 63) / 64 * p.segments * (p.dtype == VECTRA_F32 ? 6 : 1);
@@ -41,7 +42,7 @@ TcShape tc_shape(const GemmProblem& p) {
     if (most > steps / 4) most = steps / 4;
     if (most > 64) most = 64;
     for (const int64_t split : {int64_t(1), most}) {
-      if (split < 1) continue;
+      if (split < 1 || (split > 1 && p.epilogue == kEpiGatedGrad)) continue;
       const int64_t per = (steps + split - 1) / split;
       const int64_t waves = (tiles * split + slots - 1) / slots;
       double t = double(waves) * double(per) * o.step + kTile;
@@ -70,7 +71,7 @@ cudaError_t run_gemm(const GemmProblem& p, Workspace& ws,
     if (e == cudaSuccess) count_launches(1);
     return e;
   }
-  if (gemm_rows_supports(p)) {
+  if (p.epilogue != kEpiGatedGrad && gemm_rows_supports(p)) {
     if (ws.dry) return cudaSuccess;
     const cudaError_t e = launch_gemm_rows(p, stream);
     if (e == cudaSuccess) count_launches(1);

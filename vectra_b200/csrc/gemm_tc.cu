@@ -168,7 +168,8 @@ cudaError_t split_planes(const MatView& m, int64_t rows, int64_t k, bool mn,
 
 cudaError_t run_gemm_tc(const GemmProblem& p, const TcShape& shape,
                         Workspace& ws, cudaStream_t stream) {
-  const bool gated = p.epilogue == kEpiGated;
+  const bool gated =
+      p.epilogue == kEpiGated || p.epilogue == kEpiGatedGrad;
   const int tile_n = gated ? shape.bn / 2 : shape.bn;
   if (tile_n < 64 || (shape.bn == 256) != (shape.cg == 2) ||
       (shape.cg == 2 && p.dtype == VECTRA_F32))
@@ -224,19 +225,11 @@ cudaError_t run_gemm_tc(const GemmProblem& p, const TcShape& shape,
         size_t(g.split) * (gated ? 2 : 1) * p.M * p.N * sizeof(float)));
   if (ws.dry || ws.overflow) return cudaSuccess;
 
-  const auto vec = [](const void* q, int64_t ld, int64_t es) {
-    return uint8_t(aligned16(q) && (ld * es) % 16 == 0);
-  };
   const int64_t es = f32 ? 4 : 2;
-  const bool whole = p.N * es % 16 == 0;
-  g.vec_out = whole && vec(p.out, p.out_ld, es);
-  g.vec_pre = whole && vec(p.pre, p.pre_ld, es);
-  g.vec_res = whole && p.res_sn == 1 && vec(p.res, p.res_sm, es);
-  g.vec_f32 = g.split > 1 ? p.N % 4 == 0
-                          : p.N % 4 == 0 && vec(p.gate, p.gate_ld, 4) &&
-                                vec(p.up, p.up_ld, 4);
+  g.vec_res = p.N * es % 16 == 0 && p.res_sn == 1 && aligned16(p.res) &&
+              p.res_sm * es % 16 == 0;
 
-  CUtensorMap maps[4];
+  CUtensorMap maps[7] = {};
   const int b_rows = gated && shape.cg == 1 ? shape.bn / 2
                                             : shape.bn / shape.cg;
   for (int i = 0; i < 4; ++i) {
@@ -247,6 +240,23 @@ cudaError_t run_gemm_tc(const GemmProblem& p, const TcShape& shape,
                        p.dtype == VECTRA_F16 ? VECTRA_F16 : VECTRA_BF16,
                        o.mn ? rows : p.K, o.lines * o.planes, o.ld, box))
       return cudaErrorInvalidValue;
+  }
+  // Results, 32 rows of 64 bytes at a time.
+  const auto result = [&](CUtensorMap* map, const void* q, int dtype,
+                          int64_t ld, int64_t planes) {
+    return uint8_t(q != nullptr && make_result_map(map, q, dtype, p.N, p.M,
+                                                   planes, ld));
+  };
+  if (g.split > 1) {
+    g.tma_out = result(&maps[4], g.partial, VECTRA_F32, p.N,
+                       int64_t(g.split) * (gated ? 2 : 1));
+  } else {
+    g.tma_out = result(&maps[4], p.out, p.dtype, p.out_ld, 1);
+    if (p.pre)
+      g.tma_pre = result(&maps[5], p.pre, p.dtype, p.pre_ld, 1);
+    else if (p.epilogue == kEpiGated && p.gate)
+      g.tma_pre = result(&maps[5], p.gate, VECTRA_F32, p.gate_ld, 1) &&
+                  result(&maps[6], p.up, VECTRA_F32, p.up_ld, 1);
   }
   const int epilogue =
       g.split == 1 ? p.epilogue : (gated ? kEpiGatedPartial : kEpiPartial);

@@ -33,12 +33,13 @@ struct TcArgs {
   int steps_part;     // steps of one part
   int64_t units;      // tiles * split
   uint8_t a_mn, b_mn;  // operand staged MN-major
-  uint8_t vec_out, vec_pre, vec_res, vec_f32;
+  uint8_t tma_out, tma_pre;  // results, saved values: by tensor map
+  uint8_t vec_res;           // residual in 16-byte pieces
   TcSegment seg[kMostSegments];
 };
 
 // Epilogues of the kernels beyond GemmEpilogue: float32 sums of one part.
-enum { kEpiPartial = 3, kEpiGatedPartial = 4 };
+enum { kEpiPartial = 4, kEpiGatedPartial = 5 };
 
 template <typename T>
 cudaError_t launch_tc_linear(int bn, int cg, const CUtensorMap* maps,

@@ -50,8 +50,10 @@ namespace {
 using namespace tc;
 
 constexpr int kCtrlWarps = 2;
-constexpr int kStagePitch = 80;  // epilogue turning buffer: rows of 64 B + 16
-constexpr int kEpiWarpBytes = 32 * kStagePitch + 512;  // and the biases
+// A warp's turning buffer, 32 rows of 64 bytes in the 64-byte-swizzled order
+// of the tensor maps' stores, and its biases.
+constexpr int kTurnBytes = 2048;
+constexpr int kBiasBytes = 512;
 
 template <int BN, int CG>
 struct Cfg {
@@ -67,7 +69,7 @@ struct Cfg {
   static constexpr int A_BYTES = kTcRows * kTcStep * 2;
   static constexpr int B_BYTES = B_ROWS * kTcStep * 2;
   static constexpr int STAGE = A_BYTES + B_BYTES;
-  static constexpr int EPI_BYTES = EPI_WARPS * kEpiWarpBytes;
+  static constexpr int EPI_BYTES = EPI_WARPS * (kTurnBytes + kBiasBytes);
   static constexpr int MAX_BYTES = 227 * 1024 - 2048 - EPI_BYTES;
   static constexpr int STAGES = MAX_BYTES / STAGE < 8 ? MAX_BYTES / STAGE : 8;
   static constexpr int OFF_EPI = STAGES * STAGE;
@@ -235,6 +237,7 @@ __device__ __forceinline__ void dealloc_cols(uint32_t addr, uint32_t cols) {
 // so a value costs 1.5 MUFU operations instead of 2. z is capped from below
 // (NaN kept) where x reaches 63, so that ab stays finite; the result there
 // is within 3e-10 of the activation, and -infinity gives that, not NaN.
+// Packed multiplications and additions halve the instructions.
 // ---------------------------------------------------------------------------
 __device__ __forceinline__ float max_nan(float a, float b) {
   float r;
@@ -242,14 +245,51 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   return r;
 }
 
-// -log2(e) logit(Phi(z)) / z as a polynomial in t = z^2.
-__device__ __forceinline__ float gelu_q(float t) {
-  float q = fmaf(-5.2620424e-09f, t, 3.8715868e-07f);
-  q = fmaf(q, t, -1.1483583e-05f);
-  q = fmaf(q, t, 1.5959822e-04f);
-  q = fmaf(q, t, 9.4943171e-05f);
-  q = fmaf(q, t, -1.0483774e-01f);
-  return fmaf(q, t, -2.3022075f);
+__device__ __forceinline__ uint64_t fmul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t both(float c) { return f2pk(c, c); }
+
+// -log2(e) logit(Phi(z)) / z as a polynomial in t = z^2, of two values.
+__device__ __forceinline__ uint64_t gelu_q(uint64_t t) {
+  uint64_t q = ffma2(both(-5.2620424e-09f), t, both(3.8715868e-07f));
+  q = ffma2(q, t, both(-1.1483583e-05f));
+  q = ffma2(q, t, both(1.5959822e-04f));
+  q = ffma2(q, t, both(9.4943171e-05f));
+  q = ffma2(q, t, both(-1.0483774e-01f));
+  return ffma2(q, t, both(-2.3022075f));
+}
+
+// The sigmoids of two smooth activations; z is capped first, where x would
+// pass 63.
+template <int ACT>
+__device__ __forceinline__ void sigmoid2(float& z0, float& z1, float& s0,
+                                         float& s1) {
+  constexpr float kLow = ACT == VECTRA_ACT_SILU        ? -43.6f
+                         : ACT == VECTRA_ACT_GELU_TANH ? -7.6f
+                                                       : -6.5f;
+  z0 = max_nan(z0, kLow);
+  z1 = max_nan(z1, kLow);
+  const uint64_t z = f2pk(z0, z1);
+  uint64_t x;
+  if constexpr (ACT == VECTRA_ACT_SILU) {
+    x = fmul2(z, both(-kLog2e));
+  } else {
+    const uint64_t t = fmul2(z, z);
+    if constexpr (ACT == VECTRA_ACT_GELU_TANH) {
+      constexpr float k0 = -2.f * kGeluTanhC * kLog2e;
+      x = fmul2(z, ffma2(t, both(k0 * kGeluTanhA), both(k0)));
+    } else {
+      x = fmul2(z, gelu_q(t));
+    }
+  }
+  const float2 xs = f2upk(x);
+  const float a = 1.f + fast_exp2(xs.x), b = 1.f + fast_exp2(xs.y);
+  const float r = fast_rcp(a * b);
+  s0 = b * r;
+  s1 = a * r;
 }
 
 template <int ACT>
@@ -258,31 +298,46 @@ __device__ __forceinline__ void activate2(float& z0, float& z1) {
     z0 = max_nan(z0, 0.f);
     z1 = max_nan(z1, 0.f);
   } else if constexpr (ACT != VECTRA_ACT_NONE) {
-    // Below kLow, x would pass 63.
-    constexpr float kLow = ACT == VECTRA_ACT_SILU        ? -43.6f
-                           : ACT == VECTRA_ACT_GELU_TANH ? -7.6f
-                                                         : -6.5f;
-    z0 = max_nan(z0, kLow);
-    z1 = max_nan(z1, kLow);
-    float x0, x1;
-    if constexpr (ACT == VECTRA_ACT_SILU) {
-      x0 = -kLog2e * z0;
-      x1 = -kLog2e * z1;
-    } else {
-      const float t0 = z0 * z0, t1 = z1 * z1;
-      if constexpr (ACT == VECTRA_ACT_GELU_TANH) {
-        constexpr float k0 = -2.f * kGeluTanhC * kLog2e;
-        x0 = fmaf(k0 * kGeluTanhA, t0, k0) * z0;
-        x1 = fmaf(k0 * kGeluTanhA, t1, k0) * z1;
-      } else {
-        x0 = gelu_q(t0) * z0;
-        x1 = gelu_q(t1) * z1;
-      }
-    }
-    const float a = 1.f + fast_exp2(x0), b = 1.f + fast_exp2(x1);
-    const float r = fast_rcp(a * b);
-    z0 *= b * r;
-    z1 *= a * r;
+    float s0, s1;
+    sigmoid2<ACT>(z0, z1, s0, s1);
+    z0 *= s0;
+    z1 *= s1;
+  }
+}
+
+// act'(z) from z (capped) and its sigmoid s: s + z ds/dz.
+template <int ACT>
+__device__ __forceinline__ float slope_of(float z, float s) {
+  if constexpr (ACT == VECTRA_ACT_SILU) {
+    return fmaf(z * s, 1.f - s, s);
+  } else if constexpr (ACT == VECTRA_ACT_GELU_TANH) {
+    // 0 * z^2 far out has to stay 0.
+    const float t = fminf(z * z, 1e4f);
+    const float du = 2.f * kGeluTanhC * fmaf(3.f * kGeluTanhA, t, 1.f);
+    return fmaf(z * s * (1.f - s), du, s);
+  } else {  // gelu: s is Phi, and Phi' the normal density
+    const float t = fminf(z * z, 1e4f);
+    return fmaf(z * 0.3989422804f, fast_exp2(-0.5f * kLog2e * t), s);
+  }
+}
+// z0, z1 become act(z), s0, s1 act'(z).
+template <int ACT>
+__device__ __forceinline__ void activate_grad2(float& z0, float& z1,
+                                               float& s0, float& s1) {
+  if constexpr (ACT == VECTRA_ACT_NONE) {
+    s0 = s1 = 1.f;
+  } else if constexpr (ACT == VECTRA_ACT_RELU) {
+    s0 = z0 > 0.f ? 1.f : 0.f;
+    s1 = z1 > 0.f ? 1.f : 0.f;
+    z0 = max_nan(z0, 0.f);
+    z1 = max_nan(z1, 0.f);
+  } else {
+    float p0, p1;
+    sigmoid2<ACT>(z0, z1, p0, p1);
+    s0 = slope_of<ACT>(z0, p0);
+    s1 = slope_of<ACT>(z1, p1);
+    z0 *= p0;
+    z1 *= p1;
   }
 }
 
@@ -309,89 +364,155 @@ __device__ __forceinline__ void activate(float* v) {
 }
 
 // ---------------------------------------------------------------------------
-// Epilogue pieces. `stage` is the warp's 32 x kStagePitch turning buffer.
+// Epilogue pieces. `stage` is the warp's turning buffer: a lane writes (or
+// reads) its row, and rows are moved whole by the copy engine where the
+// result's layout allows a tensor map, else by the warp. The copy engine
+// spares the shared-memory reads and the stores of the warp: with K = 256
+// the SM's one 128 B/clk path through L1 and shared memory, which the
+// operands also take, is what bounds a tile.
 // ---------------------------------------------------------------------------
-// Where a warp's 32-row block lies: rows left in the matrix (0 .. 32) and
-// the pointer walk of the coalesced passes.
 struct RowBlock {
   int64_t row0;
-  int rows;
+  int rows;  // of the 32 that lie in the matrix
 };
 
-// Writes the warp's 32 x 32 block (row = lane, packed 16-bit pairs) to rows
-// row0.., columns col.. through the turning buffer: four lanes per row of
-// 64 bytes.
-template <typename T>
-__device__ __forceinline__ void store_block(uint8_t* stage, const uint32_t* pk,
-                                            T* out, int64_t ld,
-                                            const RowBlock& rb, int64_t col,
-                                            int64_t cols, bool vec,
-                                            int lane) {
-#pragma unroll
-  for (int c = 0; c < 4; ++c)
-    *reinterpret_cast<uint4*>(stage + lane * kStagePitch + c * 16) =
-        make_uint4(pk[4 * c], pk[4 * c + 1], pk[4 * c + 2], pk[4 * c + 3]);
-  __syncwarp();
-  if (vec) {
-    const int r = lane / 4, c = (lane % 4) * 8;
-    if (col + c < cols) {
-      T* q = out + (rb.row0 + r) * ld + col + c;
-      const uint8_t* s = stage + r * kStagePitch + c * 2;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if (r + 8 * i < rb.rows)
-          *reinterpret_cast<uint4*>(q) =
-              *reinterpret_cast<const uint4*>(s + i * 8 * kStagePitch);
-        q += 8 * ld;
-      }
-    }
-  } else if (col + lane < cols) {
-    T* q = out + rb.row0 * ld + col + lane;
-    for (int r = 0; r < rb.rows; ++r, q += ld)
-      *q = reinterpret_cast<const T*>(stage + r * kStagePitch)[lane];
-  }
+// Byte offset of 16-byte chunk c of row r.
+__device__ __forceinline__ int turn_at(int r, int c) {
+  return r * 64 + ((c ^ ((r >> 1) & 3)) << 4);
+}
+
+// The buffer is free: the last store has read it. (Lane 0 issues them all.)
+__device__ __forceinline__ void turn_acquire(int lane) {
+  if (lane == 0)
+    asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
   __syncwarp();
 }
 
-// The same for 16 columns of float32.
-__device__ __forceinline__ void store_half_f32(uint8_t* stage, const float* v,
-                                               float* out, int64_t ld,
-                                               const RowBlock& rb,
-                                               int64_t col, int64_t cols,
-                                               bool vec, int lane) {
+// The buffer's rows to rows `row`.. and columns `col`.. of the matrix; what
+// lies outside it is not written.
+__device__ __forceinline__ void turn_store_2d(const CUtensorMap* map,
+                                              uint8_t* stage, int col,
+                                              int row, int lane) {
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  __syncwarp();
+  if (lane == 0) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.global.shared::cta.bulk_group "
+        "[%0, {%2, %3}], [%1];" ::"l"(reinterpret_cast<uint64_t>(map)),
+        "r"(smem_addr(stage)), "r"(col), "r"(row)
+        : "memory");
+    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+  }
+}
+__device__ __forceinline__ void turn_store_3d(const CUtensorMap* map,
+                                              uint8_t* stage, int col,
+                                              int row, int plane, int lane) {
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  __syncwarp();
+  if (lane == 0) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.global.shared::cta.bulk_group "
+        "[%0, {%2, %3, %4}], [%1];" ::"l"(reinterpret_cast<uint64_t>(map)),
+        "r"(smem_addr(stage)), "r"(col), "r"(row), "r"(plane)
+        : "memory");
+    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+  }
+}
+
+// Where a block of results goes: by the copy engine through `map`, else to
+// rows of `ld` elements at `out`.
+template <typename T>
+struct Target {
+  const CUtensorMap* map;
+  bool tma;
+  T* out;
+  int64_t ld, cols;
+};
+
+// Writes 32 rows of 64 bytes (a lane's row in `words`) to columns col..:
+// 32 16-bit or 16 float32 columns.
+template <typename T>
+__device__ __forceinline__ void store_rows(uint8_t* stage,
+                                           const uint32_t* words,
+                                           const Target<T>& to,
+                                           const RowBlock& rb, int64_t col,
+                                           int lane) {
+  constexpr int kCols = 64 / int(sizeof(T));
+  turn_acquire(lane);
 #pragma unroll
   for (int c = 0; c < 4; ++c)
-    *reinterpret_cast<float4*>(stage + lane * kStagePitch + c * 16) =
-        make_float4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
-  __syncwarp();
-  if (vec) {
-    const int r = lane / 4, c = (lane % 4) * 4;
-    if (col + c < cols) {
-      float* q = out + (rb.row0 + r) * ld + col + c;
-      const uint8_t* s = stage + r * kStagePitch + c * 4;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if (r + 8 * i < rb.rows)
-          *reinterpret_cast<float4*>(q) =
-              *reinterpret_cast<const float4*>(s + i * 8 * kStagePitch);
-        q += 8 * ld;
-      }
+    *reinterpret_cast<uint4*>(stage + turn_at(lane, c)) =
+        make_uint4(words[4 * c], words[4 * c + 1], words[4 * c + 2],
+                   words[4 * c + 3]);
+  if (to.tma) {
+    turn_store_2d(to.map, stage, int(col), int(rb.row0), lane);
+  } else {
+    __syncwarp();
+    for (int e = lane; e < 32 * kCols; e += 32) {
+      const int r = e / kCols, c = e % kCols;
+      if (r < rb.rows && col + c < to.cols)
+        to.out[(rb.row0 + r) * to.ld + col + c] =
+            *reinterpret_cast<const T*>(
+                stage + turn_at(r, c * int(sizeof(T)) / 16) +
+                c * int(sizeof(T)) % 16);
     }
-  } else if (col + lane % 16 < cols) {
-    float* q = out + (rb.row0 + lane / 16) * ld + col + lane % 16;
-    for (int r = lane / 16; r < rb.rows; r += 2, q += 2 * ld)
-      *q =
-          reinterpret_cast<const float*>(stage + r * kStagePitch)[lane % 16];
+    __syncwarp();
   }
-  __syncwarp();
 }
-__device__ __forceinline__ void store_block_f32(uint8_t* stage, const float* v,
-                                                float* out, int64_t ld,
-                                                const RowBlock& rb,
-                                                int64_t col, int64_t cols,
-                                                bool vec, int lane) {
-  store_half_f32(stage, v, out, ld, rb, col, cols, vec, lane);
-  store_half_f32(stage, v + 16, out, ld, rb, col + 16, cols, vec, lane);
+__device__ __forceinline__ void store_half_f32(uint8_t* stage, const float* v,
+                                               const Target<float>& to,
+                                               const RowBlock& rb,
+                                               int64_t col, int lane) {
+  uint32_t w[16];
+#pragma unroll
+  for (int j = 0; j < 16; ++j) w[j] = __float_as_uint(v[j]);
+  if (col < to.cols) store_rows<float>(stage, w, to, rb, col, lane);
+}
+
+// A block of 32 x 32 results (or saved values) in T.
+template <typename T>
+__device__ __forceinline__ void store_values(uint8_t* stage, const float* v,
+                                             const Target<T>& to,
+                                             const RowBlock& rb, int64_t col,
+                                             int lane) {
+  if constexpr (std::is_same<T, float>::value) {
+    store_half_f32(stage, v, to, rb, col, lane);
+    store_half_f32(stage, v + 16, to, rb, col + 16, lane);
+  } else {
+    uint32_t pk[16];
+#pragma unroll
+    for (int j = 0; j < 16; ++j) pk[j] = pack2<T>(v[2 * j], v[2 * j + 1]);
+    store_rows<T>(stage, pk, to, rb, col, lane);
+  }
+}
+
+// 32 columns of one part's float32 sums.
+__device__ __forceinline__ void store_partial(uint8_t* stage, const float* v,
+                                              const TcArgs& g,
+                                              const CUtensorMap* map,
+                                              const RowBlock& rb, int plane,
+                                              int64_t col0, int lane) {
+#pragma unroll
+  for (int h = 0; h < 32; h += 16) {
+    const int64_t col = col0 + h;
+    if (col >= g.p.N) continue;
+    uint32_t w[16];
+#pragma unroll
+    for (int j = 0; j < 16; ++j) w[j] = __float_as_uint(v[h + j]);
+    if (g.tma_out) {
+      turn_acquire(lane);
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+        *reinterpret_cast<uint4*>(stage + turn_at(lane, c)) = make_uint4(
+            w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]);
+      turn_store_3d(map, stage, int(col), int(rb.row0), plane, lane);
+    } else {
+      const Target<float> to{
+          nullptr, false, g.partial + int64_t(plane) * g.p.M * g.p.N, g.p.N,
+          g.p.N};
+      store_rows<float>(stage, w, to, rb, col, lane);
+    }
+  }
 }
 
 // The residual's 32 x 32 block: asynchronous copies into the turning buffer
@@ -402,15 +523,15 @@ __device__ __forceinline__ void fetch_residual(uint8_t* stage,
                                                const GemmProblem& p,
                                                const RowBlock& rb,
                                                int64_t col, int lane) {
-  const int r = lane / 4, c = (lane % 4) * 8;
+  turn_acquire(lane);
+  const int r = lane / 4, c = lane % 4;
   const T* q = static_cast<const T*>(p.res) + (rb.row0 + r) * p.res_sm + col +
-               c;
-  const uint32_t dst = smem_addr(stage) + r * kStagePitch + c * 2;
+               c * 8;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    if (r + 8 * i < rb.rows && col + c < p.N)
+    if (r + 8 * i < rb.rows && col + c * 8 < p.N)
       asm volatile("cp.async.ca.shared.global [%0], [%1], 16;" ::"r"(
-                       dst + i * 8 * kStagePitch),
+                       smem_addr(stage + turn_at(r + 8 * i, c))),
                    "l"(q)
                    : "memory");
     q += 8 * p.res_sm;
@@ -427,25 +548,37 @@ __device__ __forceinline__ float2 unpack2(uint32_t w) {
     return __half22float2(*reinterpret_cast<const __half2*>(&w));
 }
 
+// The residual block's rows are in the turning buffer: waits for the copies,
+// or, without whole 16-byte pieces, reads it here.
+template <typename T>
+__device__ __forceinline__ void residual_ready(uint8_t* stage, bool vec,
+                                               const GemmProblem& p,
+                                               const RowBlock& rb,
+                                               int64_t col, int lane) {
+  if (vec) {
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+  } else {
+    turn_acquire(lane);
+    const T* q = static_cast<const T*>(p.res) + rb.row0 * p.res_sm +
+                 (col + lane) * p.res_sn;
+    if (col + lane < p.N)
+      for (int r = 0; r < rb.rows; ++r, q += p.res_sm)
+        *reinterpret_cast<T*>(stage + turn_at(r, lane / 8) + lane % 8 * 2) =
+            *q;
+  }
+  __syncwarp();
+}
+
 template <typename T>
 __device__ __forceinline__ void add_residual(uint8_t* stage, float* v,
                                              bool vec, const GemmProblem& p,
                                              const RowBlock& rb, int64_t col,
                                              int lane) {
-  if (vec) {
-    asm volatile("cp.async.wait_group 0;" ::: "memory");
-  } else {
-    const T* q = static_cast<const T*>(p.res) + rb.row0 * p.res_sm +
-                 (col + lane) * p.res_sn;
-    for (int r = 0; r < rb.rows; ++r, q += p.res_sm)
-      if (col + lane < p.N)
-        reinterpret_cast<T*>(stage + r * kStagePitch)[lane] = *q;
-  }
-  __syncwarp();
+  residual_ready<T>(stage, vec, p, rb, col, lane);
 #pragma unroll
   for (int c = 0; c < 4; ++c) {
-    const uint4 q = *reinterpret_cast<const uint4*>(
-        stage + lane * kStagePitch + c * 16);
+    const uint4 q =
+        *reinterpret_cast<const uint4*>(stage + turn_at(lane, c));
     const uint32_t w[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -457,7 +590,25 @@ __device__ __forceinline__ void add_residual(uint8_t* stage, float* v,
   __syncwarp();
 }
 
-// Adds a float32 residual, 16 columns at a time.
+// Adds 16 columns over the warp's 32 rows (lanes), destroying x: every step
+// halves the columns a lane keeps and hands the other half to its partner,
+// so that lanes 2 c and 2 c + 1 end with column c.
+__device__ __forceinline__ float column_sums16(float* x, int lane) {
+#pragma unroll
+  for (int n = 8; n >= 1; n >>= 1) {
+    const bool upper = (lane & (2 * n)) != 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if (i >= n) break;
+      const float keep = upper ? x[i + n] : x[i];
+      const float give = upper ? x[i] : x[i + n];
+      x[i] = keep + __shfl_xor_sync(0xffffffffu, give, 2 * n);
+    }
+  }
+  return x[0] + __shfl_xor_sync(0xffffffffu, x[0], 1);
+}
+
+// A float32 residual, 16 columns at a time.
 __device__ __forceinline__ void add_residual_f32(uint8_t* stage, float* v,
                                                  bool vec,
                                                  const GemmProblem& p,
@@ -467,50 +618,34 @@ __device__ __forceinline__ void add_residual_f32(uint8_t* stage, float* v,
 #pragma unroll
   for (int h = 0; h < 32; h += 16) {
     const int64_t col = col0 + h;
+    turn_acquire(lane);
     if (vec) {
-      const int r = lane / 4, c = (lane % 4) * 4;
-      const float* q = res + (rb.row0 + r) * p.res_sm + col + c;
+      const int r = lane / 4, c = lane % 4;
+      const float* q = res + (rb.row0 + r) * p.res_sm + col + c * 4;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        if (r + 8 * i < rb.rows && col + c < p.N)
-          *reinterpret_cast<float4*>(stage + (r + 8 * i) * kStagePitch +
-                                     c * 4) =
+        if (r + 8 * i < rb.rows && col + c * 4 < p.N)
+          *reinterpret_cast<float4*>(stage + turn_at(r + 8 * i, c)) =
               __ldg(reinterpret_cast<const float4*>(q));
         q += 8 * p.res_sm;
       }
     } else if (col + lane % 16 < p.N) {
       for (int r = lane / 16; r < rb.rows; r += 2)
-        reinterpret_cast<float*>(stage + r * kStagePitch)[lane % 16] =
+        *reinterpret_cast<float*>(stage + turn_at(r, lane % 16 / 4) +
+                                  lane % 4 * 4) =
             res[(rb.row0 + r) * p.res_sm + (col + lane % 16) * p.res_sn];
     }
     __syncwarp();
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
-      const float4 q = *reinterpret_cast<const float4*>(
-          stage + lane * kStagePitch + c * 16);
+      const float4 q =
+          *reinterpret_cast<const float4*>(stage + turn_at(lane, c));
       v[h + 4 * c] += q.x;
       v[h + 4 * c + 1] += q.y;
       v[h + 4 * c + 2] += q.z;
       v[h + 4 * c + 3] += q.w;
     }
     __syncwarp();
-  }
-}
-
-// A block of 32 x 32 results (or saved values) in T.
-template <typename T>
-__device__ __forceinline__ void store_values(uint8_t* stage, const float* v,
-                                             T* out, int64_t ld,
-                                             const RowBlock& rb, int64_t col,
-                                             int64_t cols, bool vec,
-                                             int lane) {
-  if constexpr (std::is_same<T, float>::value) {
-    store_block_f32(stage, v, out, ld, rb, col, cols, vec, lane);
-  } else {
-    uint32_t pk[16];
-#pragma unroll
-    for (int j = 0; j < 16; ++j) pk[j] = pack2<T>(v[2 * j], v[2 * j + 1]);
-    store_block<T>(stage, pk, out, ld, rb, col, cols, vec, lane);
   }
 }
 
@@ -546,17 +681,21 @@ __device__ __forceinline__ void add_bias(float* v, const float* cols) {
 // instructions for each result where the bare store takes 6.
 template <int EPI, int ACT, bool RES, bool PRE, typename T, int TILE_N,
           int WARP_COLS, typename Wait, typename Release>
-__device__ __forceinline__ void epilogue_tile(const TcArgs& g, uint8_t* stage,
-                                              float* cols, int chunks,
+__device__ __forceinline__ void epilogue_tile(const TcArgs& g,
+                                              const CUtensorMap* const* maps,
+                                              uint8_t* stage, float* cols,
+                                              int chunks,
                                               const RowBlock& rb,
                                               int64_t tile_col, int part,
                                               int lane, Wait&& wait,
                                               Release&& release) {
-  constexpr bool kGated = EPI == kEpiGated || EPI == kEpiGatedPartial;
+  constexpr bool kGated = EPI == kEpiGated || EPI == kEpiGatedPartial ||
+                          EPI == kEpiGatedGrad;
   constexpr bool kPartial = EPI == kEpiPartial || EPI == kEpiGatedPartial;
   static_assert(WARP_COLS % 32 == 0 && WARP_COLS <= 64, "columns");
   const GemmProblem& p = g.p;
-  if constexpr (EPI == kEpiLinear || EPI == kEpiGated) {
+  if constexpr (EPI == kEpiLinear || EPI == kEpiGated ||
+                EPI == kEpiGatedGrad) {
     load_bias<T>(cols, p.bias[0], p.bias_stride[0], tile_col, p.N, WARP_COLS,
                  lane);
     if constexpr (kGated)
@@ -564,6 +703,13 @@ __device__ __forceinline__ void epilogue_tile(const TcArgs& g, uint8_t* stage,
                    WARP_COLS, lane);
     __syncwarp();
   }
+  const Target<T> out{maps[0], g.tma_out != 0, static_cast<T*>(p.out),
+                      p.out_ld, p.N};
+  const Target<T> pre{maps[1], g.tma_pre != 0, static_cast<T*>(p.pre),
+                      p.pre_ld, p.N};
+  const Target<float> gate_to{maps[1], g.tma_pre != 0, p.gate, p.gate_ld,
+                              p.N};
+  const Target<float> up_to{maps[2], g.tma_pre != 0, p.up, p.up_ld, p.N};
   // With saved values in the same buffer the residual comes after them.
   constexpr bool kF32 = std::is_same<T, float>::value;
   constexpr bool kEarly = RES && !PRE && !kF32;
@@ -573,18 +719,15 @@ __device__ __forceinline__ void epilogue_tile(const TcArgs& g, uint8_t* stage,
   auto finish = [&](float* v, float* up, int c0) {
     const int64_t col = tile_col + c0;
     if constexpr (kPartial) {
-      const int64_t plane = p.M * p.N;
-      float* q = g.partial + int64_t(part) * (kGated ? 2 : 1) * plane;
-      store_block_f32(stage, v, q, p.N, rb, col, p.N, g.vec_f32, lane);
+      const int plane = part * (kGated ? 2 : 1);
+      store_partial(stage, v, g, maps[0], rb, plane, col, lane);
       if constexpr (kGated)
-        store_block_f32(stage, up, q + plane, p.N, rb, col, p.N, g.vec_f32,
-                        lane);
+        store_partial(stage, up, g, maps[0], rb, plane + 1, col, lane);
     } else {
       if constexpr (EPI == kEpiLinear) {
         add_bias<32>(v, cols + c0);
         if constexpr (PRE) {
-          store_values<T>(stage, v, static_cast<T*>(p.pre), p.pre_ld, rb,
-                          col, p.N, g.vec_pre, lane);
+          store_values<T>(stage, v, pre, rb, col, lane);
           if constexpr (RES && !kF32)
             if (g.vec_res) fetch_residual<T>(stage, p, rb, col, lane);
         }
@@ -598,17 +741,14 @@ __device__ __forceinline__ void epilogue_tile(const TcArgs& g, uint8_t* stage,
         add_bias<32>(v, cols + c0);
         add_bias<32>(up, cols + 64 + c0);
         if constexpr (PRE) {
-          store_block_f32(stage, v, p.gate, p.gate_ld, rb, col, p.N,
-                          g.vec_f32, lane);
-          store_block_f32(stage, up, p.up, p.up_ld, rb, col, p.N, g.vec_f32,
-                          lane);
+          store_values<float>(stage, v, gate_to, rb, col, lane);
+          store_values<float>(stage, up, up_to, rb, col, lane);
         }
         activate<ACT, 32>(v);
 #pragma unroll
         for (int j = 0; j < 32; ++j) v[j] *= up[j];
       }
-      store_values<T>(stage, v, static_cast<T*>(p.out), p.out_ld, rb, col,
-                      p.N, g.vec_out, lane);
+      store_values<T>(stage, v, out, rb, col, lane);
     }
   };
   if constexpr (kF32) {
@@ -636,6 +776,82 @@ __device__ __forceinline__ void epilogue_tile(const TcArgs& g, uint8_t* stage,
     for (int c0 = 0; c0 < WARP_COLS; c0 += 32)
       if (rb.rows > 0 && tile_col + c0 < p.N)
         finish(sum + c0, sum + (kGated ? WARP_COLS + c0 : 0), c0);
+  } else if constexpr (EPI == kEpiGatedGrad) {
+    // g and u again, and with dh (read like a residual) dg = dh u act'(g)
+    // and du = dh act(g). RES: their sums over the warp's rows as well, from
+    // the unrounded values.
+    uint32_t acc = 0;
+    if (g.vec_res) fetch_residual<T>(stage, p, rb, tile_col, lane);
+    if (!wait(&acc)) return;
+#pragma unroll 1
+    for (int c0 = 0; c0 < WARP_COLS; c0 += 32) {
+      const int64_t col = tile_col + c0;
+      const bool live = rb.rows > 0 && col < p.N;
+      if (g.vec_res && c0 > 0) fetch_residual<T>(stage, p, rb, col, lane);
+      residual_ready<T>(stage, g.vec_res, p, rb, col, lane);
+      uint32_t dg[16], du[16];
+#pragma unroll
+      for (int h = 0; h < 32; h += 16) {
+        uint32_t dh[8];
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const uint4 q = *reinterpret_cast<const uint4*>(
+              stage + turn_at(lane, h / 8 + c));
+          const bool in = lane < rb.rows;  // rows past the end count nothing
+          dh[4 * c] = in ? q.x : 0;
+          dh[4 * c + 1] = in ? q.y : 0;
+          dh[4 * c + 2] = in ? q.z : 0;
+          dh[4 * c + 3] = in ? q.w : 0;
+        }
+        uint32_t r0[16], r1[16];
+        tmem_ld16u(acc + c0 + h, r0);
+        tmem_ld16u(acc + TILE_N + c0 + h, r1);
+        tmem_wait_ld();
+        regs_tie16(r0);
+        regs_tie16(r1);
+        if (c0 + h + 16 == WARP_COLS) release();
+        float v[16], up[16];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          v[j] = __uint_as_float(r0[j]);
+          up[j] = __uint_as_float(r1[j]);
+        }
+        add_bias<16>(v, cols + c0 + h);
+        add_bias<16>(up, cols + 64 + c0 + h);
+#pragma unroll
+        for (int j = 0; j < 16; j += 2) {
+          if (j % 8 == 0) tie8(v + j);
+          float s0, s1;
+          activate_grad2<ACT>(v[j], v[j + 1], s0, s1);
+          const float2 d = unpack2<T>(dh[j / 2]);
+          up[j] *= d.x * s0;
+          up[j + 1] *= d.y * s1;
+          v[j] *= d.x;
+          v[j + 1] *= d.y;
+          if (j % 8 == 6) tie8(v + j - 6);
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          dg[h / 2 + j] = pack2<T>(up[2 * j], up[2 * j + 1]);
+          du[h / 2 + j] = pack2<T>(v[2 * j], v[2 * j + 1]);
+        }
+        if constexpr (RES) {
+          const float sg = column_sums16(up, lane);
+          const float su = column_sums16(v, lane);
+          const int64_t c = col + h + (lane >> 1);
+          if (live && (lane & 1) == 0 && c < p.N) {
+            const int64_t at = rb.row0 / 32 * p.N + c;
+            p.gate[at] = sg;
+            p.up[at] = su;
+          }
+        }
+      }
+      __syncwarp();  // dh's rows are read
+      if (live) {
+        store_rows<T>(stage, dg, out, rb, col, lane);
+        store_rows<T>(stage, du, pre, rb, col, lane);
+      }
+    }
   } else if constexpr (EPI == kEpiGated) {
     // Both factors of 16 columns at a time: 32 of each would not fit the 96
     // registers beside the packed results.
@@ -665,10 +881,8 @@ __device__ __forceinline__ void epilogue_tile(const TcArgs& g, uint8_t* stage,
         add_bias<16>(up, cols + 64 + c0 + h);
         if constexpr (PRE) {
           if (live) {
-            store_half_f32(stage, v, p.gate, p.gate_ld, rb, col + h, p.N,
-                           g.vec_f32, lane);
-            store_half_f32(stage, up, p.up, p.up_ld, rb, col + h, p.N,
-                           g.vec_f32, lane);
+            store_half_f32(stage, v, gate_to, rb, col + h, lane);
+            store_half_f32(stage, up, up_to, rb, col + h, lane);
           }
         }
         activate<ACT, 16>(v);
@@ -678,8 +892,7 @@ __device__ __forceinline__ void epilogue_tile(const TcArgs& g, uint8_t* stage,
                                    v[2 * j + 1] * up[2 * j + 1]);
       }
       if (live)
-        store_block<T>(stage, pk, static_cast<T*>(p.out), p.out_ld, rb, col,
-                       p.N, g.vec_out, lane);
+        store_rows<T>(stage, pk, out, rb, col, lane);
     }
   } else {
     uint32_t acc = 0;
@@ -715,9 +928,13 @@ __global__ void __launch_bounds__(Cfg<BN, CG>::THREADS, 1)
                    const __grid_constant__ CUtensorMap ta1,
                    const __grid_constant__ CUtensorMap tb0,
                    const __grid_constant__ CUtensorMap tb1,
+                   const __grid_constant__ CUtensorMap tout,
+                   const __grid_constant__ CUtensorMap tpre,
+                   const __grid_constant__ CUtensorMap tpre2,
                    const __grid_constant__ TcArgs g) {
   using C = Cfg<BN, CG>;
-  constexpr bool kGated = EPI == kEpiGated || EPI == kEpiGatedPartial;
+  constexpr bool kGated = EPI == kEpiGated || EPI == kEpiGatedPartial ||
+                          EPI == kEpiGatedGrad;
   constexpr bool kF32 = std::is_same<T, float>::value;
   constexpr int kTileN = kGated ? BN / 2 : BN;  // output columns of a tile
   // Operand format: bf16 (also float32's planes) or f16.
@@ -899,8 +1116,10 @@ __global__ void __launch_bounds__(Cfg<BN, CG>::THREADS, 1)
     const int w = warp - kCtrlWarps;
     constexpr int kWarpCols = kTileN / (C::EPI_WARPS / 4);
     const int quarter = warp & 3, share = w >> 2;
-    uint8_t* stage = smem + C::OFF_EPI + w * kEpiWarpBytes;
-    float* cols = reinterpret_cast<float*>(stage + 32 * kStagePitch);
+    uint8_t* stage = smem + C::OFF_EPI + w * kTurnBytes;
+    float* cols = reinterpret_cast<float*>(
+        smem + C::OFF_EPI + C::EPI_WARPS * kTurnBytes + w * kBiasBytes);
+    const CUtensorMap* const maps[3] = {&tout, &tpre, &tpre2};
     const uint32_t lanes = tmem + (uint32_t(quarter * 32) << 16);
     // One copy of the whole loop per activation: with the choice inside it,
     // the copies' registers met again after every tile and spilled.
@@ -944,11 +1163,12 @@ __global__ void __launch_bounds__(Cfg<BN, CG>::THREADS, 1)
           if (buf == 0) buf_phase ^= 1;
         };
         epilogue_tile<EPI, decltype(act)::value, RES, PRE, T, kTileN,
-                      kWarpCols>(g, stage, cols, chunks, rb, tile_col,
+                      kWarpCols>(g, maps, stage, cols, chunks, rb, tile_col,
                                  t.part, lane, wait, release);
       }
     };
-    if constexpr (EPI != kEpiLinear && EPI != kEpiGated) {
+    if constexpr (EPI != kEpiLinear && EPI != kEpiGated &&
+                  EPI != kEpiGatedGrad) {
       role(std::integral_constant<int, VECTRA_ACT_NONE>{});
     } else {
       switch (p.act) {
@@ -969,6 +1189,8 @@ __global__ void __launch_bounds__(Cfg<BN, CG>::THREADS, 1)
           break;
       }
     }
+    // The last stores have left shared memory and reached global memory.
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
   }
 
   // Teardown: every TMEM access is done before the allocating warp frees it,
@@ -1013,7 +1235,7 @@ cudaError_t launch_cfg(const CUtensorMap* maps, const TcArgs& g,
   cfg.attrs = attr;
   cfg.numAttrs = CG == 1 ? 1 : 2;
   return cudaLaunchKernelEx(&cfg, kern, maps[0], maps[1], maps[2], maps[3],
-                            g);
+                            maps[4], maps[5], maps[6], g);
 }
 
 template <int EPI, bool RES, bool PRE, typename T>
@@ -1024,7 +1246,8 @@ cudaError_t launch_shape(int bn, int cg, const CUtensorMap* maps,
   if constexpr (!std::is_same<T, float>::value)
     if (cg == 2)
       return launch_cfg<EPI, RES, PRE, T, 256, 2>(maps, g, stream);
-  if constexpr (EPI != kEpiGated && EPI != kEpiGatedPartial)
+  if constexpr (EPI != kEpiGated && EPI != kEpiGatedPartial &&
+                EPI != kEpiGatedGrad)
     if (bn == 64) return launch_cfg<EPI, RES, PRE, T, 64, 1>(maps, g, stream);
   return launch_cfg<EPI, RES, PRE, T, 128, 1>(maps, g, stream);
 }
@@ -1057,6 +1280,15 @@ cudaError_t launch_tc_other(int epilogue, int bn, int cg,
                                                                 g, stream)
                       : launch_shape<kEpiGated, false, false, T>(bn, cg, maps,
                                                                  g, stream);
+    case kEpiGatedGrad:
+      if constexpr (std::is_same<T, float>::value)
+        return cudaErrorInvalidValue;
+      else
+        return g.p.gate
+                   ? launch_shape<kEpiGatedGrad, true, false, T>(bn, cg, maps,
+                                                                 g, stream)
+                   : launch_shape<kEpiGatedGrad, false, false, T>(
+                         bn, cg, maps, g, stream);
     case kEpiPartial:
       return launch_shape<kEpiPartial, false, false, T>(bn, cg, maps, g,
                                                         stream);

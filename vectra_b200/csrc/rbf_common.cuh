@@ -379,6 +379,12 @@ bool make_tile_map(CUtensorMap* map, const void* base, int dtype, int64_t B,
 bool make_line_map(CUtensorMap* map, const void* base, int dtype,
                    int64_t inner, int64_t outer, int64_t ld, int box_lines);
 
+// A result matrix of `rows` by `cols` elements (f32, bf16 or f16), rows `ld`
+// apart, and `planes` of them one behind the other (3-D when more than one):
+// box of 64 bytes by 32 rows, SWIZZLE_64B. False when the layout has no map.
+bool make_result_map(CUtensorMap* map, const void* base, int dtype,
+                     int64_t cols, int64_t rows, int64_t planes, int64_t ld);
+
 // Streaming-multiprocessor count of the current device (cached).
 int device_sm_count();
 

@@ -92,4 +92,29 @@ bool make_line_map(CUtensorMap* map, const void* base, int dtype,
   });
 }
 
+bool make_result_map(CUtensorMap* map, const void* base, int dtype,
+                     int64_t cols, int64_t rows, int64_t planes, int64_t ld) {
+  auto fn = encode_fn();
+  const int64_t es = dtype == VECTRA_F32 ? 4 : 2;
+  if (rows == 1) ld = (cols * es + 15) / 16 * 16 / es;
+  if (!fn || (reinterpret_cast<uintptr_t>(base) & 15) || ld * es % 16 != 0 ||
+      (planes > 1 && ld != cols))
+    return false;
+  cuuint64_t dims[3] = {cuuint64_t(cols), cuuint64_t(rows),
+                        cuuint64_t(planes)};
+  cuuint64_t strides[2] = {cuuint64_t(ld * es), cuuint64_t(ld * es * rows)};
+  cuuint32_t box[3] = {cuuint32_t(64 / es), 32, 1};
+  cuuint32_t estr[3] = {1, 1, 1};
+  const CUtensorMapDataType type =
+      dtype == VECTRA_F32    ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+      : dtype == VECTRA_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                             : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  return encode([&] {
+    return fn(map, type, planes > 1 ? 3 : 2, const_cast<void*>(base), dims,
+              strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+              CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_NONE,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  });
+}
+
 }  // namespace vectra

@@ -22,16 +22,18 @@ TcShape tc_shape(const GemmProblem& p) {
   };
   constexpr Option kOptions[] = {
       {256, 2, 0.28}, {128, 1, 0.25}, {64, 1, 0.19}};
+  // float32 stages hold three planes and are multiplied six times.
+  constexpr double kPlanes = 3.4;
   constexpr double kTile = 2.0, kSecondLaunch = 2.5, kBytesPerUs = 5.0e6;
   const bool gated =
       p.epilogue == kEpiGated || p.epilogue == kEpiGatedGrad;
   const double sms = device_sm_count();
-  const int64_t steps =
-      (p.K + 63) / 64 * p.segments * (p.dtype == VECTRA_F32 ? 6 : 1);
+  const bool f32 = p.dtype == VECTRA_F32;
+  const int64_t steps = (p.K + 63) / 64 * p.segments;
   TcShape best;
   double least = 1e30;
   for (const Option& o : kOptions) {
-    if (o.cg == 2 && (p.dtype == VECTRA_F32 || p.M <= 128)) continue;
+    if (o.cg == 2 && (f32 || p.M <= 128)) continue;
     if (gated && o.bn < 128) continue;
     const int64_t cols = gated ? o.bn / 2 : o.bn;
     const int64_t rows = int64_t(kTcRows) * o.cg;
@@ -45,7 +47,8 @@ TcShape tc_shape(const GemmProblem& p) {
       if (split < 1 || (split > 1 && p.epilogue == kEpiGatedGrad)) continue;
       const int64_t per = (steps + split - 1) / split;
       const int64_t waves = (tiles * split + slots - 1) / slots;
-      double t = double(waves) * double(per) * o.step + kTile;
+      double t = double(waves) * double(per) * o.step * (f32 ? kPlanes : 1.0) +
+                 kTile;
       if (split > 1)
         t += kSecondLaunch + 8.0 * double(split) * double(p.M) *
                                  double(p.N) * (gated ? 2 : 1) / kBytesPerUs;

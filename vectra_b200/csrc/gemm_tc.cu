@@ -180,7 +180,7 @@ cudaError_t run_gemm_tc(const GemmProblem& p, const TcShape& shape,
   g.tiles_n = int((p.N + tile_n - 1) / tile_n);
   g.steps_seg = int((p.K + kTcStep - 1) / kTcStep);
   const bool f32 = p.dtype == VECTRA_F32;
-  g.steps = g.steps_seg * p.segments * (f32 ? 6 : 1);
+  g.steps = g.steps_seg * p.segments;
   g.split = shape.split;
   g.steps_part = (g.steps + g.split - 1) / g.split;
   g.split = (g.steps + g.steps_part - 1) / g.steps_part;  // no empty parts
@@ -210,16 +210,8 @@ cudaError_t run_gemm_tc(const GemmProblem& p, const TcShape& shape,
     if (n == 1) op[2 * side + 1] = op[2 * side];
     (side ? g.b_mn : g.a_mn) = uint8_t(mn);
   }
-  // hi, mid and lo are planes 0, 1 and 2.
-  constexpr int kPlanes[6][2] = {{2, 0}, {0, 2}, {1, 1},
-                                 {1, 0}, {0, 1}, {0, 0}};
-  for (int s = 0; s < p.segments; ++s)
-    for (int i = 0; i < (f32 ? 6 : 1); ++i) {
-      TcSegment& seg = g.seg[f32 ? i * p.segments + s : s];
-      seg.map = s;
-      seg.a_line = f32 ? int(kPlanes[i][0] * op[0].lines) : 0;
-      seg.b_line = f32 ? int(kPlanes[i][1] * op[2].lines) : 0;
-    }
+  g.a_lines = int(op[0].lines);
+  g.b_lines = int(op[2].lines);
   if (g.split > 1)
     g.partial = static_cast<float*>(ws.take(
         size_t(g.split) * (gated ? 2 : 1) * p.M * p.N * sizeof(float)));

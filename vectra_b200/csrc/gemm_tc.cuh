@@ -16,13 +16,6 @@ struct TcShape {
 constexpr int kTcRows = 128;  // rows of a tile per CTA
 constexpr int kTcStep = 64;   // reduction per stage: one 128-byte row
 
-// One product of the sum: which tensor maps (0 or 1), and where the operands'
-// lines start in them (float32 operands keep three planes in one map).
-struct TcSegment {
-  int32_t map, a_line, b_line;
-};
-constexpr int kMostSegments = 12;
-
 struct TcArgs {
   GemmProblem p;
   float* partial;     // split > 1: [split][planes][M][N]
@@ -35,7 +28,7 @@ struct TcArgs {
   uint8_t a_mn, b_mn;  // operand staged MN-major
   uint8_t tma_out, tma_pre;  // results, saved values: by tensor map
   uint8_t vec_res;           // residual in 16-byte pieces
-  TcSegment seg[kMostSegments];
+  int32_t a_lines, b_lines;  // float32: lines of one plane
 };
 
 // Epilogues of the kernels beyond GemmEpilogue: float32 sums of one part.

@@ -28,10 +28,10 @@
 // output in its row.
 //
 // float32 tensors: each operand is first split into three bf16 planes, hi +
-// mid + lo, 24 bits in all, and the product is the sum of the six plane
-// products that matter (lo hi, hi lo, mid mid, mid hi, hi mid, hi hi, small
-// ones first), as further segments of the same reduction: 6 bf16 products
-// run at 3.5 times the FP32 pipe's rate.
+// mid + lo, 24 bits in all; a stage brings in all planes of both, and the
+// product is the sum of the six plane products that matter (lo hi, hi lo,
+// mid mid, mid hi, hi mid, hi hi): 6 bf16 products run at 3.5 times the FP32
+// pipe's rate.
 //
 // A reduction too long for its few tiles is cut into parts that write
 // float32 sums to the workspace; launch_split_finish adds them in order.
@@ -55,7 +55,7 @@ constexpr int kCtrlWarps = 2;
 constexpr int kTurnBytes = 2048;
 constexpr int kBiasBytes = 512;
 
-template <int BN, int CG>
+template <int BN, int CG, bool F32>
 struct Cfg {
   // Epilogue warps: each TMEM lane quarter (a warp reads the quarter of its
   // index modulo 4) is shared by EPI_WARPS / 4 of them, with at least 32
@@ -68,7 +68,10 @@ struct Cfg {
   static constexpr int B_ROWS = BN / CG;  // rows of B staged per CTA
   static constexpr int A_BYTES = kTcRows * kTcStep * 2;
   static constexpr int B_BYTES = B_ROWS * kTcStep * 2;
-  static constexpr int STAGE = A_BYTES + B_BYTES;
+  static constexpr int PLANES = F32 ? 3 : 1;
+  static constexpr int PLANE = A_BYTES + B_BYTES;  // one plane's A, then B
+  static constexpr int STAGE = PLANES * PLANE;
+  static constexpr int ACC_COLS = F32 ? 2 * BN : BN;  // see multiply_planes
   static constexpr int EPI_BYTES = EPI_WARPS * (kTurnBytes + kBiasBytes);
   static constexpr int MAX_BYTES = 227 * 1024 - 2048 - EPI_BYTES;
   static constexpr int STAGES = MAX_BYTES / STAGE < 8 ? MAX_BYTES / STAGE : 8;
@@ -77,7 +80,7 @@ struct Cfg {
   static constexpr int NBAR = 2 * STAGES + 4;
   static constexpr int SMEM = OFF_BAR + NBAR * 8 + 16;
   static constexpr int SMEM_ALLOC = SMEM + 1024;  // 1024-byte alignment
-  static constexpr int TMEM_COLS = 2 * BN;        // two accumulators
+  static constexpr int TMEM_COLS = 2 * ACC_COLS;  // two accumulators
   static_assert(SMEM_ALLOC <= 227 * 1024, "shared memory");
   static_assert(TMEM_COLS == 512 || TMEM_COLS == 256 || TMEM_COLS == 128,
                 "TMEM columns");
@@ -110,16 +113,11 @@ __device__ __forceinline__ Unit unit_of(const TcArgs& a, int64_t u) {
 // float32: where the accumulation that starts at step `from` ends. The tensor
 // cores add into the accumulator rounding toward zero, so a long sum drifts
 // (by -2e-8 of itself for every 16 products: 1.4e-5 after 4,096 positive
-// ones). The five small plane products are too small for that to matter, but
-// of the last, hi hi, every 512 of the reduction is accumulated apart and
-// added by the epilogue, which rounds to nearest.
+// ones). Every 512 of the reduction is accumulated apart and added by the
+// epilogue, which rounds to nearest.
 constexpr int kChunkSteps = 8;
-__device__ __forceinline__ int chunk_end(const TcArgs& g, int from,
-                                         int last) {
-  const int small = g.steps / 6 * 5;  // steps before hi hi
-  const int at = from < small ? 0 : (from - small) / kChunkSteps;
-  const int end = small + (at + 1) * kChunkSteps;
-  return end < last ? end : last;
+__device__ __forceinline__ int chunk_end(int from, int last) {
+  return from + kChunkSteps < last ? from + kChunkSteps : last;
 }
 
 // ---------------------------------------------------------------------------
@@ -761,14 +759,21 @@ __device__ __forceinline__ void epilogue_tile(const TcArgs& g,
       if (!wait(&acc)) return;
 #pragma unroll
       for (int c = 0; c < kSums; c += 16) {
-        uint32_t r[16];
-        tmem_ld16u(acc + (c < WARP_COLS ? c : TILE_N + c - WARP_COLS), r);
+        // hi hi, and the five small products.
+        constexpr int kSmall = kGated ? 2 * TILE_N : TILE_N;
+        const uint32_t at =
+            acc + (c < WARP_COLS ? c : TILE_N + c - WARP_COLS);
+        uint32_t r[16], q[16];
+        tmem_ld16u(at, r);
+        tmem_ld16u(at + kSmall, q);
         tmem_wait_ld();
         regs_tie16(r);
+        regs_tie16(q);
 #pragma unroll
-        for (int j = 0; j < 16; ++j)
-          sum[c + j] = chunk == 0 ? __uint_as_float(r[j])
-                                  : sum[c + j] + __uint_as_float(r[j]);
+        for (int j = 0; j < 16; ++j) {
+          const float part_sum = __uint_as_float(r[j]) + __uint_as_float(q[j]);
+          sum[c + j] = chunk == 0 ? part_sum : sum[c + j] + part_sum;
+        }
       }
       release();
     }
@@ -923,7 +928,7 @@ __device__ __forceinline__ void epilogue_tile(const TcArgs& g,
 }
 
 template <int EPI, bool RES, bool PRE, typename T, int BN, int CG>
-__global__ void __launch_bounds__(Cfg<BN, CG>::THREADS, 1)
+__global__ void __launch_bounds__(Cfg<BN, CG, std::is_same<T, float>::value>::THREADS, 1)
     gemm_tc_kernel(const __grid_constant__ CUtensorMap ta0,
                    const __grid_constant__ CUtensorMap ta1,
                    const __grid_constant__ CUtensorMap tb0,
@@ -932,7 +937,7 @@ __global__ void __launch_bounds__(Cfg<BN, CG>::THREADS, 1)
                    const __grid_constant__ CUtensorMap tpre,
                    const __grid_constant__ CUtensorMap tpre2,
                    const __grid_constant__ TcArgs g) {
-  using C = Cfg<BN, CG>;
+  using C = Cfg<BN, CG, std::is_same<T, float>::value>;
   constexpr bool kGated = EPI == kEpiGated || EPI == kEpiGatedPartial ||
                           EPI == kEpiGatedGrad;
   constexpr bool kF32 = std::is_same<T, float>::value;
@@ -995,9 +1000,8 @@ __global__ void __launch_bounds__(Cfg<BN, CG>::THREADS, 1)
         const int k_last = k_first + g.steps_part < g.steps
                                ? k_first + g.steps_part
                                : g.steps;
-        int seg_at = k_first / g.steps_seg;
-        int in_seg = k_first - seg_at * g.steps_seg;
-        TcSegment seg = g.seg[seg_at];
+        int seg = k_first / g.steps_seg;
+        int in_seg = k_first - seg * g.steps_seg;
         for (int k = k_first; k < k_last; ++k) {
           ok = mbar_wait(bar_empty(s), phase ^ 1, p.err);
           if (!ok) break;
@@ -1007,37 +1011,41 @@ __global__ void __launch_bounds__(Cfg<BN, CG>::THREADS, 1)
           if constexpr (CG == 2) full = map_cta(full, 0);
           if (in_seg == g.steps_seg) {
             in_seg = 0;
-            seg = g.seg[++seg_at];
+            ++seg;
           }
           const int k0 = in_seg++ * kTcStep;
-          const uint32_t sa = sbase + uint32_t(s) * C::STAGE;
-          const uint32_t sb = sa + C::A_BYTES;
-          const CUtensorMap* ma = seg.map ? &ta1 : &ta0;
-          if (g.a_mn) {
+          const CUtensorMap* ma = seg ? &ta1 : &ta0;
 #pragma unroll
-            for (int i = 0; i < kTcRows / 64; ++i)
-              tma_load_2d<CG>(sa + i * 8192, ma, full, m0 + i * 64,
-                              k0 + seg.a_line);
-          } else {
-            tma_load_2d<CG>(sa, ma, full, k0, m0 + seg.a_line);
-          }
-          // Rows of B: in a pair, half each. A gated tile's first half is
-          // the gate weight's rows, its second half the up weight's.
-          constexpr int kBoxRows = kGated && CG == 1 ? BN / 2 : C::B_ROWS;
+          for (int plane = 0; plane < C::PLANES; ++plane) {
+            const int a_line = plane * g.a_lines, b_line = plane * g.b_lines;
+            const uint32_t sa =
+                sbase + uint32_t(s) * C::STAGE + plane * C::PLANE;
+            const uint32_t sb = sa + C::A_BYTES;
+            if (g.a_mn) {
 #pragma unroll
-          for (int h = 0; h < C::B_ROWS / kBoxRows; ++h) {
-            const CUtensorMap* mb =
-                (kGated ? (CG == 2 ? int(rank) : h) : seg.map) ? &tb1 : &tb0;
-            const int row =
-                kGated ? n0 : n0 + int(rank) * C::B_ROWS;
-            const uint32_t dst = sb + h * kBoxRows * 128;
-            if (g.b_mn) {
-#pragma unroll
-              for (int i = 0; i < kBoxRows / 64; ++i)
-                tma_load_2d<CG>(dst + i * 8192, mb, full, row + i * 64,
-                                k0 + seg.b_line);
+              for (int i = 0; i < kTcRows / 64; ++i)
+                tma_load_2d<CG>(sa + i * 8192, ma, full, m0 + i * 64,
+                                k0 + a_line);
             } else {
-              tma_load_2d<CG>(dst, mb, full, k0, row + seg.b_line);
+              tma_load_2d<CG>(sa, ma, full, k0, m0 + a_line);
+            }
+            // Rows of B: in a pair, half each. A gated tile's first half is
+            // the gate weight's rows, its second half the up weight's.
+            constexpr int kBoxRows = kGated && CG == 1 ? BN / 2 : C::B_ROWS;
+#pragma unroll
+            for (int h = 0; h < C::B_ROWS / kBoxRows; ++h) {
+              const CUtensorMap* mb =
+                  (kGated ? (CG == 2 ? int(rank) : h) : seg) ? &tb1 : &tb0;
+              const int row = kGated ? n0 : n0 + int(rank) * C::B_ROWS;
+              const uint32_t dst = sb + h * kBoxRows * 128;
+              if (g.b_mn) {
+#pragma unroll
+                for (int i = 0; i < kBoxRows / 64; ++i)
+                  tma_load_2d<CG>(dst + i * 8192, mb, full, row + i * 64,
+                                  k0 + b_line);
+              } else {
+                tma_load_2d<CG>(dst, mb, full, k0, row + b_line);
+              }
             }
           }
           ++issued;
@@ -1082,21 +1090,37 @@ __global__ void __launch_bounds__(Cfg<BN, CG>::THREADS, 1)
                                ? k_first + g.steps_part
                                : g.steps;
         for (int from = k_first; from < k_last && ok;) {
-        const int to = kF32 ? chunk_end(g, from, k_last) : k_last;
+        const int to = kF32 ? chunk_end(from, k_last) : k_last;
         ok = mbar_wait(bar_acc_empty(buf), buf_phase ^ 1, p.err);
         if (!ok) break;
         tc_fence_after();
-        const uint32_t d = tmem + uint32_t(buf * BN);
+        const uint32_t d = tmem + uint32_t(buf * C::ACC_COLS);
         for (int k = from; k < to; ++k) {
           ok = mbar_wait(bar_full(s), phase, p.err);
           if (!ok) break;
           tc_fence_after();
           const uint64_t da = da0 + uint64_t((uint32_t(s) * C::STAGE) >> 4);
           const uint64_t db = db0 + uint64_t((uint32_t(s) * C::STAGE) >> 4);
+          if constexpr (kF32) {
+            // Planes 0, 1, 2 are hi, mid, lo. hi hi has an accumulator of its
+            // own: the others are too small beside it for their truncation
+            // to matter, but would add five more truncations of its sum.
+            constexpr int kPairs[6][2] = {{2, 0}, {0, 2}, {1, 1},
+                                          {1, 0}, {0, 1}, {0, 0}};
 #pragma unroll
-          for (int i = 0; i < kTcStep / 16; ++i)
-            mma_f16<CG>(d, da + i * ka, db + i * kb, idesc,
-                        k > from || i > 0);
+            for (int i = 0; i < kTcStep / 16; ++i)
+#pragma unroll
+              for (int q = 0; q < 6; ++q)
+                mma_f16<CG>(q == 5 ? d : d + BN,
+                            da + i * ka + ((kPairs[q][0] * C::PLANE) >> 4),
+                            db + i * kb + ((kPairs[q][1] * C::PLANE) >> 4),
+                            idesc, k > from || i > 0 || (q > 0 && q < 5));
+          } else {
+#pragma unroll
+            for (int i = 0; i < kTcStep / 16; ++i)
+              mma_f16<CG>(d, da + i * ka, db + i * kb, idesc,
+                          k > from || i > 0);
+          }
           commit_all<CG>(bar_empty(s));
           if (++s == C::STAGES) {
             s = 0;
@@ -1140,14 +1164,14 @@ __global__ void __launch_bounds__(Cfg<BN, CG>::THREADS, 1)
                                  ? k_first + g.steps_part
                                  : g.steps;
           chunks = 0;
-          for (int k = k_first; k < k_last; k = chunk_end(g, k, k_last))
+          for (int k = k_first; k < k_last; k = chunk_end(k, k_last))
             ++chunks;
         }
         auto wait = [&](uint32_t* acc) {
           ok = mbar_wait(bar_acc_full(buf), buf_phase, p.err);
           ok = __all_sync(0xffffffffu, ok);
           if (ok) tc_fence_after();
-          *acc = lanes + uint32_t(buf * BN + share * kWarpCols);
+          *acc = lanes + uint32_t(buf * C::ACC_COLS + share * kWarpCols);
           return ok;
         };
         auto release = [&] {
@@ -1207,7 +1231,7 @@ __global__ void __launch_bounds__(Cfg<BN, CG>::THREADS, 1)
 template <int EPI, bool RES, bool PRE, typename T, int BN, int CG>
 cudaError_t launch_cfg(const CUtensorMap* maps, const TcArgs& g,
                        cudaStream_t stream) {
-  using C = Cfg<BN, CG>;
+  using C = Cfg<BN, CG, std::is_same<T, float>::value>;
   auto kern = gemm_tc_kernel<EPI, RES, PRE, T, BN, CG>;
   static std::atomic<int> configured[64];
   int dev = 0;

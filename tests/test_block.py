@@ -13,6 +13,7 @@ summed against the other factor's magnitudes. float16's subnormal spacing
 adds 2^-24 per rounding.
 """
 
+import ctypes
 import math
 
 import numpy as np
@@ -20,6 +21,7 @@ import pytest
 import torch
 
 import vectra_b200
+from vectra_b200 import _lib
 from vectra_b200 import block
 from vectra_b200 import custom_ops
 
@@ -746,7 +748,6 @@ def test_exports():
     """The library exports what include/vectra_block.h declares."""
     import os
     import re
-    from vectra_b200 import _lib
     header = os.path.join(os.path.dirname(os.path.dirname(
         os.path.abspath(__file__))), 'include', 'vectra_block.h')
     text = re.sub(r'/\*.*?\*/', '', open(header, encoding='utf-8').read(),
@@ -758,6 +759,72 @@ def test_exports():
         assert hasattr(_lib.LIB, name), name
     assert block.strerror(-13).startswith('the workspace')
     assert block.strerror(0) == 'ok'
+
+
+class _LinearArgs(ctypes.Structure):
+    """vectra_linear_args."""
+    _fields_ = [(n, _lib.Tensor) for n in ('x', 'weight', 'bias', 'residual',
+                                           'y', 'pre')] + [
+        ('activation', ctypes.c_int32), ('workspace', ctypes.c_void_p),
+        ('workspace_bytes', ctypes.c_size_t)]
+
+
+def _abi_tensor(shape, dtype=_lib.BF16, strides=None, addr=0x10000):
+    t = _lib.Tensor()
+    t.data, t.dtype, t.ndim = addr, dtype, len(shape)
+    step = 1
+    for i in reversed(range(len(shape))):
+        t.size[i] = shape[i]
+        t.stride[i] = step if strides is None else strides[i]
+        step *= shape[i]
+    return t
+
+
+def test_abi_statuses():
+    """The C entries answer statuses and sizes without touching a device."""
+    size = _lib.LIB.vectra_linear_forward_workspace_bytes
+    size.restype, size.argtypes = ctypes.c_int64, [ctypes.c_void_p]
+    call = _lib.LIB.vectra_linear_forward
+    call.restype, call.argtypes = ctypes.c_int, [ctypes.c_void_p,
+                                                 ctypes.c_void_p]
+
+    def args(**over):
+        a = _LinearArgs()
+        a.x, a.weight = _abi_tensor((64, 4096)), _abi_tensor((512, 4096))
+        a.y = _abi_tensor((64, 512))
+        for name, value in over.items():
+            setattr(a, name, value)
+        return a
+
+    def status(**over):
+        return size(ctypes.byref(args(**over)))
+
+    # 64 x 512 over 4,096: cut into parts, whose sums need the workspace.
+    need = status()
+    assert need > 0 and need % 256 == 0
+    assert call(ctypes.byref(args()), None) == -13  # no workspace given
+    assert call(ctypes.byref(args(workspace=0x10001,
+                                  workspace_bytes=need)), None) == -13
+    assert call(ctypes.byref(args(workspace=0x10000,
+                                  workspace_bytes=need - 1)), None) == -13
+    assert status(x=_abi_tensor((64, 4096), strides=(4100, 1))) > need
+    assert size(None) == _lib.ERR_NULL
+    assert status(x=_abi_tensor((64,))) == _lib.ERR_RANK
+    assert status(weight=_abi_tensor((512, 4095))) == _lib.ERR_SHAPE
+    assert status(y=_abi_tensor((64, 511))) == _lib.ERR_SHAPE
+    assert status(x=_abi_tensor((64, 4096), _lib.F64)) == _lib.ERR_DTYPE
+    assert status(weight=_abi_tensor((512, 4096), _lib.F16)) == _lib.ERR_DTYPE
+    assert status(bias=_abi_tensor((511,))) == _lib.ERR_SHAPE
+    assert status(residual=_abi_tensor((64, 512), _lib.F32)) == _lib.ERR_DTYPE
+    assert status(y=_abi_tensor((64, 512), addr=None)) == _lib.ERR_NULL
+    assert status(y=_abi_tensor((64, 512), strides=(512, 2))) == -12
+    assert status(y=_abi_tensor((64, 512), strides=(500, 1))) == -12
+    assert status(activation=5) == _lib.ERR_UNSUPPORTED
+    assert status(x=_abi_tensor((2**30, 4096)),
+                  y=_abi_tensor((2**30, 512))) == _lib.ERR_UNSUPPORTED
+    # A handful of rows needs none; nor does an empty product.
+    assert status(x=_abi_tensor((4, 4096)), y=_abi_tensor((4, 512))) == 0
+    assert status(x=_abi_tensor((0, 4096)), y=_abi_tensor((0, 512))) == 0
 
 
 # ---------------------------------------------------------------------------

@@ -171,7 +171,7 @@ struct GemmProblem {
   float* gate = nullptr;  // kEpiGated: g and u
   float* up = nullptr;
   int64_t gate_ld = 0, up_ld = 0;
-  unsigned int* err = nullptr;
+  unsigned int* err = nullptr;  // device error word (set at launch)
 };
 
 // Bump allocator over the caller's workspace. With no base it only counts,

@@ -19,6 +19,7 @@
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/library.h>
 
+#include <initializer_list>
 #include <optional>
 #include <string>
 #include <tuple>
@@ -916,6 +917,21 @@ struct BelowUnlessRecording {
   }
 };
 
+// What a backward pass has to know, in one number: which inputs want a
+// gradient, and the activation.
+int64_t pack_call(const std::string& activation,
+                  std::initializer_list<bool> wants) {
+  int64_t packed = int64_t(activation_of(activation)) << 8;
+  int i = 0;
+  for (const bool w : wants) packed |= int64_t(w) << i++;
+  return packed;
+}
+const char* activation_name(int64_t activation) {
+  static const char* const names[] = {"none", "relu", "gelu", "gelu_tanh",
+                                      "silu"};
+  return names[activation];
+}
+
 struct LinearFunction : public Function<LinearFunction> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x,
                         const Tensor& w, const OptTensor& bias,
@@ -927,26 +943,23 @@ struct LinearFunction : public Function<LinearFunction> {
     auto [y, pre] = call_linear(x, w, bias, residual, activation,
                                 layer && activation != "none");
     ctx->save_for_backward({x, w, pre});
-    ctx->saved_data["activation"] = activation;
-    ctx->saved_data["dx"] = wants_grad(x);
-    ctx->saved_data["dw"] = wants_grad(w);
-    ctx->saved_data["db"] = wants_grad(bias);
-    ctx->saved_data["dr"] = wants_grad(residual);
+    ctx->saved_data["call"] = pack_call(
+        activation, {wants_grad(x), wants_grad(w), wants_grad(bias),
+                     wants_grad(residual)});
     return y;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const auto saved = ctx->get_saved_variables();
-    const bool dx = ctx->saved_data["dx"].toBool();
-    const bool dw = ctx->saved_data["dw"].toBool();
-    const bool db = ctx->saved_data["db"].toBool();
-    const bool dr = ctx->saved_data["dr"].toBool();
+    const int64_t packed = ctx->saved_data["call"].toInt();
+    const bool dx = packed & 1, dw = packed & 2, db = packed & 4,
+               dr = packed & 8;
     variable_list out(5);
     if (!grads[0].defined()) return out;
     if (dx || dw || db) {
       BelowUnlessRecording below;
       auto [gx, gw, gb] = call_linear_backward(
-          grads[0], saved[0], saved[1], saved[2],
-          ctx->saved_data["activation"].toStringRef(), dx, dw, db);
+          grads[0], saved[0], saved[1], saved[2], activation_name(packed >> 8),
+          dx, dw, db);
       if (dx) out[0] = gx;
       if (dw) out[1] = gw;
       if (db) out[2] = gb;
@@ -970,24 +983,21 @@ struct GatedFunction : public Function<GatedFunction> {
     auto [h, gate, up] = call_gated(x, wg, wu, bg, bu, activation, save);
     ctx->save_for_backward({x, wg, wu, gate, up, bg.value_or(Tensor()),
                             bu.value_or(Tensor())});
-    ctx->saved_data["activation"] = activation;
-    const bool needs[5] = {wants_grad(x), wants_grad(wg), wants_grad(wu),
-                           wants_grad(bg), wants_grad(bu)};
-    int64_t mask = 0;
-    for (int i = 0; i < 5; ++i) mask |= int64_t(needs[i]) << i;
-    ctx->saved_data["mask"] = mask;
+    ctx->saved_data["call"] = pack_call(
+        activation, {wants_grad(x), wants_grad(wg), wants_grad(wu),
+                     wants_grad(bg), wants_grad(bu)});
     return h;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const auto s = ctx->get_saved_variables();
-    const int64_t mask = ctx->saved_data["mask"].toInt();
+    const int64_t mask = ctx->saved_data["call"].toInt();
     variable_list out(6);
     if (!grads[0].defined()) return out;
     BelowUnlessRecording below;
     auto [dx, dw, db] = call_gated_backward(
         grads[0], s[0], s[1], s[2], optional(s[5]), optional(s[6]), s[3],
-        s[4], ctx->saved_data["activation"].toStringRef(), (mask & 1) != 0,
-        (mask & 6) != 0, (mask & 24) != 0);
+        s[4], activation_name(mask >> 8), (mask & 1) != 0, (mask & 6) != 0,
+        (mask & 24) != 0);
     if (mask & 1) out[0] = dx;
     for (int i = 0; i < 2; ++i) {
       if (mask >> (1 + i) & 1) out[1 + i] = dw.select(0, i);
@@ -1011,17 +1021,15 @@ struct QkFunction : public Function<QkFunction> {
                             kw.value_or(Tensor()),
                             positions.value_or(Tensor())});
     ctx->saved_data["eps"] = eps;
-    ctx->saved_data["interleaved"] = interleaved;
-    ctx->saved_data["dq"] = wants_grad(q);
-    ctx->saved_data["dk"] = wants_grad(k);
-    ctx->saved_data["dqw"] = wants_grad(qw);
-    ctx->saved_data["dkw"] = wants_grad(kw);
+    ctx->saved_data["call"] =
+        pack_call("none", {wants_grad(q), wants_grad(k), wants_grad(qw),
+                           wants_grad(kw), interleaved});
     return {qo, ko};
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const auto s = ctx->get_saved_variables();
-    const bool dqw = ctx->saved_data["dqw"].toBool();
-    const bool dkw = ctx->saved_data["dkw"].toBool();
+    const int64_t packed = ctx->saved_data["call"].toInt();
+    const bool dqw = packed & 4, dkw = packed & 8;
     variable_list out(9);
     if (!grads[0].defined() && !grads[1].defined()) return out;
     BelowUnlessRecording below;
@@ -1033,9 +1041,9 @@ struct QkFunction : public Function<QkFunction> {
     auto [dq, dk, gqw, gkw] = call_qk_backward(
         gq, gk, s[0], s[1], s[2], s[3], optional(s[4]), optional(s[5]),
         optional(s[6]), ctx->saved_data["eps"].toDouble(),
-        ctx->saved_data["interleaved"].toBool(), dqw || dkw);
-    if (ctx->saved_data["dq"].toBool()) out[0] = dq;
-    if (ctx->saved_data["dk"].toBool()) out[1] = dk;
+        (packed & 16) != 0, dqw || dkw);
+    if (packed & 1) out[0] = dq;
+    if (packed & 2) out[1] = dk;
     if (dqw) out[4] = gqw;
     if (dkw) out[5] = gkw;
     return out;

@@ -41,17 +41,23 @@ __device__ __forceinline__ void split3(float x, __nv_bfloat16* hi,
   *lo = __float2bfloat16_rn(r - __bfloat162float(m));
 }
 
-// dst[plane][line][i], lines past `outer` zero; VEC elements per thread.
+// One operand's splitting: dst[plane][line][i], lines past `outer` zero.
+struct SplitJob {
+  const float* src;
+  int64_t s_outer, s_inner;
+  __nv_bfloat16* dst;
+  int64_t ld, outer, lines, inner;
+  int vec;  // eight elements per thread, else one
+};
+struct SplitJobs {
+  SplitJob job[4];
+};
+
 template <int VEC>
-__global__ void __launch_bounds__(256)
-    split_planes_kernel(const float* src, int64_t s_outer, int64_t s_inner,
-                        __nv_bfloat16* dst, int64_t ld, int64_t outer,
-                        int64_t lines, int64_t inner) {
-  allow_dependents();
-  grid_dependency_wait();
-  const int64_t per_line = (inner + VEC - 1) / VEC;
-  const int64_t total = lines * per_line;
-  const int64_t plane = lines * ld;
+__device__ __forceinline__ void split_operand(const SplitJob& j) {
+  const int64_t per_line = (j.inner + VEC - 1) / VEC;
+  const int64_t total = j.lines * per_line;
+  const int64_t plane = j.lines * j.ld;
   const int64_t step = int64_t(gridDim.x) * blockDim.x;
   for (int64_t e = int64_t(blockIdx.x) * blockDim.x + threadIdx.x; e < total;
        e += step) {
@@ -65,29 +71,43 @@ __global__ void __launch_bounds__(256)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (o < outer)
-          f = __ldg(reinterpret_cast<const float4*>(src + o * s_outer + i) +
-                    h);
+        if (o < j.outer)
+          f = __ldg(
+              reinterpret_cast<const float4*>(j.src + o * j.s_outer + i) + h);
         x[4 * h] = f.x;
         x[4 * h + 1] = f.y;
         x[4 * h + 2] = f.z;
         x[4 * h + 3] = f.w;
       }
     } else {
-      x[0] = o < outer ? src[o * s_outer + i * s_inner] : 0.f;
+      x[0] = o < j.outer ? j.src[o * j.s_outer + i * j.s_inner] : 0.f;
     }
 #pragma unroll
     for (int v = 0; v < VEC; ++v)
       split3(x[v], &q[0].e[v], &q[1].e[v], &q[2].e[v]);
 #pragma unroll
     for (int s = 0; s < 3; ++s) {
-      __nv_bfloat16* d = dst + s * plane + o * ld + i;
+      __nv_bfloat16* d = j.dst + s * plane + o * j.ld + i;
       if constexpr (VEC == 8)
         *reinterpret_cast<uint4*>(d) = q[s].u[0];
       else
         *d = q[s].e[0];
     }
   }
+}
+
+// Memory-bound: reads 4 bytes and writes 6 per element; all operands of a
+// product in one launch (blockIdx.y). 33 MB of x and a small weight take 12
+// us of the 51 of 65,536 x 128 x 256.
+__global__ void __launch_bounds__(256)
+    split_planes_kernel(const __grid_constant__ SplitJobs jobs) {
+  allow_dependents();
+  grid_dependency_wait();
+  const SplitJob& j = jobs.job[blockIdx.y];
+  if (j.vec)
+    split_operand<8>(j);
+  else
+    split_operand<1>(j);
 }
 
 bool aligned16(const void* p) {
@@ -137,29 +157,37 @@ cudaError_t pack(const MatView& m, int64_t rows, int64_t k, bool mn,
 
 // float32 to planes. The lines of a reduction are padded with zeros to whole
 // stages: a stage that ran past one plane would read the next.
-cudaError_t split_planes(const MatView& m, int64_t rows, int64_t k, bool mn,
-                         Workspace& ws, TmaOperand* out,
-                         cudaStream_t stream) {
-  const int64_t outer = mn ? k : rows, inner = mn ? rows : k;
-  const int64_t lines =
-      mn ? (k + kTcStep - 1) / kTcStep * kTcStep : rows;
-  const int64_t ld = (inner + 7) / 8 * 8;
-  auto* dst = static_cast<__nv_bfloat16*>(
-      ws.take(size_t(3) * lines * ld * 2));
-  *out = {dst, mn, ld, lines, 3};
-  if (ws.dry || ws.overflow) return cudaSuccess;
-  const int64_t s_outer = mn ? m.sk : m.sr, s_inner = mn ? m.sr : m.sk;
-  const bool vec = inner % 8 == 0 && (s_inner == 1 || inner == 1) &&
-                   aligned16(m.p) && (outer <= 1 || s_outer % 4 == 0);
-  const int64_t blocks = (lines * (inner / (vec ? 8 : 1) + 1) + 255) / 256;
+SplitJob split_planes(const MatView& m, int64_t rows, int64_t k, bool mn,
+                      Workspace& ws, TmaOperand* out) {
+  SplitJob j{};
+  j.outer = mn ? k : rows;
+  j.inner = mn ? rows : k;
+  j.lines = mn ? (k + kTcStep - 1) / kTcStep * kTcStep : rows;
+  j.ld = (j.inner + 7) / 8 * 8;
+  j.dst = static_cast<__nv_bfloat16*>(
+      ws.take(size_t(3) * j.lines * j.ld * 2));
+  j.src = static_cast<const float*>(m.p);
+  j.s_outer = mn ? m.sk : m.sr;
+  j.s_inner = mn ? m.sr : m.sk;
+  j.vec = j.inner % 8 == 0 && j.s_inner == 1 && aligned16(m.p) &&
+          (j.outer <= 1 || j.s_outer % 4 == 0);
+  *out = {j.dst, mn, j.ld, j.lines, 3};
+  return j;
+}
+
+cudaError_t launch_splits(const SplitJobs& jobs, int n, cudaStream_t stream) {
+  int64_t blocks = 1;
+  for (int i = 0; i < n; ++i) {
+    const SplitJob& j = jobs.job[i];
+    const int64_t need =
+        (j.lines * (j.inner / (j.vec ? 8 : 1) + 1) + 255) / 256;
+    if (need > blocks) blocks = need;
+  }
   const int64_t most = int64_t(device_sm_count()) * 16;
-  const dim3 grid(unsigned(blocks < most ? blocks : most));
-  const float* src = static_cast<const float*>(m.p);
-  const cudaError_t e =
-      vec ? launch_pdl(split_planes_kernel<8>, grid, dim3(256), 0, stream,
-                       src, s_outer, s_inner, dst, ld, outer, lines, inner)
-          : launch_pdl(split_planes_kernel<1>, grid, dim3(256), 0, stream,
-                       src, s_outer, s_inner, dst, ld, outer, lines, inner);
+  const cudaError_t e = launch_pdl(
+      split_planes_kernel,
+      dim3(unsigned(blocks < most ? blocks : most), unsigned(n)), dim3(256),
+      0, stream, jobs);
   if (e == cudaSuccess) count_launches(1);
   return e;
 }
@@ -189,6 +217,8 @@ cudaError_t run_gemm_tc(const GemmProblem& p, const TcShape& shape,
   // Both A's (and both B's) of a call are staged in one form.
   const int n_a = p.segments, n_b = gated ? 2 : p.segments;
   TmaOperand op[4];
+  SplitJobs jobs{};
+  int n_jobs = 0;
   for (int side = 0; side < 2; ++side) {
     const MatView* v = side ? p.b : p.a;
     const int n = side ? n_b : n_a;
@@ -200,7 +230,7 @@ cudaError_t run_gemm_tc(const GemmProblem& p, const TcShape& shape,
       TmaOperand* o = &op[2 * side + i];
       cudaError_t e = cudaSuccess;
       if (f32)
-        e = split_planes(v[i], rows, p.K, mn, ws, o, stream);
+        jobs.job[n_jobs++] = split_planes(v[i], rows, p.K, mn, ws, o);
       else if (describable(v[i], rows, p.K, mn))
         *o = {v[i].p, mn, mn ? v[i].sk : v[i].sr, mn ? p.K : rows, 1};
       else
@@ -216,6 +246,12 @@ cudaError_t run_gemm_tc(const GemmProblem& p, const TcShape& shape,
     g.partial = static_cast<float*>(ws.take(
         size_t(g.split) * (gated ? 2 : 1) * p.M * p.N * sizeof(float)));
   if (ws.dry || ws.overflow) return cudaSuccess;
+  if (f32) {
+    const cudaError_t e = launch_splits(jobs, n_jobs, stream);
+    if (e != cudaSuccess) return e;
+  }
+  g.p.err = device_error_ptr();
+  if (g.p.err == nullptr) return cudaErrorNotSupported;
 
   const int64_t es = f32 ? 4 : 2;
   g.vec_res = p.N * es % 16 == 0 && p.res_sn == 1 && aligned16(p.res) &&

@@ -9,7 +9,9 @@
 // thread keeps the sums of its columns in float32 (from the unrounded dz),
 // the warps' sums are joined in shared memory and written per chunk, and a
 // second kernel adds the chunks in order, so the result does not depend on
-// scheduling.
+// scheduling. Measured (B200): gated, 66,560 x 704 bf16, 106 us for 656 MB (6.2
+// TB/s, 0.95 of the copy rate) with the sums; rows' loads one at a time took
+// 203.
 #include "block_common.cuh"
 
 namespace vectra {

@@ -1,5 +1,5 @@
-// gemm_tc_kernel.cuh: the matrix products of the transformer-block operators in
-// bf16 / f16 on the 5th-generation tensor cores (tcgen05 + TMEM).
+// gemm_tc_kernel.cuh: the matrix products of the transformer-block operators
+// on the 5th-generation tensor cores (tcgen05 + TMEM).
 //
 //   acc[m, n] = sum over segments s, k of a[s](m, k) b[s](n, k)
 //
@@ -20,9 +20,8 @@
 //    only). Two accumulators in TMEM, so the next tile's product runs during
 //    this one's epilogue.
 //  * the other warps are the epilogue: two or four per TMEM lane quarter,
-//    which share its columns. A lane holds one row;
-//    results are packed and turned through shared memory so that global
-//    loads (the residual) and stores run along rows.
+//    which share its columns. A lane holds one row; results are packed and
+//    turned through shared memory, from where the copy engine stores them.
 // A gated layer's B tile is BN / 2 gate rows and the same BN / 2 up rows:
 // one MMA makes both projections, and the epilogue finds both factors of an
 // output in its row.
@@ -36,6 +35,12 @@
 // A reduction too long for its few tiles is cut into parts that write
 // float32 sums to the workspace; launch_split_finish adds them in order.
 // Every wait is bounded (error word and early exit).
+//
+// Measured (B200): 8,191 x 4096 -> 4096 f16 with a whole epilogue 187-202 us,
+// 1.4 PFLOP/s, 0.87 of the library's burst rate, the tensor pipe 91 % busy;
+// gated 8,192 x 4096 -> 10240 840 us, 1.64 PFLOP/s. With a reduction of 256
+// the results bound it: 66,560 x 256 -> 1024 bare 39 us (3.5 TB/s of writes,
+// a fill's rate), with bias and GELU 63.
 #pragma once
 
 #include <atomic>
@@ -59,10 +64,10 @@ template <int BN, int CG, bool F32>
 struct Cfg {
   // Epilogue warps: each TMEM lane quarter (a warp reads the quarter of its
   // index modulo 4) is shared by EPI_WARPS / 4 of them, with at least 32
-  // accumulator columns each. Four per scheduler at
-  // BN = 256: an epilogue with an activation is bound by instruction
-  // latency (two per scheduler issued on 39 % of cycles and took 109 us for
-  // 66,560 x 256 x 1,024 with GELU).
+  // accumulator columns each. Four per scheduler at BN = 256: an epilogue
+  // with an activation is bound by instruction latency (66,560 x 256 -> 1024
+  // with GELU took 109 us with two, which issued on 39 % of cycles, and 95
+  // with four).
   static constexpr int EPI_WARPS = BN == 256 ? 16 : 8;
   static constexpr int THREADS = (kCtrlWarps + EPI_WARPS) * 32;
   static constexpr int B_ROWS = BN / CG;  // rows of B staged per CTA
@@ -675,8 +680,8 @@ __device__ __forceinline__ void add_bias(float* v, const float* cols) {
 // and gives the TMEM address of the warp's rows and first column, `release`
 // gives it back after the last read. What a call does not need is compiled out: with
 // the residual, the saved values and the partial sums behind run-time
-// branches the values were copied between registers at every join, 10
-// instructions for each result where the bare store takes 6.
+// branches the values were copied between registers at every join: 10
+// instructions for each result where the bare store took 6.
 template <int EPI, int ACT, bool RES, bool PRE, typename T, int TILE_N,
           int WARP_COLS, typename Wait, typename Release>
 __device__ __forceinline__ void epilogue_tile(const TcArgs& g,

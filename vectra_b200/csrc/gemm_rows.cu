@@ -1,8 +1,7 @@
 // gemm_rows.cu: the products of a serving step, act(x W^T + b) + r or the
-// gated layer for up to eight rows of x.
+// gated layer for a few rows of x, eight at a time.
 //
-// Bound by reading the weights once: 2 N K bytes against 2 M N K operations
-// with M <= 8. There is no reuse to stage for, so the weights go straight
+// Bound by reading the weights: 2 N K bytes against 16 N K operations. There is no reuse to stage for, so the weights go straight
 // from global memory into mma.sync operands: in m16n8k16 the weight rows are
 // the 16 rows, the tokens the 8 columns, and since a sum may run over the
 // reduction in any order, a lane's 16-byte load (eight neighbours of one
@@ -17,8 +16,8 @@
 // flight, which covers DRAM latency at full rate. Measured (B200): the gated
 // layer of one token, 4096 -> 10240, 27.8 us (6.0 TB/s, 0.92 of the copy
 // rate), 8 x 4096 -> 4096 8.0 us (33 MB: 4.2 TB/s, start and join included);
-// the tensor-core kernel takes 48 and 13. From 9 rows on that one is as fast
-// (16 rows 10.7 us; this kernel with two token tiles took 12.7).
+// the tensor-core kernel takes 48 and 13. (Two token tiles per pass, for 16
+// rows, took 12.7 us where that kernel takes 10.1.)
 #include "block_common.cuh"
 #include "gemm_rows.cuh"
 #include "mma_sync.cuh"
@@ -58,17 +57,18 @@ __device__ __forceinline__ float act_any(float z, int act) {
 // The warps' sums, added in order, and the epilogue: one output per thread.
 template <typename T, bool GATED>
 __device__ __forceinline__ void finish_rows(
-    const GemmProblem& p, const float (*sums)[kTokens][16 + 1], int64_t n0) {
+    const GemmProblem& p, const float (*sums)[kTokens][16 + 1], int64_t n0,
+    int64_t m0) {
   constexpr int kCols = GATED ? 8 : 16;
   constexpr bool kExact = std::is_same<T, float>::value;
-  const int m = threadIdx.x / kCols, r = threadIdx.x % kCols;
-  const int64_t n = n0 + r;
-  if (m >= p.M || m >= kTokens || n >= p.N) return;
+  const int t = threadIdx.x / kCols, r = threadIdx.x % kCols;
+  const int64_t n = n0 + r, m = m0 + t;
+  if (m >= p.M || t >= kTokens || n >= p.N) return;
   float z = 0.f, u = 0.f;
 #pragma unroll
   for (int w = 0; w < kWarps; ++w) {
-    z += sums[w][m][r];
-    if constexpr (GATED) u += sums[w][m][8 + r];
+    z += sums[w][t][r];
+    if constexpr (GATED) u += sums[w][t][8 + r];
   }
   if (p.bias[0])
     z += to_f32(static_cast<const T*>(p.bias[0])[n * p.bias_stride[0]]);
@@ -116,9 +116,10 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
     wok[h] = n < p.N;
     wp[h] = static_cast<const T*>(w.p) + (wok[h] ? n : 0) * w.sr + t * 8;
   }
-  const bool xok = g < p.M;
-  const T* xp =
-      static_cast<const T*>(p.a[0].p) + (xok ? g : 0) * p.a[0].sr + t * 8;
+  const int64_t m0 = int64_t(blockIdx.y) * kTokens;
+  const bool xok = m0 + g < p.M;
+  const T* xp = static_cast<const T*>(p.a[0].p) +
+                (xok ? m0 + g : 0) * p.a[0].sr + t * 8;
 
   float acc[4] = {0.f, 0.f, 0.f, 0.f};
   for (int64_t step = s0; step < s1; step += kDepth) {
@@ -147,7 +148,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
   for (int c = 0; c < 4; ++c)
     sums[warp][2 * t + (c & 1)][g + 8 * (c >> 1)] = acc[c];
   __syncthreads();
-  finish_rows<T, GATED>(p, sums, n0);
+  finish_rows<T, GATED>(p, sums, n0, m0);
 }
 
 // The same for float32, on the FP32 pipe: a lane's 16 bytes are four
@@ -178,11 +179,12 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
     wp[h] = static_cast<const float*>(w.p) + (wok[h] ? n : 0) * w.sr + t * 4;
   }
   // Tokens past M repeat the last one; nothing of theirs is written.
+  const int64_t m0 = int64_t(blockIdx.y) * kTokens;
   const float* xp[TOKENS];
 #pragma unroll
   for (int m = 0; m < TOKENS; ++m)
     xp[m] = static_cast<const float*>(p.a[0].p) +
-            (m < p.M ? m : p.M - 1) * p.a[0].sr + t * 4;
+            (m0 + m < p.M ? m0 + m : p.M - 1) * p.a[0].sr + t * 4;
   float acc[2][TOKENS];
 #pragma unroll
   for (int m = 0; m < TOKENS; ++m) acc[0][m] = acc[1][m] = 0.f;
@@ -231,7 +233,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
       if (t == 0) sums[warp][m][g + 8 * h] = v;
     }
   __syncthreads();
-  finish_rows<float, GATED>(p, sums, n0);
+  finish_rows<float, GATED>(p, sums, n0, m0);
 }
 
 bool line_view(const MatView& m, int64_t rows, int64_t es) {
@@ -241,9 +243,25 @@ bool line_view(const MatView& m, int64_t rows, int64_t es) {
 
 }  // namespace
 
+// Up to eight rows read the weights once and always run here. More rows take
+// passes over them, which still beats the tensor-core kernel's start and
+// second launch while the blocks' work is small. B200, us, here against
+// there: bf16 32 x 1024 -> 1024 3.1 and 5.9, 64 x 1024 -> 1024 5.3 and 6.0,
+// 32 x 1472 -> 1984 6.0 and 7.4, 64 x 1472 -> 1984 9.7 and 7.4, 16 x 4096 ->
+// 4096 13.5 and 10.1; f32, whose other kernel also splits its operands first,
+// 16 x 4096 -> 4096 41 and 56, 32 x 1024 -> 1024 6.2 and 11.5, 32 x 1472 ->
+// 1984 16.1 and 15.2.
 bool gemm_rows_supports(const GemmProblem& p) {
-  const int64_t es = p.dtype == VECTRA_F32 ? 4 : 2;
-  if (p.M > kRowsMost || p.segments != 1 || p.K * es % 16 != 0) return false;
+  const bool f32 = p.dtype == VECTRA_F32;
+  const int64_t es = f32 ? 4 : 2;
+  if (p.segments != 1 || p.K * es % 16 != 0) return false;
+  if (p.M > (f32 ? 2 * kTokens : kTokens)) {
+    const int64_t cols = p.epilogue == kEpiGated ? 8 : 16;
+    const int64_t blocks =
+        ((p.N + cols - 1) / cols) * ((p.M + kTokens - 1) / kTokens);
+    if (p.M > kRowsMost || blocks * p.K > (f32 ? 400000 : 800000))
+      return false;
+  }
   return line_view(p.a[0], p.M, es) && line_view(p.b[0], p.N, es) &&
          (p.epilogue != kEpiGated || line_view(p.b[1], p.N, es));
 }
@@ -251,7 +269,9 @@ bool gemm_rows_supports(const GemmProblem& p) {
 cudaError_t launch_gemm_rows(const GemmProblem& p, cudaStream_t stream) {
   const bool gated = p.epilogue == kEpiGated;
   const int64_t cols = gated ? 8 : 16;
-  const dim3 grid(unsigned((p.N + cols - 1) / cols)), block(kWarps * 32);
+  const dim3 grid(unsigned((p.N + cols - 1) / cols),
+                  unsigned((p.M + kTokens - 1) / kTokens));
+  const dim3 block(kWarps * 32);
   auto run = [&](auto kernel) {
     return launch_pdl(kernel, grid, block, 0, stream, p);
   };

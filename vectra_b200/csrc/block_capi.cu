@@ -75,6 +75,9 @@ int check_common(const vectra_tensor& x, const vectra_tensor& w,
   return VECTRA_OK;
 }
 
+// Above the few-row kernel's sizes, float32 gradients are split once.
+constexpr int64_t kSplitOnceRows = 64;
+
 // Rows of the gradients in the workspace start on 16-byte boundaries, which
 // the tensor-core products need.
 int64_t pad8(int64_t n) { return (n + 7) / 8 * 8; }
@@ -155,6 +158,12 @@ int linear_backward(const vectra_linear_grad_args& a, Workspace& ws,
     g.db = const_cast<void*>(a.dbias.data);
     VECTRA_TRY(to_status(run_grad(g, ws, stream), ws));
   }
+  // float32: dz is split once for both products.
+  if (dt == VECTRA_F32 && present(a.dx) && present(a.dweight) &&
+      M > kSplitOnceRows && N > 0 && K > 0)
+    VECTRA_TRY(to_status(
+        split_for_products(dz_rows.p, M, N, dz_rows.sr, dz_rows.sk, ws,
+                           &dz_rows, &dz_cols, stream), ws));
   GemmProblem p;
   p.dtype = dt;
   p.epilogue = kEpiStore;
@@ -321,6 +330,21 @@ int gated_backward(const vectra_gated_grad_args& a, Workspace& ws,
     g.db2 = db2;
     VECTRA_TRY(to_status(run_grad(g, ws, stream), ws));
   }
+  MatView dg_rows{d, ld, 1}, du_rows{d2, ld, 1};
+  MatView dg_cols{d, 1, ld}, du_cols{d2, 1, ld};
+  if (dt == VECTRA_F32 && present(a.dx) && present(a.dw_gate) &&
+      M > kSplitOnceRows && F > 0 && K > 0) {
+    // dg and du are split once for both products, as one matrix.
+    VECTRA_TRY(to_status(
+        split_for_products(d, M, ld, ld, 1, ws, &dg_rows, &dg_cols, stream),
+        ws));
+    const int64_t half = ld / 2 * 2;  // bytes of a bf16 row's half
+    du_rows = dg_rows;
+    du_cols = dg_cols;
+    du_rows.p = dg_rows.p ? static_cast<const char*>(dg_rows.p) + half
+                          : nullptr;
+    du_cols.p = du_rows.p;
+  }
   GemmProblem p;
   p.dtype = dt;
   p.epilogue = kEpiStore;
@@ -329,8 +353,8 @@ int gated_backward(const vectra_gated_grad_args& a, Workspace& ws,
     p.N = K;
     p.K = F;
     p.segments = 2;
-    p.a[0] = {d, ld, 1};
-    p.a[1] = {d2, ld, 1};
+    p.a[0] = dg_rows;
+    p.a[1] = du_rows;
     p.b[0] = cols_of(a.w_gate);
     p.b[1] = cols_of(a.w_up);
     p.out = const_cast<void*>(a.dx.data);
@@ -351,7 +375,7 @@ int gated_backward(const vectra_gated_grad_args& a, Workspace& ws,
       p.M = joined ? 2 * F : F;
       p.N = K;
       p.K = M;
-      p.a[0] = {i ? d2 : d, 1, ld};
+      p.a[0] = i ? du_cols : dg_cols;
       p.b[0] = cols_of(a.x);
       p.out = const_cast<void*>(out[i]->data);
       p.out_ld = out[i]->stride[0];

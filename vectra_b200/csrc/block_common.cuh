@@ -140,6 +140,9 @@ cudaError_t with_dtype(int dtype, F&& f) {
 struct MatView {
   const void* p = nullptr;
   int64_t sr = 0, sk = 0;
+  // float32 split beforehand (split_for_products): p holds three bf16 planes
+  // of this many lines, in the order of the view's own rows in memory.
+  int64_t plane_lines = 0;
 };
 
 // What happens to acc[m, n].
@@ -196,6 +199,15 @@ struct Workspace {
 
 // Runs (or, when ws.dry, sizes) one product; picks the kernel.
 cudaError_t run_gemm(const GemmProblem& p, Workspace& ws, cudaStream_t stream);
+
+// A float32 matrix [lines][inner] (rows `ld` apart, unit inner stride) split
+// into planes once for several products; returns it as the operand that
+// reduces over the lines (`cols`) and the one that reduces over the inner
+// dimension (`rows`).
+cudaError_t split_for_products(const void* p, int64_t lines, int64_t inner,
+                               int64_t s_line, int64_t s_inner, Workspace& ws,
+                               MatView* rows, MatView* cols,
+                               cudaStream_t stream);
 
 // gemm_finish.cu: `partial` holds [split][M][N] float32 sums (for kEpiGated
 // [split][2][M][N]).

@@ -254,7 +254,8 @@ bool line_view(const MatView& m, int64_t rows, int64_t es) {
 bool gemm_rows_supports(const GemmProblem& p) {
   const bool f32 = p.dtype == VECTRA_F32;
   const int64_t es = f32 ? 4 : 2;
-  if (p.segments != 1 || p.K * es % 16 != 0) return false;
+  if (p.segments != 1 || p.K * es % 16 != 0 || p.a[0].plane_lines)
+    return false;
   if (p.M > (f32 ? 2 * kTokens : kTokens)) {
     const int64_t cols = p.epilogue == kEpiGated ? 8 : 16;
     const int64_t blocks =

@@ -194,6 +194,21 @@ cudaError_t launch_splits(const SplitJobs& jobs, int n, cudaStream_t stream) {
 
 }  // namespace
 
+cudaError_t split_for_products(const void* p, int64_t lines, int64_t inner,
+                               int64_t s_line, int64_t s_inner, Workspace& ws,
+                               MatView* rows, MatView* cols,
+                               cudaStream_t stream) {
+  SplitJobs jobs{};
+  TmaOperand o;
+  // As an operand reduced over the lines, whose padding both uses can share.
+  jobs.job[0] =
+      split_planes({p, s_inner, s_line}, inner, lines, true, ws, &o);
+  *rows = {o.p, o.ld, 1, o.lines};
+  *cols = {o.p, 1, o.ld, o.lines};
+  if (ws.dry || ws.overflow) return cudaSuccess;
+  return launch_splits(jobs, 1, stream);
+}
+
 cudaError_t run_gemm_tc(const GemmProblem& p, const TcShape& shape,
                         Workspace& ws, cudaStream_t stream) {
   const bool gated =
@@ -229,7 +244,9 @@ cudaError_t run_gemm_tc(const GemmProblem& p, const TcShape& shape,
     for (int i = 0; i < n; ++i) {
       TmaOperand* o = &op[2 * side + i];
       cudaError_t e = cudaSuccess;
-      if (f32)
+      if (v[i].plane_lines)
+        *o = {v[i].p, mn, mn ? v[i].sk : v[i].sr, v[i].plane_lines, 3};
+      else if (f32)
         jobs.job[n_jobs++] = split_planes(v[i], rows, p.K, mn, ws, o);
       else if (describable(v[i], rows, p.K, mn))
         *o = {v[i].p, mn, mn ? v[i].sk : v[i].sr, mn ? p.K : rows, 1};
@@ -246,7 +263,7 @@ cudaError_t run_gemm_tc(const GemmProblem& p, const TcShape& shape,
     g.partial = static_cast<float*>(ws.take(
         size_t(g.split) * (gated ? 2 : 1) * p.M * p.N * sizeof(float)));
   if (ws.dry || ws.overflow) return cudaSuccess;
-  if (f32) {
+  if (n_jobs > 0) {
     const cudaError_t e = launch_splits(jobs, n_jobs, stream);
     if (e != cudaSuccess) return e;
   }

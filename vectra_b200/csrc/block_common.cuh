@@ -17,7 +17,8 @@
 namespace vectra {
 
 // ---------------------------------------------------------------------------
-// Activations. kExact: CUDA's expf / erff / tanhf, for float32 tensors.
+// Activations. kExact: CUDA's expf / erff / tanhf, for float32 tensors
+// outside the tensor-core epilogue (which has its own, gemm_tc_kernel.cuh).
 // Otherwise forms on ex2.approx and rcp.approx whose error (below 1e-6
 // absolute) is far under the rounding of the 16-bit results.
 // ---------------------------------------------------------------------------

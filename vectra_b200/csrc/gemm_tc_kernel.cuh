@@ -240,7 +240,8 @@ __device__ __forceinline__ void dealloc_cols(uint32_t addr, uint32_t cols) {
 // so a value costs 1.5 MUFU operations instead of 2. z is capped from below
 // (NaN kept) where x reaches 63, so that ab stays finite; the result there
 // is within 3e-10 of the activation, and -infinity gives that, not NaN.
-// Packed multiplications and additions halve the instructions.
+// float32 results take the same forms: their error is below that of the
+// product before them. Packed multiplications and additions halve the instructions.
 // ---------------------------------------------------------------------------
 __device__ __forceinline__ float max_nan(float a, float b) {
   float r;

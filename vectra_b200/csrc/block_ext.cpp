@@ -904,6 +904,20 @@ using torch::autograd::variable_list;
 bool wants_grad(const Tensor& t) { return t.defined() && t.requires_grad(); }
 bool wants_grad(const OptTensor& t) { return has(t) && t->requires_grad(); }
 
+bool has_tangent(const Tensor& t) {
+  return t.defined() && t._fw_grad(/*level=*/0).defined();
+}
+bool has_tangent(const OptTensor& t) { return has(t) && has_tangent(*t); }
+
+// The operators have no forward-mode formula; below autograd a tangent would
+// be dropped, which reads as zero.
+template <typename... Args>
+void refuse_tangents(const char* op, const Args&... args) {
+  TORCH_CHECK_NOT_IMPLEMENTED(
+      !(has_tangent(args) || ...), "vectra_b200::", op,
+      ": forward-mode differentiation is not implemented");
+}
+
 OptTensor optional(const Tensor& t) {
   return t.defined() ? OptTensor(t) : OptTensor();
 }
@@ -1053,6 +1067,7 @@ struct QkFunction : public Function<QkFunction> {
 Tensor linear_autograd(const Tensor& x, const Tensor& w,
                        const OptTensor& bias, const OptTensor& residual,
                        c10::string_view activation) {
+  refuse_tangents("linear", x, w, bias, residual);
   if (at::GradMode::is_enabled() &&
       (wants_grad(x) || wants_grad(w) || wants_grad(bias) ||
        wants_grad(residual)))
@@ -1065,6 +1080,7 @@ Tensor linear_autograd(const Tensor& x, const Tensor& w,
 Tensor gated_autograd(const Tensor& x, const Tensor& wg, const Tensor& wu,
                       const OptTensor& bg, const OptTensor& bu,
                       c10::string_view activation) {
+  refuse_tangents("gated_linear", x, wg, wu, bg, bu);
   if (at::GradMode::is_enabled() &&
       (wants_grad(x) || wants_grad(wg) || wants_grad(wu) || wants_grad(bg) ||
        wants_grad(bu)))
@@ -1077,6 +1093,7 @@ std::tuple<Tensor, Tensor> qk_autograd(
     const Tensor& q, const Tensor& k, const Tensor& cos, const Tensor& sin,
     const OptTensor& qw, const OptTensor& kw, const OptTensor& positions,
     double eps, bool interleaved) {
+  refuse_tangents("qk_norm_rope", q, k, cos, sin, qw, kw);
   if (at::GradMode::is_enabled() && (wants_grad(q) || wants_grad(k) ||
                                      wants_grad(qw) || wants_grad(kw))) {
     auto out = QkFunction::apply(q, k, cos, sin, qw, kw, positions, eps,

@@ -7,8 +7,10 @@ Tolerances are those of test_block.py unless a test derives its own.
 import pytest
 import torch
 
+from tests.test_block import ACTS
 from tests.test_block import DEVICES
 from tests.test_block import Rand
+from tests.test_block import TYPES
 from vectra_b200 import block
 
 
@@ -52,3 +54,56 @@ def test_forward_mode_is_refused(device, op, grad):
                 torch.func.jacfwd(one)(t)
         # Outside the level the same tensors run.
         fun(*args)
+
+
+# ---------------------------------------------------------------------------
+# Values that are not finite
+# ---------------------------------------------------------------------------
+# (rows, K, N) of a few rows, one CTA's tiles, a reduction in parts, and CTA
+# pairs (16-bit types); odd columns among them.
+KERNELS = [(4, 64, 72), (150, 64, 520), (130, 4096, 96), (2570, 192, 1032),
+           (70, 72, 33)]
+
+
+def _others_equal(got, clean, columns, dim, what):
+    """All of `dim` but `columns` as without the special values."""
+    keep = [i for i in range(clean.shape[dim]) if i not in columns]
+    index = torch.tensor(keep, device=got.device)
+    assert torch.equal(got.index_select(dim, index),
+                       clean.index_select(dim, index)), what
+
+
+@pytest.mark.parametrize('device', DEVICES)
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('act', ACTS)
+@pytest.mark.parametrize('size', KERNELS)
+def test_nan_stays_in_its_column(device, dtype, act, size):
+    """NaN in one weight row and in one bias entry: those columns only, in
+    the result and in the gradients of the parameters."""
+    m, k, n = size
+    rand = Rand(m + k + n, device, dtype)
+    x, dy = rand(m, k), rand(m, n)
+    w, b = rand(n, k, scale=k**-0.5), rand(n)
+    wu, bu = rand(n, k, scale=k**-0.5), rand(n)
+    bad = (3, 6)
+
+    def linear(*leaves):
+        leaves = [t.clone().requires_grad_() for t in leaves]
+        y = block.linear(x, *leaves, activation=act)
+        return (y, *torch.autograd.grad(y, leaves, dy))
+
+    def gated(*leaves):
+        leaves = [t.clone().requires_grad_() for t in leaves]
+        h = block.gated_linear(x, leaves[0], leaves[2], leaves[1], leaves[3],
+                               act)
+        return (h, *torch.autograd.grad(h, leaves, dy))
+
+    clean, clean_h = linear(w, b), gated(w, b, wu, bu)
+    w[bad[0], k // 2] = float('nan')
+    b[bad[1]] = float('nan')
+    for got, want, what in ((linear(w, b), clean, 'linear'),
+                            (gated(w, b, wu, bu), clean_h, 'gated')):
+        assert got[0][:, list(bad)].isnan().all(), what
+        _others_equal(got[0], want[0], bad, 1, what)
+        for i in range(1, len(got)):
+            _others_equal(got[i], want[i], bad, 0, f'{what} gradient {i}')

@@ -236,9 +236,9 @@ __device__ __forceinline__ void dealloc_cols(uint32_t addr, uint32_t cols) {
 // 0.044715 z^3), and gelu g = logit(Phi(z)) = z Q(z^2) with a polynomial Q
 // fitted on |z| <= 5 for the least error of the result (7e-8; beyond, its
 // leading term keeps driving the sigmoid to 0 or 1). With x = -g log2(e),
-// sigmoid = 1 / (1 + 2^x); two of them share one reciprocal, 1/a = b / (ab),
-// so a value costs 1.5 MUFU operations instead of 2. z is capped from below
-// (NaN kept) where x reaches 63, so that ab stays finite; the result there
+// sigmoid = 1 / (1 + 2^x). Each value has a reciprocal of its own: one for
+// two, 1/a = b / (ab), would carry a NaN into the neighbouring column. z is
+// capped from below (NaN kept) where x reaches 63; the result there
 // is within 3e-10 of the activation, and -infinity gives that, not NaN.
 // float32 results take the same forms: their error is below that of the
 // product before them. Packed multiplications and additions halve the instructions.
@@ -290,10 +290,8 @@ __device__ __forceinline__ void sigmoid2(float& z0, float& z1, float& s0,
     }
   }
   const float2 xs = f2upk(x);
-  const float a = 1.f + fast_exp2(xs.x), b = 1.f + fast_exp2(xs.y);
-  const float r = fast_rcp(a * b);
-  s0 = b * r;
-  s1 = a * r;
+  s0 = fast_rcp(1.f + fast_exp2(xs.x));
+  s1 = fast_rcp(1.f + fast_exp2(xs.y));
 }
 
 template <int ACT>

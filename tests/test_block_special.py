@@ -10,7 +10,14 @@ import torch
 from tests.test_block import ACTS
 from tests.test_block import DEVICES
 from tests.test_block import Rand
+from tests.test_block import TINY
 from tests.test_block import TYPES
+from tests.test_block import U
+from tests.test_block import act64
+from tests.test_block import close
+from tests.test_block import d
+from tests.test_block import slope64
+from tests.test_block import sums
 from vectra_b200 import block
 
 
@@ -107,3 +114,58 @@ def test_nan_stays_in_its_column(device, dtype, act, size):
         _others_equal(got[0], want[0], bad, 1, what)
         for i in range(1, len(got)):
             _others_equal(got[i], want[i], bad, 0, f'{what} gradient {i}')
+
+
+def _close_or_past(got, want, bound, what):
+    """`close`; what lies past the type's range is infinite (within its bound
+    of the edge it may be either)."""
+    most = torch.finfo(got.dtype).max
+    sure = want.abs() - bound > most
+    near = want.abs() + bound < most
+    assert torch.equal(d(got)[sure], want[sure].sign() * float('inf')), what
+    close(got[near], want[near], bound[near], what)
+
+
+@pytest.mark.parametrize('device', DEVICES)
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('act', ACTS)
+@pytest.mark.parametrize('rows', [40, 300])
+@pytest.mark.parametrize('saved', [False, True])
+def test_slopes_far_out(device, dtype, act, rows, saved):
+    """Gates of up to 1e4 either side of zero, beside ordinary ones. The
+    weights are zero, so the gates are the biases, exactly, and the slope is
+    off by the 4e-6 (its float32 form), act by 2e-6 of the gate."""
+    u = U[dtype]
+    rand = Rand(rows, device, dtype)
+    far = [50., 100., 1e3, 1e4, 25., 12., 7., -7., -12., -50., -1e3, -1e4]
+    gates = torch.tensor([v for f in far for v in (f, -0.7, f, 2.5, f, 6.)])
+    bg = gates.to(device, dtype)
+    n, k = bg.numel(), 64
+    x, dh = rand(rows, k), rand(rows, n)
+    zero = x.new_zeros(n, k)
+    bu = torch.full_like(bg, 0.75)
+    ops = torch.ops.vectra_b200
+    h, gate, up = ops.gated_linear_with_pre(x, zero, zero, bg, bu, act, True)
+    if not saved:
+        gate, up = gate.new_empty(0), up.new_empty(0)
+    _, dw, db = ops.gated_linear_backward(dh, x, zero, zero, bg, bu, gate, up,
+                                          act, True, True, True)
+    g, dy = d(bg).expand(rows, n), d(dh)
+    a, slope = act64(g, act), slope64(g, act)
+    ab = 2e-6 * g.abs().clamp(min=1)
+    tiny = TINY[dtype]
+    close(h, 0.75 * a, 0.75 * ab * (1 + u) + u * 0.75 * a.abs() + tiny, 'h')
+    for i, (want, off) in enumerate(((dy * 0.75 * slope,
+                                      dy.abs() * 0.75 * 4e-6),
+                                     (dy * a, dy.abs() * ab))):
+        spread = off.sum(0) + sums(rows) * want.abs().sum(0)
+        total = want.sum(0)
+        _close_or_past(db[i], total,
+                       spread * (1 + u) + u * total.abs() + tiny, 'db')
+        # As rounded for the product.
+        off = off * (1 + u) + u * want.abs() + tiny
+        total = want.t() @ d(x)
+        spread = off.t() @ d(x).abs() + sums(rows) * (
+            want.abs().t() @ d(x).abs())
+        _close_or_past(dw[i], total,
+                       spread * (1 + u) + u * total.abs() + tiny, 'dw')

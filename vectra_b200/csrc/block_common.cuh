@@ -33,6 +33,15 @@ __device__ __forceinline__ float sigmoid_f(float z) {
   if constexpr (kExact) return 1.f / (1.f + expf(-z));
   return fast_rcp(1.f + fast_exp2(-kLog2e * z));
 }
+// The same, and in `rest` 1 - sigmoid without the difference's cancellation,
+// which the slopes would multiply by z or z^3.
+template <bool kExact>
+__device__ __forceinline__ float sigmoid_f(float z, float* rest) {
+  const float e = kExact ? expf(-z) : fast_exp2(-kLog2e * z);
+  const float s = kExact ? 1.f / (1.f + e) : fast_rcp(1.f + e);
+  *rest = fminf(e, 0x1p126f) * s;  // s is 0 where e is infinite
+  return s;
+}
 
 constexpr float kGeluTanhC = 0.7978845608028654f;  // sqrt(2 / pi)
 constexpr float kGeluTanhA = 0.044715f;
@@ -81,9 +90,10 @@ __device__ __forceinline__ float act_grad(float z, float* value) {
     *value = z > 0.f || z != z ? z : 0.f;
     return z > 0.f ? 1.f : 0.f;
   } else if constexpr (ACT == VECTRA_ACT_SILU) {
-    const float s = sigmoid_f<kExact>(z);
+    float rest;
+    const float s = sigmoid_f<kExact>(z, &rest);
     *value = z * s;
-    return s * (1.f + z * (1.f - s));
+    return s * (1.f + z * rest);
   } else if constexpr (ACT == VECTRA_ACT_GELU) {
     float phi, e;
     if constexpr (kExact) {
@@ -99,10 +109,11 @@ __device__ __forceinline__ float act_grad(float z, float* value) {
     // the product 0 * z^2 finite.
     const float c = fminf(fmaxf(z, -100.f), 100.f);
     const float u = kGeluTanhC * fmaf(kGeluTanhA * c * c, c, c);
-    const float s = sigmoid_f<kExact>(2.f * u);
+    float rest;
+    const float s = sigmoid_f<kExact>(2.f * u, &rest);
     *value = z * s;
     const float du = kGeluTanhC * fmaf(3.f * kGeluTanhA * c, c, 1.f);
-    return s + 2.f * c * s * (1.f - s) * du;
+    return s + 2.f * c * s * rest * du;
   } else {
     *value = z;
     return 1.f;

@@ -266,11 +266,13 @@ __device__ __forceinline__ uint64_t gelu_q(uint64_t t) {
   return ffma2(q, t, both(-2.3022075f));
 }
 
-// The sigmoids of two smooth activations; z is capped first, where x would
+// The sigmoids s of two smooth activations and r = 1 - s, formed as 2^x s:
+// far out, where s is 1 but for its last bit, a difference would leave that
+// bit for the slope to multiply by z^3. z is capped first, where x would
 // pass 63.
 template <int ACT>
 __device__ __forceinline__ void sigmoid2(float& z0, float& z1, float& s0,
-                                         float& s1) {
+                                         float& s1, float& r0, float& r1) {
   constexpr float kLow = ACT == VECTRA_ACT_SILU        ? -43.6f
                          : ACT == VECTRA_ACT_GELU_TANH ? -7.6f
                                                        : -6.5f;
@@ -290,8 +292,11 @@ __device__ __forceinline__ void sigmoid2(float& z0, float& z1, float& s0,
     }
   }
   const float2 xs = f2upk(x);
-  s0 = fast_rcp(1.f + fast_exp2(xs.x));
-  s1 = fast_rcp(1.f + fast_exp2(xs.y));
+  const float e0 = fast_exp2(xs.x), e1 = fast_exp2(xs.y);
+  s0 = fast_rcp(1.f + e0);
+  s1 = fast_rcp(1.f + e1);
+  r0 = e0 * s0;
+  r1 = e1 * s1;
 }
 
 template <int ACT>
@@ -300,23 +305,23 @@ __device__ __forceinline__ void activate2(float& z0, float& z1) {
     z0 = max_nan(z0, 0.f);
     z1 = max_nan(z1, 0.f);
   } else if constexpr (ACT != VECTRA_ACT_NONE) {
-    float s0, s1;
-    sigmoid2<ACT>(z0, z1, s0, s1);
+    float s0, s1, r0, r1;
+    sigmoid2<ACT>(z0, z1, s0, s1, r0, r1);
     z0 *= s0;
     z1 *= s1;
   }
 }
 
-// act'(z) from z (capped) and its sigmoid s: s + z ds/dz.
+// act'(z) from z (capped), its sigmoid s and r = 1 - s: s + z ds/dz.
 template <int ACT>
-__device__ __forceinline__ float slope_of(float z, float s) {
+__device__ __forceinline__ float slope_of(float z, float s, float r) {
   if constexpr (ACT == VECTRA_ACT_SILU) {
-    return fmaf(z * s, 1.f - s, s);
+    return fmaf(z * s, r, s);
   } else if constexpr (ACT == VECTRA_ACT_GELU_TANH) {
     // 0 * z^2 far out has to stay 0.
     const float t = fminf(z * z, 1e4f);
     const float du = 2.f * kGeluTanhC * fmaf(3.f * kGeluTanhA, t, 1.f);
-    return fmaf(z * s * (1.f - s), du, s);
+    return fmaf(z * s * r, du, s);
   } else {  // gelu: s is Phi, and Phi' the normal density
     const float t = fminf(z * z, 1e4f);
     return fmaf(z * 0.3989422804f, fast_exp2(-0.5f * kLog2e * t), s);
@@ -334,10 +339,10 @@ __device__ __forceinline__ void activate_grad2(float& z0, float& z1,
     z0 = max_nan(z0, 0.f);
     z1 = max_nan(z1, 0.f);
   } else {
-    float p0, p1;
-    sigmoid2<ACT>(z0, z1, p0, p1);
-    s0 = slope_of<ACT>(z0, p0);
-    s1 = slope_of<ACT>(z1, p1);
+    float p0, p1, r0, r1;
+    sigmoid2<ACT>(z0, z1, p0, p1, r0, r1);
+    s0 = slope_of<ACT>(z0, p0, r0);
+    s1 = slope_of<ACT>(z1, p1, r1);
     z0 *= p0;
     z1 *= p1;
   }

@@ -169,3 +169,58 @@ def test_slopes_far_out(device, dtype, act, rows, saved):
             want.abs().t() @ d(x).abs())
         _close_or_past(dw[i], total,
                        spread * (1 + u) + u * total.abs() + tiny, 'dw')
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('act', ACTS)
+@pytest.mark.parametrize('size', KERNELS)
+def test_infinite_preactivations(dtype, act, size):
+    """Biases that are infinite, NaN or very large: every kernel gives what
+    the definition gives in floating point (act(-inf) is -inf * 0, NaN, for
+    the smooth ones), and so do the slopes."""
+    m, k, n = size
+    rand = Rand(m * 3 + n, 'cuda', dtype)
+    big = 6e4 if dtype == torch.float16 else 1e30
+    x, dy = rand(m, k), rand(m, n)
+    w, b = rand(n, k, scale=k**-0.5), rand(n)
+    far = [float('inf'), float('-inf'), float('nan'), big, -big]
+    b[2:12:2] = torch.tensor(far, device='cuda')
+    columns = torch.arange(2, 12, 2)
+    z = torch.tensor(far, dtype=torch.float64)
+    want, slope = act64(z, act), slope64(z, act)
+    leaf = b.clone().requires_grad_()
+    y = block.linear(x, w, leaf, activation=act)
+    db, = torch.autograd.grad(y, leaf, dy)
+    checks = [('linear', y, want, db, slope)]
+    wu, bu = rand(n, k, scale=0.01 / k), torch.ones_like(b)
+    ops = torch.ops.vectra_b200
+    h, gate, up = ops.gated_linear_with_pre(x, w, wu, b, bu, act, True)
+    for saved in (True, False):
+        if not saved:
+            gate, up = gate.new_empty(0), up.new_empty(0)
+        _, _, both = ops.gated_linear_backward(
+            dy, x, w, wu, b, bu, gate, up, act, False, False, True)
+        checks += [('dg', h, want, both[0], slope),
+                   ('du', h, want, both[1], want)]
+    for what, result, value, grad, factor in checks:
+        got = d(result)[:, columns]
+        value = value.expand(m, 5)
+        assert torch.equal(got.isnan(), value.isnan()), what
+        inf = value.isinf()
+        assert torch.equal(got[inf], value[inf]), what
+        fin = value.isfinite()
+        # Beside the bias the product is nothing, or within the rounding of
+        # the type; the up factor is 1 to within 0.01 x sqrt(k) / k.
+        err = (got - value)[fin].abs()
+        assert (err <= 0.03 * value[fin].abs()).all(), what
+        total = (d(dy)[:, columns] * factor).sum(0)
+        got = d(grad)[columns]
+        keep = torch.ones(5, dtype=torch.bool)
+        if act == 'relu':
+            keep[2] = False  # a NaN has no slope
+        assert torch.equal(got.isnan()[keep], total.isnan()[keep]), what
+        if what != 'du':
+            fin = total.isfinite() & keep
+            spread = (d(dy).abs().sum(0)[columns][fin] * 0.03)
+            assert ((got - total)[fin].abs() <= spread).all(), what

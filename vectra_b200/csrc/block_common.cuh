@@ -105,15 +105,15 @@ __device__ __forceinline__ float act_grad(float z, float* value) {
     *value = z * phi;
     return phi + z * 0.3989422804f * e;
   } else if constexpr (ACT == VECTRA_ACT_GELU_TANH) {
-    // Past |z| = 100 the sigmoid is exactly 0 or 1; the clamp keeps z^3 and
-    // the product 0 * z^2 finite.
-    const float c = fminf(fmaxf(z, -100.f), 100.f);
-    const float u = kGeluTanhC * fmaf(kGeluTanhA * c * c, c, c);
+    const float u = kGeluTanhC * fmaf(kGeluTanhA * z * z, z, z);
     float rest;
     const float s = sigmoid_f<kExact>(2.f * u, &rest);
     *value = z * s;
-    const float du = kGeluTanhC * fmaf(3.f * kGeluTanhA * c, c, 1.f);
-    return s + 2.f * c * s * rest * du;
+    // Past |z| = 100, s or rest is exactly 0; its product with z^2 has to
+    // stay 0.
+    const float t = fminf(z * z, 1e4f);
+    const float du = kGeluTanhC * fmaf(3.f * kGeluTanhA, t, 1.f);
+    return s + 2.f * z * s * rest * du;
   } else {
     *value = z;
     return 1.f;

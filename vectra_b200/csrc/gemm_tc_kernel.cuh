@@ -237,9 +237,10 @@ __device__ __forceinline__ void dealloc_cols(uint32_t addr, uint32_t cols) {
 // fitted on |z| <= 5 for the least error of the result (7e-8; beyond, its
 // leading term keeps driving the sigmoid to 0 or 1). With x = -g log2(e),
 // sigmoid = 1 / (1 + 2^x). Each value has a reciprocal of its own: one for
-// two, 1/a = b / (ab), would carry a NaN into the neighbouring column. z is
-// capped from below (NaN kept) where x reaches 63; the result there
-// is within 3e-10 of the activation, and -infinity gives that, not NaN.
+// two, 1/a = b / (ab), would carry a NaN into the neighbouring column. Far
+// out, 2^x is 0 or infinity and the sigmoid 1 or 0; an infinite z gives what
+// the definition gives in floating point, infinity or (-infinity times 0)
+// NaN, here as in every other kernel of the operators.
 // float32 results take the same forms: their error is below that of the
 // product before them. Packed multiplications and additions halve the instructions.
 // ---------------------------------------------------------------------------
@@ -268,16 +269,10 @@ __device__ __forceinline__ uint64_t gelu_q(uint64_t t) {
 
 // The sigmoids s of two smooth activations and r = 1 - s, formed as 2^x s:
 // far out, where s is 1 but for its last bit, a difference would leave that
-// bit for the slope to multiply by z^3. z is capped first, where x would
-// pass 63.
+// bit for the slope to multiply by z^3. Where 2^x passes 2^126, s is 0.
 template <int ACT>
-__device__ __forceinline__ void sigmoid2(float& z0, float& z1, float& s0,
+__device__ __forceinline__ void sigmoid2(float z0, float z1, float& s0,
                                          float& s1, float& r0, float& r1) {
-  constexpr float kLow = ACT == VECTRA_ACT_SILU        ? -43.6f
-                         : ACT == VECTRA_ACT_GELU_TANH ? -7.6f
-                                                       : -6.5f;
-  z0 = max_nan(z0, kLow);
-  z1 = max_nan(z1, kLow);
   const uint64_t z = f2pk(z0, z1);
   uint64_t x;
   if constexpr (ACT == VECTRA_ACT_SILU) {
@@ -295,8 +290,8 @@ __device__ __forceinline__ void sigmoid2(float& z0, float& z1, float& s0,
   const float e0 = fast_exp2(xs.x), e1 = fast_exp2(xs.y);
   s0 = fast_rcp(1.f + e0);
   s1 = fast_rcp(1.f + e1);
-  r0 = e0 * s0;
-  r1 = e1 * s1;
+  r0 = fminf(e0, 0x1p126f) * s0;
+  r1 = fminf(e1, 0x1p126f) * s1;
 }
 
 template <int ACT>
@@ -312,7 +307,7 @@ __device__ __forceinline__ void activate2(float& z0, float& z1) {
   }
 }
 
-// act'(z) from z (capped), its sigmoid s and r = 1 - s: s + z ds/dz.
+// act'(z) from z, its sigmoid s and r = 1 - s: s + z ds/dz.
 template <int ACT>
 __device__ __forceinline__ float slope_of(float z, float s, float r) {
   if constexpr (ACT == VECTRA_ACT_SILU) {

@@ -4,6 +4,8 @@ values that are not finite or far out, and uses that a call has to refuse.
 Tolerances are those of test_block.py unless a test derives its own.
 """
 
+import math
+
 import pytest
 import torch
 
@@ -224,3 +226,41 @@ def test_infinite_preactivations(dtype, act, size):
             fin = total.isfinite() & keep
             spread = (d(dy).abs().sum(0)[columns][fin] * 0.03)
             assert ((got - total)[fin].abs() <= spread).all(), what
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('act', ['gelu', 'gelu_tanh', 'silu'])
+@pytest.mark.parametrize('size', KERNELS)
+def test_float32_tails(act, size):
+    """float32 activations of -8 to -4 to a relative accuracy, by every
+    kernel. The weights are zero, so z is the bias, exactly. An exponent of
+    size e takes at most four roundings (its polynomial included) and so puts
+    4 e 2^-24 on its exponential; the rest of the form is within 16 of
+    them."""
+    m, k, n = size
+    rand = Rand(m, 'cuda', torch.float32)
+    x, zero = rand(m, k), torch.zeros(n, k, device='cuda')
+    b = torch.linspace(-8, -4, n, device='cuda')
+    z = d(b)
+    e = {'gelu': z * z / 2, 'silu': -z,
+         'gelu_tanh': -math.sqrt(8 / math.pi) * (z + 0.044715 * z**3)}[act]
+    # (act64's 1 + tanh is 0 from z = -6 on, in float64 too.)
+    want = (z * torch.sigmoid(-e) if act == 'gelu_tanh' else
+            act64(z, act)).expand(m, n)
+    bound = (4 * e + 16) * 2.0**-24 * want.abs()
+    close(block.linear(x, zero, b, activation=act), want, bound, 'linear')
+    one = torch.ones_like(b)
+    h = block.gated_linear(x, zero, zero, b, one, activation=act)
+    close(h, want, bound, 'gated')
+    # The slope, act(z) / z + z phi(z) or its like: terms of one size.
+    leaf = b.clone().requires_grad_()
+    db, = torch.autograd.grad(block.linear(x, zero, leaf, activation=act),
+                              leaf, torch.full((m, n), 1.0, device='cuda'))
+    slope = slope64(z, act)
+    if act == 'gelu_tanh':
+        s = torch.sigmoid(-e)
+        slope = s + z * s * (1 - s) * math.sqrt(8 / math.pi) * (
+            1 + 3 * 0.044715 * z * z)
+    size = (want[0] / z).abs() * (1 + z * z * (3 if act == 'gelu_tanh' else
+                                               1))
+    close(db, m * slope, m * (4 * e + 16 + m) * 2.0**-24 * size, 'db')

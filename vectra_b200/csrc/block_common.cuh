@@ -17,8 +17,9 @@
 namespace vectra {
 
 // ---------------------------------------------------------------------------
-// Activations. kExact: CUDA's expf / erff / tanhf, for float32 tensors
-// outside the tensor-core epilogue (which has its own, gemm_tc_kernel.cuh).
+// Activations. kExact: CUDA's expf and erfcf, for float32 tensors, in forms
+// that keep their relative accuracy in the negative tail (0.5 z (1 + erf),
+// and the same with tanh, lose it from z = -3 on).
 // Otherwise forms on ex2.approx and rcp.approx whose error (below 1e-6
 // absolute) is far under the rounding of the 16-bit results.
 // ---------------------------------------------------------------------------
@@ -70,13 +71,13 @@ __device__ __forceinline__ float act_fwd(float z) {
     if constexpr (kExact) return z / (1.f + expf(-z));
     return z * sigmoid_f<false>(z);
   } else if constexpr (ACT == VECTRA_ACT_GELU) {
-    if constexpr (kExact) return 0.5f * z * (1.f + erff(z * 0.70710678118f));
+    if constexpr (kExact) return 0.5f * z * erfcf(z * -0.70710678118f);
     float e;
     return z * phi_fast(z, &e);
   } else if constexpr (ACT == VECTRA_ACT_GELU_TANH) {
     const float u = kGeluTanhC * fmaf(kGeluTanhA * z * z, z, z);
-    if constexpr (kExact) return 0.5f * z * (1.f + tanhf(u));
     // (1 + tanh u) / 2 = sigmoid(2 u)
+    if constexpr (kExact) return z / (1.f + expf(-2.f * u));
     return z * sigmoid_f<false>(2.f * u);
   } else {
     return z;
@@ -97,7 +98,7 @@ __device__ __forceinline__ float act_grad(float z, float* value) {
   } else if constexpr (ACT == VECTRA_ACT_GELU) {
     float phi, e;
     if constexpr (kExact) {
-      phi = 0.5f * (1.f + erff(z * 0.70710678118f));
+      phi = 0.5f * erfcf(z * -0.70710678118f);
       e = expf(-0.5f * z * z);
     } else {
       phi = phi_fast(z, &e);

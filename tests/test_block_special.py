@@ -264,3 +264,43 @@ def test_float32_tails(act, size):
     size = (want[0] / z).abs() * (1 + z * z * (3 if act == 'gelu_tanh' else
                                                1))
     close(db, m * slope, m * (4 * e + 16 + m) * 2.0**-24 * size, 'db')
+
+
+def _same_kinds(got, want, what):
+    """NaN and infinities where `want` (float64) has them."""
+    got = d(got)
+    assert torch.equal(got.isnan(), want.isnan()), what
+    inf = want.isinf()
+    assert torch.equal(got[inf], want[inf]), what
+    assert got[want.isfinite()].isfinite().all(), what
+
+
+@pytest.mark.parametrize('device', DEVICES)
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('size', KERNELS)
+def test_infinite_operands(device, dtype, size):
+    """Infinities in x, the weight and the gradient: against finite numbers
+    of either sign, zeros, other infinities and NaN, as in any product."""
+    m, k, n = size
+    rand = Rand(k + n, device, dtype)
+    x, w, dy = rand(m, k), rand(n, k, scale=k**-0.5), rand(m, n)
+    inf, nan = float('inf'), float('nan')
+    w[2, 3] = 0
+    clean = block.linear(x, w)
+    x[0, 3], x[1, 5], x[2, 1], x[2, 9], x[3, 7] = inf, -inf, inf, -inf, -inf
+    w[4, 5], w[6, 7], w[8, 3], w[10, 7] = inf, -inf, nan, inf
+    dy[1, 4], dy[3, 12], dy[0, 6] = inf, -inf, 0
+    xs, ws, g = d(x), d(w), d(dy)
+    x.requires_grad_(), w.requires_grad_()
+    y = block.linear(x, w)
+    dx, dw = torch.autograd.grad(y, [x, w], dy)
+    _same_kinds(y, xs @ ws.t(), 'y')
+    _same_kinds(dx, g @ ws, 'dx')
+    _same_kinds(dw, g.t() @ xs, 'dw')
+    rows = list(range(4, m))
+    cols = [i for i in range(n) if i not in (4, 6, 8, 10)]
+    assert torch.equal(y[rows][:, cols], clean[rows][:, cols])
+    r = block.linear(x, w, activation='relu')
+    _same_kinds(r, (xs @ ws.t()).clamp(min=0), 'relu')
+    h = block.gated_linear(x, w, torch.ones_like(w), activation='none')
+    _same_kinds(h, (xs @ ws.t()) * xs.sum(1, keepdim=True), 'gated')

@@ -26,8 +26,11 @@ __global__ void __launch_bounds__(256)
 
 // Splits float32 into three bf16 planes: hi the nearest bf16, mid the
 // nearest to the rest, lo the rest's rest (exact: 8 + 8 + 8 bits). A value
-// that would round up to infinity is truncated instead; infinities and NaN
-// stand in hi alone.
+// that would round up to infinity is truncated instead; NaN stands in hi
+// alone. An infinity is (1, 0, infinity) with its sign: lo meets nothing but
+// the other operand's hi, so one product of the pair is infinite (NaN where
+// that hi is 0: a zero, or a number below 2^-134), the finite others change
+// nothing, and infinity times infinity is hi times lo.
 __device__ __forceinline__ void split3(float x, __nv_bfloat16* hi,
                                        __nv_bfloat16* mid,
                                        __nv_bfloat16* lo) {
@@ -36,9 +39,10 @@ __device__ __forceinline__ void split3(float x, __nv_bfloat16* hi,
   if (finite && fabsf(x) >= 3.39e38f) h = __float2bfloat16_rz(x);
   const float r = finite ? x - __bfloat162float(h) : 0.f;
   const __nv_bfloat16 m = __float2bfloat16_rn(r);
-  *hi = h;
+  const bool inf = fabsf(x) > 3.402823466e38f;  // not NaN
+  *hi = inf ? __float2bfloat16_rn(copysignf(1.f, x)) : h;
   *mid = m;
-  *lo = __float2bfloat16_rn(r - __bfloat162float(m));
+  *lo = __float2bfloat16_rn(inf ? x : r - __bfloat162float(m));
 }
 
 // One operand's splitting: dst[plane][line][i], lines past `outer` zero.

@@ -304,3 +304,57 @@ def test_infinite_operands(device, dtype, size):
     _same_kinds(r, (xs @ ws.t()).clamp(min=0), 'relu')
     h = block.gated_linear(x, w, torch.ones_like(w), activation='none')
     _same_kinds(h, (xs @ ws.t()) * xs.sum(1, keepdim=True), 'gated')
+
+
+# ---------------------------------------------------------------------------
+# RbfBlock
+# ---------------------------------------------------------------------------
+CASTS = {
+    'half': lambda m, device: m.half(),
+    'bfloat16': lambda m, device: m.bfloat16(),
+    'to': lambda m, device: m.to(torch.float16),
+    'both': lambda m, device: m.to(device, torch.bfloat16),
+    'back': lambda m, device: m.half().float(),
+    'parent': lambda m, device: torch.nn.Sequential(m).to(torch.bfloat16)[0],
+}
+
+
+@pytest.mark.parametrize('device', DEVICES)
+@pytest.mark.parametrize('cast', CASTS)
+def test_block_can_be_cast(device, cast):
+    """The rotation tables and the attention's scale stay float32, bit for
+    bit; everything else takes the type, and the block runs and trains."""
+    torch.manual_seed(0)
+    blk = block.RbfBlock(64, 4, 96, max_positions=32).to(device)
+    blk.log_scale.data.uniform_(-2.5, -1.5)
+    x = Rand(47, device, torch.float32)(3, 17, 64)
+    blk(x).square().mean().backward()
+    scale, grad = blk.log_scale.detach().clone(), blk.log_scale.grad.clone()
+    blk = CASTS[cast](blk, device)
+    dtype = blk.out.weight.dtype
+    tables = block.rotation_tables(32, 16, device=device)
+    for got, want in ((blk.cos, tables[0]), (blk.sin, tables[1]),
+                      (blk.log_scale, scale), (blk.log_scale.grad, grad)):
+        assert got.dtype == torch.float32 and torch.equal(got, want)
+    assert {p.dtype for n, p in blk.named_parameters()
+            if n != 'log_scale'} == {dtype}
+    x = x.to(dtype)
+    with torch.no_grad():
+        served = blk(x)
+    blk.zero_grad()
+    trained = blk(x)
+    assert served.dtype == trained.dtype == dtype
+    assert torch.isfinite(served).all()
+    trained.float().square().mean().backward()
+    for name, p in blk.named_parameters():
+        assert p.grad is not None and torch.isfinite(p.grad).all(), name
+        assert p.grad.dtype == p.dtype, name
+
+
+def test_block_from_meta():
+    """Tables that never had values are made on the first real device."""
+    blk = block.RbfBlock(64, 4, 96, max_positions=32, device='meta')
+    assert blk.cos.is_meta and blk.half().cos.dtype == torch.float32
+    blk = blk.to_empty(device='cpu')
+    cos, sin = block.rotation_tables(32, 16)
+    assert torch.equal(blk.cos, cos) and torch.equal(blk.sin, sin)

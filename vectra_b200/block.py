@@ -220,7 +220,8 @@ class RbfBlock(nn.Module):
     Serving (no gradient needed) runs attention on
     torch.ops.vectra.rbf_attention. That operator has no backward pass, so
     with gradients the same formula runs as matrix products, and the layers
-    around it train through this module's operators.
+    around it train through this module's operators. `.to(dtype)` and its
+    like leave the rotation tables and `log_scale` in float32.
     """
 
     def __init__(self, d_model: int, heads: int, ffn: int,
@@ -238,7 +239,8 @@ class RbfBlock(nn.Module):
         self.k_weight = nn.Parameter(torch.ones(self.head_dim, **kw))
         self.out = nn.Linear(d_model, d_model, **kw)
         self.log_scale = nn.Parameter(
-            torch.full((1, heads, 1, 1), -2.0, device=device))
+            torch.full((1, heads, 1, 1), -2.0, device=device,
+                       dtype=torch.float32))
         self.norm2 = nn.LayerNorm(d_model, **kw)
         self.gate = nn.Linear(d_model, ffn, **kw)
         self.up = nn.Linear(d_model, ffn, **kw)
@@ -247,6 +249,27 @@ class RbfBlock(nn.Module):
                                    device=device)
         self.register_buffer('cos', cos, persistent=False)
         self.register_buffer('sin', sin, persistent=False)
+
+    def _apply(self, fn, recurse=True):
+        # What .to(), .half() and the like do to every tensor. The operators
+        # take float32 tables only, and a scale rounded to 16 bits would move
+        # every logit: these keep their type and values.
+        tables, scale = (self.cos, self.sin), self.log_scale.detach()
+        grad = self.log_scale.grad
+        if grad is not None:
+            grad = grad.detach()
+        super()._apply(fn, recurse)
+        if self.cos.is_meta < tables[0].is_meta:
+            tables = rotation_tables(tables[0].shape[0], self.head_dim)
+        elif self.cos.dtype == torch.float32:
+            tables = (self.cos, self.sin)
+        self.cos, self.sin = (t.to(self.cos.device) for t in tables)
+        if self.log_scale.dtype != torch.float32:
+            self.log_scale.grad = None
+            self.log_scale.data = scale.to(self.log_scale.device)
+            if grad is not None:
+                self.log_scale.grad = grad.to(self.log_scale.device)
+        return self
 
     def _attend(self, q, k, v, bias):
         scale = self.log_scale.exp()

@@ -358,3 +358,17 @@ def test_block_from_meta():
     blk = blk.to_empty(device='cpu')
     cos, sin = block.rotation_tables(32, 16)
     assert torch.equal(blk.cos, cos) and torch.equal(blk.sin, sin)
+
+
+@pytest.mark.parametrize('device', DEVICES)
+def test_block_refuses_longer_sequences(device):
+    """More tokens than rotations, without positions, raise instead of
+    giving NaN; positions inside the tables serve them."""
+    blk = block.RbfBlock(32, 2, 48, max_positions=8).to(device)
+    x = Rand(5, device, torch.float32)(2, 9, 32)
+    with torch.no_grad():
+        assert torch.isfinite(blk(x[:, :8])).all()
+        with pytest.raises(ValueError, match='max_positions'):
+            blk(x)
+        at = torch.arange(9, device=device) % 8
+        assert torch.isfinite(blk(x, positions=at)).all()

@@ -286,8 +286,13 @@ class RbfBlock(nn.Module):
 
     def forward(self, x, key_bias=None, positions=None):
         """x [B, N, d_model]; key_bias broadcastable to [B, 1|H, 1, N] (0 or
-        -inf); positions as in `qk_norm_rope`."""
+        -inf); positions as in `qk_norm_rope` (one outside the tables of
+        max_positions rows makes its token NaN). Without positions, N above
+        max_positions raises ValueError."""
         b, n, _ = x.shape
+        if positions is None and n > self.cos.shape[0]:
+            raise ValueError(f'{n} tokens, but max_positions is '
+                             f'{self.cos.shape[0]}')
         qkv = linear(self.norm1(x), self.qkv.weight, self.qkv.bias)
         q, k, v = qkv.view(b, n, 3, self.heads,
                            self.head_dim).permute(2, 0, 3, 1, 4)

@@ -372,3 +372,40 @@ def test_block_refuses_longer_sequences(device):
             blk(x)
         at = torch.arange(9, device=device) % 8
         assert torch.isfinite(blk(x, positions=at)).all()
+
+
+# ---------------------------------------------------------------------------
+# Saved values
+# ---------------------------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('act', ['none', 'gelu', 'silu'])
+@pytest.mark.parametrize('size', [(2570, 192, 2056), (5001, 72, 1032),
+                                  (257, 1100, 5000), (150, 64, 520)])
+def test_saved_values(dtype, act, size):
+    """The pre-activation beside the result, with and without a residual:
+    within their bounds, the same with and without the other, and the same
+    every time."""
+    m, k, n = size
+    u, tiny = U[dtype], TINY[dtype]
+    rand = Rand(m, 'cuda', dtype)
+    x, w, b, r = rand(m, k), rand(n, k, scale=k**-0.5), rand(n), rand(m, n)
+    z = d(x) @ d(w).t() + d(b)
+    off = sums(k) * (d(x).abs() @ d(w).abs().t() + d(b).abs())
+    run = torch.ops.vectra_b200.linear_with_pre
+    plain, pre = run(x, w, b, None, act, True)
+    close(pre, z, off * (1 + u) + u * z.abs() + tiny, 'pre')
+    want = act64(z, act)
+    bound = 1.13 * off + 2e-6 * z.abs().clamp(min=1) + tiny
+    close(plain, want, bound * (1 + u) + u * want.abs(), 'y')
+    first = None
+    for _ in range(20):
+        y, again = run(x, w, b, r, act, True)
+        assert torch.equal(again, pre)
+        if first is None:
+            first = y
+            want = want + d(r)
+            bound = bound + 2.0**-23 * want.abs()
+            close(y, want, bound * (1 + u) + u * want.abs(), 'y + r')
+            assert torch.equal(y, run(x, w, b, r, act, False)[0])
+        assert torch.equal(y, first)

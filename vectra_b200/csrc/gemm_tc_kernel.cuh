@@ -805,11 +805,7 @@ __device__ __forceinline__ void epilogue_tile(const TcArgs& g,
         const uint32_t at =
             acc + (c < WARP_COLS ? c : TILE_N + c - WARP_COLS);
         uint32_t r[16], q[16];
-        tmem_ld16u(at, r);
-        tmem_ld16u(at + kSmall, q);
-        tmem_wait_ld();
-        regs_tie16(r);
-        regs_tie16(q);
+        tmem_load16x2(at, r, at + kSmall, q);
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
           const float part_sum = __uint_as_float(r[j]) + __uint_as_float(q[j]);
@@ -850,11 +846,7 @@ __device__ __forceinline__ void epilogue_tile(const TcArgs& g,
           dh[4 * c + 3] = in ? q.w : 0;
         }
         uint32_t r0[16], r1[16];
-        tmem_ld16u(acc + c0 + h, r0);
-        tmem_ld16u(acc + TILE_N + c0 + h, r1);
-        tmem_wait_ld();
-        regs_tie16(r0);
-        regs_tie16(r1);
+        tmem_load16x2(acc + c0 + h, r0, acc + TILE_N + c0 + h, r1);
         if (c0 + h + 16 == WARP_COLS) release();
         float v[16], up[16];
 #pragma unroll
@@ -911,11 +903,7 @@ __device__ __forceinline__ void epilogue_tile(const TcArgs& g,
 #pragma unroll
       for (int h = 0; h < 32; h += 16) {
         uint32_t r0[16], r1[16];
-        tmem_ld16u(acc + c0 + h, r0);
-        tmem_ld16u(acc + TILE_N + c0 + h, r1);
-        tmem_wait_ld();
-        regs_tie16(r0);
-        regs_tie16(r1);
+        tmem_load16x2(acc + c0 + h, r0, acc + TILE_N + c0 + h, r1);
         if (c0 + h + 16 == WARP_COLS) release();
         float v[16], up[16];
 #pragma unroll
@@ -950,10 +938,8 @@ __device__ __forceinline__ void epilogue_tile(const TcArgs& g,
           fetch_residual<T>(stage, p, rb, tile_col + c0, lane);
       uint32_t r0[32];
       uint32_t r1[kGated ? 32 : 1];
-      tmem_ld32u(acc + c0, r0);
-      if constexpr (kGated) tmem_ld32u(acc + TILE_N + c0, r1);
-      tmem_wait_ld_tied(r0);
-      if constexpr (kGated) regs_tie32(r1);
+      tmem_load32(acc + c0, r0);
+      if constexpr (kGated) tmem_load32(acc + TILE_N + c0, r1);
       if (c0 + 32 == WARP_COLS) release();
       if (rb.rows <= 0 || tile_col + c0 >= p.N) continue;
       float v[32], up[32];

@@ -198,14 +198,42 @@ __device__ __forceinline__ void regs_tie32(uint32_t* r) {
                :
                : "memory");
 }
-__device__ __forceinline__ void regs_tie16(uint32_t* r) {
-  asm volatile(""
-               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]),
-                 "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]),
-                 "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]),
-                 "+r"(r[14]), "+r"(r[15])
-               :
-               : "memory");
+// Loads that have landed when the statement ends: the load and its wait are
+// one, so that no copy or spill of a destination can come between them.
+__device__ __forceinline__ void tmem_load32(uint32_t taddr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, "
+      "%7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, "
+      "%21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=&r"(r[0]), "=&r"(r[1]), "=&r"(r[2]), "=&r"(r[3]), "=&r"(r[4]),
+        "=&r"(r[5]), "=&r"(r[6]), "=&r"(r[7]), "=&r"(r[8]), "=&r"(r[9]),
+        "=&r"(r[10]), "=&r"(r[11]), "=&r"(r[12]), "=&r"(r[13]), "=&r"(r[14]),
+        "=&r"(r[15]), "=&r"(r[16]), "=&r"(r[17]), "=&r"(r[18]), "=&r"(r[19]),
+        "=&r"(r[20]), "=&r"(r[21]), "=&r"(r[22]), "=&r"(r[23]), "=&r"(r[24]),
+        "=&r"(r[25]), "=&r"(r[26]), "=&r"(r[27]), "=&r"(r[28]), "=&r"(r[29]),
+        "=&r"(r[30]), "=&r"(r[31])
+      : "r"(taddr)
+      : "memory");
+}
+// 16 columns at each of two addresses.
+__device__ __forceinline__ void tmem_load16x2(uint32_t t0, uint32_t* r,
+                                              uint32_t t1, uint32_t* q) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, "
+      "%7, %8, %9, %10, %11, %12, %13, %14, %15}, [%32];\n\t"
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%16, %17, %18, %19, %20, %21, "
+      "%22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%33];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=&r"(r[0]), "=&r"(r[1]), "=&r"(r[2]), "=&r"(r[3]), "=&r"(r[4]),
+        "=&r"(r[5]), "=&r"(r[6]), "=&r"(r[7]), "=&r"(r[8]), "=&r"(r[9]),
+        "=&r"(r[10]), "=&r"(r[11]), "=&r"(r[12]), "=&r"(r[13]), "=&r"(r[14]),
+        "=&r"(r[15]), "=&r"(q[0]), "=&r"(q[1]), "=&r"(q[2]), "=&r"(q[3]),
+        "=&r"(q[4]), "=&r"(q[5]), "=&r"(q[6]), "=&r"(q[7]), "=&r"(q[8]),
+        "=&r"(q[9]), "=&r"(q[10]), "=&r"(q[11]), "=&r"(q[12]), "=&r"(q[13]),
+        "=&r"(q[14]), "=&r"(q[15])
+      : "r"(t0), "r"(t1)
+      : "memory");
 }
 __device__ __forceinline__ uint64_t f2pk(float x, float y) {
   uint64_t r;

@@ -409,3 +409,80 @@ def test_saved_values(dtype, act, size):
             close(y, want, bound * (1 + u) + u * want.abs(), 'y + r')
             assert torch.equal(y, run(x, w, b, r, act, False)[0])
         assert torch.equal(y, first)
+
+
+# ---------------------------------------------------------------------------
+# What a backward pass keeps
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize('device', DEVICES)
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize('k', [64, 1024])
+@pytest.mark.parametrize('want', [(0,), (1,), (2,), (3,), (0, 2), (1, 2)])
+def test_unneeded_inputs_may_change(device, dtype, k, want):
+    """A backward pass holds only the inputs that its gradients read: the
+    others may be written in place between forward and backward, and the
+    gradients are those of the values before."""
+    rand = Rand(k, device, dtype)
+    m, n = 33, 48
+    args = [rand(m, k), rand(n, k, scale=k**-0.5), rand(n), rand(m, n)]
+    dy = rand(m, n)
+
+    def grads(change):
+        leaves = [t.clone().requires_grad_(i in want)
+                  for i, t in enumerate(args)]
+        # x, weight, bias and residual as intermediate results.
+        use = [t * 1 for t in leaves]
+        y = block.linear(*use, activation='gelu')
+        held = {0: (1,), 1: (0,)}
+        needed = {j for i in want for j in held.get(i, ())}
+        if change:
+            for j, t in enumerate(use):
+                if j not in needed:
+                    t.add_(1)
+        return torch.autograd.grad(y, [leaves[i] for i in want], dy)
+
+    for got, expected in zip(grads(True), grads(False)):
+        assert torch.equal(got, expected)
+
+
+@pytest.mark.parametrize('device', DEVICES)
+@pytest.mark.parametrize('want', [(0,), (1,), (2,), (3,), (4,), (0, 3)])
+def test_unneeded_inputs_may_change_gated(device, want):
+    """The same where a gated layer's projections were saved (float32)."""
+    rand = Rand(7, device, torch.float32)
+    m, k, n = 33, 64, 48
+    args = [rand(m, k), rand(n, k, scale=0.1), rand(n, k, scale=0.1), rand(n),
+            rand(n)]
+    dy = rand(m, n)
+
+    def grads(change):
+        leaves = [t.clone().requires_grad_(i in want)
+                  for i, t in enumerate(args)]
+        use = [t * 1 for t in leaves]
+        y = block.gated_linear(*use)
+        needed = {j for i in want for j in {0: (1, 2), 1: (0,),
+                                            2: (0,)}.get(i, ())}
+        if change:
+            for j, t in enumerate(use):
+                if j not in needed:
+                    t.add_(1)
+        return torch.autograd.grad(y, [leaves[i] for i in want], dy)
+
+    for got, expected in zip(grads(True), grads(False)):
+        assert torch.equal(got, expected)
+
+
+@pytest.mark.parametrize('device', DEVICES)
+@pytest.mark.parametrize('op', ['linear', 'gated_linear'])
+def test_partial_gradients_trace(device, op):
+    """Calls with frozen inputs go through AOT dispatch with static and
+    dynamic shapes."""
+    rand = Rand(5, device, torch.float32)
+    args = [rand(6, 8), rand(4, 8), rand(4, 8)][:2 if op == 'linear' else 3]
+    for i in range(len(args)):
+        call = [t.clone().requires_grad_(i == j) for j, t in enumerate(args)]
+        torch.library.opcheck(
+            getattr(torch.ops.vectra_b200, op).default, tuple(call),
+            test_utils=('test_schema', 'test_faketensor',
+                        'test_aot_dispatch_static',
+                        'test_aot_dispatch_dynamic'))

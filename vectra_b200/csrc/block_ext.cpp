@@ -946,6 +946,13 @@ const char* activation_name(int64_t activation) {
   return names[activation];
 }
 
+// What stands for an input that the backward pass reads the shape of only:
+// one element, expanded. Saving the input itself would keep its memory and
+// forbid writing it in place.
+Tensor shape_of(const Tensor& t) {
+  return at::empty({1}, t.options()).expand_symint(t.sym_sizes());
+}
+
 struct LinearFunction : public Function<LinearFunction> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x,
                         const Tensor& w, const OptTensor& bias,
@@ -956,7 +963,9 @@ struct LinearFunction : public Function<LinearFunction> {
         wants_grad(x) || wants_grad(w) || wants_grad(bias);
     auto [y, pre] = call_linear(x, w, bias, residual, activation,
                                 layer && activation != "none");
-    ctx->save_for_backward({x, w, pre});
+    // dx reads the weight, dw reads x.
+    ctx->save_for_backward({wants_grad(w) ? x : shape_of(x),
+                            wants_grad(x) ? w : shape_of(w), pre});
     ctx->saved_data["call"] = pack_call(
         activation, {wants_grad(x), wants_grad(w), wants_grad(bias),
                      wants_grad(residual)});
@@ -995,8 +1004,16 @@ struct GatedFunction : public Function<GatedFunction> {
                       wg.size(1) > (sums ? VECTRA_GATED_RECOMPUTE_K_SUMS
                                          : VECTRA_GATED_RECOMPUTE_K);
     auto [h, gate, up] = call_gated(x, wg, wu, bg, bu, activation, save);
-    ctx->save_for_backward({x, wg, wu, gate, up, bg.value_or(Tensor()),
-                            bu.value_or(Tensor())});
+    if (save) {
+      // dx reads the weights, dw reads x; the biases are in gate and up.
+      const bool dw = wants_grad(wg) || wants_grad(wu), dx = wants_grad(x);
+      ctx->save_for_backward({dw ? x : shape_of(x), dx ? wg : shape_of(wg),
+                              dx ? wu : shape_of(wu), gate, up, Tensor(),
+                              Tensor()});
+    } else {
+      ctx->save_for_backward({x, wg, wu, gate, up, bg.value_or(Tensor()),
+                              bu.value_or(Tensor())});
+    }
     ctx->saved_data["call"] = pack_call(
         activation, {wants_grad(x), wants_grad(wg), wants_grad(wu),
                      wants_grad(bg), wants_grad(bu)});

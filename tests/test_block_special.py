@@ -20,6 +20,7 @@ from tests.test_block import close
 from tests.test_block import d
 from tests.test_block import slope64
 from tests.test_block import sums
+from tests.test_block import turn64
 from vectra_b200 import block
 
 
@@ -486,3 +487,50 @@ def test_partial_gradients_trace(device, op):
             test_utils=('test_schema', 'test_faketensor',
                         'test_aot_dispatch_static',
                         'test_aot_dispatch_dynamic'))
+
+
+# ---------------------------------------------------------------------------
+# qk_norm_rope
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize('device', DEVICES)
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('interleaved', [False, True])
+@pytest.mark.parametrize('dims', [(64, 16), (64, 32), (64, 64), (48, 0),
+                                  (40, 16), (7, 6)])
+@pytest.mark.parametrize('aligned', [True, False])
+def test_infinite_components(device, dtype, interleaved, dims, aligned):
+    """An infinite component of a vector, or of its gradient, reaches what
+    the formula says, and its partner only where the two are rotated: the
+    same for the 16-byte and the general kernel."""
+    dim, r = dims
+    rand = Rand(dim + r, device, dtype)
+    b, h, n = 2, 3, 7
+    cos, sin = block.rotation_tables(20, r, device=device)
+    pos = torch.randint(1, 20, (b, n), generator=rand.gen)
+    q, dq = rand(b, h, n, dim), rand(b, h, n, dim)
+    inf = float('inf')
+    for t in (q, dq):
+        for e in range(dim):  # one vector each, as far as there are any
+            i, j = divmod(e * 5 % dim, n)
+            if i < h:
+                t[0 if t is q else 1, i, j, e] = inf if e % 2 else -inf
+    w = 1 + rand(dim, scale=0.1)
+    if not aligned:
+        wide = rand(b, h, n, dim + 1)
+        wide[..., 1:] = q
+        q = wide[..., 1:]
+    q = q.detach().requires_grad_()
+    w.requires_grad_()
+    out, _ = block.qk_norm_rope(q, q.detach(), cos, sin, w, None,
+                                pos.to(device), 1e-6, interleaved)
+    dx, dw = torch.autograd.grad(out, [q, w], dq)
+    c, s = d(cos)[pos][:, None], d(sin)[pos][:, None]
+    v, g = d(q), d(dq)
+    scale = (v.square().mean(-1, keepdim=True) + 1e-6).rsqrt()
+    nrm = v * scale
+    _same_kinds(out, turn64(nrm * d(w), c, s, interleaved), 'y')
+    g = turn64(g, c, -s, interleaved)
+    gw = g * d(w)
+    _same_kinds(dx, scale * (gw - nrm * (gw * nrm).mean(-1, keepdim=True)),
+                'dx')
+    _same_kinds(dw, (g * nrm).sum((0, 1, 2)), 'dw')

@@ -5,10 +5,12 @@ Tolerances are those of test_block.py unless a test derives its own.
 """
 
 import math
+import threading
 
 import pytest
 import torch
 
+import vectra_b200
 from tests.test_block import ACTS
 from tests.test_block import DEVICES
 from tests.test_block import Rand
@@ -534,3 +536,79 @@ def test_infinite_components(device, dtype, interleaved, dims, aligned):
     _same_kinds(dx, scale * (gw - nrm * (gw * nrm).mean(-1, keepdim=True)),
                 'dx')
     _same_kinds(dw, (g * nrm).sum((0, 1, 2)), 'dw')
+
+
+# ---------------------------------------------------------------------------
+# Products with tensor maps, in threads and graphs
+# ---------------------------------------------------------------------------
+# More than 64 rows, which the few-row kernel never takes: one CTA's tiles, a
+# reduction in parts (two launches), CTA pairs.
+TENSOR_MAPS = {'tile': (150, 64, 520), 'parts': (130, 4096, 96),
+               'pair': (2570, 192, 2056)}
+
+
+def _launches(call):
+    before = vectra_b200.launch_count()
+    out = call()
+    return out, vectra_b200.launch_count() - before
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize('size', TENSOR_MAPS)
+def test_products_from_a_fresh_thread(dtype, size):
+    """A thread without a current CUDA context encodes tensor maps, of
+    operands and of results."""
+    m, k, n = TENSOR_MAPS[size]
+    rand = Rand(m, 'cuda', dtype)
+    x, w, b, wu = rand(m, k), rand(n, k), rand(n), rand(n, k)
+    for call in (lambda: block.linear(x, w, b, None, 'gelu'),
+                 lambda: block.gated_linear(x, w, wu)):
+        want, launches = _launches(call)
+        planes = dtype == torch.float32  # split first, in a launch
+        if size == 'parts':
+            assert launches == 2 + planes
+        torch.cuda.synchronize()
+        got = []
+        thread = threading.Thread(target=lambda c=call: got.append(c()))
+        thread.start()
+        thread.join()
+        assert len(got) == 1 and torch.equal(got[0], want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize('size', TENSOR_MAPS)
+def test_products_in_a_cuda_graph(dtype, size):
+    """Forward and backward passes, captured and replayed on new inputs:
+    tensor maps, clusters and workspaces of parts."""
+    m, k, n = TENSOR_MAPS[size]
+    rand = Rand(n, 'cuda', dtype)
+    x, w, wu, b, dy = rand(m, k), rand(n, k), rand(n, k), rand(n), rand(m, n)
+    ops = torch.ops.vectra_b200
+    none = torch.empty(0, device='cuda')
+
+    def step():
+        y, pre = ops.linear_with_pre(x, w, b, dy, 'gelu', True)
+        h = block.gated_linear(x, w, wu, b, b)
+        return (y, h, *ops.linear_backward(dy, x, w, pre, 'gelu', True, True,
+                                           True),
+                *ops.gated_linear_backward(dy, x, w, wu, b, b, none, none,
+                                           'silu', True, True, True))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        _, launches = _launches(step)
+    torch.cuda.current_stream().wait_stream(side)
+    assert launches >= 8 + (size == 'parts')
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for t in (x, w, dy):
+        t.copy_(rand(*t.shape))
+    for _ in range(2):
+        graph.replay()
+    want = step()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(out, want))

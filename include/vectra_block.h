@@ -89,13 +89,15 @@ typedef struct {
 } vectra_gated_args;
 
 /* With a reduction (K) up to this long, forming gate and up again in the
- * backward pass takes no more time than writing and reading them (bf16 /
- * f16; forward and elementwise backward of 66,560 x 256 -> 704 on a B200:
- * 160 us against 207; of 16,384 x 1024 -> 2816: 275 against 274). The second
- * limit holds when db_gate and db_up are wanted, whose sums cost the
- * recomputing kernel more (209 against 212, 298 against 279). */
+ * backward pass takes less time than writing and reading them (bf16 / f16;
+ * forward and whole backward on a B200, us, saved against formed again, for
+ * 66,560 x K -> 704, 16,384 x K -> 2816, 4,096 x K -> 5632: K = 768, 497 / 468,
+ * 517 / 432, 247 / 234; K = 1536, 799 / 870, 742 / 787, 393 / 421; level
+ * around 1024). The second limit holds when db_gate and db_up are wanted,
+ * whose sums cost the recomputing kernel more (K = 512, 404 / 400, 396 / 381,
+ * 222 / 211; K = 768, 499 / 523, 467 / 466, 251 / 252). */
 #define VECTRA_GATED_RECOMPUTE_K 768
-#define VECTRA_GATED_RECOMPUTE_K_SUMS 256
+#define VECTRA_GATED_RECOMPUTE_K_SUMS 512
 
 /* Gradients of the above for dh [M,F]: dg = dh * up * act'(gate), du = dh *
  * act(gate), with gate and up as the forward saved them, or formed again

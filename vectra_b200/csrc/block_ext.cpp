@@ -184,14 +184,28 @@ void call_with_workspace(const char* op, Args& a, const Tensor& like,
 // ---------------------------------------------------------------------------
 // Float32 formulation on CPU tensors.
 // ---------------------------------------------------------------------------
+// The kernels' forms (block_common.cuh): ATen's GELU and its gradient lose
+// the negative tail, and some infinite or very large arguments, in float32.
+constexpr double kGeluTanhC = 0.7978845608028654;  // sqrt(2 / pi)
+constexpr double kGeluTanhA = 0.044715;
+
+// Phi(z).
+Tensor cpu_cdf(const Tensor& z) {
+  return at::special_erfc(z * -0.7071067811865476) * 0.5;
+}
+// The argument of tanh GELU's sigmoid.
+Tensor cpu_tanh_argument(const Tensor& z) {
+  return (z + z * z * z * kGeluTanhA) * (2 * kGeluTanhC);
+}
+
 Tensor cpu_act(const Tensor& z, int32_t act) {
   switch (act) {
     case VECTRA_ACT_RELU:
       return at::relu(z);
     case VECTRA_ACT_GELU:
-      return at::gelu(z);
+      return z * cpu_cdf(z);
     case VECTRA_ACT_GELU_TANH:
-      return at::gelu(z, "tanh");
+      return z * at::sigmoid(cpu_tanh_argument(z));
     case VECTRA_ACT_SILU:
       return at::silu(z);
     default:
@@ -199,16 +213,25 @@ Tensor cpu_act(const Tensor& z, int32_t act) {
   }
 }
 
+// dy act'(z).
 Tensor cpu_act_grad(const Tensor& dy, const Tensor& z, int32_t act) {
   switch (act) {
     case VECTRA_ACT_RELU:
-      return at::threshold_backward(dy, z, 0);
+      return dy * (z > 0);
     case VECTRA_ACT_GELU:
-      return at::gelu_backward(dy, z);
-    case VECTRA_ACT_GELU_TANH:
-      return at::gelu_backward(dy, z, "tanh");
-    case VECTRA_ACT_SILU:
-      return at::silu_backward(dy, z);
+      return dy * (cpu_cdf(z) +
+                   z * at::exp(z * z * -0.5) * 0.3989422804014327);
+    case VECTRA_ACT_GELU_TANH: {
+      const Tensor x = cpu_tanh_argument(z), s = at::sigmoid(x);
+      // 0 * z^2 far out has to stay 0.
+      const Tensor t = at::clamp_max(z * z, 1e4);
+      return dy * (s + z * s * at::sigmoid(-x) *
+                           ((t * (3 * kGeluTanhA) + 1) * (2 * kGeluTanhC)));
+    }
+    case VECTRA_ACT_SILU: {
+      const Tensor s = at::sigmoid(z);
+      return dy * (s * (z * at::sigmoid(-z) + 1));
+    }
     default:
       return dy;
   }

@@ -12,7 +12,16 @@
  * are asynchronous on the given stream; functions return VECTRA_OK or a
  * negative status, whose text vectra_block_strerror gives. Sums, norms and
  * activations are computed in 32 bits and each result is rounded once to
- * its type.
+ * its type. With 16-bit tensors two inner values are rounded as well, which
+ * the tensor cores take in 16 bits or the caller keeps: a gradient dz (of a
+ * gated layer dg and du) before its products with the weight and with x, and
+ * vectra_linear's pre. A gated layer's gradients are then off by 2.3e-3 of
+ * their size in bfloat16, where one rounding alone is 1.7e-3.
+ *
+ * A wait that runs out inside a kernel ends it early with an unfinished
+ * result; the call has returned VECTRA_OK by then.
+ * vectra_rbf_check_device_errors (vectra_rbf.h) reports it, for these calls
+ * as for the attention's.
  *
  * The backward calls and some forward calls need a workspace, sized by the
  * matching *_workspace_bytes (which may answer 0) for the same arguments
@@ -47,6 +56,10 @@ typedef enum {
   VECTRA_ACT_GELU_TANH = 3,
   VECTRA_ACT_SILU = 4
 } vectra_activation;
+/* Their float32 values keep a relative accuracy down the negative tail; for
+ * 16-bit results GELU is good to 1.5e-7 absolute. An infinite argument gives
+ * what the formula gives in floating point: NaN for GELU, GELU_TANH or SILU
+ * of minus infinity. */
 
 /* y = act(x W^T + b) + r.
  *  x [M,K], weight [N,K], bias [N] (data NULL: none), residual [M,N] (data
@@ -101,8 +114,9 @@ typedef struct {
 
 /* Gradients of the above for dh [M,F]: dg = dh * up * act'(gate), du = dh *
  * act(gate), with gate and up as the forward saved them, or formed again
- * from x, the weights and the biases when both are NULL; dx = dg Wg + du Wu; dw_gate = dg^T x, dw_up = du^T x; db_gate
- * and db_up the sums of dg and du over rows. Unwanted results: data NULL
+ * from x, the weights and the biases when both are NULL; dx = dg Wg + du Wu;
+ * dw_gate = dg^T x, dw_up = du^T x; db_gate and db_up the sums of dg and du
+ * (before their rounding) over rows. Unwanted results: data NULL
  * (dw_gate and dw_up together, db_gate and db_up together). dw_up directly
  * behind dw_gate in memory saves a pass over x. */
 typedef struct {

@@ -15,8 +15,14 @@ Tensors are float32, float16 or bfloat16 with any strides, one type per
 call. CUDA tensors run this library's sm_100a kernels on the current stream
 (include/vectra_block.h is their C ABI); CPU tensors run an ATen formulation
 in float32. Sums, norms and activations are in float32 and each result is
-rounded once. All three differentiate (once); under torch.no_grad(), or when
-no argument needs a gradient, nothing is kept for a backward pass.
+rounded once; with 16-bit tensors a gradient is also rounded before its
+products with the weight and the input, and `linear` keeps act's argument for
+the backward pass in its type. All three differentiate (once, in reverse;
+forward mode raises NotImplementedError); under torch.no_grad(), or when no
+argument needs a gradient, nothing is kept for a backward pass.
+torch.autocast does not reach them: cast the inputs, mixed types raise.
+A kernel whose wait runs out leaves its result unfinished, which
+`_lib.check_device_errors` reports.
 
 `RbfBlock` is a pre-norm transformer block built from them.
 """

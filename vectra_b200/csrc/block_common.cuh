@@ -229,6 +229,10 @@ cudaError_t launch_split_finish(const GemmProblem& p, int split,
                                 const float* partial, cudaStream_t stream);
 
 // block_grad.cu: elementwise parts of the backward passes.
+// dz (and du) are written in the operands' type: 16-bit tensors' products run
+// on 16-bit operands, and two planes of them would double both products of a
+// backward pass. It costs a gated layer's bf16 gradients 2.3e-3 of their size
+// against 1.7e-3 for the result's rounding alone; db is of the unrounded sums.
 struct GradProblem {
   int32_t dtype = VECTRA_F32;
   int32_t act = VECTRA_ACT_NONE;

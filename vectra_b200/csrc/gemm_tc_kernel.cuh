@@ -30,17 +30,19 @@
 // mid + lo, 24 bits in all; a stage brings in all planes of both, and the
 // product is the sum of the six plane products that matter (lo hi, hi lo,
 // mid mid, mid hi, hi mid, hi hi): 6 bf16 products run at 3.5 times the FP32
-// pipe's rate.
+// pipe's rate. (What that costs beside the product: splitting x and a small
+// weight is 12 of the 52 us of 65,536 x 128 -> 256.)
 //
 // A reduction too long for its few tiles is cut into parts that write
 // float32 sums to the workspace; launch_split_finish adds them in order.
 // Every wait is bounded (error word and early exit).
 //
-// Measured (B200): 8,191 x 4096 -> 4096 f16 with a whole epilogue 187-202 us,
-// 1.4 PFLOP/s, 0.87 of the library's burst rate, the tensor pipe 91 % busy;
-// gated 8,192 x 4096 -> 10240 840 us, 1.64 PFLOP/s. With a reduction of 256
-// the results bound it: 66,560 x 256 -> 1024 bare 39 us (3.5 TB/s of writes,
-// a fill's rate), with bias and GELU 63.
+// Measured (B200): 8,191 x 4096 -> 4096 f16 with a whole epilogue 187-212 us
+// for a few calls at a time, the tensor pipe 91 % busy, and 232-245 us call
+// after call, where the power limit lowers the clock: 1.12-1.47 PFLOP/s, 0.68
+// to 0.89 of the library's burst rate. Gated 8,192 x 4096 -> 10240 840 us,
+// 1.64 PFLOP/s. With a reduction of 256 the results bound it: 66,560 x 256 ->
+// 1024 bare 39 us (3.5 TB/s of writes, a fill's rate), with bias and GELU 62.
 #pragma once
 
 #include <atomic>
@@ -272,11 +274,10 @@ __device__ __forceinline__ uint64_t gelu_q(uint64_t t) {
 
 // Phi of two values, to 5e-7 of itself for z < 0 and to 3e-7 for z > 0, beside
 // the exponential's argument (z^2 2^-24): with a = |z|, Phi(-a) =
-// exp(-a^2 / 2) F(a), where (a + k) F(a) is smooth down to its limit at
-// infinity and a polynomial of degree 9 in (a - k) / (a + k), fitted for the
-// least relative error on 0 <= a <= 14.5 (2e-8). Measured, 65,536 x 128 -> 256
-// with it 52 us, with the fit of the 16-bit
-// results 47, with erfcf 82.
+// exp(-a^2 / 2) F(a), where (a + k) F(a) is smooth up to its limit at infinity
+// and a polynomial of degree 9 in (a - k) / (a + k), fitted for the
+// least relative error on 0 <= a <= 14.5 (2e-8). Measured: 65,536 x 128 -> 256
+// takes 52 us with it, 47 with the fit of the 16-bit results, 82 with erfcf.
 __device__ __forceinline__ void normal_cdf2(float z0, float z1, float& p0,
                                             float& p1) {
   constexpr float k = 2.75f;
@@ -1117,48 +1118,49 @@ __global__ void __launch_bounds__(Cfg<BN, CG, std::is_same<T, float>::value>::TH
                                ? k_first + g.steps_part
                                : g.steps;
         for (int from = k_first; from < k_last && ok;) {
-        const int to = kF32 ? chunk_end(from, k_last) : k_last;
-        ok = mbar_wait(bar_acc_empty(buf), buf_phase ^ 1, p.err);
-        if (!ok) break;
-        tc_fence_after();
-        const uint32_t d = tmem + uint32_t(buf * C::ACC_COLS);
-        for (int k = from; k < to; ++k) {
-          ok = mbar_wait(bar_full(s), phase, p.err);
+          const int to = kF32 ? chunk_end(from, k_last) : k_last;
+          ok = mbar_wait(bar_acc_empty(buf), buf_phase ^ 1, p.err);
           if (!ok) break;
           tc_fence_after();
-          const uint64_t da = da0 + uint64_t((uint32_t(s) * C::STAGE) >> 4);
-          const uint64_t db = db0 + uint64_t((uint32_t(s) * C::STAGE) >> 4);
-          if constexpr (kF32) {
-            // Planes 0, 1, 2 are hi, mid, lo. hi hi has an accumulator of its
-            // own: the others are too small beside it for their truncation
-            // to matter, but would add five more truncations of its sum.
-            constexpr int kPairs[6][2] = {{2, 0}, {0, 2}, {1, 1},
-                                          {1, 0}, {0, 1}, {0, 0}};
+          const uint32_t d = tmem + uint32_t(buf * C::ACC_COLS);
+          for (int k = from; k < to; ++k) {
+            ok = mbar_wait(bar_full(s), phase, p.err);
+            if (!ok) break;
+            tc_fence_after();
+            const uint64_t da = da0 + uint64_t((uint32_t(s) * C::STAGE) >> 4);
+            const uint64_t db = db0 + uint64_t((uint32_t(s) * C::STAGE) >> 4);
+            if constexpr (kF32) {
+              // Planes 0, 1, 2 are hi, mid, lo. hi hi has an accumulator of
+              // its own: the others are too small beside it for their
+              // truncation to matter, but would add five more truncations of
+              // its sum.
+              constexpr int kPairs[6][2] = {{2, 0}, {0, 2}, {1, 1},
+                                            {1, 0}, {0, 1}, {0, 0}};
 #pragma unroll
-            for (int i = 0; i < kTcStep / 16; ++i)
+              for (int i = 0; i < kTcStep / 16; ++i)
 #pragma unroll
-              for (int q = 0; q < 6; ++q)
-                mma_f16<CG>(q == 5 ? d : d + BN,
-                            da + i * ka + ((kPairs[q][0] * C::PLANE) >> 4),
-                            db + i * kb + ((kPairs[q][1] * C::PLANE) >> 4),
-                            idesc, k > from || i > 0 || (q > 0 && q < 5));
-          } else {
+                for (int q = 0; q < 6; ++q)
+                  mma_f16<CG>(q == 5 ? d : d + BN,
+                              da + i * ka + ((kPairs[q][0] * C::PLANE) >> 4),
+                              db + i * kb + ((kPairs[q][1] * C::PLANE) >> 4),
+                              idesc, k > from || i > 0 || (q > 0 && q < 5));
+            } else {
 #pragma unroll
-            for (int i = 0; i < kTcStep / 16; ++i)
-              mma_f16<CG>(d, da + i * ka, db + i * kb, idesc,
-                          k > from || i > 0);
+              for (int i = 0; i < kTcStep / 16; ++i)
+                mma_f16<CG>(d, da + i * ka, db + i * kb, idesc,
+                            k > from || i > 0);
+            }
+            commit_all<CG>(bar_empty(s));
+            if (++s == C::STAGES) {
+              s = 0;
+              phase ^= 1;
+            }
           }
-          commit_all<CG>(bar_empty(s));
-          if (++s == C::STAGES) {
-            s = 0;
-            phase ^= 1;
-          }
-        }
-        if (!ok) break;
-        commit_all<CG>(bar_acc_full(buf));
-        buf ^= 1;
-        if (buf == 0) buf_phase ^= 1;
-        from = to;
+          if (!ok) break;
+          commit_all<CG>(bar_acc_full(buf));
+          buf ^= 1;
+          if (buf == 0) buf_phase ^= 1;
+          from = to;
         }
       }
     }

@@ -13,7 +13,12 @@
 // 65 us for the 16,384 tokens of 32 + 8 heads of 128, bf16, views of one
 // projection (344 MB: 5.3 TB/s, 0.81 of the copy rate; writes alone reach
 // 3.7 TB/s here, so their half takes 46 us); 2.9 us for 64 single tokens;
-// forward and backward of 6,147 tokens of 16 + 16 heads of 64, f16, 46 us.
+// forward and backward of 6,147 tokens of 16 + 16 heads of 64, f16, half
+// rotated, 47 us for 101 MB. There the backward kernel is bound by latency: its
+// 146 registers leave one block of eight warps an SM (12 % occupancy, DRAM
+// 10 %, issue 0.32 per scheduler), in waves of load, compute and store. float32,
+// 8,192 tokens of 32 + 8 heads of 128: forward 58.7 us (336 MB), forward and
+// backward 150.6 (671 MB).
 #include "block_common.cuh"
 #include "tcgen05.cuh"
 

@@ -181,7 +181,9 @@ def draw(rng):
         batch = _log_int(rng, 1, 1024)
         kv_heads = rng.choice([1, 2, 4, 8, 16])
         heads = kv_heads * rng.choice([1, 1, 2, 3, 4, 8])
-        queries, keys = _log_int(rng, 1, 4096), _log_int(rng, 1, 8192)
+        # Over a single state all gradients but that of v are zero.
+        queries = _log_int(rng, 1, 4096)
+        keys = _log_int(rng, 4 if train else 1, 8192)
         if rng.random() < 0.25:
             queries = 1
         dim = rng.choice([32, 64, 64, 80, 96, 128, 128])

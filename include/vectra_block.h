@@ -6,6 +6,14 @@
  *  - vectra_gated_linear_*:  h = act(x Wg^T + bg) * (x Wu^T + bu)
  *  - vectra_qk_norm_rope_*:  the RMS norm of every query and key head vector
  *                            and the rotation of its position, in one pass
+ *                            (vectra_qk_norm_rope_axes_*: of its positions
+ *                            on several axes)
+ *  - vectra_dropout:         zeros a share of a tensor by a mask that is a
+ *                            function of an element's index
+ *  - vectra_residual_norm_*: x_out = a x + gate dropout(norm(branch)) and the
+ *                            next sublayer's norm of x_out, in one pass
+ *  - vectra_cross_attention_*: RBF attention to an encoder's states, of
+ *                            another length, with shared key heads
  *
  * each with its backward pass. Conventions are those of vectra_rbf.h: plain
  * pointers, sizes and element strides; the caller owns every buffer; calls
@@ -157,12 +165,138 @@ typedef struct {
   size_t workspace_bytes;
 } vectra_qk_grad_args;
 
+/* qk_norm_rope with positions on up to VECTRA_MAX_AXES axes: positions[axis]
+ * starts `stride` elements behind positions[axis - 1], and the R2 pairs
+ * belong to the axes in order, section[axis] of them to each: pair i turns by
+ * entry i of the table row that its axis' position names. A position outside
+ * [0, P) on any axis makes its vectors NaN. */
+#define VECTRA_MAX_AXES 4
+typedef struct {
+  int32_t count;                       /* 1 to VECTRA_MAX_AXES */
+  int32_t section[VECTRA_MAX_AXES];    /* not negative, sum R2 */
+  int64_t stride;
+} vectra_qk_axes;
+typedef struct {
+  vectra_qk_args qk; /* positions must not be NULL */
+  vectra_qk_axes axes;
+} vectra_qk_axes_args;
+typedef struct {
+  vectra_qk_grad_args qk;
+  vectra_qk_axes axes;
+} vectra_qk_axes_grad_args;
+
+/* Dropout. Element e of a tensor, counted in row-major order of its sizes
+ * (whatever its strides), is kept when its 16-bit random number is at least
+ * cut = round(65536 p), and then scaled by 65536 / (65536 - cut); the others
+ * become 0, whatever they hold. The random numbers are those of Philox4x32-10
+ * (Salmon et al., "Parallel random numbers: as easy as 1, 2, 3", 2011) with
+ * the key rng[0] (its low, then its high half) and the counter
+ * (e / 8 low half, e / 8 high half, rng[1] low half, stream): number e % 8 is
+ * the low (even) or high half of output word (e % 8) / 2. */
+typedef struct {
+  double p;             /* 0 to 1 */
+  const int64_t* rng;   /* device memory: seed, step. NULL: p is 0 */
+  uint32_t stream;      /* keeps the masks of one step apart */
+} vectra_drop;
+
+/* y = dropout(x), which is also its own gradient.
+ *  x [M,C], one of F32 / F16 / BF16, any strides; y [M,C] contiguous. */
+typedef struct {
+  vectra_tensor x, y;
+  vectra_drop drop;
+} vectra_dropout_args;
+
+/* u = norm(branch) * branch_weight  (branch_weight's data NULL: u = branch)
+ * x_out = residual_scale x + gate * dropout(u)
+ * y = norm(x_out) * weight + bias
+ * with norm(v) = v / sqrt(mean(v^2) + eps) over C, of v - mean(v) first when
+ * `kind` is VECTRA_NORM_LAYER.
+ *  x, branch [M,C]: one dtype of F32 / F16 / BF16, any strides. branch's data
+ *  NULL: x_out is x itself and not written; residual_scale must be 1 and p 0
+ *  then, gate and branch_weight NULL.
+ *  weight, bias, branch_weight [C] (data NULL: none), gate [G,C] (NULL: 1)
+ *  with M a multiple of G: row r takes gate row r / (M / G).
+ *  x_out, y [M,C]: contiguous. y's data NULL: no second norm (weight and bias
+ *  NULL then). The norm is of x_out before its rounding.
+ *  stats [M,4] F32, contiguous: mean and factor of the second norm, mean and
+ *  factor of the first, for the backward pass; data NULL: not wanted.
+ * C is at most 16384. */
+typedef enum { VECTRA_NORM_RMS = 0, VECTRA_NORM_LAYER = 1 } vectra_norm_kind;
+typedef struct {
+  vectra_tensor x, branch, weight, bias, branch_weight, gate;
+  vectra_tensor x_out, y, stats;
+  vectra_drop drop;
+  double residual_scale, eps;
+  int32_t kind; /* vectra_norm_kind */
+} vectra_residual_norm_args;
+
+/* Gradients of the above for dx_out and dy [M,C] (any strides; dx_out's data
+ * NULL: zero; dy's: y had none, its norm is left out). Of fwd, x_out and
+ * stats are read as the forward wrote them (x_out is x, strides and all, where
+ * there was no branch), branch, weight, branch_weight and gate as it read
+ * them. x, y and bias are not read, x_out only with dy, stats only with dy or
+ * branch_weight, branch only with branch_weight or dgate.
+ *  dx, dbranch [M,C], dgate [G,C], dweight, dbias, dbranch_weight [C]:
+ *  contiguous; data NULL when not wanted. */
+typedef struct {
+  vectra_residual_norm_args fwd;
+  vectra_tensor dx_out, dy;
+  vectra_tensor dx, dbranch, dweight, dbias, dbranch_weight, dgate;
+  void* workspace;
+  size_t workspace_bytes;
+} vectra_residual_norm_grad_args;
+
+/* out[b,h,i] = sum over j < len_b of softmax_j(-scale |q_i - k_j|^2) v_j, with
+ * q of head h and k, v of head h / (H / Hk).
+ *  q [B,H,Nq,D], k [B,Hk,Nk,D], v [B,Hk,Nk,Dv]: one dtype of F32 / F16 / BF16,
+ *  any strides; H a multiple of Hk; D and Dv at most 256.
+ *  scale [B|1,H|1,1,1]: any float type; zero and negative values are legal.
+ *  key_lengths [B]: int32 or int64, or NULL: Nk. Values outside [0, Nk] count
+ *  as the nearer end. Keys and values at or past a length are never used; a
+ *  sequence of length 0 has zero results (and gradients).
+ *  out [B,H,Nq,Dv]: unit inner stride.
+ * For the backward pass (data NULL: not wanted):
+ *  lse [B,H,Nq] F32, contiguous: log2 of the sum of each row's weights before
+ *  division, infinity for a sequence of length 0.
+ *  rest [B,H,Nq,Dv], of 16-bit tensors only, contiguous, their type: what out's
+ *  rounding left, itself rounded. The backward pass subtracts numbers that are
+ *  nearly equal where a row has one large weight, and out alone would decide
+ *  their difference. */
+typedef struct {
+  vectra_tensor q, k, v, scale;
+  const void* key_lengths;
+  int32_t length_bytes;  /* 4 or 8 */
+  int64_t length_stride;
+  vectra_tensor out, lse, rest;
+  void* workspace;
+  size_t workspace_bytes;
+} vectra_cross_args;
+
+/* Gradients for dout [B,H,Nq,Dv] (any strides), with out, lse and rest as the
+ * forward wrote them:
+ *  dq, dk, dv: as q, k and v, unit inner stride; rows of dk and dv at or past
+ *  the length are zero. dscale [B,H] F32, contiguous. data NULL when not
+ *  wanted (dk and dv together). */
+typedef struct {
+  vectra_cross_args fwd;
+  vectra_tensor dout, dq, dk, dv, dscale;
+  void* workspace;
+  size_t workspace_bytes;
+} vectra_cross_grad_args;
+
 VECTRA_API int vectra_linear_forward(const vectra_linear_args* args, void* stream);
 VECTRA_API int vectra_linear_backward(const vectra_linear_grad_args* args, void* stream);
 VECTRA_API int vectra_gated_linear_forward(const vectra_gated_args* args, void* stream);
 VECTRA_API int vectra_gated_linear_backward(const vectra_gated_grad_args* args, void* stream);
 VECTRA_API int vectra_qk_norm_rope_forward(const vectra_qk_args* args, void* stream);
 VECTRA_API int vectra_qk_norm_rope_backward(const vectra_qk_grad_args* args, void* stream);
+VECTRA_API int vectra_qk_norm_rope_axes_forward(const vectra_qk_axes_args* args, void* stream);
+VECTRA_API int vectra_qk_norm_rope_axes_backward(const vectra_qk_axes_grad_args* args, void* stream);
+VECTRA_API int vectra_dropout(const vectra_dropout_args* args, void* stream);
+VECTRA_API int vectra_residual_norm_forward(const vectra_residual_norm_args* args, void* stream);
+VECTRA_API int vectra_residual_norm_backward(const vectra_residual_norm_grad_args* args, void* stream);
+VECTRA_API int vectra_cross_attention_forward(const vectra_cross_args* args, void* stream);
+VECTRA_API int vectra_cross_attention_backward(const vectra_cross_grad_args* args, void* stream);
 
 /* Workspace of the call with these arguments, in bytes; a negative status
  * for invalid ones. */
@@ -171,6 +305,10 @@ VECTRA_API int64_t vectra_linear_backward_workspace_bytes(const vectra_linear_gr
 VECTRA_API int64_t vectra_gated_linear_forward_workspace_bytes(const vectra_gated_args* args);
 VECTRA_API int64_t vectra_gated_linear_backward_workspace_bytes(const vectra_gated_grad_args* args);
 VECTRA_API int64_t vectra_qk_norm_rope_backward_workspace_bytes(const vectra_qk_grad_args* args);
+VECTRA_API int64_t vectra_qk_norm_rope_axes_backward_workspace_bytes(const vectra_qk_axes_grad_args* args);
+VECTRA_API int64_t vectra_residual_norm_backward_workspace_bytes(const vectra_residual_norm_grad_args* args);
+VECTRA_API int64_t vectra_cross_attention_forward_workspace_bytes(const vectra_cross_args* args);
+VECTRA_API int64_t vectra_cross_attention_backward_workspace_bytes(const vectra_cross_grad_args* args);
 
 /* Message for a status of these calls. */
 VECTRA_API const char* vectra_block_strerror(int status);

@@ -10,6 +10,17 @@
                         interleaved)
         the RMS norm of every query and key head vector and the rotation of
         its position in one pass, ready for torch.ops.vectra.rbf_attention.
+    q, k = qk_norm_rope_axes(q, k, cos, sin, positions, sections, ...)
+        the same with positions on several axes (time, height, width).
+    x, y = residual_norm(x, branch, weight, bias, gate, branch_weight,
+                         residual_scale, p, rng, ...)
+        a sublayer's result normalised, dropped out, gated and added to the
+        scaled residual, and the next sublayer's norm, in one pass.
+    y = dropout(x, p, rng, stream)
+        dropout whose mask is a function of an element's index.
+    o = cross_attention(q, k, v, scale, key_lengths)
+        RBF attention to an encoder's states of another length, with shared
+        key heads; with gradients, unlike torch.ops.vectra.rbf_attention.
 
 Tensors are float32, float16 or bfloat16 with any strides, one type per
 call. CUDA tensors run this library's sm_100a kernels on the current stream
@@ -17,15 +28,20 @@ call. CUDA tensors run this library's sm_100a kernels on the current stream
 in float32. Sums, norms and activations are in float32 and each result is
 rounded once; with 16-bit tensors a gradient is also rounded before its
 products with the weight and the input, and `linear` keeps act's argument for
-the backward pass in its type. All three differentiate (once, in reverse;
+the backward pass in its type. `cross_attention` rounds weights and their
+gradients to 16 bits before the products that take them, with 16-bit tensors.
+All differentiate (once, in reverse, `dropout` again and again;
 forward mode raises NotImplementedError); under torch.no_grad(), or when no
 argument needs a gradient, nothing is kept for a backward pass.
 torch.autocast does not reach them: cast the inputs, mixed types raise.
 A kernel whose wait runs out leaves its result unfinished, which
 `_lib.check_device_errors` reports.
 
-`RbfBlock` is a pre-norm transformer block built from them.
+`RbfBlock` is a pre-norm transformer block built from them, `RbfCrossBlock`
+one that reads an encoder's states.
 """
+
+import math
 
 import torch
 from torch import nn
@@ -48,6 +64,17 @@ EXPORTED = (
     'vectra_gated_linear_forward_workspace_bytes',
     'vectra_gated_linear_backward_workspace_bytes',
     'vectra_qk_norm_rope_backward_workspace_bytes',
+    'vectra_qk_norm_rope_axes_forward',
+    'vectra_qk_norm_rope_axes_backward',
+    'vectra_dropout',
+    'vectra_residual_norm_forward',
+    'vectra_residual_norm_backward',
+    'vectra_cross_attention_forward',
+    'vectra_cross_attention_backward',
+    'vectra_qk_norm_rope_axes_backward_workspace_bytes',
+    'vectra_residual_norm_backward_workspace_bytes',
+    'vectra_cross_attention_forward_workspace_bytes',
+    'vectra_cross_attention_backward_workspace_bytes',
     'vectra_block_strerror',
 )
 
@@ -55,6 +82,10 @@ _OPS = torch.ops.vectra_b200
 _LINEAR = _OPS.linear.default
 _GATED = _OPS.gated_linear.default
 _QK = _OPS.qk_norm_rope.default
+_AXES = _OPS.qk_norm_rope_axes.default
+_DROPOUT = _OPS.dropout.default
+_NORM = _OPS.residual_norm.default
+_CROSS = _OPS.cross_attention.default
 
 
 def linear(x, weight, bias=None, residual=None,
@@ -128,6 +159,124 @@ def qk_norm_rope(q, k, cos, sin, q_weight=None, k_weight=None,
     """
     return _QK(q, k, cos, sin, q_weight, k_weight, positions, eps,
                interleaved)
+
+
+def qk_norm_rope_axes(q, k, cos, sin, positions, sections, q_weight=None,
+                      k_weight=None, eps: float = 1e-6,
+                      interleaved: bool = False):
+    """`qk_norm_rope` with positions on one to four axes.
+
+    The tables' pairs belong to the axes in order, sections[a] of them to axis
+    a: pair i turns by entry i of the row that its axis' position names, so
+    the tables' columns decide every pair's frequency.
+
+    Args:
+      q, k, cos, sin, q_weight, k_weight, eps, interleaved: As in
+        `qk_norm_rope`.
+      positions: int32 or int64, broadcastable to [A, B, N] (its first size is
+        A). A position outside the tables makes its token's vectors NaN.
+      sections: A pair counts, not negative, that add up to cos.shape[1].
+
+    Returns, raises:
+      As `qk_norm_rope`.
+    """
+    return _AXES(q, k, cos, sin, positions, sections, q_weight, k_weight, eps,
+                 interleaved)
+
+
+def dropout(x, p: float, rng=None, stream: int = 0) -> torch.Tensor:
+    """Zeros a share p of x and scales the rest by the inverse of what is kept.
+
+    The mask is a function of rng, stream and an element's index in row-major
+    order (whatever the strides) and is never stored: the backward pass makes
+    it again, and a captured graph takes a new one when rng is written between
+    replays. Masks of different steps or streams are independent. An element
+    that is not kept is 0, whatever it holds. p is taken to the nearest
+    multiple of 2^-16 (the numbers: include/vectra_block.h, vectra_drop).
+
+    Args:
+      x: Any shape and strides.
+      p: From 0 to 1.
+      rng: int64 [2] on x's device, contiguous: (seed, step). All 64 bits of
+        the seed and the low 32 of the step count. Not needed for p = 0. It
+        must not change between a forward pass and its backward pass.
+      stream: Keeps the masks of one step apart: a number for each place of
+        a model that drops; its low 32 bits count.
+
+    Returns:
+      A tensor like x, contiguous.
+
+    Raises:
+      ValueError: p outside [0, 1], a type that is not supported, or an rng
+        that is missing or not as above.
+    """
+    return _DROPOUT(x, p, rng, stream)
+
+
+def residual_norm(x, branch=None, weight=None, bias=None, gate=None,
+                  branch_weight=None, residual_scale: float = 1.0,
+                  p: float = 0.0, rng=None, stream: int = 0,
+                  eps: float = 1e-6, kind: str = 'rms', norm: bool = True):
+    """What stands between two sublayers:
+
+        u = norm(branch) * branch_weight    (u = branch without one)
+        x_out = residual_scale * x + gate * dropout(u, p, rng, stream)
+        y = norm(x_out) * weight + bias
+
+    with norm(v) = v / sqrt(mean(v^2) + eps), of v - mean(v) for 'layer'.
+
+    Args:
+      x: [..., C], the residual stream, C at most 16384.
+      branch: Like x, a sublayer's result; None: x_out is x.
+      weight, bias: Optional [C], of the norm behind.
+      gate: Optional, C last and before it x's sizes up to some dimension and
+        ones from there on: [C], [B, 1, C] or [B, N, C] for x [B, N, C].
+      branch_weight: Optional [C]: the branch is normalised first.
+      residual_scale: Multiplies x.
+      p, rng, stream: As in `dropout`, of the branch.
+      kind: 'rms' or 'layer', of both norms.
+      norm: False: no norm behind; y is None.
+
+    Returns:
+      (x_out, y), contiguous. y is formed from x_out before its rounding.
+      Without a branch x_out is x itself.
+
+    Raises:
+      ValueError: shapes, dtypes or devices that do not agree, arguments of a
+        branch or norm that is not there.
+      NotImplementedError: C above 16384.
+    """
+    x_out, y = _NORM(x, branch, weight, bias, branch_weight, gate,
+                     residual_scale, p, rng, stream, eps, kind, norm)
+    return x if branch is None else x_out, y if norm else None
+
+
+def cross_attention(q, k, v, scale, key_lengths=None) -> torch.Tensor:
+    """RBF attention to states of another length: for query i of head h
+
+        sum over j < key_lengths[b] of softmax_j(-scale |q_i - k_j|^2) v_j
+
+    with the keys of head h // (H / Hk).
+
+    Args:
+      q: [B, H, Nq, D], D at most 256.
+      k: [B, Hk, Nk, D], H a multiple of Hk.
+      v: [B, Hk, Nk, Dv], Dv at most 256.
+      scale: Broadcastable to [B, H, 1, 1], any float type. Zero and negative
+        values are legal.
+      key_lengths: Optional int32 or int64 [B]; values outside [0, Nk] count
+        as the nearer end. Keys and values at or past a length are never used
+        and have zero gradients, whatever they hold; a sequence of length 0
+        has zero results.
+
+    Returns:
+      [B, H, Nq, Dv], laid out as `custom_ops.output_strides` says.
+
+    Raises:
+      ValueError: shapes, dtypes or devices that do not agree.
+      NotImplementedError: D or Dv above 256.
+    """
+    return _CROSS(q, k, v, scale, key_lengths)
 
 
 def rotation_tables(length: int, dim: int, base: float = 10000.0,
@@ -216,8 +365,97 @@ def _qk_backward_fake(dq_out, dk_out, q, k, cos, sin, q_weight, k_weight,
             weight(k_weight))
 
 
+@torch.library.register_fake('vectra_b200::qk_norm_rope_axes')
+def _axes_fake(q, k, cos, sin, positions, sections, q_weight=None,
+               k_weight=None, eps=1e-6, interleaved=False):
+    del cos, sin, positions, sections, q_weight, k_weight, eps, interleaved
+    return _heads_like(q), _heads_like(k)
+
+
+@torch.library.register_fake('vectra_b200::qk_norm_rope_axes_backward')
+def _axes_backward_fake(dq_out, dk_out, q, k, cos, sin, positions, sections,
+                        q_weight, k_weight, eps, interleaved, need_dw):
+    del sections
+    return _qk_backward_fake(dq_out, dk_out, q, k, cos, sin, q_weight,
+                             k_weight, positions, eps, interleaved, need_dw)
+
+
+@torch.library.register_fake('vectra_b200::dropout')
+def _dropout_fake(x, p, rng=None, stream=0):
+    del p, rng, stream
+    return x.new_empty(x.shape)
+
+
+@torch.library.register_fake('vectra_b200::residual_norm')
+def _norm_fake(x, branch=None, weight=None, bias=None, branch_weight=None,
+               gate=None, residual_scale=1.0, p=0.0, rng=None, stream=0,
+               eps=1e-6, kind='rms', norm=True):
+    return _norm_with_stats_fake(x, branch, weight, bias, branch_weight, gate,
+                                 residual_scale, p, rng, stream, eps, kind,
+                                 norm, False)[:2]
+
+
+@torch.library.register_fake('vectra_b200::residual_norm_with_stats')
+def _norm_with_stats_fake(x, branch, weight, bias, branch_weight, gate,
+                          residual_scale, p, rng, stream, eps, kind, norm,
+                          want_stats):
+    del weight, bias, branch_weight, gate, residual_scale, p, rng, stream
+    del eps, kind
+    rows = math.prod(x.shape[:-1]) if want_stats and x.shape[-1] else 0
+    return (x.new_empty(x.shape if branch is not None else (0,)),
+            x.new_empty(x.shape if norm else (0,)),
+            x.new_empty((rows, 4), dtype=torch.float32))
+
+
+@torch.library.register_fake('vectra_b200::residual_norm_backward')
+def _norm_backward_fake(dx_out, dy, x_out, stats, branch, weight,
+                        branch_weight, gate, residual_scale, p, rng, stream,
+                        eps, kind, need):
+    del x_out, stats, branch, weight, branch_weight, residual_scale, p, rng
+    del stream, eps, kind
+    g = dx_out if dy is None else dy
+    c = g.shape[-1:]
+    shapes = (g.shape, g.shape, c, c, c, () if gate is None else gate.shape)
+    return tuple(g.new_empty(shape if need >> i & 1 else (0,))
+                 for i, shape in enumerate(shapes))
+
+
+def _rows_like(t, width):
+    return t.new_empty_strided((*t.shape[:-1], width),
+                               custom_ops.output_strides(t, width))
+
+
+@torch.library.register_fake('vectra_b200::cross_attention')
+def _cross_fake(q, k, v, scale, key_lengths=None):
+    del k, scale, key_lengths
+    return _rows_like(q, v.shape[-1])
+
+
+@torch.library.register_fake('vectra_b200::cross_attention_with_lse')
+def _cross_with_lse_fake(q, k, v, scale, key_lengths, want_lse):
+    del k, scale, key_lengths
+    rest = want_lse and q.dtype != torch.float32
+    return (_rows_like(q, v.shape[-1]),
+            q.new_empty(q.shape[:-1] if want_lse else (0, *q.shape[1:3]),
+                        dtype=torch.float32),
+            q.new_empty((*q.shape[:-1], v.shape[-1]) if rest else (0,)))
+
+
+@torch.library.register_fake('vectra_b200::cross_attention_backward')
+def _cross_backward_fake(dout, q, k, v, scale, key_lengths, out, lse, rest,
+                         need_dq, need_dkv, need_dscale):
+    del dout, scale, key_lengths, out, lse, rest
+
+    def grad(t, need):
+        return _rows_like(t, t.shape[-1]) if need else t.new_empty((0,))
+
+    return (grad(q, need_dq), grad(k, need_dkv), grad(v, need_dkv),
+            q.new_empty((q.shape[0] if need_dscale else 0, q.shape[1]),
+                        dtype=torch.float32))
+
+
 # ---------------------------------------------------------------------------
-# A block that runs them together.
+# Blocks that run them together.
 # ---------------------------------------------------------------------------
 class RbfBlock(nn.Module):
     """A pre-norm transformer block: RBF attention over normalised, rotated

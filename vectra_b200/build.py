@@ -37,7 +37,9 @@ CU_SOURCES = ['capi.cu', 'rbf_generic.cu', 'rbf_decode.cu', 'rbf_tc.cu',
               'gemm_rows.cu', 'gemm_select.cu', 'gemm_tc.cu', 'gemm_tc_linear_bf16.cu',
               'gemm_tc_linear_f16.cu', 'gemm_tc_other_bf16.cu',
               'gemm_tc_other_f16.cu', 'gemm_tc_linear_f32.cu',
-              'gemm_tc_other_f32.cu', 'qk_norm_rope.cu']
+              'gemm_tc_other_f32.cu', 'qk_norm_rope.cu', 'qk_norm_rope_axes.cu',
+              'residual_norm.cu', 'cross_simple.cu', 'cross_finish.cu',
+              'decoder_capi.cu']
 ARCH = ['-gencode', 'arch=compute_100a,code=sm_100a']
 
 
@@ -127,7 +129,7 @@ def build_library(force=False, verbose=False, extra_flags=(), lib_path=LIB,
 def build_torch_extension(force=False, verbose=False):
     """Compiles the PyTorch binding against the installed torch: the
     operator's registration and CUDA launcher (torch_ext.cpp), the
-    transformer-block operators' (block_ext.cpp) and the CPU implementation
+    transformer-block operators' (block_ext.cpp, decoder_ext.cpp) and the CPU implementation
     of attention (rbf_cpu.cpp, parallel over planes with ATen's OpenMP
     thread pool, so it is compiled with -fopenmp and linked against the
     libgomp that torch itself loads)."""
@@ -137,7 +139,8 @@ def build_torch_extension(force=False, verbose=False):
     src = os.path.join(CSRC, 'torch_ext.cpp')
     cpu_src = os.path.join(CSRC, 'rbf_cpu.cpp')
     block_src = os.path.join(CSRC, 'block_ext.cpp')
-    sources = [src, cpu_src, block_src]
+    decoder_src = os.path.join(CSRC, 'decoder_ext.cpp')
+    sources = [src, cpu_src, block_src, decoder_src]
     if not (force or _stale(TORCH_EXT, sources + [LIB] + _headers())):
         return TORCH_EXT
     abi = int(torch._C._GLIBCXX_USE_CXX11_ABI)  # pylint: disable=protected-access
@@ -152,18 +155,21 @@ def build_torch_extension(force=False, verbose=False):
     cpu_obj = os.path.join(BUILD, 'rbf_cpu.o')
     ext_obj = os.path.join(BUILD, 'torch_ext.o')
     block_obj = os.path.join(BUILD, 'block_ext.o')
-    headers = [h for h in _headers() if h.endswith('.h')]
+    decoder_obj = os.path.join(BUILD, 'decoder_ext.o')
+    headers = [h for h in _headers()
+               if h.endswith(('.h', 'philox.cuh'))]
     jobs = [['g++', '-c', '-O3', '-fopenmp'] + common +
             [cpu_src, '-o', cpu_obj],
             ['g++', '-c', '-O2'] + common + [src, '-o', ext_obj],
-            ['g++', '-c', '-O2'] + common + [block_src, '-o', block_obj]]
+            ['g++', '-c', '-O2'] + common + [block_src, '-o', block_obj],
+            ['g++', '-c', '-O2'] + common + [decoder_src, '-o', decoder_obj]]
     jobs = [job for job in jobs
             if force or _stale(job[-1], [job[-3]] + headers)]
     if jobs:
         with concurrent.futures.ThreadPoolExecutor(len(jobs)) as pool:
             list(pool.map(lambda c: _run(c, verbose), jobs))
-    cmd = ['g++', '-shared', ext_obj, cpu_obj, block_obj, '-o', TORCH_EXT,
-           '-L', PKG, '-lvectra_rbf']
+    cmd = ['g++', '-shared', ext_obj, cpu_obj, block_obj, decoder_obj,
+           '-o', TORCH_EXT, '-L', PKG, '-lvectra_rbf']
     for libdir in cpp_extension.library_paths(device_type='cuda'):
         cmd += ['-L', libdir]
     cmd += ['-lc10', '-lc10_cuda', '-ltorch', '-ltorch_cpu', '-ltorch_cuda',

@@ -2,62 +2,16 @@
 // (include/vectra_block.h): argument checks, and each operator's forward and
 // backward pass as a short sequence of matrix products and elementwise
 // kernels on the caller's stream.
-#include "block_common.cuh"
+#include "block_checks.cuh"
 
 namespace vectra {
 namespace {
-
-bool io_dtype_ok(int32_t d) {
-  return d == VECTRA_F32 || d == VECTRA_F16 || d == VECTRA_BF16;
-}
-
-// Checks one tensor: rank, sizes, dtype, and the pointer when it holds
-// elements.
-int check(const vectra_tensor& t, int32_t dtype,
-          std::initializer_list<int64_t> sizes) {
-  if (t.ndim != int32_t(sizes.size())) return VECTRA_ERR_RANK;
-  int64_t count = 1;
-  int i = 0;
-  for (const int64_t s : sizes) {
-    if (t.size[i] != s) return VECTRA_ERR_SHAPE;
-    count *= s;
-    ++i;
-  }
-  if (t.dtype != dtype) return VECTRA_ERR_DTYPE;
-  if (count > 0 && t.data == nullptr) return VECTRA_ERR_NULL;
-  return VECTRA_OK;
-}
-
-// Results need a unit inner stride and rows that do not overlap.
-int check_result(const vectra_tensor& t, int32_t dtype,
-                 std::initializer_list<int64_t> sizes) {
-  const int st = check(t, dtype, sizes);
-  if (st != VECTRA_OK) return st;
-  const int last = t.ndim - 1;
-  if (t.size[last] > 1 && t.stride[last] != 1) return VECTRA_ERR_LAYOUT;
-  if (t.ndim == 2 && t.size[0] > 1 && t.stride[0] < t.size[1])
-    return VECTRA_ERR_LAYOUT;
-  return VECTRA_OK;
-}
-
-bool present(const vectra_tensor& t) { return t.data != nullptr; }
 
 MatView rows_of(const vectra_tensor& t) {  // reduced over the columns
   return {t.data, t.stride[0], t.stride[1]};
 }
 MatView cols_of(const vectra_tensor& t) {  // reduced over the rows
   return {t.data, t.stride[1], t.stride[0]};
-}
-
-#define VECTRA_TRY(expr)                 \
-  do {                                   \
-    const int st_ = (expr);              \
-    if (st_ != VECTRA_OK) return st_;    \
-  } while (0)
-
-int to_status(cudaError_t e, const Workspace& ws) {
-  if (ws.overflow) return VECTRA_ERR_WORKSPACE;
-  return e == cudaSuccess ? VECTRA_OK : VECTRA_ERR_CUDA;
 }
 
 int check_common(const vectra_tensor& x, const vectra_tensor& w,
@@ -385,7 +339,8 @@ int gated_backward(const vectra_gated_grad_args& a, Workspace& ws,
   return VECTRA_OK;
 }
 
-int build_qk(const vectra_qk_args& a, QkProblem* p) {
+int build_qk(const vectra_qk_args& a, const vectra_qk_axes* axes,
+             QkProblem* p) {
   if (a.q.ndim != 4 || a.k.ndim != 4 || a.cos.ndim != 2 || a.sin.ndim != 2)
     return VECTRA_ERR_RANK;
   if (!io_dtype_ok(a.q.dtype)) return VECTRA_ERR_DTYPE;
@@ -405,6 +360,21 @@ int build_qk(const vectra_qk_args& a, QkProblem* p) {
   if (a.positions && a.position_bytes != 4 && a.position_bytes != 8)
     return VECTRA_ERR_DTYPE;
   *p = QkProblem{};
+  if (axes != nullptr) {
+    if (axes->count < 1 || axes->count > VECTRA_MAX_AXES)
+      return VECTRA_ERR_UNSUPPORTED;
+    if (a.positions == nullptr && B * N > 0) return VECTRA_ERR_NULL;
+    int64_t sum = 0;
+    for (int i = 0; i < axes->count; ++i) {
+      if (axes->section[i] < 0) return VECTRA_ERR_SHAPE;
+      p->first_pair[i] = int32_t(sum);
+      sum += axes->section[i];
+      if (sum > R2) return VECTRA_ERR_SHAPE;
+    }
+    if (sum != R2) return VECTRA_ERR_SHAPE;
+    p->axes = axes->count;
+    p->pos_sa = axes->stride;
+  }
   const vectra_tensor* x[2] = {&a.q, &a.k};
   const vectra_tensor* w[2] = {&a.q_weight, &a.k_weight};
   for (int i = 0; i < 2; ++i) {
@@ -450,19 +420,20 @@ int set_result(const vectra_tensor& t, const vectra_tensor& like,
   return VECTRA_OK;
 }
 
-int qk_forward(const vectra_qk_args& a, cudaStream_t stream) {
+int qk_forward(const vectra_qk_args& a, const vectra_qk_axes* axes,
+               cudaStream_t stream) {
   QkProblem p;
-  VECTRA_TRY(build_qk(a, &p));
+  VECTRA_TRY(build_qk(a, axes, &p));
   VECTRA_TRY(set_result(a.q_out, a.q, &p.side[0]));
   VECTRA_TRY(set_result(a.k_out, a.k, &p.side[1]));
   return launch_qk_forward(p, stream) == cudaSuccess ? VECTRA_OK
                                                      : VECTRA_ERR_CUDA;
 }
 
-int qk_backward(const vectra_qk_grad_args& a, Workspace& ws,
-                cudaStream_t stream) {
+int qk_backward_with(const vectra_qk_grad_args& a, const vectra_qk_axes* axes,
+                     Workspace& ws, cudaStream_t stream) {
   QkProblem p;
-  VECTRA_TRY(build_qk(a.fwd, &p));
+  VECTRA_TRY(build_qk(a.fwd, axes, &p));
   const vectra_tensor* x[2] = {&a.fwd.q, &a.fwd.k};
   const vectra_tensor* dy[2] = {&a.dq_out, &a.dk_out};
   const vectra_tensor* dx[2] = {&a.dq, &a.dk};
@@ -483,29 +454,16 @@ int qk_backward(const vectra_qk_grad_args& a, Workspace& ws,
   }
   return to_status(run_qk_backward(p, ws, stream), ws);
 }
-
-template <typename Args, typename F>
-int run_with_workspace(const Args* a, void* stream, F&& f) {
-  if (a == nullptr) return VECTRA_ERR_NULL;
-  Workspace ws;
-  ws.base = static_cast<char*>(a->workspace);
-  ws.size = a->workspace ? a->workspace_bytes : 0;
-  ws.dry = false;
-  if (reinterpret_cast<uintptr_t>(ws.base) & 255) return VECTRA_ERR_WORKSPACE;
-  // Size it first: nothing is launched when it does not fit.
-  Workspace need;
-  const int st = f(*a, need, nullptr);
-  if (st != VECTRA_OK) return st;
-  if (need.used > ws.size) return VECTRA_ERR_WORKSPACE;
-  return f(*a, ws, static_cast<cudaStream_t>(stream));
+int qk_backward(const vectra_qk_grad_args& a, Workspace& ws,
+                cudaStream_t stream) {
+  return qk_backward_with(a, nullptr, ws, stream);
 }
-
-template <typename Args, typename F>
-int64_t workspace_of(const Args* a, F&& f) {
-  if (a == nullptr) return VECTRA_ERR_NULL;
-  Workspace need;
-  const int st = f(*a, need, nullptr);
-  return st != VECTRA_OK ? st : int64_t(need.used);
+// The workspace of the axes' call is its qk part's.
+auto qk_axes_backward(const vectra_qk_axes& axes) {
+  return [&axes](const vectra_qk_grad_args& a, Workspace& ws,
+                 cudaStream_t stream) {
+    return qk_backward_with(a, &axes, ws, stream);
+  };
 }
 
 }  // namespace
@@ -530,11 +488,26 @@ int vectra_gated_linear_backward(const vectra_gated_grad_args* a,
 }
 int vectra_qk_norm_rope_forward(const vectra_qk_args* a, void* stream) {
   if (a == nullptr) return VECTRA_ERR_NULL;
-  return qk_forward(*a, static_cast<cudaStream_t>(stream));
+  return qk_forward(*a, nullptr, static_cast<cudaStream_t>(stream));
 }
 int vectra_qk_norm_rope_backward(const vectra_qk_grad_args* a,
                                  void* stream) {
   return run_with_workspace(a, stream, qk_backward);
+}
+int vectra_qk_norm_rope_axes_forward(const vectra_qk_axes_args* a,
+                                     void* stream) {
+  if (a == nullptr) return VECTRA_ERR_NULL;
+  return qk_forward(a->qk, &a->axes, static_cast<cudaStream_t>(stream));
+}
+int vectra_qk_norm_rope_axes_backward(const vectra_qk_axes_grad_args* a,
+                                      void* stream) {
+  if (a == nullptr) return VECTRA_ERR_NULL;
+  return run_with_workspace(&a->qk, stream, qk_axes_backward(a->axes));
+}
+int64_t vectra_qk_norm_rope_axes_backward_workspace_bytes(
+    const vectra_qk_axes_grad_args* a) {
+  if (a == nullptr) return VECTRA_ERR_NULL;
+  return workspace_of(&a->qk, qk_axes_backward(a->axes));
 }
 
 int64_t vectra_linear_forward_workspace_bytes(const vectra_linear_args* a) {
@@ -570,8 +543,9 @@ const char* vectra_block_strerror(int status) {
              "tables float32, norm weights that type or float32, positions "
              "int32 or int64)";
     case VECTRA_ERR_UNSUPPORTED:
-      return "unsupported activation, a head width above 512, or a size "
-             "above 2^29 - 256";
+      return "unsupported activation, a head width above 512 (in cross "
+             "attention 256), a normalised row above 16384, more than 4 axes, "
+             "or a size above 2^29 - 256";
     case VECTRA_ERR_LAYOUT:
       return "results and rotation tables need a unit inner stride and rows "
              "that do not overlap";

@@ -285,11 +285,20 @@ struct QkProblem {
   const void* pos = nullptr;
   int32_t pos_bytes = 8;
   int64_t pos_sb = 0, pos_sn = 0;
+  // Positions on several axes, pos_sa apart: pairs from first_pair[a] on take
+  // axis a's.
+  int32_t axes = 1;
+  int32_t first_pair[VECTRA_MAX_AXES] = {0};
+  int64_t pos_sa = 0;
   float eps = 0.f;
 };
 cudaError_t launch_qk_forward(const QkProblem& p, cudaStream_t stream);
 cudaError_t run_qk_backward(const QkProblem& p, Workspace& ws,
                             cudaStream_t stream);
+// qk_norm_rope_axes.cu: the same for positions on several axes.
+cudaError_t launch_qk_forward_axes(const QkProblem& p, cudaStream_t stream);
+cudaError_t run_qk_backward_axes(const QkProblem& p, Workspace& ws,
+                                 cudaStream_t stream);
 
 // Largest size of one dimension: tensor-map coordinates are 32-bit, and
 // float32 operands keep three planes of lines in one map.

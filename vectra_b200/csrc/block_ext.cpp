@@ -1,37 +1,31 @@
 // block_ext.cpp: PyTorch registration of the transformer-block operators
 // (include/vectra_block.h) in the vectra_b200 namespace:
 //
-//   linear, gated_linear, qk_norm_rope        differentiable entry points
+//   linear, gated_linear, qk_norm_rope,
+//   qk_norm_rope_axes                         differentiable entry points
 //   linear_with_pre, gated_linear_with_pre    the forward that also returns
 //                                             what the backward needs
 //   linear_backward, gated_linear_backward,
-//   qk_norm_rope_backward                     gradients
+//   qk_norm_rope_backward,
+//   qk_norm_rope_axes_backward                gradients
 //
 // CUDA tensors run the kernels of libvectra_rbf.so on the current stream,
 // with results and workspace from PyTorch's allocator; CPU tensors run the
 // ATen formulation below in float32. The entry points differentiate through
 // C++ autograd functions; the backward operators are not differentiable
 // again (they raise). Fake implementations are in vectra_b200/block.py.
-#include <ATen/ATen.h>
-#include <ATen/cuda/CUDAContext.h>
-#include <c10/cuda/CUDAGuard.h>
 #include <torch/csrc/autograd/autograd_not_implemented_fallback.h>
-#include <torch/csrc/autograd/custom_function.h>
-#include <torch/library.h>
 
 #include <initializer_list>
-#include <optional>
-#include <string>
 #include <tuple>
 #include <utility>
 #include <vector>
 
-#include "vectra_block.h"
+#include "block_ext.h"
 
 namespace {
 
-using at::Tensor;
-using OptTensor = std::optional<Tensor>;
+using namespace vectra_ext;
 
 // ---------------------------------------------------------------------------
 // Shared checks.
@@ -44,37 +38,6 @@ int32_t activation_of(c10::string_view name) {
   if (name == "silu") return VECTRA_ACT_SILU;
   TORCH_CHECK_VALUE(false, "activation must be 'none', 'relu', 'gelu', "
                            "'gelu_tanh' or 'silu', got '", std::string(name), "'");
-}
-
-bool io_dtype(at::ScalarType t) {
-  return t == at::kFloat || t == at::kHalf || t == at::kBFloat16;
-}
-
-int32_t abi_dtype(at::ScalarType t) {
-  switch (t) {
-    case at::kFloat:
-      return VECTRA_F32;
-    case at::kHalf:
-      return VECTRA_F16;
-    case at::kBFloat16:
-      return VECTRA_BF16;
-    default:
-      return -1;
-  }
-}
-
-bool has(const OptTensor& t) { return t.has_value() && t->defined(); }
-
-void check_like(const Tensor& t, const char* name, const Tensor& x) {
-  TORCH_CHECK_VALUE(t.device() == x.device(), name, " must be on ",
-                    x.device(), ", got ", t.device());
-  TORCH_CHECK_VALUE(t.scalar_type() == x.scalar_type(), name, " must be ",
-                    x.scalar_type(), ", got ", t.scalar_type());
-}
-
-void check_sizes(const Tensor& t, const char* name, at::IntArrayRef sizes) {
-  TORCH_CHECK_VALUE(t.sizes() == sizes, name, " must have shape ", sizes,
-                    ", got ", t.sizes());
 }
 
 void check_layer(const Tensor& x, const Tensor& w, const char* w_name) {
@@ -92,93 +55,6 @@ std::vector<int64_t> with_last(at::IntArrayRef sizes, int64_t last) {
   std::vector<int64_t> s = sizes.vec();
   s.back() = last;
   return s;
-}
-
-// [..., C] as [rows, C]: a view where the leading dimensions allow one.
-Tensor as_rows(const Tensor& t) {
-  int64_t rows = 1;
-  for (int64_t i = 0; i + 1 < t.dim(); ++i) rows *= t.size(i);
-  return t.dim() == 2 ? t : t.reshape({rows, t.size(-1)});
-}
-
-vectra_tensor describe(const Tensor& t) {
-  vectra_tensor d{};
-  d.data = t.data_ptr();
-  d.dtype = abi_dtype(t.scalar_type());
-  d.ndim = int32_t(t.dim());
-  for (int64_t i = 0; i < t.dim(); ++i) {
-    d.size[i] = t.size(i);
-    d.stride[i] = t.stride(i);
-  }
-  return d;
-}
-
-vectra_tensor describe(const OptTensor& t) {
-  return has(t) ? describe(*t) : vectra_tensor{};
-}
-
-// The same view as the ABI's description, without making a tensor of it;
-// where the leading dimensions do not allow one, `copy` keeps the copy.
-vectra_tensor describe_rows(const Tensor& t, Tensor* copy) {
-  const int64_t last = t.dim() - 1;
-  int64_t rows = 1, ld = 0;
-  bool regular = true;
-  for (int64_t i = last - 1; i >= 0; --i) {
-    if (t.size(i) != 1) {
-      if (rows == 1) {
-        ld = t.stride(i);
-      } else if (t.stride(i) != ld * rows) {
-        regular = false;
-      }
-    }
-    rows *= t.size(i);
-  }
-  if (!regular && rows > 0) {
-    *copy = as_rows(t);
-    return describe(*copy);
-  }
-  vectra_tensor d{};
-  d.data = t.data_ptr();
-  d.dtype = abi_dtype(t.scalar_type());
-  d.ndim = 2;
-  d.size[0] = rows;
-  d.size[1] = t.size(last);
-  d.stride[0] = rows > 1 ? ld : t.size(last);
-  d.stride[1] = t.stride(last);
-  return d;
-}
-
-[[noreturn]] void raise_status(const char* op, int status) {
-  const char* msg = vectra_block_strerror(status);
-  switch (status) {
-    case VECTRA_ERR_UNSUPPORTED:
-      TORCH_CHECK_NOT_IMPLEMENTED(false, "vectra_b200::", op, ": ", msg);
-    case VECTRA_ERR_CUDA:
-    case VECTRA_ERR_DEVICE:
-    case VECTRA_ERR_WORKSPACE:
-      TORCH_CHECK(false, "vectra_b200::", op, ": ", msg);
-    default:
-      TORCH_CHECK_VALUE(false, "vectra_b200::", op, ": ", msg);
-  }
-  TORCH_CHECK(false, "unreachable");
-}
-
-// Sizes the workspace, allocates it and makes the call.
-template <typename Args, typename Size, typename Call>
-void call_with_workspace(const char* op, Args& a, const Tensor& like,
-                         Size&& size, Call&& call) {
-  const int64_t bytes = size(&a);
-  if (bytes < 0) raise_status(op, int(bytes));
-  Tensor ws;
-  if (bytes > 0) {
-    ws = at::empty({bytes + 256}, like.options().dtype(at::kByte));
-    const uintptr_t p = reinterpret_cast<uintptr_t>(ws.data_ptr());
-    a.workspace = reinterpret_cast<void*>((p + 255) & ~uintptr_t(255));
-    a.workspace_bytes = size_t(bytes);
-  }
-  const int st = call(
-      &a, at::cuda::getCurrentCUDAStream(like.device().index()).stream());
-  if (st != VECTRA_OK) raise_status(op, st);
 }
 
 // ---------------------------------------------------------------------------
@@ -235,11 +111,6 @@ Tensor cpu_act_grad(const Tensor& dy, const Tensor& z, int32_t act) {
     default:
       return dy;
   }
-}
-
-Tensor f32(const Tensor& t) { return t.to(at::kFloat); }
-OptTensor f32(const OptTensor& t) {
-  return has(t) ? OptTensor(f32(*t)) : OptTensor();
 }
 
 // ---------------------------------------------------------------------------
@@ -564,6 +435,13 @@ Grads3 gated_backward_cpu(const Tensor& dh, const Tensor& x,
 // ---------------------------------------------------------------------------
 // qk_norm_rope
 // ---------------------------------------------------------------------------
+void check_positions(const Tensor& positions, const Tensor& q) {
+  TORCH_CHECK_VALUE(positions.device() == q.device() &&
+                        (positions.scalar_type() == at::kLong ||
+                         positions.scalar_type() == at::kInt),
+                    "positions must be int64 or int32 on ", q.device());
+}
+
 void check_qk(const Tensor& q, const Tensor& k, const Tensor& cos,
               const Tensor& sin, const OptTensor& qw, const OptTensor& kw,
               const OptTensor& positions) {
@@ -600,10 +478,7 @@ void check_qk(const Tensor& q, const Tensor& k, const Tensor& cos,
     check_sizes(**w, "norm weights", {d});
   }
   if (has(positions)) {
-    TORCH_CHECK_VALUE(positions->device() == q.device() &&
-                          (positions->scalar_type() == at::kLong ||
-                           positions->scalar_type() == at::kInt),
-                      "positions must be int64 or int32 on ", q.device());
+    check_positions(*positions, q);
     TORCH_CHECK_VALUE(
         positions->dim() <= 2 &&
             (positions->dim() < 1 || positions->size(-1) == 1 ||
@@ -615,14 +490,26 @@ void check_qk(const Tensor& q, const Tensor& k, const Tensor& cos,
   }
 }
 
-// Results follow their input's order of heads and tokens, by the rule of
-// vectra::rbf_attention's output (torch_ext.cpp).
-Tensor empty_like_heads(const Tensor& t) {
-  const int64_t b = t.size(0), h = t.size(1), n = t.size(2), d = t.size(3);
-  if (h > 1 && n > 1 && t.stride(2) > t.stride(1))
-    return at::empty_strided({b, h, n, d}, {n * h * d, d, h * d, 1},
-                             t.options());
-  return at::empty({b, h, n, d}, t.options());
+// The pairs of every axis (qk_norm_rope_axes), and positions [A, B, N].
+void check_axes(const Tensor& positions, at::IntArrayRef sections,
+                const Tensor& q, const Tensor& cos) {
+  const int64_t axes = int64_t(sections.size());
+  TORCH_CHECK_VALUE(axes >= 1 && axes <= VECTRA_MAX_AXES, "1 to ",
+                    VECTRA_MAX_AXES, " axes, got ", axes, " sections");
+  int64_t sum = 0;
+  for (const int64_t n : sections) {
+    TORCH_CHECK_VALUE(n >= 0, "sections must not be negative, got ", sections);
+    sum += n;
+  }
+  TORCH_CHECK_VALUE(sum == cos.size(1), "sections ", sections,
+                    " must add up to the tables' ", cos.size(1), " pairs");
+  check_positions(positions, q);
+  TORCH_CHECK_VALUE(
+      positions.dim() == 3 && positions.size(0) == axes &&
+          (positions.size(1) == 1 || positions.size(1) == q.size(0)) &&
+          (positions.size(2) == 1 || positions.size(2) == q.size(2)),
+      "positions must broadcast to [", axes, ", B, N] = [", axes, ", ",
+      q.size(0), ", ", q.size(2), "], got ", positions.sizes());
 }
 
 vectra_qk_args describe_qk(const Tensor& q, const Tensor& k,
@@ -705,29 +592,122 @@ Grads4 qk_backward_cuda(const Tensor& dq_out, const Tensor& dk_out,
   return {dq, dk, dqw, dkw};
 }
 
-// [B, 1, N, R / 2] rows of a table; rows outside it are NaN.
-Tensor cpu_rows(const Tensor& table, const Tensor& pos) {
-  const int64_t rows = table.size(0);
-  const Tensor inside = (pos >= 0).logical_and(pos < rows);
-  Tensor got =
-      rows > 0
-          ? table.index({pos.clamp(0, rows - 1)})
-          : at::zeros({pos.size(0), pos.size(1), table.size(1)},
-                      table.options());
-  return at::where(inside.unsqueeze(-1), got,
-                   at::full({}, std::nan(""), table.options()))
-      .unsqueeze(1);
+vectra_qk_axes describe_axes(const Tensor& positions, at::IntArrayRef sections,
+                             vectra_qk_args* qk) {
+  vectra_qk_axes axes{};
+  axes.count = int32_t(sections.size());
+  for (int64_t i = 0; i < axes.count; ++i)
+    axes.section[i] = int32_t(sections[size_t(i)]);
+  axes.stride = positions.size(0) > 1 ? positions.stride(0) : 0;
+  qk->positions = positions.numel() > 0 ? positions.data_ptr() : nullptr;
+  qk->position_bytes = int32_t(positions.element_size());
+  for (int i = 0; i < 2; ++i)
+    qk->position_stride[i] =
+        positions.size(i + 1) > 1 ? positions.stride(i + 1) : 0;
+  return axes;
 }
 
-Tensor cpu_turn(const Tensor& x, const Tensor& c, const Tensor& s,
-                const Tensor& pos, int64_t table, bool interleaved) {
+std::tuple<Tensor, Tensor> axes_cuda(
+    const Tensor& q, const Tensor& k, const Tensor& cos, const Tensor& sin,
+    const Tensor& positions, at::IntArrayRef sections, const OptTensor& qw,
+    const OptTensor& kw, double eps, bool interleaved) {
+  check_qk(q, k, cos, sin, qw, kw, {});
+  check_axes(positions, sections, q, cos);
+  c10::cuda::CUDAGuard guard(q.device());
+  Tensor qo = empty_like_heads(q), ko = empty_like_heads(k);
+  vectra_qk_axes_args a{};
+  a.qk = describe_qk(q, k, cos, sin, qw, kw, {}, eps, interleaved);
+  a.axes = describe_axes(positions, sections, &a.qk);
+  a.qk.q_out = describe(qo);
+  a.qk.k_out = describe(ko);
+  const int st = vectra_qk_norm_rope_axes_forward(
+      &a, at::cuda::getCurrentCUDAStream(q.device().index()).stream());
+  if (st != VECTRA_OK) raise_status("qk_norm_rope_axes", st);
+  return {qo, ko};
+}
+
+Grads4 axes_backward_cuda(const Tensor& dq_out, const Tensor& dk_out,
+                          const Tensor& q, const Tensor& k, const Tensor& cos,
+                          const Tensor& sin, const Tensor& positions,
+                          at::IntArrayRef sections, const OptTensor& qw,
+                          const OptTensor& kw, double eps, bool interleaved,
+                          bool need_dw) {
+  check_qk(q, k, cos, sin, qw, kw, {});
+  check_axes(positions, sections, q, cos);
+  check_qk_grad(dq_out, dk_out, q, k);
+  c10::cuda::CUDAGuard guard(q.device());
+  Tensor dq = empty_like_heads(q), dk = empty_like_heads(k);
+  const auto weight = [&](const OptTensor& w) {
+    return has(w) && need_dw ? at::empty_like(*w, at::MemoryFormat::Contiguous)
+                             : at::empty({0}, q.options());
+  };
+  Tensor dqw = weight(qw), dkw = weight(kw);
+  // The workspace is the qk part's.
+  struct Args : vectra_qk_axes_grad_args {
+    void*& workspace = qk.workspace;
+    size_t& workspace_bytes = qk.workspace_bytes;
+  } a{};
+  a.qk.fwd = describe_qk(q, k, cos, sin, qw, kw, {}, eps, interleaved);
+  a.axes = describe_axes(positions, sections, &a.qk.fwd);
+  a.qk.dq_out = describe(dq_out);
+  a.qk.dk_out = describe(dk_out);
+  a.qk.dq = describe(dq);
+  a.qk.dk = describe(dk);
+  if (dqw.numel()) a.qk.dq_weight = describe(dqw);
+  if (dkw.numel()) a.qk.dk_weight = describe(dkw);
+  call_with_workspace("qk_norm_rope_axes_backward", a, q,
+                      vectra_qk_norm_rope_axes_backward_workspace_bytes,
+                      vectra_qk_norm_rope_axes_backward);
+  return {dq, dk, dqw, dkw};
+}
+
+// A token's cosines and sines [B, 1, N, R / 2], NaN for a position outside
+// the tables, and whether none is outside.
+struct CpuAngles {
+  Tensor c, s, inside;  // inside [B, 1, N, 1]
+};
+
+// [B, N, pairs] entries of the columns from `first` on.
+Tensor cpu_rows(const Tensor& table, const Tensor& pos, int64_t first,
+                int64_t pairs) {
+  const int64_t rows = table.size(0);
+  const Tensor part = table.narrow(1, first, pairs);
+  const Tensor inside = (pos >= 0).logical_and(pos < rows);
+  Tensor got = rows > 0 ? part.index({pos.clamp(0, rows - 1)})
+                        : at::zeros({pos.size(0), pos.size(1), pairs},
+                                    table.options());
+  return at::where(inside.unsqueeze(-1), got,
+                   at::full({}, std::nan(""), table.options()));
+}
+
+// positions [A, B, N]; sections: pairs of every axis.
+CpuAngles cpu_angles(const Tensor& cos, const Tensor& sin, const Tensor& pos,
+                     at::IntArrayRef sections) {
+  std::vector<Tensor> c, s;
+  Tensor inside = at::ones({pos.size(1), pos.size(2)}, at::kBool);
+  int64_t first = 0;
+  for (size_t a = 0; a < sections.size(); ++a) {
+    const Tensor p = pos.select(0, int64_t(a));
+    c.push_back(cpu_rows(cos, p, first, sections[a]));
+    s.push_back(cpu_rows(sin, p, first, sections[a]));
+    inside = inside.logical_and((p >= 0).logical_and(p < cos.size(0)));
+    first += sections[a];
+  }
+  inside = inside.unsqueeze(1).unsqueeze(-1);
+  const Tensor nan = at::full({}, std::nan(""), cos.options());
+  return {at::where(inside, at::cat(c, -1).unsqueeze(1), nan),
+          at::where(inside, at::cat(s, -1).unsqueeze(1), nan), inside};
+}
+
+// `back`: by the opposite angles.
+Tensor cpu_turn(const Tensor& x, const CpuAngles& t, bool back,
+                bool interleaved) {
+  const Tensor& c = t.c;
+  const Tensor s = back ? -t.s : t.s;
   const int64_t r2 = c.size(-1), d = x.size(-1);
   const Tensor head = x.narrow(-1, 0, 2 * r2);
   Tensor tail = x.narrow(-1, 2 * r2, d - 2 * r2);
-  const Tensor inside = (pos >= 0).logical_and(pos < table)
-                            .unsqueeze(1)
-                            .unsqueeze(-1);
-  tail = at::where(inside, tail, at::full({}, std::nan(""), x.options()));
+  tail = at::where(t.inside, tail, at::full({}, std::nan(""), x.options()));
   if (interleaved) {
     const Tensor p = head.unflatten(-1, {r2, 2});
     const Tensor a = p.select(-1, 0), b = p.select(-1, 1);
@@ -738,49 +718,42 @@ Tensor cpu_turn(const Tensor& x, const Tensor& c, const Tensor& s,
   return at::cat({a * c - b * s, b * c + a * s, tail}, -1);
 }
 
+// [1, B, N].
 Tensor cpu_positions(const OptTensor& positions, const Tensor& q) {
   const Tensor p = has(positions)
                        ? positions->to(at::kLong)
                        : at::arange(q.size(2), q.options().dtype(at::kLong));
-  return p.expand({q.size(0), q.size(2)});
+  return p.expand({q.size(0), q.size(2)}).unsqueeze(0);
 }
 
-std::tuple<Tensor, Tensor> qk_cpu(const Tensor& q, const Tensor& k,
-                                  const Tensor& cos, const Tensor& sin,
-                                  const OptTensor& qw, const OptTensor& kw,
-                                  const OptTensor& positions, double eps,
-                                  bool interleaved) {
-  check_qk(q, k, cos, sin, qw, kw, positions);
+std::tuple<Tensor, Tensor> cpu_qk_forward(const Tensor& q, const Tensor& k,
+                                          const CpuAngles& angles,
+                                          const OptTensor& qw,
+                                          const OptTensor& kw, double eps,
+                                          bool interleaved) {
   TORCH_CHECK_NOT_IMPLEMENTED(q.size(3) <= 512,
                               "vectra_b200::qk_norm_rope: a head width above "
                               "512");
-  const Tensor pos = cpu_positions(positions, q);
-  const Tensor c = cpu_rows(cos, pos), s = cpu_rows(sin, pos);
   const auto side = [&](const Tensor& x, const OptTensor& w) {
     const Tensor v = f32(x);
     Tensor y = v * at::rsqrt(v.square().mean({-1}, true) + eps);
     if (has(w)) y = y * f32(*w);
-    return empty_like_heads(x).copy_(
-        cpu_turn(y, c, s, pos, cos.size(0), interleaved));
+    return empty_like_heads(x).copy_(cpu_turn(y, angles, false, interleaved));
   };
   return {side(q, qw), side(k, kw)};
 }
 
-Grads4 qk_backward_cpu(const Tensor& dq_out, const Tensor& dk_out,
-                       const Tensor& q, const Tensor& k, const Tensor& cos,
-                       const Tensor& sin, const OptTensor& qw,
-                       const OptTensor& kw, const OptTensor& positions,
-                       double eps, bool interleaved, bool need_dw) {
-  check_qk(q, k, cos, sin, qw, kw, positions);
-  check_qk_grad(dq_out, dk_out, q, k);
-  const Tensor pos = cpu_positions(positions, q);
-  const Tensor c = cpu_rows(cos, pos), s = cpu_rows(sin, pos);
+Grads4 cpu_qk_backward(const Tensor& dq_out, const Tensor& dk_out,
+                       const Tensor& q, const Tensor& k,
+                       const CpuAngles& angles, const OptTensor& qw,
+                       const OptTensor& kw, double eps, bool interleaved,
+                       bool need_dw) {
   const auto side = [&](const Tensor& dy, const Tensor& x,
                         const OptTensor& w) {
     const Tensor v = f32(x);
     const Tensor r = at::rsqrt(v.square().mean({-1}, true) + eps);
     const Tensor n = v * r;
-    Tensor g = cpu_turn(f32(dy), c, -s, pos, cos.size(0), interleaved);
+    Tensor g = cpu_turn(f32(dy), angles, true, interleaved);
     Tensor dw = has(w) && need_dw
                     ? (g * n).sum(at::IntArrayRef{0, 1, 2})
                           .to(w->scalar_type())
@@ -792,6 +765,58 @@ Grads4 qk_backward_cpu(const Tensor& dq_out, const Tensor& dk_out,
   const auto [dq, dqw] = side(dq_out, q, qw);
   const auto [dk, dkw] = side(dk_out, k, kw);
   return {dq, dk, dqw, dkw};
+}
+
+std::tuple<Tensor, Tensor> qk_cpu(const Tensor& q, const Tensor& k,
+                                  const Tensor& cos, const Tensor& sin,
+                                  const OptTensor& qw, const OptTensor& kw,
+                                  const OptTensor& positions, double eps,
+                                  bool interleaved) {
+  check_qk(q, k, cos, sin, qw, kw, positions);
+  return cpu_qk_forward(
+      q, k, cpu_angles(cos, sin, cpu_positions(positions, q), {cos.size(1)}),
+      qw, kw, eps, interleaved);
+}
+
+Grads4 qk_backward_cpu(const Tensor& dq_out, const Tensor& dk_out,
+                       const Tensor& q, const Tensor& k, const Tensor& cos,
+                       const Tensor& sin, const OptTensor& qw,
+                       const OptTensor& kw, const OptTensor& positions,
+                       double eps, bool interleaved, bool need_dw) {
+  check_qk(q, k, cos, sin, qw, kw, positions);
+  check_qk_grad(dq_out, dk_out, q, k);
+  return cpu_qk_backward(
+      dq_out, dk_out, q, k,
+      cpu_angles(cos, sin, cpu_positions(positions, q), {cos.size(1)}), qw, kw,
+      eps, interleaved, need_dw);
+}
+
+std::tuple<Tensor, Tensor> axes_cpu(
+    const Tensor& q, const Tensor& k, const Tensor& cos, const Tensor& sin,
+    const Tensor& positions, at::IntArrayRef sections, const OptTensor& qw,
+    const OptTensor& kw, double eps, bool interleaved) {
+  check_qk(q, k, cos, sin, qw, kw, {});
+  check_axes(positions, sections, q, cos);
+  const Tensor pos = positions.to(at::kLong).expand(
+      {positions.size(0), q.size(0), q.size(2)});
+  return cpu_qk_forward(q, k, cpu_angles(cos, sin, pos, sections), qw, kw, eps,
+                        interleaved);
+}
+
+Grads4 axes_backward_cpu(const Tensor& dq_out, const Tensor& dk_out,
+                         const Tensor& q, const Tensor& k, const Tensor& cos,
+                         const Tensor& sin, const Tensor& positions,
+                         at::IntArrayRef sections, const OptTensor& qw,
+                         const OptTensor& kw, double eps, bool interleaved,
+                         bool need_dw) {
+  check_qk(q, k, cos, sin, qw, kw, {});
+  check_axes(positions, sections, q, cos);
+  check_qk_grad(dq_out, dk_out, q, k);
+  const Tensor pos = positions.to(at::kLong).expand(
+      {positions.size(0), q.size(0), q.size(2)});
+  return cpu_qk_backward(dq_out, dk_out, q, k,
+                         cpu_angles(cos, sin, pos, sections), qw, kw, eps,
+                         interleaved, need_dw);
 }
 
 // ---------------------------------------------------------------------------
@@ -920,40 +945,6 @@ Tensor gated_below(const Tensor& x, const Tensor& wg, const Tensor& wu,
   return op.call(x, wg, wu, bg, bu, activation);
 }
 
-using torch::autograd::AutogradContext;
-using torch::autograd::Function;
-using torch::autograd::variable_list;
-
-bool wants_grad(const Tensor& t) { return t.defined() && t.requires_grad(); }
-bool wants_grad(const OptTensor& t) { return has(t) && t->requires_grad(); }
-
-bool has_tangent(const Tensor& t) {
-  return t.defined() && t._fw_grad(/*level=*/0).defined();
-}
-bool has_tangent(const OptTensor& t) { return has(t) && has_tangent(*t); }
-
-// The operators have no forward-mode formula; below autograd a tangent would
-// be dropped, which reads as zero.
-template <typename... Args>
-void refuse_tangents(const char* op, const Args&... args) {
-  TORCH_CHECK_NOT_IMPLEMENTED(
-      !(has_tangent(args) || ...), "vectra_b200::", op,
-      ": forward-mode differentiation is not implemented");
-}
-
-OptTensor optional(const Tensor& t) {
-  return t.defined() ? OptTensor(t) : OptTensor();
-}
-
-// Backward calls go straight to the kernels unless their results are to be
-// differentiated again, which the operators' own autograd entry refuses.
-struct BelowUnlessRecording {
-  std::optional<at::AutoDispatchBelowADInplaceOrView> below;
-  BelowUnlessRecording() {
-    if (!at::GradMode::is_enabled()) below.emplace();
-  }
-};
-
 // What a backward pass has to know, in one number: which inputs want a
 // gradient, and the activation.
 int64_t pack_call(const std::string& activation,
@@ -967,13 +958,6 @@ const char* activation_name(int64_t activation) {
   static const char* const names[] = {"none", "relu", "gelu", "gelu_tanh",
                                       "silu"};
   return names[activation];
-}
-
-// What stands for an input that the backward pass reads the shape of only:
-// one element, expanded. Saving the input itself would keep its memory and
-// forbid writing it in place.
-Tensor shape_of(const Tensor& t) {
-  return at::empty({1}, t.options()).expand_symint(t.sym_sizes());
 }
 
 struct LinearFunction : public Function<LinearFunction> {
@@ -1104,6 +1088,96 @@ struct QkFunction : public Function<QkFunction> {
   }
 };
 
+std::tuple<Tensor, Tensor> call_axes(
+    const Tensor& q, const Tensor& k, const Tensor& cos, const Tensor& sin,
+    const Tensor& positions, at::IntArrayRef sections, const OptTensor& qw,
+    const OptTensor& kw, double eps, bool interleaved) {
+  static const auto op =
+      c10::Dispatcher::singleton()
+          .findSchemaOrThrow("vectra_b200::qk_norm_rope_axes", "")
+          .typed<std::tuple<Tensor, Tensor>(
+              const Tensor&, const Tensor&, const Tensor&, const Tensor&,
+              const Tensor&, at::IntArrayRef, const OptTensor&,
+              const OptTensor&, double, bool)>();
+  return op.call(q, k, cos, sin, positions, sections, qw, kw, eps,
+                 interleaved);
+}
+
+Grads4 call_axes_backward(const Tensor& dq, const Tensor& dk, const Tensor& q,
+                          const Tensor& k, const Tensor& cos,
+                          const Tensor& sin, const Tensor& positions,
+                          at::IntArrayRef sections, const OptTensor& qw,
+                          const OptTensor& kw, double eps, bool interleaved,
+                          bool need_dw) {
+  static const auto op =
+      c10::Dispatcher::singleton()
+          .findSchemaOrThrow("vectra_b200::qk_norm_rope_axes_backward", "")
+          .typed<Grads4(const Tensor&, const Tensor&, const Tensor&,
+                        const Tensor&, const Tensor&, const Tensor&,
+                        const Tensor&, at::IntArrayRef, const OptTensor&,
+                        const OptTensor&, double, bool, bool)>();
+  return op.call(dq, dk, q, k, cos, sin, positions, sections, qw, kw, eps,
+                 interleaved, need_dw);
+}
+
+struct AxesFunction : public Function<AxesFunction> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& q,
+                               const Tensor& k, const Tensor& cos,
+                               const Tensor& sin, const Tensor& positions,
+                               const std::vector<int64_t>& sections,
+                               const OptTensor& qw, const OptTensor& kw,
+                               double eps, bool interleaved) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    auto [qo, ko] = call_axes(q, k, cos, sin, positions, sections, qw, kw,
+                              eps, interleaved);
+    ctx->save_for_backward({q, k, cos, sin, positions, qw.value_or(Tensor()),
+                            kw.value_or(Tensor())});
+    ctx->saved_data["eps"] = eps;
+    ctx->saved_data["sections"] = sections;
+    ctx->saved_data["call"] =
+        pack_call("none", {wants_grad(q), wants_grad(k), wants_grad(qw),
+                           wants_grad(kw), interleaved});
+    return {qo, ko};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto s = ctx->get_saved_variables();
+    const int64_t packed = ctx->saved_data["call"].toInt();
+    const bool dqw = packed & 4, dkw = packed & 8;
+    variable_list out(10);
+    if (!grads[0].defined() && !grads[1].defined()) return out;
+    BelowUnlessRecording below;
+    // A result that nothing used has no gradient: its share is zero.
+    const Tensor gq = grads[0].defined() ? grads[0] : at::zeros_like(s[0]);
+    const Tensor gk = grads[1].defined() ? grads[1] : at::zeros_like(s[1]);
+    auto [dq, dk, gqw, gkw] = call_axes_backward(
+        gq, gk, s[0], s[1], s[2], s[3], s[4],
+        ctx->saved_data["sections"].toIntVector(), optional(s[5]),
+        optional(s[6]), ctx->saved_data["eps"].toDouble(),
+        (packed & 16) != 0, dqw || dkw);
+    if (packed & 1) out[0] = dq;
+    if (packed & 2) out[1] = dk;
+    if (dqw) out[6] = gqw;
+    if (dkw) out[7] = gkw;
+    return out;
+  }
+};
+
+std::tuple<Tensor, Tensor> axes_autograd(
+    const Tensor& q, const Tensor& k, const Tensor& cos, const Tensor& sin,
+    const Tensor& positions, at::IntArrayRef sections, const OptTensor& qw,
+    const OptTensor& kw, double eps, bool interleaved) {
+  refuse_tangents("qk_norm_rope_axes", q, k, cos, sin, qw, kw);
+  if (at::GradMode::is_enabled() && (wants_grad(q) || wants_grad(k) ||
+                                     wants_grad(qw) || wants_grad(kw))) {
+    auto out = AxesFunction::apply(q, k, cos, sin, positions, sections.vec(),
+                                   qw, kw, eps, interleaved);
+    return {out[0], out[1]};
+  }
+  at::AutoDispatchBelowADInplaceOrView below;
+  return call_axes(q, k, cos, sin, positions, sections, qw, kw, eps,
+                   interleaved);
+}
+
 Tensor linear_autograd(const Tensor& x, const Tensor& w,
                        const OptTensor& bias, const OptTensor& residual,
                        c10::string_view activation) {
@@ -1214,6 +1288,16 @@ TORCH_LIBRARY_FRAGMENT(vectra_b200, m) {
       "Tensor k, Tensor cos, Tensor sin, Tensor? q_weight, "
       "Tensor? k_weight, Tensor? positions, float eps, bool interleaved, "
       "bool need_dw) -> (Tensor, Tensor, Tensor, Tensor)");
+  m.def(
+      "qk_norm_rope_axes(Tensor q, Tensor k, Tensor cos, Tensor sin, "
+      "Tensor positions, int[] sections, Tensor? q_weight=None, "
+      "Tensor? k_weight=None, float eps=1e-6, bool interleaved=False) "
+      "-> (Tensor, Tensor)");
+  m.def(
+      "qk_norm_rope_axes_backward(Tensor dq_out, Tensor dk_out, Tensor q, "
+      "Tensor k, Tensor cos, Tensor sin, Tensor positions, int[] sections, "
+      "Tensor? q_weight, Tensor? k_weight, float eps, bool interleaved, "
+      "bool need_dw) -> (Tensor, Tensor, Tensor, Tensor)");
 }
 
 TORCH_LIBRARY_IMPL(vectra_b200, CUDA, m) {
@@ -1225,6 +1309,8 @@ TORCH_LIBRARY_IMPL(vectra_b200, CUDA, m) {
   m.impl("gated_linear_backward", &gated_backward_impl<gated_backward_cuda>);
   m.impl("qk_norm_rope", &qk_cuda);
   m.impl("qk_norm_rope_backward", &qk_backward_cuda);
+  m.impl("qk_norm_rope_axes", &axes_cuda);
+  m.impl("qk_norm_rope_axes_backward", &axes_backward_cuda);
 }
 
 TORCH_LIBRARY_IMPL(vectra_b200, CPU, m) {
@@ -1236,14 +1322,18 @@ TORCH_LIBRARY_IMPL(vectra_b200, CPU, m) {
   m.impl("gated_linear_backward", &gated_backward_impl<gated_backward_cpu>);
   m.impl("qk_norm_rope", &qk_cpu);
   m.impl("qk_norm_rope_backward", &qk_backward_cpu);
+  m.impl("qk_norm_rope_axes", &axes_cpu);
+  m.impl("qk_norm_rope_axes_backward", &axes_backward_cpu);
 }
 
 TORCH_LIBRARY_IMPL(vectra_b200, Autograd, m) {
   m.impl("linear", &linear_autograd);
   m.impl("gated_linear", &gated_autograd);
   m.impl("qk_norm_rope", &qk_autograd);
+  m.impl("qk_norm_rope_axes", &axes_autograd);
   for (const char* op :
        {"linear_with_pre", "linear_backward", "gated_linear_with_pre",
-        "gated_linear_backward", "qk_norm_rope_backward"})
+        "gated_linear_backward", "qk_norm_rope_backward",
+        "qk_norm_rope_axes_backward"})
     m.impl(op, torch::autograd::autogradNotImplementedFallback());
 }

@@ -1,0 +1,201 @@
+// cross_finish.cu: what attention to an encoder's states needs beside its
+// tile kernels (cross.cuh): c_i = e_i . out_i before the backward pass, and
+// the joins of an axis that was split over blocks, in the parts' order.
+#include "cross.cuh"
+
+namespace vectra {
+namespace {
+
+// One warp a row; memory-bound, a row's 64 to 512 bytes at a time.
+template <typename T>
+__global__ void __launch_bounds__(256)
+    delta_kernel(const __grid_constant__ CrossProblem p, float* delta) {
+  allow_dependents();
+  grid_dependency_wait();
+  const int64_t rows = p.B * p.H * p.Nq;
+  const int lane = threadIdx.x % 32;
+  for (int64_t r = int64_t(blockIdx.x) * 8 + threadIdx.x / 32; r < rows;
+       r += int64_t(gridDim.x) * 8) {
+    const int64_t bh = r / p.Nq, i = r - bh * p.Nq;
+    const int64_t b = bh / p.H, h = bh - b * p.H;
+    const T* o = static_cast<const T*>(p.out) + b * p.so[0] + h * p.so[1] +
+                 i * p.so[2];
+    const T* e = static_cast<const T*>(p.dout) + b * p.se[0] + h * p.se[1] +
+                 i * p.se[2];
+    const T* rest = static_cast<const T*>(p.rest) + r * p.Dv;
+    float t = 0.f;
+    for (int d = lane; d < p.Dv; d += 32) {
+      float x = to_f32(o[d]);
+      if (p.rest) x += to_f32(rest[d]);
+      t = fmaf(x, to_f32(e[d * p.se[3]]), t);
+    }
+    t = warp_sum(t);
+    if (lane == 0) delta[r] = t;
+  }
+}
+
+// One warp a row: the largest maximum over the parts, then every part's sum
+// and result brought to it.
+template <typename T>
+__global__ void __launch_bounds__(256)
+    join_kernel(const __grid_constant__ CrossProblem p) {
+  allow_dependents();
+  grid_dependency_wait();
+  const int64_t rows = p.B * p.H * p.Nq;
+  const int lane = threadIdx.x % 32;
+  for (int64_t r = int64_t(blockIdx.x) * 8 + threadIdx.x / 32; r < rows;
+       r += int64_t(gridDim.x) * 8) {
+    const int64_t bh = r / p.Nq, i = r - bh * p.Nq;
+    const int64_t b = bh / p.H, h = bh - b * p.H;
+    const float2* ml = reinterpret_cast<const float2*>(p.part_ml) + r;
+    float m = kNegInf;
+    bool nan = false;
+    for (int s = 0; s < p.splits; ++s) {
+      const float x = ml[s * rows].x;
+      m = fmaxf(m, x);
+      nan = nan || x != x;
+    }
+    if (nan) m = NAN;
+    float l = 0.f;
+    float acc[kMaxCrossWidth / 32];
+#pragma unroll
+    for (int c = 0; c < kMaxCrossWidth / 32; ++c) acc[c] = 0.f;
+    for (int s = 0; s < p.splits; ++s) {
+      const float2 t = ml[s * rows];
+      // A part whose keys all weigh nothing (or that has none) adds nothing.
+      if (t.x == kNegInf) continue;
+      const float f = fast_exp2(t.x - m);
+      l = fmaf(t.y, f, l);
+      const float* o = p.part + (s * rows + r) * p.Dv;
+#pragma unroll
+      for (int c = 0; c < kMaxCrossWidth / 32; ++c)
+        if (c * 32 + lane < p.Dv) acc[c] = fmaf(o[c * 32 + lane], f, acc[c]);
+    }
+    const bool any = cross_length(p, b) > 0;
+    T* out = static_cast<T*>(p.out) + b * p.so[0] + h * p.so[1] + i * p.so[2];
+    T* rest = p.rest ? static_cast<T*>(p.rest) + r * p.Dv : nullptr;
+#pragma unroll
+    for (int c = 0; c < kMaxCrossWidth / 32; ++c) {
+      const int d = c * 32 + lane;
+      if (d < p.Dv)
+        store_with_rest<T>(out + d, rest ? rest + d : nullptr,
+                           any ? acc[c] / l : 0.f);
+    }
+    if (p.lse && lane == 0) p.lse[r] = any ? m + log2f(l) : INFINITY;
+  }
+}
+
+struct SumArgs {
+  const float* part;
+  void* out;
+  int64_t H, N, rows;
+  int64_t so[3];
+  int splits, width;
+};
+template <typename T>
+__global__ void __launch_bounds__(256) sum_kernel(const SumArgs a) {
+  allow_dependents();
+  grid_dependency_wait();
+  const int lane = threadIdx.x % 32;
+  for (int64_t r = int64_t(blockIdx.x) * 8 + threadIdx.x / 32; r < a.rows;
+       r += int64_t(gridDim.x) * 8) {
+    const int64_t bh = r / a.N, i = r - bh * a.N;
+    const int64_t b = bh / a.H, h = bh - b * a.H;
+    T* out = static_cast<T*>(a.out) + b * a.so[0] + h * a.so[1] + i * a.so[2];
+    for (int d = lane; d < a.width; d += 32) {
+      float t = 0.f;
+      for (int s = 0; s < a.splits; ++s)
+        t += a.part[(s * a.rows + r) * a.width + d];
+      out[d] = from_f32<T>(t);
+    }
+  }
+}
+
+// One block a head of a sequence. A row's three sums over its parts are
+// X = sum z d, Y = sum P d and Z = sum z, of distances d; its share is
+// -(X - Y Z), where Z is what rounding left of zero.
+__global__ void __launch_bounds__(256)
+    dscale_kernel(const __grid_constant__ CrossProblem p, int splits) {
+  __shared__ double sums[8];
+  allow_dependents();
+  grid_dependency_wait();
+  const int64_t rows = p.B * p.H * p.Nq;
+  const int64_t first = int64_t(blockIdx.x) * p.Nq;
+  double t = 0.0;
+  for (int64_t i = threadIdx.x; i < p.Nq; i += blockDim.x) {
+    float x = 0.f, y = 0.f, z = 0.f;
+    for (int s = 0; s < splits; ++s) {
+      const float* w = p.dscale_rows + (s * rows + first + i) * 3;
+      x += w[0];
+      y += w[1];
+      z += w[2];
+    }
+    // Rounded products: over a single key the difference is exactly zero.
+    t -= double(__fsub_rn(x, __fmul_rn(y, z)));
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+  if (threadIdx.x % 32 == 0) sums[threadIdx.x / 32] = t;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    double all = 0.0;
+    for (int w = 0; w < 8; ++w) all += sums[w];
+    p.dscale[blockIdx.x] = float(all);
+  }
+}
+
+unsigned row_blocks(int64_t rows) {
+  const int64_t blocks = (rows + 7) / 8;
+  const int64_t most = int64_t(device_sm_count()) * 16;
+  return unsigned(blocks < most ? blocks : most);
+}
+
+}  // namespace
+
+cudaError_t launch_cross_delta(const CrossProblem& p, float* delta,
+                               cudaStream_t stream) {
+  const int64_t rows = p.B * p.H * p.Nq;
+  if (rows == 0) return cudaSuccess;
+  count_launches(1);
+  return with_dtype(p.dtype, [&](auto* t) {
+    using T = std::remove_pointer_t<decltype(t)>;
+    return launch_pdl(delta_kernel<T>, dim3(row_blocks(rows)), dim3(256), 0,
+                      stream, p, delta);
+  });
+}
+
+cudaError_t launch_cross_join(const CrossProblem& p, cudaStream_t stream) {
+  const int64_t rows = p.B * p.H * p.Nq;
+  if (rows == 0) return cudaSuccess;
+  count_launches(1);
+  return with_dtype(p.dtype, [&](auto* t) {
+    using T = std::remove_pointer_t<decltype(t)>;
+    return launch_pdl(join_kernel<T>, dim3(row_blocks(rows)), dim3(256), 0,
+                      stream, p);
+  });
+}
+
+cudaError_t launch_cross_sum(int32_t dtype, const float* part, int splits,
+                             int64_t B, int64_t H, int64_t N, int width,
+                             void* out, const int64_t* so,
+                             cudaStream_t stream) {
+  const SumArgs a{part, out, H, N, B * H * N, {so[0], so[1], so[2]}, splits,
+                  width};
+  if (a.rows == 0 || width == 0) return cudaSuccess;
+  count_launches(1);
+  return with_dtype(dtype, [&](auto* t) {
+    using T = std::remove_pointer_t<decltype(t)>;
+    return launch_pdl(sum_kernel<T>, dim3(row_blocks(a.rows)), dim3(256), 0,
+                      stream, a);
+  });
+}
+
+cudaError_t launch_cross_dscale(const CrossProblem& p, int splits,
+                                cudaStream_t stream) {
+  if (p.B * p.H == 0) return cudaSuccess;
+  count_launches(1);
+  return launch_pdl(dscale_kernel, dim3(unsigned(p.B * p.H)), dim3(256), 0,
+                    stream, p, splits);
+}
+
+}  // namespace vectra

@@ -54,6 +54,7 @@ struct CrossProblem {
   float* part = nullptr;     // out or dq or dk: [splits][rows][width]
   float* part_v = nullptr;   // dv
   float* part_ml = nullptr;  // forward: [splits][rows][2], maximum and sum
+  float* part_l = nullptr;   // [splits][rows]: the sum for lse, where another
   unsigned int* err = nullptr;
 };
 
@@ -91,6 +92,13 @@ cudaError_t run_cross_simple_forward(const CrossProblem& p, Workspace& ws,
                                      cudaStream_t stream);
 cudaError_t run_cross_simple_backward(const CrossProblem& p, Workspace& ws,
                                       cudaStream_t stream);
+
+// cross_tc.cu: bf16 and f16 on the tensor cores, widths up to 128.
+bool cross_tc_supports(const CrossProblem& p, bool backward);
+cudaError_t run_cross_tc_forward(const CrossProblem& p, Workspace& ws,
+                                 cudaStream_t stream);
+cudaError_t run_cross_tc_backward(const CrossProblem& p, Workspace& ws,
+                                  cudaStream_t stream);
 
 // cross_finish.cu.
 // c_i of every row into delta.

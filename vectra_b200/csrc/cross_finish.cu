@@ -56,7 +56,7 @@ __global__ void __launch_bounds__(256)
       nan = nan || x != x;
     }
     if (nan) m = NAN;
-    float l = 0.f;
+    float l = 0.f, l_lse = 0.f;
     float acc[kMaxCrossWidth / 32];
 #pragma unroll
     for (int c = 0; c < kMaxCrossWidth / 32; ++c) acc[c] = 0.f;
@@ -66,6 +66,7 @@ __global__ void __launch_bounds__(256)
       if (t.x == kNegInf) continue;
       const float f = fast_exp2(t.x - m);
       l = fmaf(t.y, f, l);
+      l_lse = fmaf(p.part_l ? p.part_l[s * rows + r] : t.y, f, l_lse);
       const float* o = p.part + (s * rows + r) * p.Dv;
 #pragma unroll
       for (int c = 0; c < kMaxCrossWidth / 32; ++c)
@@ -81,7 +82,7 @@ __global__ void __launch_bounds__(256)
         store_with_rest<T>(out + d, rest ? rest + d : nullptr,
                            any ? acc[c] / l : 0.f);
     }
-    if (p.lse && lane == 0) p.lse[r] = any ? m + log2f(l) : INFINITY;
+    if (p.lse && lane == 0) p.lse[r] = any ? m + log2f(l_lse) : INFINITY;
   }
 }
 

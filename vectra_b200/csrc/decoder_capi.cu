@@ -261,7 +261,10 @@ int cross_forward(const vectra_cross_args& a, Workspace& ws,
   CrossProblem p;
   VECTRA_TRY(build_cross(a, &p));
   p.err = ws.dry ? nullptr : device_error_ptr();
-  return to_status(run_cross_simple_forward(p, ws, stream), ws);
+  return to_status(cross_tc_supports(p, false)
+                       ? run_cross_tc_forward(p, ws, stream)
+                       : run_cross_simple_forward(p, ws, stream),
+                   ws);
 }
 
 int cross_backward(const vectra_cross_grad_args& a, Workspace& ws,
@@ -286,7 +289,10 @@ int cross_backward(const vectra_cross_grad_args& a, Workspace& ws,
     p.dscale = static_cast<float*>(const_cast<void*>(a.dscale.data));
   }
   p.err = ws.dry ? nullptr : device_error_ptr();
-  return to_status(run_cross_simple_backward(p, ws, stream), ws);
+  return to_status(cross_tc_supports(p, true)
+                       ? run_cross_tc_backward(p, ws, stream)
+                       : run_cross_simple_backward(p, ws, stream),
+                   ws);
 }
 
 }  // namespace

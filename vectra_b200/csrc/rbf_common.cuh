@@ -373,6 +373,13 @@ bool make_tile_map(CUtensorMap* map, const void* base, int dtype, int64_t B,
                    int64_t H, int64_t N, int64_t D, const int64_t* s,
                    int box_rows, int box_cols = 64);
 
+// A [B, H, N, D] view whose H = Hk * G heads are taken G at a time, as a 5-D
+// map with a box of 64 columns by G heads by `box_rows` tokens, SWIZZLE_128B:
+// rows of the box are (token, head of the group).
+bool make_group_map(CUtensorMap* map, const void* base, int dtype, int64_t B,
+                    int64_t Hk, int64_t G, int64_t N, int64_t D,
+                    const int64_t* s, int box_rows);
+
 // A matrix of `outer` lines of `inner` contiguous bf16/f16 elements, `ld`
 // apart, as a 2-D map with a box of 64 elements by `box_lines` lines,
 // SWIZZLE_128B; elements outside read as zeros.

@@ -71,6 +71,32 @@ bool make_tile_map(CUtensorMap* map, const void* base, int dtype, int64_t B,
   });
 }
 
+bool make_group_map(CUtensorMap* map, const void* base, int dtype, int64_t B,
+                    int64_t Hk, int64_t G, int64_t N, int64_t D,
+                    const int64_t* s, int box_rows) {
+  auto fn = encode_fn();
+  if (!fn) return false;
+  cuuint64_t dims[5] = {cuuint64_t(D), cuuint64_t(G), cuuint64_t(N),
+                        cuuint64_t(Hk), cuuint64_t(B)};
+  cuuint64_t strides[4] = {cuuint64_t(s[1] * 2), cuuint64_t(s[2] * 2),
+                           cuuint64_t(s[1] * G * 2), cuuint64_t(s[0] * 2)};
+  // Strides of size-1 dimensions are never used; give them valid values.
+  const cuuint64_t line = cuuint64_t(D * 2 + 15) / 16 * 16;
+  for (int i = 0; i < 4; ++i)
+    if (dims[i + 1] == 1) strides[i] = line;
+  cuuint32_t box[5] = {64, cuuint32_t(G), cuuint32_t(box_rows), 1, 1};
+  cuuint32_t estr[5] = {1, 1, 1, 1, 1};
+  return encode([&] {
+    return fn(map,
+              dtype == VECTRA_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                   : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+              5, const_cast<void*>(base), dims, strides, box, estr,
+              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+              CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  });
+}
+
 bool make_line_map(CUtensorMap* map, const void* base, int dtype,
                    int64_t inner, int64_t outer, int64_t ld, int box_lines) {
   auto fn = encode_fn();

@@ -257,7 +257,8 @@ typedef struct {
  *  out [B,H,Nq,Dv]: unit inner stride.
  * For the backward pass (data NULL: not wanted):
  *  lse [B,H,Nq] F32, contiguous: log2 of the sum of each row's weights before
- *  division, infinity for a sequence of length 0.
+ *  division (in 16-bit types without their common factor exp(-scale |q|^2)),
+ *  infinity for a sequence of length 0.
  *  rest [B,H,Nq,Dv], of 16-bit tensors only, contiguous, their type: what out's
  *  rounding left, itself rounded. The backward pass subtracts numbers that are
  *  nearly equal where a row has one large weight, and out alone would decide

@@ -466,17 +466,24 @@ class RbfBlock(nn.Module):
     with gradients the same formula runs as matrix products, and the layers
     around it train through this module's operators. `.to(dtype)` and its
     like leave the rotation tables and `log_scale` in float32.
+
+    With `sections`, positions have an axis each (`qk_norm_rope_axes`) and have
+    to be given.
     """
 
     def __init__(self, d_model: int, heads: int, ffn: int,
                  activation: str = 'silu', max_positions: int = 4096,
-                 device=None, dtype=None):
+                 device=None, dtype=None, sections=None):
         super().__init__()
         if d_model % heads or (d_model // heads) % 2:
             raise ValueError('d_model must be an even multiple of heads')
+        if sections is not None and \
+                sum(sections) != d_model // heads // 2:
+            raise ValueError('sections must add up to half the head width')
         kw = {'device': device, 'dtype': dtype}
         self.heads, self.head_dim = heads, d_model // heads
         self.activation = activation
+        self.sections = None if sections is None else tuple(sections)
         self.norm1 = nn.LayerNorm(d_model, **kw)
         self.qkv = nn.Linear(d_model, 3 * d_model, **kw)
         self.q_weight = nn.Parameter(torch.ones(self.head_dim, **kw))
@@ -531,23 +538,113 @@ class RbfBlock(nn.Module):
     def forward(self, x, key_bias=None, positions=None):
         """x [B, N, d_model]; key_bias broadcastable to [B, 1|H, 1, N] (0 or
         -inf); positions as in `qk_norm_rope` (one outside the tables of
-        max_positions rows makes its token NaN). Without positions, N above
-        max_positions raises ValueError."""
+        max_positions rows makes its token NaN), with sections as in
+        `qk_norm_rope_axes`. Without positions, sections or N above
+        max_positions raise ValueError."""
         b, n, _ = x.shape
+        if positions is None and self.sections is not None:
+            raise ValueError('a block with sections needs positions')
         if positions is None and n > self.cos.shape[0]:
             raise ValueError(f'{n} tokens, but max_positions is '
                              f'{self.cos.shape[0]}')
         qkv = linear(self.norm1(x), self.qkv.weight, self.qkv.bias)
         q, k, v = qkv.view(b, n, 3, self.heads,
                            self.head_dim).permute(2, 0, 3, 1, 4)
-        q, k = qk_norm_rope(q, k, self.cos, self.sin, self.q_weight,
-                            self.k_weight, positions)
+        if self.sections is not None:
+            q, k = qk_norm_rope_axes(q, k, self.cos, self.sin, positions,
+                                     self.sections, self.q_weight,
+                                     self.k_weight)
+        else:
+            q, k = qk_norm_rope(q, k, self.cos, self.sin, self.q_weight,
+                                self.k_weight, positions)
         a = self._attend(q, k, v, key_bias)
         a = a.transpose(1, 2).reshape(b, n, -1)
         x = linear(a, self.out.weight, self.out.bias, residual=x)
         h = gated_linear(self.norm2(x), self.gate.weight, self.up.weight,
                          self.gate.bias, self.up.bias, self.activation)
         return linear(h, self.down.weight, self.down.bias, residual=x)
+
+
+class RbfCrossBlock(nn.Module):
+    """A transformer block whose attention reads an encoder's states: RBF
+    cross attention and a gated feed-forward layer, each between two RMS
+    norms, with a learned gate and dropout on its way into the residual
+    stream.
+
+    It runs the same operators with and without gradients. `.to(dtype)` and
+    its like leave `log_scale` in float32.
+    """
+
+    # Dropout's streams of one block: attention, feed-forward, hidden layer.
+    STREAMS = 3
+
+    def __init__(self, d_model: int, d_states: int, heads: int,
+                 kv_heads: int, ffn: int, activation: str = 'silu',
+                 dropout: float = 0.0, residual_scale: float = 1.0,
+                 device=None, dtype=None):
+        super().__init__()
+        if d_model % heads or heads % kv_heads:
+            raise ValueError('d_model must be a multiple of heads, and heads '
+                             'of kv_heads')
+        kw = {'device': device, 'dtype': dtype}
+        self.heads, self.kv_heads = heads, kv_heads
+        self.head_dim = d_model // heads
+        self.activation, self.p = activation, dropout
+        self.residual_scale = residual_scale
+        for name in ('norm1', 'norm2', 'attn_norm', 'ffn_norm', 'attn_gate',
+                     'ffn_gate'):
+            setattr(self, name, nn.Parameter(torch.ones(d_model, **kw)))
+        self.q = nn.Linear(d_model, d_model, bias=False, **kw)
+        self.kv = nn.Linear(d_states, 2 * kv_heads * self.head_dim,
+                            bias=False, **kw)
+        self.out = nn.Linear(d_model, d_model, bias=False, **kw)
+        self.log_scale = nn.Parameter(
+            torch.full((1, heads, 1, 1), -2.0, device=device,
+                       dtype=torch.float32))
+        self.gate = nn.Linear(d_model, ffn, bias=False, **kw)
+        self.up = nn.Linear(d_model, ffn, bias=False, **kw)
+        self.down = nn.Linear(ffn, d_model, bias=False, **kw)
+
+    def _apply(self, fn, recurse=True):
+        # As RbfBlock's.
+        scale, grad = self.log_scale.detach(), self.log_scale.grad
+        super()._apply(fn, recurse)
+        if self.log_scale.dtype != torch.float32:
+            self.log_scale.grad = None
+            self.log_scale.data = scale.to(self.log_scale.device)
+            if grad is not None:
+                self.log_scale.grad = grad.detach().to(self.log_scale.device)
+        return self
+
+    def forward(self, x, states, state_lengths=None, rng=None,
+                stream: int = 0):
+        """x [B, N, d_model]; states [B, M, d_states], of which a sequence has
+        state_lengths[b] (int32 or int64 [B]; all M by default). In training
+        mode with dropout, rng is as in `dropout` and the block's streams are
+        stream .. stream + STREAMS - 1."""
+        b, n, _ = x.shape
+        p = self.p if self.training else 0.0
+        drop = {'p': p, 'rng': rng, 'residual_scale': self.residual_scale}
+        _, y = residual_norm(x, weight=self.norm1)
+        q = linear(y, self.q.weight).view(b, n, self.heads, self.head_dim)
+        k, v = linear(states, self.kv.weight).view(
+            b, states.shape[1], 2, self.kv_heads,
+            self.head_dim).permute(2, 0, 3, 1, 4)
+        a = cross_attention(q.transpose(1, 2), k, v, self.log_scale.exp(),
+                            state_lengths)
+        a = linear(a.transpose(1, 2).reshape(b, n, -1), self.out.weight)
+        x, y = residual_norm(x, a, self.norm2, gate=self.attn_gate,
+                             branch_weight=self.attn_norm, stream=stream,
+                             **drop)
+        h = gated_linear(y, self.gate.weight, self.up.weight,
+                         activation=self.activation)
+        if p > 0:
+            h = dropout(h, p, rng, stream + 2)
+        h = linear(h, self.down.weight)
+        x, _ = residual_norm(x, h, gate=self.ffn_gate,
+                             branch_weight=self.ffn_norm, stream=stream + 1,
+                             norm=False, **drop)
+        return x
 
 
 def strerror(status: int) -> str:

@@ -368,6 +368,7 @@ int build_qk(const vectra_qk_args& a, const vectra_qk_axes* axes,
     for (int i = 0; i < axes->count; ++i) {
       if (axes->section[i] < 0) return VECTRA_ERR_SHAPE;
       p->first_pair[i] = int32_t(sum);
+      if (sum % 4) p->whole_quads = false;
       sum += axes->section[i];
       if (sum > R2) return VECTRA_ERR_SHAPE;
     }

@@ -290,6 +290,7 @@ struct QkProblem {
   int32_t axes = 1;
   int32_t first_pair[VECTRA_MAX_AXES] = {0};
   int64_t pos_sa = 0;
+  bool whole_quads = true;  // axes' first pairs are multiples of 4
   float eps = 0.f;
 };
 cudaError_t launch_qk_forward(const QkProblem& p, cudaStream_t stream);

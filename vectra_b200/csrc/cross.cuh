@@ -48,13 +48,13 @@ struct CrossProblem {
   float* dscale = nullptr;        // [B, H]
   const float* delta = nullptr;   // [B, H, Nq]: c_i
   float* dscale_rows = nullptr;   // [splits][B, H, Nq][3]
+  const float* key_squares = nullptr;  // [B, Hk, Nk]: |k_j|^2, or not formed
   // A split axis: parts of it, and their float32 results.
   int32_t splits = 1;
   int64_t row_blocks = 1;    // blocks of one sequence's key head
   float* part = nullptr;     // out or dq or dk: [splits][rows][width]
   float* part_v = nullptr;   // dv
   float* part_ml = nullptr;  // forward: [splits][rows][2], maximum and sum
-  float* part_l = nullptr;   // [splits][rows]: the sum for lse, where another
   unsigned int* err = nullptr;
 };
 
@@ -104,6 +104,10 @@ cudaError_t run_cross_tc_backward(const CrossProblem& p, Workspace& ws,
 // c_i of every row into delta.
 cudaError_t launch_cross_delta(const CrossProblem& p, float* delta,
                                cudaStream_t stream);
+// |k_j|^2 of every key into `squares` [B, Hk, Nk] (16-byte pieces: what
+// cross_tc_supports allows).
+cudaError_t launch_cross_squares(const CrossProblem& p, float* squares,
+                                 cudaStream_t stream);
 // out and lse from the parts.
 cudaError_t launch_cross_join(const CrossProblem& p, cudaStream_t stream);
 // `out` [B, H, N, width] from [splits][B, H, N][width].

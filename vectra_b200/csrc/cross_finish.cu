@@ -6,31 +6,96 @@
 namespace vectra {
 namespace {
 
-// One warp a row; memory-bound, a row's 64 to 512 bytes at a time.
-template <typename T>
+// Sixteen lanes a row, 16-byte pieces where rows allow them (VEC); memory-bound.
+template <typename T, bool VEC>
 __global__ void __launch_bounds__(256)
     delta_kernel(const __grid_constant__ CrossProblem p, float* delta) {
   allow_dependents();
   grid_dependency_wait();
   const int64_t rows = p.B * p.H * p.Nq;
-  const int lane = threadIdx.x % 32;
-  for (int64_t r = int64_t(blockIdx.x) * 8 + threadIdx.x / 32; r < rows;
-       r += int64_t(gridDim.x) * 8) {
-    const int64_t bh = r / p.Nq, i = r - bh * p.Nq;
-    const int64_t b = bh / p.H, h = bh - b * p.H;
-    const T* o = static_cast<const T*>(p.out) + b * p.so[0] + h * p.so[1] +
-                 i * p.so[2];
-    const T* e = static_cast<const T*>(p.dout) + b * p.se[0] + h * p.se[1] +
-                 i * p.se[2];
-    const T* rest = static_cast<const T*>(p.rest) + r * p.Dv;
+  const int lane = threadIdx.x % 16;
+  // The loop runs to the warp's last row: the sums need every lane.
+  for (int64_t r0 = (int64_t(blockIdx.x) * 8 + threadIdx.x / 32) * 2; r0 < rows;
+       r0 += int64_t(gridDim.x) * 16) {
+    const int64_t r = r0 + threadIdx.x % 32 / 16;
     float t = 0.f;
-    for (int d = lane; d < p.Dv; d += 32) {
-      float x = to_f32(o[d]);
-      if (p.rest) x += to_f32(rest[d]);
-      t = fmaf(x, to_f32(e[d * p.se[3]]), t);
+    if (r < rows) {
+      const int64_t bh = r / p.Nq, i = r - bh * p.Nq;
+      const int64_t b = bh / p.H, h = bh - b * p.H;
+      const T* o = static_cast<const T*>(p.out) + b * p.so[0] + h * p.so[1] +
+                   i * p.so[2];
+      const T* e = static_cast<const T*>(p.dout) + b * p.se[0] +
+                   h * p.se[1] + i * p.se[2];
+      const T* rest =
+          p.rest ? static_cast<const T*>(p.rest) + r * p.Dv : nullptr;
+      constexpr int N = VEC ? 16 / int(sizeof(T)) : 1;
+      for (int d = lane * N; d < p.Dv; d += 16 * N) {
+        union Piece {
+          uint4 u;
+          T e[N];
+        } x, y, z;
+        if constexpr (VEC) {
+          x.u = __ldg(reinterpret_cast<const uint4*>(o + d));
+          y.u = __ldg(reinterpret_cast<const uint4*>(e + d));
+          if (rest) z.u = __ldg(reinterpret_cast<const uint4*>(rest + d));
+        } else {
+          x.e[0] = o[d];
+          y.e[0] = e[d * p.se[3]];
+          if (rest) z.e[0] = rest[d];
+        }
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+          float v = to_f32(x.e[j]);
+          if (rest) v += to_f32(z.e[j]);
+          t = fmaf(v, to_f32(y.e[j]), t);
+        }
+      }
     }
-    t = warp_sum(t);
-    if (lane == 0) delta[r] = t;
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+    if (lane == 0 && r < rows) delta[r] = t;
+  }
+}
+
+// Sixteen lanes a key, 16-byte pieces (bf16 and f16).
+template <typename T>
+__global__ void __launch_bounds__(256)
+    squares_kernel(const __grid_constant__ CrossProblem p, float* squares) {
+  allow_dependents();
+  grid_dependency_wait();
+  const int64_t rows = p.B * p.Hk * p.Nk;
+  const int lane = threadIdx.x % 16;
+  for (int64_t r0 = (int64_t(blockIdx.x) * 8 + threadIdx.x / 32) * 2; r0 < rows;
+       r0 += int64_t(gridDim.x) * 16) {
+    const int64_t r = r0 + threadIdx.x % 32 / 16;
+    float t = 0.f;
+    if (r < rows) {
+      const int64_t bh = r / p.Nk, i = r - bh * p.Nk;
+      const int64_t b = bh / p.Hk, h = bh - b * p.Hk;
+      const T* k = static_cast<const T*>(p.k) + b * p.sk[0] + h * p.sk[1] +
+                   i * p.sk[2];
+      for (int d = lane * 8; d < p.D; d += 128) {
+        union {
+          uint4 u;
+          T e[8];
+        } x;
+        if (d + 8 <= p.D) {
+          x.u = __ldg(reinterpret_cast<const uint4*>(k + d));
+        } else {
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            x.e[j] = d + j < p.D ? k[d + j] : from_f32<T>(0.f);
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float v = to_f32(x.e[j]);
+          t = fmaf(v, v, t);
+        }
+      }
+    }
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+    if (lane == 0 && r < rows) squares[r] = t;
   }
 }
 
@@ -56,7 +121,7 @@ __global__ void __launch_bounds__(256)
       nan = nan || x != x;
     }
     if (nan) m = NAN;
-    float l = 0.f, l_lse = 0.f;
+    float l = 0.f;
     float acc[kMaxCrossWidth / 32];
 #pragma unroll
     for (int c = 0; c < kMaxCrossWidth / 32; ++c) acc[c] = 0.f;
@@ -66,7 +131,6 @@ __global__ void __launch_bounds__(256)
       if (t.x == kNegInf) continue;
       const float f = fast_exp2(t.x - m);
       l = fmaf(t.y, f, l);
-      l_lse = fmaf(p.part_l ? p.part_l[s * rows + r] : t.y, f, l_lse);
       const float* o = p.part + (s * rows + r) * p.Dv;
 #pragma unroll
       for (int c = 0; c < kMaxCrossWidth / 32; ++c)
@@ -82,7 +146,7 @@ __global__ void __launch_bounds__(256)
         store_with_rest<T>(out + d, rest ? rest + d : nullptr,
                            any ? acc[c] / l : 0.f);
     }
-    if (p.lse && lane == 0) p.lse[r] = any ? m + log2f(l_lse) : INFINITY;
+    if (p.lse && lane == 0) p.lse[r] = any ? m + log2f(l) : INFINITY;
   }
 }
 
@@ -160,9 +224,33 @@ cudaError_t launch_cross_delta(const CrossProblem& p, float* delta,
   count_launches(1);
   return with_dtype(p.dtype, [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
-    return launch_pdl(delta_kernel<T>, dim3(row_blocks(rows)), dim3(256), 0,
-                      stream, p, delta);
+    const int64_t sizes[3] = {p.B, p.H, p.Nq};
+    const auto whole = [&](const void* base, const int64_t* s) {
+      bool ok = (reinterpret_cast<uintptr_t>(base) & 15) == 0;
+      for (int i = 0; i < 3; ++i)
+        ok = ok && (sizes[i] <= 1 || s[i] * int64_t(sizeof(T)) % 16 == 0);
+      return ok;
+    };
+    const bool vec = p.Dv * sizeof(T) % 16 == 0 && whole(p.out, p.so) &&
+                     whole(p.dout, p.se) && (p.se[3] == 1 || p.Dv == 1) &&
+                     (reinterpret_cast<uintptr_t>(p.rest) & 15) == 0;
+    return launch_pdl(vec ? delta_kernel<T, true> : delta_kernel<T, false>,
+                      dim3(row_blocks((rows + 1) / 2)), dim3(256), 0, stream,
+                      p, delta);
   });
+}
+
+cudaError_t launch_cross_squares(const CrossProblem& p, float* squares,
+                                 cudaStream_t stream) {
+  const int64_t rows = p.B * p.Hk * p.Nk;
+  if (rows == 0) return cudaSuccess;
+  count_launches(1);
+  const dim3 grid(row_blocks((rows + 1) / 2));
+  if (p.dtype == VECTRA_BF16)
+    return launch_pdl(squares_kernel<__nv_bfloat16>, grid, dim3(256), 0,
+                      stream, p, squares);
+  return launch_pdl(squares_kernel<__half>, grid, dim3(256), 0, stream, p,
+                    squares);
 }
 
 cudaError_t launch_cross_join(const CrossProblem& p, cudaStream_t stream) {

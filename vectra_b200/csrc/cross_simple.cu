@@ -70,6 +70,13 @@ __device__ __forceinline__ void stage(float* dst, const void* base,
   }
 }
 
+// lse leaves out the factor 2^(-g log2e |q_i|^2) of all of a row's weights in
+// 16-bit types, as the tensor cores' kernels, which do not form it, do: the
+// passes of one call may run on either (a copy of an argument may be aligned
+// another way). float32 has these kernels alone, and keeps the whole logits.
+template <typename T>
+constexpr bool kLeaveOut = !std::is_same<T, float>::value;
+
 // Rounded once, in all passes alike: a single key weighs exactly 1.
 __device__ __forceinline__ float logit(float g, float distance) {
   return __fmul_rn(-g * kLog2e, distance);
@@ -118,12 +125,13 @@ __global__ void __launch_bounds__(kThreads)
       stage<T, W, R, S::LR>(sr2, p.v, p.sv, b, hk, 1, first, rows, p.Dv);
     }
   }
-  // Rows that are queries: scale, lse and c_i of each.
-  float g2[RT], lse[RT], delta[RT];
+  // Rows that are queries: scale, lse and c_i of each, and what lse leaves
+  // out.
+  float g2[RT], lse[RT], delta[RT], left_out[RT];
   int64_t qrow[RT];  // of [B, H, Nq]; -1: none
 #pragma unroll
   for (int i = 0; i < RT; ++i) {
-    g2[i] = lse[i] = delta[i] = 0.f;
+    g2[i] = lse[i] = delta[i] = left_out[i] = 0.f;
     qrow[i] = -1;
     const int64_t r = first + ty * RT + i;
     if (kRowsAreQueries && r < rows) {
@@ -133,6 +141,25 @@ __global__ void __launch_bounds__(kThreads)
       if constexpr (PASS == kQueries) {
         lse[i] = p.lse[qrow[i]];
         delta[i] = p.delta[qrow[i]];
+      }
+    }
+  }
+
+  if constexpr (kLeaveOut<T> && kRowsAreQueries) {
+    __syncthreads();
+    if (t0 < t1) {
+#pragma unroll
+      for (int i = 0; i < RT; ++i) {
+        float sq = 0.f;
+        for (int d = tx; d < p.D; d += 16) {
+          const float x = sr[d * S::LR + ty * RT + i];
+          sq = fmaf(x, x, sq);
+        }
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1)
+          sq += __shfl_xor_sync(0xffffffffu, sq, o);
+        left_out[i] = g2[i] * kLog2e * sq;
+        lse[i] -= left_out[i];
       }
     }
   }
@@ -175,26 +202,54 @@ __global__ void __launch_bounds__(kThreads)
       }
     }
     __syncthreads();
+    if constexpr (kLeaveOut<T> && !kRowsAreQueries) {
+      // Four threads a column.
+      for (int c = threadIdx.x / 4; c < CN; c += kThreads / 4) {
+        float sq = 0.f;
+        for (int d = threadIdx.x % 4; d < p.D; d += 4) {
+          const float x = sc[d * S::LC + c];
+          sq = fmaf(x, x, sq);
+        }
+        sq += __shfl_xor_sync(0xffffffffu, sq, 1);
+        sq += __shfl_xor_sync(0xffffffffu, sq, 2);
+        if (threadIdx.x % 4 == 0) col_lse[c] -= col_g[c] * kLog2e * sq;
+      }
+      __syncthreads();
+    }
 
     float s[RT][CT], u[RT][CT];
 #pragma unroll
     for (int i = 0; i < RT; ++i)
 #pragma unroll
       for (int j = 0; j < CT; ++j) s[i][j] = u[i][j] = 0.f;
-#pragma unroll 4
-    for (int d = 0; d < p.D; ++d) {
-      float r[RT], c[CT];
-#pragma unroll
-      for (int i = 0; i < RT; ++i) r[i] = sr[d * S::LR + ty * RT + i];
-#pragma unroll
-      for (int j = 0; j < CT; ++j) c[j] = sc[d * S::LC + tx * CT + j];
+    // Sums of eight components at a time: a sum of D terms one by one would
+    // be off by twice as much, and the weights' exponents with it.
+#pragma unroll 1
+    for (int d0 = 0; d0 < p.D; d0 += 8) {
+      float eight[RT][CT];
 #pragma unroll
       for (int i = 0; i < RT; ++i)
 #pragma unroll
-        for (int j = 0; j < CT; ++j) {
-          const float x = r[i] - c[j];
-          s[i][j] = fmaf(x, x, s[i][j]);
-        }
+        for (int j = 0; j < CT; ++j) eight[i][j] = 0.f;
+#pragma unroll
+      for (int d = d0; d < d0 + 8; ++d) {  // zeros past the width
+        float r[RT], c[CT];
+#pragma unroll
+        for (int i = 0; i < RT; ++i) r[i] = sr[d * S::LR + ty * RT + i];
+#pragma unroll
+        for (int j = 0; j < CT; ++j) c[j] = sc[d * S::LC + tx * CT + j];
+#pragma unroll
+        for (int i = 0; i < RT; ++i)
+#pragma unroll
+          for (int j = 0; j < CT; ++j) {
+            const float x = r[i] - c[j];
+            eight[i][j] = fmaf(x, x, eight[i][j]);
+          }
+      }
+#pragma unroll
+      for (int i = 0; i < RT; ++i)
+#pragma unroll
+        for (int j = 0; j < CT; ++j) s[i][j] += eight[i][j];
     }
     if constexpr (S::kBack) {
 #pragma unroll 4
@@ -355,10 +410,11 @@ __global__ void __launch_bounds__(kThreads)
         }
         if (tx == 0) {
           if (!whole) {
-            p.part_ml[at * 2] = m[i];
+            p.part_ml[at * 2] = m[i] + left_out[i];
             p.part_ml[at * 2 + 1] = l[i];
           } else if (p.lse) {
-            p.lse[qrow[i]] = len > 0 ? m[i] + log2f(l[i]) : INFINITY;
+            p.lse[qrow[i]] =
+                len > 0 ? m[i] + left_out[i] + log2f(l[i]) : INFINITY;
           }
         }
       } else {

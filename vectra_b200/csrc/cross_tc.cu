@@ -14,11 +14,14 @@
 // from TMEM, rounded to 16 bits, where they lie as the first operand has to:
 // the transposed form of the keys' pass needs no transposition.
 //
-// Warps: two warpgroups form P and z, one thread a row, of alternate tiles, so
-// that the tensor cores work on one tile while the other is formed; a TMA
-// producer; an MMA issuer; two warps for the columns' terms, which are
-// |k_j|^2 from the tile in shared memory, or a query's lse, c_i and scale
-// from global memory. In the forward pass every warpgroup has its own
+// Warps: two warpgroups form P and z, one thread a row, each of one half of a
+// tile's columns, while the tensor cores work on the next tile's S and T (two
+// tiles are in TMEM); a TMA producer; an MMA issuer; a warpgroup for the columns' terms, which are
+// |k_j|^2, or a query's lse, c_i and scale. Where several blocks walk the same
+// keys their |k_j|^2 are formed once beforehand; a lone block (a decoding step)
+// forms them from the tile in shared memory (two warps doing that in every
+// block set the pace: 627 us of 4,096 queries on 5,003 keys, 32 heads of 128,
+// against 432 without). In the forward pass every warpgroup has its own
 // accumulator, maximum and sum, joined once at the end: nothing is exchanged
 // on the way.
 //
@@ -27,10 +30,12 @@
 // zeros in shared memory, so that what they held (NaN included) meets no
 // weight.
 //
-// Rounding, beside each result's: P and z enter their products in 16 bits. The
-// forward pass divides by the sum of the rounded weights, so a row with one
-// large weight gets that key's value and not 2^-9 of it less, while lse, which
-// the backward pass forms P from, is of the unrounded ones.
+// Rounding, beside each result's: P and z enter their products in 16 bits. For
+// a backward pass the forward one multiplies what P's rounding left as well
+// (KEEP): c_i of a
+// result that is off by 2^-9 of its weights would put 2^-9 of the distance
+// between q_i and the mean key into dq, as much as all other roundings of dq
+// together (bf16: 3.2e-3 of dq against 2.4e-3).
 #include <atomic>
 #include <type_traits>
 
@@ -45,16 +50,16 @@ using namespace tc;
 enum Pass { kForward = 0, kQueries = 1, kKeys = 2 };
 
 constexpr int kRows = 128;
-constexpr int kThreads = 384;
+constexpr int kThreads = 512;
 constexpr int kProducerWarp = 8;
 constexpr int kMmaWarp = 9;
-constexpr int kTermWarp = 10;
-constexpr int kTermThreads = 64;
+constexpr int kTermWarp = 12;
+constexpr int kTermThreads = 128;
 constexpr float kRescaleThreshold = 8.f;  // log2 of the lazy-rescale factor
 // Registers after the launch's equal share: the warpgroups that hold a row of
 // a tile, and the others (checked against the launch's total on the host).
 constexpr int kRowRegs = 200;
-constexpr int kOtherRegs = 104;
+constexpr int kOtherRegs = 56;
 
 template <int W, int PASS>
 struct Cfg {
@@ -81,8 +86,8 @@ struct Cfg {
   static constexpr int SMEM = OFF_TMEM + 16;
   static constexpr int SMEM_ALLOC = SMEM + 1024;  // for 1024-byte alignment
   static_assert(SMEM_ALLOC <= 232448, "shared memory");
-  // TMEM columns: S of both warpgroups, T of both (backward), accumulators.
-  // P overlays S, z overlays T.
+  // TMEM columns: S of two tiles, T of two (backward), accumulators. Each
+  // warpgroup's P overlays its half of S, z that of T.
   static constexpr int S0 = 0, T0 = 2 * CN, A0 = kBack ? 4 * CN : 2 * CN;
   static constexpr int TMEM_COLS = 512;
   static_assert(A0 + 2 * W <= TMEM_COLS, "TMEM");
@@ -172,23 +177,22 @@ __device__ __forceinline__ uint32_t chunk_at(int block, int r, int kb, int c) {
   return uint32_t(kb * block + r * 128 + ((c ^ (r & 7)) << 4));
 }
 
-template <typename T, int KB>
+// The sum of squares of chunks [from, from + N) of row r.
+template <typename T, int N>
 __device__ __forceinline__ float row_square(const uint8_t* tile, int block,
-                                            int r) {
+                                            int r, int from) {
   uint64_t a = 0, b = 0;
-#pragma unroll
-  for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-    for (int c = 0; c < 8; ++c) {
-      const uint4 raw =
-          *reinterpret_cast<const uint4*>(tile + chunk_at(block, r, kb, c));
-      const uint64_t x = unpack2<T>(raw.x), y = unpack2<T>(raw.y),
-                     z = unpack2<T>(raw.z), w = unpack2<T>(raw.w);
-      a = ffma2(x, x, a);
-      b = ffma2(y, y, b);
-      a = ffma2(z, z, a);
-      b = ffma2(w, w, b);
-    }
+#pragma unroll 4
+  for (int i = from; i < from + N; ++i) {
+    const uint4 raw = *reinterpret_cast<const uint4*>(
+        tile + chunk_at(block, r, i / 8, i % 8));
+    const uint64_t x = unpack2<T>(raw.x), y = unpack2<T>(raw.y),
+                   z = unpack2<T>(raw.z), w = unpack2<T>(raw.w);
+    a = ffma2(x, x, a);
+    b = ffma2(y, y, b);
+    a = ffma2(z, z, a);
+    b = ffma2(w, w, b);
+  }
   return halves(fadd2(a, b));
 }
 
@@ -233,7 +237,7 @@ __device__ __forceinline__ void store8f(float* out, const float* v, int live) {
     if (i < live) out[i] = v[i];
 }
 
-template <typename T, int W, int PASS>
+template <typename T, int W, int PASS, bool KEEP>
 __global__ void __launch_bounds__(kThreads, 1)
     cross_tc_kernel(const __grid_constant__ CUtensorMap tr,
                     const __grid_constant__ CUtensorMap tr2,
@@ -251,7 +255,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const uint32_t sbase = smem_addr(smem);
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);
-  // 0 rows loaded; 1, 2 S (and T) of a warpgroup formed; 3, 4 its P (and z)
+  // 0 rows loaded; 1, 2 S (and T) of a buffer formed; 3, 4 its P (and z)
   // written; 5 accumulators final; then per stage loaded, free, terms written.
   const uint32_t bar_r = smem_addr(&bars[0]);
   auto bar_s = [&](int x) { return smem_addr(&bars[1 + x]); };
@@ -305,7 +309,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(bar_end, 1);
       for (int x = 0; x < 2; ++x) {
         mbar_init(bar_s(x), 1);
-        mbar_init(bar_p(x), 4);
+        mbar_init(bar_p(x), 8);
       }
       for (int s = 0; s < NS; ++s) {
         mbar_init(bar_full(s), 1);
@@ -393,13 +397,14 @@ __global__ void __launch_bounds__(kThreads, 1)
             inner(C::T0 + x * CN, dr2, col + uint64_t(C::CTILE >> 4), dv16);
           tc_commit(bar_s(x));
         };
+        // acc += A B of warpgroup x's columns, A its 16-bit pairs in TMEM.
         auto sum = [&](uint32_t dst, uint32_t src, uint64_t db, uint32_t idesc,
-                       bool first) {
+                       int x, bool first) {
 #pragma unroll
-          for (int k = 0; k < CN / 16; ++k)
-            tc_mma_ts(tmem + dst, tmem + src + k * 8,
-                      db + uint64_t((k * 16 * 128) >> 4), idesc,
-                      !first || k > 0);
+          for (int k = 0; k < CN / 32; ++k)
+            tc_mma_ts(tmem + dst, tmem + src + x * (CN / 2) + k * 8,
+                      db + uint64_t(((x * (CN / 2) + k * 16) * 128) >> 4),
+                      idesc, !first || k > 0);
         };
         ok = mbar_wait(bar_r, 0, p.err);
         for (int t = 0; t < 2 && t < n && ok; ++t) {
@@ -415,12 +420,19 @@ __global__ void __launch_bounds__(kThreads, 1)
           tc_fence_after();
           const uint64_t col = dcm + uint64_t((s * C::STAGE) >> 4);
           const uint64_t col2 = col + uint64_t(C::CTILE >> 4);
-          if (PASS == kForward) {
-            sum(C::A0 + x * W, C::S0 + x * CN, col2, idesc_a2, t < 2);
-          } else {
-            sum(C::A0, C::T0 + x * CN, col, idesc_a, t == 0);
-            if (PASS == kKeys)
-              sum(C::A0 + W, C::S0 + x * CN, col2, idesc_a2, t == 0);
+#pragma unroll
+          for (int g = 0; g < 2; ++g) {
+            if (PASS == kForward) {
+              const uint32_t src = C::S0 + x * CN;
+              sum(C::A0 + g * W, src, col2, idesc_a2, g, t == 0);
+              if (KEEP)
+                sum(C::A0 + g * W, src + CN / 4, col2, idesc_a2, g, false);
+            } else {
+              sum(C::A0, C::T0 + x * CN, col, idesc_a, g, t == 0 && g == 0);
+              if (PASS == kKeys)
+                sum(C::A0 + W, C::S0 + x * CN, col2, idesc_a2, g,
+                    t == 0 && g == 0);
+            }
           }
           tc_commit(bar_free(s));
           if (t + 2 < n) {
@@ -433,54 +445,65 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         if (ok) tc_commit(bar_end);
       }
-    } else {
+    } else if (warp >= kTermWarp) {
       // ------------------------------------------------------- column terms
-      const int th = threadIdx.x - kTermWarp * 32;  // 0 .. 63
+      const int th = threadIdx.x - kTermWarp * 32;  // 0 .. 127
       for (int t = 0; t < n && ok; ++t) {
         const int s = t % NS;
         float* out = term + s * C::TERMS * CN;
         if constexpr (kRowsAreQueries) {
-          ok = mbar_wait(bar_full(s), uint32_t((t / NS) & 1), p.err);
+          // Threads of a column, which are neighbours, and this one's part.
+          constexpr int PER = kTermThreads / CN, CHUNKS = 8 * C::KB / PER;
+          const int c = th / PER, part_of = th % PER;
+          const int first = (t0 + t) * CN;
+          const bool known = p.key_squares != nullptr;
+          const bool last = first + CN > len;
+          ok = known ? mbar_wait(bar_free(s), uint32_t(((t / NS) & 1) ^ 1),
+                                 p.err)
+                     : true;
+          float sq = 0.f;
+          if (known && ok && first + c < len)
+            sq = __ldg(p.key_squares + plane * p.Nk + first + c);
+          if (ok && (!known || last))
+            ok = mbar_wait(bar_full(s), uint32_t((t / NS) & 1), p.err);
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
           uint8_t* k_tile = smem + C::OFF_C + s * C::STAGE;
-          // The operand that a product sums these rows of.
-          uint8_t* summed = k_tile + (PASS == kForward ? C::CTILE : 0);
-          const int first = (t0 + t) * CN;
-#pragma unroll
-          for (int i = 0; i < CN / kTermThreads; ++i) {
-            const int c = th + i * kTermThreads;
-            float sq = 0.f;
-            if (first + c < len) {
-              sq = row_square<T, C::KB>(k_tile, C::CBLOCK, c);
-            } else {
-#pragma unroll
-              for (int kb = 0; kb < C::KB; ++kb)
-#pragma unroll
-                for (int q = 0; q < 8; ++q)
-                  *reinterpret_cast<uint4*>(
-                      summed + chunk_at(C::CBLOCK, c, kb, q)) =
-                      make_uint4(0, 0, 0, 0);
-            }
-            out[c] = -sq;
+          if (!known) {
+            sq = row_square<T, CHUNKS>(k_tile, C::CBLOCK, c, part_of * CHUNKS);
+            if (PER == 2) sq += __shfl_xor_sync(0xffffffffu, sq, 1);
           }
-          fence_proxy_async_smem();
+          if (last) {
+            // Unseen rows of the operand that a product sums.
+            uint8_t* summed = k_tile + (PASS == kForward ? C::CTILE : 0);
+            if (first + c >= len) {
+              sq = 0.f;
+              for (int i = part_of * CHUNKS; i < (part_of + 1) * CHUNKS; ++i)
+                *reinterpret_cast<uint4*>(
+                    summed + chunk_at(C::CBLOCK, c, i / 8, i % 8)) =
+                    make_uint4(0, 0, 0, 0);
+            }
+            fence_proxy_async_smem();
+          }
+          if (part_of == 0) out[c] = -sq;
         } else {
           ok = mbar_wait(bar_free(s), uint32_t(((t / NS) & 1) ^ 1), p.err);
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
           const int i = (t0 + t) * a.cols_i + th / G, h = hk * G + th % G;
-          float lse = INFINITY, ci = 0.f, g = 0.f;  // weighs nothing
-          if (th < a.cols_i * G && i < nq) {
-            const int64_t q = (int64_t(b) * p.H + h) * p.Nq + i;
-            lse = __ldg(p.lse + q);
-            ci = __ldg(p.delta + q);
-            g = cross_scale(p, b, h);
+          if (th < CN) {
+            float lse = INFINITY, ci = 0.f, g = 0.f;  // weighs nothing
+            if (th < a.cols_i * G && i < nq) {
+              const int64_t q = (int64_t(b) * p.H + h) * p.Nq + i;
+              lse = __ldg(p.lse + q);
+              ci = __ldg(p.delta + q);
+              g = cross_scale(p, b, h);
+            }
+            out[th] = -lse;
+            out[CN + th] = -ci;
+            out[2 * CN + th] = g * kLog2e;
+            out[3 * CN + th] = 2.f * g;
           }
-          out[th] = -lse;
-          out[CN + th] = -ci;
-          out[2 * CN + th] = g * kLog2e;
-          out[3 * CN + th] = 2.f * g;
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(bar_term(s));
@@ -491,8 +514,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     setmaxnreg_inc<kRowRegs>();
     const int x = warp >> 2;
     const uint32_t lane_base = uint32_t((warp & 3) * 32) << 16;
-    const uint32_t s_col = tmem + lane_base + C::S0 + x * CN;
-    const uint32_t t_col = tmem + lane_base + C::T0 + x * CN;
+    constexpr int HALF = CN / 2;  // columns of this warpgroup
+    const uint32_t s_base = tmem + lane_base + C::S0 + x * HALF;
+    const uint32_t t_base = tmem + lane_base + C::T0 + x * HALF;
     const uint32_t acc = tmem + lane_base + C::A0;
     // A warp none of whose rows lives only keeps step.
     const bool warp_live = __any_sync(0xffffffffu, row_live);
@@ -502,50 +526,59 @@ __global__ void __launch_bounds__(kThreads, 1)
 
     if constexpr (PASS == kForward) {
       const uint32_t o_col = acc + x * W;
-      const uint64_t two = both(2.f), gl2 = both(gl);
-      float m_used = kNegInf, l = 0.f, l_rounded = 0.f;
-      for (int t = x; t < n && ok; t += 2) {
-        const int s = t % NS;
-        const float* nk = term + s * CN;
-        ok = mbar_wait(bar_s(x), uint32_t((t >> 1) & 1), p.err) &&
+      const uint64_t two = both(2.f);
+      const bool warp_negative = __any_sync(0xffffffffu, gl < 0.f);
+      // A scale of 0 keeps masked columns at weight 0 through a tiny one.
+      const float gle = warp_negative ? 1.f : (gl == 0.f ? 1e-37f : gl);
+      const uint64_t gl2 = both(gle);
+      float m_used = kNegInf, l = 0.f;
+      for (int t = 0; t < n && ok; ++t) {
+        const int s = t % NS, buf = t & 1;
+        const float* nk = term + s * CN + x * HALF;
+        const uint32_t s_col = s_base + buf * CN;
+        ok = mbar_wait(bar_s(buf), uint32_t((t >> 1) & 1), p.err) &&
              mbar_wait(bar_term(s), uint32_t((t / NS) & 1), p.err);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         tc_fence_after();
         if (warp_live) {
-          uint32_t v[CN];
+          uint32_t v[HALF];
           tmem_load64(s_col, v);
-          tmem_load64(s_col + 64, v + 64);
           float mx[4] = {kNegInf, kNegInf, kNegInf, kNegInf};
+          // u = 2 S - |k|^2; the logit is gl u.
 #pragma unroll
-          for (int j = 0; j < CN; j += 4) {
+          for (int j = 0; j < HALF; j += 4) {
             const float4 n4 = *reinterpret_cast<const float4*>(nk + j);
-            const float2 lo = f2upk(
-                mul2(gl2, ffma2(two, bits2(v + j), f2pk(n4.x, n4.y))));
-            const float2 hi = f2upk(
-                mul2(gl2, ffma2(two, bits2(v + j + 2), f2pk(n4.z, n4.w))));
+            const float2 lo = f2upk(ffma2(two, bits2(v + j), f2pk(n4.x, n4.y)));
+            const float2 hi =
+                f2upk(ffma2(two, bits2(v + j + 2), f2pk(n4.z, n4.w)));
             v[j] = __float_as_uint(lo.x);
             v[j + 1] = __float_as_uint(lo.y);
             v[j + 2] = __float_as_uint(hi.x);
             v[j + 3] = __float_as_uint(hi.y);
           }
-          const int live = len - (t0 + t) * CN;
-          if (live < CN) {
+          if (warp_negative) {  // the largest logit is not that of the largest u
 #pragma unroll
-            for (int j = 0; j < CN; ++j)
+            for (int j = 0; j < HALF; ++j)
+              v[j] = __float_as_uint(gl * __uint_as_float(v[j]));
+          }
+          const int live = len - (t0 + t) * CN - x * HALF;
+          if (live < HALF) {
+#pragma unroll
+            for (int j = 0; j < HALF; ++j)
               if (j >= live) v[j] = __float_as_uint(kNegInf);
           }
 #pragma unroll
-          for (int j = 0; j < CN; j += 8)
+          for (int j = 0; j < HALF; j += 8)
 #pragma unroll
             for (int q = 0; q < 4; ++q)
               mx[q] = fmax3(mx[q], __uint_as_float(v[j + 2 * q]),
                             __uint_as_float(v[j + 2 * q + 1]));
-          const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+          const float u_top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+          // (A scale of 0 has logits 0; 0 * -inf only where nothing is live.)
+          const float top = u_top == kNegInf ? kNegInf : gle * u_top;
           // The reference maximum moves when the new one is more than 2^8
           // larger; the warp rescales O if any of its rows moved.
-          // (This warpgroup's last product has completed: S of this tile was
-          // issued behind it.)
           const bool need = top > m_used + kRescaleThreshold ||
                             (m_used == kNegInf && top != kNegInf);
           float factor = 1.f;
@@ -553,9 +586,15 @@ __global__ void __launch_bounds__(kThreads, 1)
             factor = m_used == kNegInf ? 0.f : fast_exp2(m_used - top);
             m_used = top;
             l *= factor;
-            l_rounded *= factor;
           }
-          if (t >= 2 && __any_sync(0xffffffffu, need)) {
+          if (t > 0 && __any_sync(0xffffffffu, need)) {
+            // The tile before's product into O, which may still run: this
+            // tile's S was issued ahead of it. Its stage is free behind it.
+            ok = mbar_wait(bar_free((t - 1) % NS),
+                           uint32_t(((t - 1) / NS) & 1), p.err);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            tc_fence_after();
 #pragma unroll
             for (int c = 0; c < W / 32; ++c) {
               uint32_t o[32];
@@ -569,59 +608,63 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           const float ref = m_used == kNegInf ? 0.f : m_used;
           const uint64_t neg = both(-ref);
-          uint64_t sa = 0, sb = 0, ra = 0, rb = 0;
+          const uint64_t minus = both(-1.f);
+          uint64_t sa = 0, sb = 0;
 #pragma unroll
-          for (int c = 0; c < CN / 32; ++c) {
-            uint32_t w[16];
+          for (int c = 0; c < HALF / 32; ++c) {
+            uint32_t w[16], rest[16];
 #pragma unroll
             for (int j = 0; j < 16; j += 2) {
               const int k = c * 32 + 2 * j;
-              const float2 e0 = f2upk(fadd2(bits2(v + k), neg));
-              const float2 e1 = f2upk(fadd2(bits2(v + k + 2), neg));
-              const float p0 = fast_exp2(e0.x), p1 = fast_exp2(e0.y);
-              const float p2 = fast_exp2(e1.x), p3 = fast_exp2(e1.y);
-              sa = fadd2(sa, f2pk(p0, p1));
-              sb = fadd2(sb, f2pk(p2, p3));
-              w[j] = pack2<T>(p0, p1);
-              w[j + 1] = pack2<T>(p2, p3);
-              ra = fadd2(ra, unpack2<T>(w[j]));
-              rb = fadd2(rb, unpack2<T>(w[j + 1]));
+              const float2 e0 = f2upk(ffma2(gl2, bits2(v + k), neg));
+              const float2 e1 = f2upk(ffma2(gl2, bits2(v + k + 2), neg));
+              const uint64_t p0 = f2pk(fast_exp2(e0.x), fast_exp2(e0.y));
+              const uint64_t p1 = f2pk(fast_exp2(e1.x), fast_exp2(e1.y));
+              w[j] = pack2<T>(f2upk(p0).x, f2upk(p0).y);
+              w[j + 1] = pack2<T>(f2upk(p1).x, f2upk(p1).y);
+              sa = fadd2(sa, p0);
+              sb = fadd2(sb, p1);
+              if constexpr (KEEP) {
+                const uint64_t r0 = unpack2<T>(w[j]),
+                               r1 = unpack2<T>(w[j + 1]);
+                const float2 d0 = f2upk(ffma2(r0, minus, p0));
+                const float2 d1 = f2upk(ffma2(r1, minus, p1));
+                rest[j] = pack2<T>(d0.x, d0.y);
+                rest[j + 1] = pack2<T>(d1.x, d1.y);
+              }
             }
             tmem_st16(s_col + c * 16, w);
+            if constexpr (KEEP) tmem_st16(s_col + HALF / 2 + c * 16, rest);
           }
           l += halves(fadd2(sa, sb));
-          l_rounded += halves(fadd2(ra, rb));
           tmem_wait_st();
         }
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(bar_p(x));
+        if (lane == 0) mbar_arrive(bar_p(buf));
       }
       if (ok) ok = mbar_wait(bar_end, 0, p.err);
       ok = __all_sync(0xffffffffu, ok);
       tc_fence_after();
       // The warpgroups' maxima and sums, through the row operand's memory
       // (every product has read it by now).
-      float4* join = reinterpret_cast<float4*>(smem + C::OFF_R);
-      join[x * kRows + r] = make_float4(m_used, l, l_rounded, 0.f);
+      float2* join = reinterpret_cast<float2*>(smem + C::OFF_R);
+      join[x * kRows + r] = make_float2(m_used, l);
       sync_rows();
-      const float4 j0 = join[r], j1 = join[kRows + r];
+      const float2 j0 = join[r], j1 = join[kRows + r];
       const float m = fmaxf(j0.x, j1.x);
       const float f0 = j0.x == kNegInf ? 0.f : fast_exp2(j0.x - m);
       const float f1 = j1.x == kNegInf ? 0.f : fast_exp2(j1.x - m);
-      const bool has1 = n > 1;
       // Without a finite maximum nothing was weighed: 0 / 0.
       const float sum = f0 * j0.y + f1 * j1.y;
-      const float div = f0 * j0.z + f1 * j1.z;
-      const float inv = whole ? 1.f / div : 1.f;
+      const float inv = whole ? 1.f / sum : 1.f;
       const float lse = m + log2f(sum);
       if (ok && warp_live) {
         if (row_live && x == 0) {
           const int64_t k = part * all_rows + at;
           if (!whole) {
             p.part_ml[2 * k] = m;
-            p.part_ml[2 * k + 1] = div;
-            if (p.part_l) p.part_l[k] = sum;
+            p.part_ml[2 * k + 1] = sum;
           } else if (p.lse) {
             p.lse[at] = lse;
           }
@@ -643,10 +686,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             float v[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-              // The second warpgroup's accumulator holds nothing before its
-              // first tile.
-              const float y1 = has1 ? __uint_as_float(o1[q + i]) * f1 : 0.f;
-              v[i] = (__uint_as_float(o0[q + i]) * f0 + y1) * inv;
+              v[i] = (__uint_as_float(o0[q + i]) * f0 +
+                      __uint_as_float(o1[q + i]) * f1) * inv;
             }
             const int d = d0 + q, live = p.Dv - d;
             if (live <= 0) break;
@@ -667,23 +708,25 @@ __global__ void __launch_bounds__(kThreads, 1)
       ok = mbar_wait(bar_r, 0, p.err);
       ok = __all_sync(0xffffffffu, ok);
       if (!kRowsAreQueries && ok)
-        nkr = -row_square<T, C::KB>(smem + C::OFF_R, C::RBLOCK, r);
+        nkr = -row_square<T, 8 * C::KB>(smem + C::OFF_R, C::RBLOCK, r, 0);
       const uint64_t nkr2 = both(nkr), gl2 = both(gl), lse2 = both(-lse),
                      ci2 = both(-ci);
       uint64_t zs = 0, zx = 0, xs = 0, ys = 0;  // of rounded z; for dscale
       const bool want_scale = PASS == kQueries && p.dscale_rows != nullptr;
-      for (int t = x; t < n && ok; t += 2) {
-        const int s = t % NS;
-        const float* col = term + s * C::TERMS * CN;
-        ok = mbar_wait(bar_s(x), uint32_t((t >> 1) & 1), p.err) &&
+      for (int t = 0; t < n && ok; ++t) {
+        const int s = t % NS, buf = t & 1;
+        const float* col = term + s * C::TERMS * CN + x * HALF;
+        const uint32_t s_col = s_base + buf * CN, t_col = t_base + buf * CN;
+        ok = mbar_wait(bar_s(buf), uint32_t((t >> 1) & 1), p.err) &&
              mbar_wait(bar_term(s), uint32_t((t / NS) & 1), p.err);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         tc_fence_after();
         if (warp_live) {
-          const int live = kRowsAreQueries ? len - (t0 + t) * CN : CN;
+          const int live =
+              kRowsAreQueries ? len - (t0 + t) * CN - x * HALF : HALF;
 #pragma unroll
-          for (int c = 0; c < CN; c += 32) {
+          for (int c = 0; c < HALF; c += 32) {
             uint32_t sv[32], tv[32];
             tmem_load32x2(s_col + c, sv, t_col + c, tv);
             uint32_t pw[16], zw[16];
@@ -722,7 +765,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const float2 e = f2upk(lg[q]);
                 float w0 = fast_exp2(e.x), w1 = fast_exp2(e.y);
                 float2 z = f2upk(mul2(f2pk(w0, w1), zc[q]));
-                if (kRowsAreQueries && live < CN) {
+                if (kRowsAreQueries && live < HALF) {
                   const int k = c + j + 2 * q;
                   if (k >= live) w0 = z.x = 0.f;
                   if (k + 1 >= live) w1 = z.y = 0.f;
@@ -750,7 +793,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(bar_p(x));
+        if (lane == 0) mbar_arrive(bar_p(buf));
       }
       if (ok) ok = mbar_wait(bar_end, 0, p.err);
       ok = __all_sync(0xffffffffu, ok);
@@ -861,7 +904,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (!whole) {
       p.part_ml[2 * k] = kNegInf;
       p.part_ml[2 * k + 1] = 0.f;
-      if (p.part_l) p.part_l[k] = 0.f;
     } else if (p.lse) {
       p.lse[at] = INFINITY;
     }
@@ -881,7 +923,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 // ---------------------------------------------------------------------------
 // Host side.
 // ---------------------------------------------------------------------------
-template <typename T, int W, int PASS>
+template <typename T, int W, int PASS, bool KEEP>
 cudaError_t launch(const CrossProblem& problem, cudaStream_t stream) {
   using C = Cfg<W, PASS>;
   TcArgs a{};
@@ -913,7 +955,7 @@ cudaError_t launch(const CrossProblem& problem, cudaStream_t stream) {
                           qi);
   if (!made) return cudaErrorInvalidValue;
 
-  auto kern = cross_tc_kernel<T, W, PASS>;
+  auto kern = cross_tc_kernel<T, W, PASS, KEEP>;
   static std::atomic<int> configured[64];
   int dev = 0;
   cudaError_t err = cudaGetDevice(&dev);
@@ -925,7 +967,7 @@ cudaError_t launch(const CrossProblem& problem, cudaStream_t stream) {
     err = cudaFuncGetAttributes(&attr, kern);
     if (err != cudaSuccess) return err;
     if (int64_t(attr.numRegs) * kThreads <
-        int64_t(256) * kRowRegs + int64_t(128) * kOtherRegs)
+        int64_t(256) * (kRowRegs + kOtherRegs))
       return cudaErrorInvalidConfiguration;
     err = cudaFuncSetAttribute(
         kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM_ALLOC);
@@ -941,14 +983,14 @@ cudaError_t launch(const CrossProblem& problem, cudaStream_t stream) {
                     v, a);
 }
 
-template <int PASS>
+template <int PASS, bool KEEP = false>
 cudaError_t launch_pass(const CrossProblem& p, cudaStream_t stream) {
   const bool wide = p.D > 64 || p.Dv > 64;
   if (p.dtype == VECTRA_BF16)
-    return wide ? launch<__nv_bfloat16, 128, PASS>(p, stream)
-                : launch<__nv_bfloat16, 64, PASS>(p, stream);
-  return wide ? launch<__half, 128, PASS>(p, stream)
-              : launch<__half, 64, PASS>(p, stream);
+    return wide ? launch<__nv_bfloat16, 128, PASS, KEEP>(p, stream)
+                : launch<__nv_bfloat16, 64, PASS, KEEP>(p, stream);
+  return wide ? launch<__half, 128, PASS, KEEP>(p, stream)
+              : launch<__half, 64, PASS, KEEP>(p, stream);
 }
 
 // Parts of the axis that a block walks, where the rows alone leave SMs
@@ -970,6 +1012,11 @@ int splits_for(const CrossProblem& p, int pass) {
 
 float* take_floats(Workspace& ws, int64_t n) {
   return static_cast<float*>(ws.take(size_t(n) * sizeof(float)));
+}
+
+// |k_j|^2 of every key, where more than one block of a pass would form it.
+bool want_squares(const CrossProblem& p) {
+  return p.Nq > kRows / p.G && p.Nk > 0;
 }
 
 bool map_ok(const void* base, const int64_t* s, const int64_t* sizes) {
@@ -998,10 +1045,17 @@ cudaError_t run_cross_tc_forward(const CrossProblem& problem, Workspace& ws,
   if (p.splits > 1) {
     p.part = take_floats(ws, p.splits * rows * p.Dv);
     p.part_ml = take_floats(ws, p.splits * rows * 2);
-    if (p.lse) p.part_l = take_floats(ws, p.splits * rows);
   }
+  float* squares =
+      want_squares(p) ? take_floats(ws, p.B * p.Hk * p.Nk) : nullptr;
+  p.key_squares = squares;
   if (ws.dry || ws.overflow || rows == 0) return cudaSuccess;
-  const cudaError_t e = launch_pass<kForward>(p, stream);
+  if (squares) {
+    const cudaError_t st = launch_cross_squares(p, squares, stream);
+    if (st != cudaSuccess) return st;
+  }
+  const cudaError_t e = p.lse ? launch_pass<kForward, true>(p, stream)
+                              : launch_pass<kForward>(p, stream);
   return e != cudaSuccess || p.splits == 1 ? e : launch_cross_join(p, stream);
 }
 
@@ -1011,6 +1065,10 @@ cudaError_t run_cross_tc_backward(const CrossProblem& problem, Workspace& ws,
   const int64_t rows = p.B * p.H * p.Nq, keys = p.B * p.Hk * p.Nk;
   float* delta = take_floats(ws, rows);
   p.delta = delta;
+  float* squares = (p.dq || p.dscale) && want_squares(p)
+                       ? take_floats(ws, p.B * p.Hk * p.Nk)
+                       : nullptr;
+  p.key_squares = squares;
   CrossProblem pq = p, pk = p;
   const bool want_q = p.dq || p.dscale;
   if (want_q) {
@@ -1028,6 +1086,8 @@ cudaError_t run_cross_tc_backward(const CrossProblem& problem, Workspace& ws,
   }
   if (ws.dry || ws.overflow) return cudaSuccess;
   cudaError_t e = launch_cross_delta(p, delta, stream);
+  if (e == cudaSuccess && squares)
+    e = launch_cross_squares(p, squares, stream);
   if (e == cudaSuccess && want_q && rows > 0) {
     e = launch_pass<kQueries>(pq, stream);
     if (e == cudaSuccess && pq.part)

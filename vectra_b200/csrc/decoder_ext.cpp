@@ -159,6 +159,8 @@ void check_norm(const Tensor& x, const OptTensor& branch,
                 const NormCall& call, bool norm) {
   check_io(x);
   TORCH_CHECK_VALUE(x.dim() >= 1, "x must be [..., C]");
+  TORCH_CHECK_NOT_IMPLEMENTED(x.size(-1) <= 16384,
+                              "vectra_b200::residual_norm: rows above 16384");
   check_drop(x, call.p, call.rng);
   if (has(branch)) {
     check_like(*branch, "branch", x);
@@ -471,6 +473,9 @@ void check_cross(const Tensor& q, const Tensor& k, const Tensor& v,
                     "k ", k.sizes());
   TORCH_CHECK_VALUE(q.size(3) >= 1 && v.size(3) >= 1,
                     "head vectors must not be empty");
+  TORCH_CHECK_NOT_IMPLEMENTED(q.size(3) <= 256 && v.size(3) <= 256,
+                              "vectra_b200::cross_attention: a head width "
+                              "above 256");
   TORCH_CHECK_VALUE(k.size(1) > 0 ? q.size(1) % k.size(1) == 0
                                   : q.size(1) == 0,
                     "q's ", q.size(1), " heads must be a multiple of k's ",
@@ -627,9 +632,6 @@ struct CpuCross {
 };
 CpuCross cpu_cross(const Tensor& q, const Tensor& k, const Tensor& v,
                    const Tensor& scale, const OptTensor& lengths) {
-  TORCH_CHECK_NOT_IMPLEMENTED(q.size(3) <= 256 && v.size(3) <= 256,
-                              "vectra_b200::cross_attention: a head width "
-                              "above 256");
   const int64_t b = q.size(0), h = q.size(1), hk = k.size(1), nk = k.size(2);
   const int64_t g = hk > 0 ? h / hk : 1;
   CpuCross t;
@@ -647,6 +649,13 @@ CpuCross cpu_cross(const Tensor& q, const Tensor& k, const Tensor& v,
   t.dist = at::cdist(t.q, t.k.expand({b, hk, g, nk, k.size(3)}), 2.0, 2)
                .square();
   return t;
+}
+
+// What lse leaves out (include/vectra_block.h).
+Tensor cpu_left_out(const CpuCross& t, const Tensor& q) {
+  return q.scalar_type() == at::kFloat
+             ? at::zeros({}, at::kFloat)
+             : t.scale * t.q.square().sum({-1}, true) * 1.4426950408889634;
 }
 
 Three cross_cpu(const Tensor& q, const Tensor& k, const Tensor& v,
@@ -674,7 +683,9 @@ Three cross_cpu(const Tensor& q, const Tensor& k, const Tensor& v,
   out.copy_(o);
   if (rest.numel()) rest.copy_(o - f32(out));
   if (want_lse)
-    lse.copy_(at::where(any, at::logsumexp(s, {-1}, true) * 1.4426950408889634,
+    lse.copy_(at::where(any,
+                        at::logsumexp(s, {-1}, true) * 1.4426950408889634 +
+                            cpu_left_out(t, q),
                         -inf)
                   .reshape(lse.sizes()));
   return {out, lse, rest};
@@ -705,7 +716,8 @@ Four cross_backward_cpu(const Tensor& dout, const Tensor& q, const Tensor& k,
   if (q.scalar_type() != at::kFloat) o = o + f32(rest);
   o = o.reshape(e.sizes());
   const Tensor zero = at::zeros({}, at::kFloat);
-  const Tensor from = lse.reshape({b, hk, g, nq, 1});
+  const Tensor from =
+      lse.reshape({b, hk, g, nq, 1}) - cpu_left_out(t, q);
   const Tensor w = at::where(
       t.seen,
       at::exp2(-t.scale * t.dist * 1.4426950408889634 - from), zero);

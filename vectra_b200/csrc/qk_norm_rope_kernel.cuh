@@ -285,7 +285,22 @@ __device__ __forceinline__ void load_angles(const QkProblem& p,
     a->s[i] = 0.f;
   }
   if (!rows.known) return;
-  // Four pairs that are loaded together are of one axis (vec_ok).
+  if constexpr (MULTI) {
+    // Sections that end inside four neighbouring pairs: one pair at a time.
+    if (!p.whole_quads) {
+#pragma unroll
+      for (int i = 0; i < VE; ++i) {
+        const int c = INTER && i >= VE / 2 ? c1 : c0;
+        const int j = INTER ? c * (VE / 2) + i % (VE / 2) : c0 * VE + i;
+        if (c < 0 || j >= p.R2) continue;
+        const int64_t row = row_of(p, rows, j);
+        a->c[i] = __ldg(p.cos + row * p.cos_ld + j);
+        a->s[i] = __ldg(p.sin + row * p.sin_ld + j);
+      }
+      return;
+    }
+  }
+  // Pairs that are loaded together are of one axis.
   if constexpr (!INTER) {
     if (c0 >= 0 && c0 * VE < p.R2) {
 #pragma unroll
@@ -744,8 +759,6 @@ bool vec_ok(const QkProblem& p, bool backward) {
   const int ve = 16 / es;
   if (p.D % ve || p.D / ve > 64) return false;
   if ((p.interleaved ? 2 * p.R2 : p.R2) % ve) return false;
-  for (int a = 1; a < p.axes; ++a)
-    if (p.first_pair[a] % 4) return false;
   if (p.R2 > 0 && ((reinterpret_cast<uintptr_t>(p.cos) & 15) ||
                    (reinterpret_cast<uintptr_t>(p.sin) & 15) ||
                    p.cos_ld % 4 || p.sin_ld % 4))

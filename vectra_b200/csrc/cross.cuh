@@ -100,6 +100,13 @@ cudaError_t run_cross_tc_forward(const CrossProblem& p, Workspace& ws,
 cudaError_t run_cross_tc_backward(const CrossProblem& p, Workspace& ws,
                                   cudaStream_t stream);
 
+// cross_rows.cu: bf16 and f16, up to 16 packed rows, widths up to 128.
+bool cross_rows_supports(const CrossProblem& p, bool backward);
+cudaError_t run_cross_rows_forward(const CrossProblem& p, Workspace& ws,
+                                   cudaStream_t stream);
+cudaError_t run_cross_rows_backward(const CrossProblem& p, Workspace& ws,
+                                    cudaStream_t stream);
+
 // cross_finish.cu.
 // c_i of every row into delta.
 cudaError_t launch_cross_delta(const CrossProblem& p, float* delta,

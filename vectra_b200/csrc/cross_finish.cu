@@ -176,18 +176,19 @@ __global__ void __launch_bounds__(256) sum_kernel(const SumArgs a) {
   }
 }
 
-// One block a head of a sequence. A row's three sums over its parts are
+// One warp a head of a sequence. A row's three sums over its parts are
 // X = sum z d, Y = sum P d and Z = sum z, of distances d; its share is
 // -(X - Y Z), where Z is what rounding left of zero.
 __global__ void __launch_bounds__(256)
     dscale_kernel(const __grid_constant__ CrossProblem p, int splits) {
-  __shared__ double sums[8];
   allow_dependents();
   grid_dependency_wait();
   const int64_t rows = p.B * p.H * p.Nq;
-  const int64_t first = int64_t(blockIdx.x) * p.Nq;
+  const int64_t head = int64_t(blockIdx.x) * 8 + threadIdx.x / 32;
+  if (head >= p.B * p.H) return;
+  const int64_t first = head * p.Nq;
   double t = 0.0;
-  for (int64_t i = threadIdx.x; i < p.Nq; i += blockDim.x) {
+  for (int64_t i = threadIdx.x % 32; i < p.Nq; i += 32) {
     float x = 0.f, y = 0.f, z = 0.f;
     for (int s = 0; s < splits; ++s) {
       const float* w = p.dscale_rows + (s * rows + first + i) * 3;
@@ -200,13 +201,7 @@ __global__ void __launch_bounds__(256)
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
-  if (threadIdx.x % 32 == 0) sums[threadIdx.x / 32] = t;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    double all = 0.0;
-    for (int w = 0; w < 8; ++w) all += sums[w];
-    p.dscale[blockIdx.x] = float(all);
-  }
+  if (threadIdx.x % 32 == 0) p.dscale[head] = float(t);
 }
 
 unsigned row_blocks(int64_t rows) {
@@ -283,8 +278,8 @@ cudaError_t launch_cross_dscale(const CrossProblem& p, int splits,
                                 cudaStream_t stream) {
   if (p.B * p.H == 0) return cudaSuccess;
   count_launches(1);
-  return launch_pdl(dscale_kernel, dim3(unsigned(p.B * p.H)), dim3(256), 0,
-                    stream, p, splits);
+  return launch_pdl(dscale_kernel, dim3(unsigned((p.B * p.H + 7) / 8)),
+                    dim3(256), 0, stream, p, splits);
 }
 
 }  // namespace vectra

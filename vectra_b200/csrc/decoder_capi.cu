@@ -261,7 +261,9 @@ int cross_forward(const vectra_cross_args& a, Workspace& ws,
   CrossProblem p;
   VECTRA_TRY(build_cross(a, &p));
   p.err = ws.dry ? nullptr : device_error_ptr();
-  return to_status(cross_tc_supports(p, false)
+  return to_status(cross_rows_supports(p, false)
+                       ? run_cross_rows_forward(p, ws, stream)
+                   : cross_tc_supports(p, false)
                        ? run_cross_tc_forward(p, ws, stream)
                        : run_cross_simple_forward(p, ws, stream),
                    ws);
@@ -289,7 +291,9 @@ int cross_backward(const vectra_cross_grad_args& a, Workspace& ws,
     p.dscale = static_cast<float*>(const_cast<void*>(a.dscale.data));
   }
   p.err = ws.dry ? nullptr : device_error_ptr();
-  return to_status(cross_tc_supports(p, true)
+  return to_status(cross_rows_supports(p, true)
+                       ? run_cross_rows_backward(p, ws, stream)
+                   : cross_tc_supports(p, true)
                        ? run_cross_tc_backward(p, ws, stream)
                        : run_cross_simple_backward(p, ws, stream),
                    ws);

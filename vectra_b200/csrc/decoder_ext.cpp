@@ -607,12 +607,22 @@ Four cross_backward_cuda(const Tensor& dout, const Tensor& q, const Tensor& k,
     return {dq, dk, dv, dscale};
   }
   const Tensor s4 = rank4(scale);
+  // The 16-bit kernels read rows in 16-byte pieces: an upstream gradient that
+  // has none (an expanded one) is packed.
+  Tensor e = dout;
+  if (q.scalar_type() != at::kFloat && dout.numel() > 0) {
+    bool pieces = dout.stride(3) == 1 &&
+                  reinterpret_cast<uintptr_t>(dout.data_ptr()) % 16 == 0;
+    for (int i = 0; i < 3; ++i)
+      pieces = pieces && (dout.size(i) == 1 || dout.stride(i) % 8 == 0);
+    if (!pieces) e = heads_like(q, v.size(3)).copy_(dout);
+  }
   vectra_cross_grad_args a{};
   a.fwd = describe_cross(q, k, v, s4, lengths);
   a.fwd.out = describe(out);
   a.fwd.lse = describe(lse);
   if (rest.numel() && q.scalar_type() != at::kFloat) a.fwd.rest = describe(rest);
-  a.dout = describe(dout);
+  a.dout = describe(e);
   if (need_dq) a.dq = describe(dq);
   if (need_dkv) {
     a.dk = describe(dk);

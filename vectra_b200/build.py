@@ -38,7 +38,8 @@ CU_SOURCES = ['capi.cu', 'rbf_generic.cu', 'rbf_decode.cu', 'rbf_tc.cu',
               'gemm_tc_linear_f16.cu', 'gemm_tc_other_bf16.cu',
               'gemm_tc_other_f16.cu', 'gemm_tc_linear_f32.cu',
               'gemm_tc_other_f32.cu', 'qk_norm_rope.cu', 'qk_norm_rope_axes.cu',
-              'residual_norm.cu', 'cross_simple.cu', 'cross_finish.cu',
+              'residual_norm.cu', 'residual_norm_bf16.cu', 'residual_norm_f16.cu',
+              'residual_norm_f32.cu', 'cross_simple.cu', 'cross_finish.cu',
               'cross_tc.cu', 'cross_rows.cu', 'decoder_capi.cu']
 ARCH = ['-gencode', 'arch=compute_100a,code=sm_100a']
 

@@ -55,9 +55,36 @@ __device__ __forceinline__ void stage(float* dst, const void* base,
                                       const int64_t* s, int64_t b, int64_t h0,
                                       int64_t group, int64_t first,
                                       int64_t rows, int width) {
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+  if constexpr (std::is_same<T, float>::value) {
+    // Whole 16-byte pieces: a warp takes one of 32 rows, whose components it
+    // stores without conflicts.
+    if (width % 4 == 0 && s[3] == 1 && s[0] % 4 == 0 && s[1] % 4 == 0 &&
+        s[2] % 4 == 0 && (reinterpret_cast<uintptr_t>(base) & 15) == 0) {
+      constexpr int ROWS = N < 32 ? N : 32, SIDE = 32 / ROWS;
+      const int r0 = lane % ROWS, d0 = lane / ROWS;
+      for (int at = warp; at < N / ROWS * (W / 4) / SIDE; at += kThreads / 32) {
+        const int r = at % (N / ROWS) * ROWS + r0;
+        const int d = (at / (N / ROWS) * SIDE + d0) * 4;
+        const int64_t row = first + r;
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (row < rows && d < width) {
+          const int64_t i = group == 1 ? row : row / group;
+          const int64_t g = group == 1 ? 0 : row - i * group;
+          v = __ldg(reinterpret_cast<const float4*>(
+              static_cast<const float*>(base) + b * s[0] + (h0 + g) * s[1] +
+              i * s[2] + d));
+        }
+        dst[d * L + r] = v.x;
+        dst[(d + 1) * L + r] = v.y;
+        dst[(d + 2) * L + r] = v.z;
+        dst[(d + 3) * L + r] = v.w;
+      }
+      return;
+    }
+  }
   // A warp reads 8 components of 4 rows a step: whole 32-byte sectors of
   // 32-bit values, and stores that meet in at most 2 ways.
-  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
   const int dl = lane % 8, rl = lane / 8;
   for (int r = warp * 4 + rl; r < N; r += (kThreads / 32) * 4) {
     const int64_t row = first + r;
@@ -529,15 +556,22 @@ cudaError_t launch_pass(const CrossProblem& p, cudaStream_t stream) {
   });
 }
 
-// Parts of the axis that a block walks: enough for two blocks an SM, each of
-// two tiles at least.
-int splits_for(const CrossProblem& p, int64_t rows, int64_t cols) {
+// Parts of the axis that a block walks: enough for twice the blocks that the
+// SMs hold (`per_sm` by their shared memory), each of two tiles at least.
+int splits_for(const CrossProblem& p, int64_t rows, int64_t cols,
+               bool backward) {
   int r, c;
   tile_of(p, rows, &r, &c);
   const int64_t blocks = (rows + r - 1) / r * p.B * p.Hk;
   const int64_t tiles = (cols + c - 1) / c;
   if (blocks == 0) return 1;
-  int64_t s = 2 * int64_t(device_sm_count()) / blocks;
+  const int64_t w = width_of(p);
+  const int64_t bytes =
+      4 * (backward ? 2 * w * (r + c + 8) + 2 * r * (c + 4)
+                    : w * (r + 2 * c + 12) + r * (c + 4));
+  int64_t per_sm = 227 * 1024 / (bytes + 1024);
+  if (per_sm > 4) per_sm = 4;
+  int64_t s = 2 * per_sm * device_sm_count() / blocks;
   if (s > tiles / 2) s = tiles / 2;
   if (s > 64) s = 64;
   return s < 1 ? 1 : int(s);
@@ -553,7 +587,7 @@ cudaError_t run_cross_simple_forward(const CrossProblem& problem,
                                      Workspace& ws, cudaStream_t stream) {
   CrossProblem p = problem;
   const int64_t rows = p.B * p.H * p.Nq;
-  p.splits = splits_for(p, p.Nq * p.G, p.Nk);
+  p.splits = splits_for(p, p.Nq * p.G, p.Nk, false);
   if (p.splits > 1) {
     p.part = take_floats(ws, p.splits * rows * p.Dv);
     p.part_ml = take_floats(ws, p.splits * rows * 2);
@@ -572,12 +606,12 @@ cudaError_t run_cross_simple_backward(const CrossProblem& problem,
   CrossProblem pq = p, pk = p;
   const bool want_q = p.dq || p.dscale;
   if (want_q) {
-    pq.splits = splits_for(p, p.Nq * p.G, p.Nk);
+    pq.splits = splits_for(p, p.Nq * p.G, p.Nk, true);
     if (p.dscale) pq.dscale_rows = take_floats(ws, pq.splits * rows * 3);
     if (pq.splits > 1 && p.dq) pq.part = take_floats(ws, pq.splits * rows * p.D);
   }
   if (p.dk) {
-    pk.splits = splits_for(p, p.Nk, p.Nq * p.G);
+    pk.splits = splits_for(p, p.Nk, p.Nq * p.G, true);
     if (pk.splits > 1) {
       pk.part = take_floats(ws, pk.splits * keys * p.D);
       pk.part_v = take_floats(ws, pk.splits * keys * p.Dv);

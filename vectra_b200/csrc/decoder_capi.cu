@@ -56,7 +56,7 @@ int build_norm(const vectra_residual_norm_args& a, const vectra_tensor& rows,
   if (!io_dtype_ok(dtype)) return VECTRA_ERR_DTYPE;
   const int64_t m = rows.size[0], c = rows.size[1];
   if (m < 0 || c < 0) return VECTRA_ERR_SHAPE;
-  if (c > kMaxNormCols) return VECTRA_ERR_UNSUPPORTED;
+  if (c > kMaxNormCols || m > kMaxSize) return VECTRA_ERR_UNSUPPORTED;
   if (a.kind != VECTRA_NORM_RMS && a.kind != VECTRA_NORM_LAYER)
     return VECTRA_ERR_UNSUPPORTED;
   VECTRA_TRY(check_drop(a.drop));

@@ -113,28 +113,46 @@ __global__ void __launch_bounds__(256)
     const int64_t bh = r / p.Nq, i = r - bh * p.Nq;
     const int64_t b = bh / p.H, h = bh - b * p.H;
     const float2* ml = reinterpret_cast<const float2*>(p.part_ml) + r;
-    float m = kNegInf;
-    bool nan = false;
-    for (int s = 0; s < p.splits; ++s) {
-      const float x = ml[s * rows].x;
-      m = fmaxf(m, x);
-      nan = nan || x != x;
+    // Two parts a lane (64 at most): their factors, then the sums over parts
+    // with four parts' loads under way.
+    float2 own[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int s = lane + 32 * i;
+      own[i] = s < p.splits ? ml[s * rows] : make_float2(kNegInf, 0.f);
     }
-    if (nan) m = NAN;
-    float l = 0.f;
+    const bool nan = __any_sync(0xffffffffu, own[0].x != own[0].x ||
+                                                 own[1].x != own[1].x);
+    const float m = nan ? NAN : warp_max(fmaxf(own[0].x, own[1].x));
+    float f[2], l = 0.f;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      // A part whose keys all weigh nothing (or that has none) adds nothing.
+      f[i] = own[i].x == kNegInf ? 0.f : fast_exp2(own[i].x - m);
+      l += own[i].x == kNegInf ? 0.f : own[i].y * f[i];
+    }
+    l = warp_sum(l);
     float acc[kMaxCrossWidth / 32];
 #pragma unroll
     for (int c = 0; c < kMaxCrossWidth / 32; ++c) acc[c] = 0.f;
-    for (int s = 0; s < p.splits; ++s) {
-      const float2 t = ml[s * rows];
-      // A part whose keys all weigh nothing (or that has none) adds nothing.
-      if (t.x == kNegInf) continue;
-      const float f = fast_exp2(t.x - m);
-      l = fmaf(t.y, f, l);
-      const float* o = p.part + (s * rows + r) * p.Dv;
+    for (int s0 = 0; s0 < p.splits; s0 += 4) {
+      float v[4][kMaxCrossWidth / 32];
+      float by[4];
 #pragma unroll
-      for (int c = 0; c < kMaxCrossWidth / 32; ++c)
-        if (c * 32 + lane < p.Dv) acc[c] = fmaf(o[c * 32 + lane], f, acc[c]);
+      for (int i = 0; i < 4; ++i) {
+        const int s = s0 + i;
+        by[i] = __shfl_sync(0xffffffffu, s < 32 ? f[0] : f[1], s & 31);
+        const float* o = p.part + (s * rows + r) * p.Dv;
+#pragma unroll
+        for (int c = 0; c < kMaxCrossWidth / 32; ++c)
+          v[i][c] = s < p.splits && c * 32 + lane < p.Dv ? o[c * 32 + lane]
+                                                         : 0.f;
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int c = 0; c < kMaxCrossWidth / 32; ++c)
+          if (by[i] != 0.f) acc[c] = fmaf(v[i][c], by[i], acc[c]);
     }
     const bool any = cross_length(p, b) > 0;
     T* out = static_cast<T*>(p.out) + b * p.so[0] + h * p.so[1] + i * p.so[2];
@@ -169,39 +187,50 @@ __global__ void __launch_bounds__(256) sum_kernel(const SumArgs a) {
     T* out = static_cast<T*>(a.out) + b * a.so[0] + h * a.so[1] + i * a.so[2];
     for (int d = lane; d < a.width; d += 32) {
       float t = 0.f;
+#pragma unroll 4
       for (int s = 0; s < a.splits; ++s)
-        t += a.part[(s * a.rows + r) * a.width + d];
+        t += __ldg(a.part + (s * a.rows + r) * a.width + d);
       out[d] = from_f32<T>(t);
     }
   }
 }
 
-// One warp a head of a sequence. A row's three sums over its parts are
-// X = sum z d, Y = sum P d and Z = sum z, of distances d; its share is
-// -(X - Y Z), where Z is what rounding left of zero.
+// `warps` warps (of a block of eight) a head of a sequence. A row's three sums
+// over its parts are X = sum z d, Y = sum P d and Z = sum z, of distances d; its
+// share is -(X - Y Z), where Z is what rounding left of zero.
 __global__ void __launch_bounds__(256)
-    dscale_kernel(const __grid_constant__ CrossProblem p, int splits) {
+    dscale_kernel(const __grid_constant__ CrossProblem p, int splits,
+                  int warps) {
+  __shared__ double sums[8];
   allow_dependents();
   grid_dependency_wait();
   const int64_t rows = p.B * p.H * p.Nq;
-  const int64_t head = int64_t(blockIdx.x) * 8 + threadIdx.x / 32;
-  if (head >= p.B * p.H) return;
-  const int64_t first = head * p.Nq;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int64_t head = int64_t(blockIdx.x) * (8 / warps) + warp / warps;
   double t = 0.0;
-  for (int64_t i = threadIdx.x % 32; i < p.Nq; i += 32) {
-    float x = 0.f, y = 0.f, z = 0.f;
-    for (int s = 0; s < splits; ++s) {
-      const float* w = p.dscale_rows + (s * rows + first + i) * 3;
-      x += w[0];
-      y += w[1];
-      z += w[2];
+  if (head < p.B * p.H) {
+    const int64_t first = head * p.Nq;
+    for (int64_t i = warp % warps * 32 + lane; i < p.Nq; i += warps * 32) {
+      float x = 0.f, y = 0.f, z = 0.f;
+#pragma unroll 4
+      for (int s = 0; s < splits; ++s) {
+        const float* w = p.dscale_rows + (s * rows + first + i) * 3;
+        x += __ldg(w);
+        y += __ldg(w + 1);
+        z += __ldg(w + 2);
+      }
+      // Rounded products: over a single key the difference is exactly zero.
+      t -= double(__fsub_rn(x, __fmul_rn(y, z)));
     }
-    // Rounded products: over a single key the difference is exactly zero.
-    t -= double(__fsub_rn(x, __fmul_rn(y, z)));
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
-  if (threadIdx.x % 32 == 0) p.dscale[head] = float(t);
+  if (lane == 0) sums[warp] = t;
+  __syncthreads();
+  if (lane == 0 && warp % warps == 0 && head < p.B * p.H) {
+    for (int w = 1; w < warps; ++w) t += sums[warp + w];
+    p.dscale[head] = float(t);
+  }
 }
 
 unsigned row_blocks(int64_t rows) {
@@ -278,8 +307,10 @@ cudaError_t launch_cross_dscale(const CrossProblem& p, int splits,
                                 cudaStream_t stream) {
   if (p.B * p.H == 0) return cudaSuccess;
   count_launches(1);
-  return launch_pdl(dscale_kernel, dim3(unsigned((p.B * p.H + 7) / 8)),
-                    dim3(256), 0, stream, p, splits);
+  const int warps = p.Nq > 64 ? 8 : 1;
+  const int64_t per = 8 / warps;
+  return launch_pdl(dscale_kernel, dim3(unsigned((p.B * p.H + per - 1) / per)),
+                    dim3(256), 0, stream, p, splits, warps);
 }
 
 }  // namespace vectra

@@ -365,6 +365,206 @@ __global__ void __launch_bounds__(kWarps * 32)
   }
 }
 
+// Up to 8 rows: the rows are the fragments' 8 columns and the keys, or the
+// components of out, their 16 rows, which takes half as many instructions on
+// the tensor cores (whose warp-level form set the pace of a decoding step: 48 a
+// step of 16 keys of 128 with the rows as rows, 79 us for 32 sequences over up
+// to 4,001 keys; REST false, without a backward pass to come, leaves out the
+// products with what P's rounding left).
+//   S^T = k q^T, out^T += v^T P^T
+template <typename T, int NB, bool REST>
+__global__ void __launch_bounds__(kWarps * 32)
+    few_rows_forward_kernel(const __grid_constant__ CrossProblem p) {
+  allow_dependents();
+  grid_dependency_wait();
+  const int lane = threadIdx.x % 32, g = lane / 4, t = lane % 4;
+  const int64_t unit = int64_t(blockIdx.x) * kWarps + threadIdx.x / 32;
+  const int64_t plane = unit / p.splits;
+  if (plane >= p.B * p.Hk) return;
+  const int part = int(unit - plane * p.splits);
+  const int64_t b = plane / p.Hk, hk = plane - b * p.Hk;
+  const int len = cross_length(p, b);
+  int t0, t1;
+  split_range((len + kKeys - 1) / kKeys, part, p.splits, &t0, &t1);
+
+  extern __shared__ uint4 ring_memory[];
+  constexpr int STAGES = kForwardStages<NB>;
+  Ring<T, NB, STAGES> ring{ring_memory + threadIdx.x};
+#pragma unroll
+  for (int i = 0; i < STAGES - 1; ++i)
+    ring.fetch(p, b, hk, t0 + i, t1, len, lane);
+
+  const Row own = packed_row(p, b, hk, g);
+  uint32_t q[NB][4];
+  load_row<NB>(q, row_of<T>(p.q, p.sq, b, own.h, own.i), own.live, p.D, t);
+  // Rows 2 t and 2 t + 1, the columns of this thread's fragments.
+  float gl[2], m[2] = {kNegInf, kNegInf}, l[2] = {0.f, 0.f};
+#pragma unroll
+  for (int c = 0; c < 2; ++c) {
+    const Row r = packed_row(p, b, hk, 2 * t + c);
+    gl[c] = r.live ? cross_scale(p, b, r.h) * kLog2e : 0.f;
+  }
+  float acc[NB * 2][4];
+#pragma unroll
+  for (int n = 0; n < NB * 2; ++n)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[n][i] = 0.f;
+
+  for (int step = t0; step < t1; ++step) {
+    ring.fetch(p, b, hk, step + STAGES - 1, t1, len, lane);
+    ring.wait();
+    float s[4] = {0.f, 0.f, 0.f, 0.f};
+    float nk[2];
+    {
+      uint32_t k[2][NB][4];
+      ring.read(step, 0, 0, k[0]);
+      ring.read(step, 0, 1, k[1]);
+      float sq[2] = {0.f, 0.f};
+#pragma unroll
+      for (int n = 0; n < NB; ++n) {
+#pragma unroll
+        for (int w = 0; w < 4; w += 2) {
+          const uint32_t f[4] = {k[0][n][w], k[1][n][w], k[0][n][w + 1],
+                                 k[1][n][w + 1]};
+          mma16816<T>(s, f, q[n][w], q[n][w + 1]);
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            const float2 f = pair<T>(k[h][n][w]);
+            sq[h] = fmaf(f.x, f.x, sq[h]);
+            sq[h] = fmaf(f.y, f.y, sq[h]);
+          }
+      }
+      nk[0] = quad_sum(sq[0]);
+      nk[1] = quad_sum(sq[1]);
+    }
+    // s[2 h + c]: key g + 8 h, row 2 t + c.
+    float x[4];
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const bool in = step * kKeys + 8 * h + g < len;
+        x[2 * h + c] =
+            in ? gl[c] * fmaf(2.f, s[2 * h + c], -nk[h]) : kNegInf;
+      }
+    bool grows = false;
+    float top[2];
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      top[c] = fmaxf(x[c], x[2 + c]);
+#pragma unroll
+      for (int o = 4; o < 32; o *= 2)
+        top[c] = fmaxf(top[c], __shfl_xor_sync(0xffffffffu, top[c], o));
+      grows = grows || top[c] > m[c];
+    }
+    if (__any_sync(0xffffffffu, grows)) {
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const float next = fmaxf(m[c], top[c]);
+        const float f = m[c] == kNegInf ? 0.f : fast_exp2(m[c] - next);
+        m[c] = next;
+        l[c] *= f;
+#pragma unroll
+        for (int n = 0; n < NB * 2; ++n) {
+          acc[n][c] *= f;
+          acc[n][2 + c] *= f;
+        }
+      }
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        x[2 * h + c] =
+            fast_exp2(x[2 * h + c] - (m[c] == kNegInf ? 0.f : m[c]));
+        l[c] += x[2 * h + c];
+      }
+    uint32_t hi[2], lo[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const uint32_t w = pack_pair<T>(x[2 * h], x[2 * h + 1]);
+      hi[h] = turn(w);
+      if constexpr (REST) {
+        const float2 f = pair<T>(w);
+        lo[h] = turn(pack_pair<T>(x[2 * h] - f.x, x[2 * h + 1] - f.y));
+      }
+    }
+    uint32_t v[2][NB][4];
+    ring.read(step, 1, 0, v[0]);
+    ring.read(step, 1, 1, v[1]);
+#pragma unroll
+    for (int n = 0; n < NB; ++n)
+#pragma unroll
+      for (int w = 0; w < 4; w += 2) {
+        const uint32_t f[4] = {turn(v[0][n][w]), turn(v[0][n][w + 1]),
+                               turn(v[1][n][w]), turn(v[1][n][w + 1])};
+        mma16816<T>(acc[n * 2 + w / 2], f, hi[0], hi[1]);
+        if constexpr (REST) mma16816<T>(acc[n * 2 + w / 2], f, lo[0], lo[1]);
+      }
+  }
+
+  const int64_t rows = p.B * p.H * p.Nq;
+  const bool whole = p.splits == 1;
+  float inv[2];
+#pragma unroll
+  for (int c = 0; c < 2; ++c) {
+#pragma unroll
+    for (int o = 4; o < 32; o *= 2)
+      l[c] += __shfl_xor_sync(0xffffffffu, l[c], o);
+    inv[c] = whole ? (len > 0 ? 1.f / l[c] : 0.f) : 1.f;
+    const Row r = packed_row(p, b, hk, 2 * t + c);
+    if (g != 0 || !r.live) continue;
+    if (!whole) {
+      const int64_t at = part * rows + r.at;
+      p.part_ml[2 * at] = m[c];
+      p.part_ml[2 * at + 1] = l[c];
+    } else if (p.lse) {
+      p.lse[r.at] = len > 0 ? m[c] + log2f(l[c]) : INFINITY;
+    }
+  }
+  if (!whole) {
+    // acc[2 n + w / 2][2 (w % 2) + c]: row 2 t + c, component
+    // 32 n + 8 (g / 2) + 2 w + g % 2.
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      const Row r = packed_row(p, b, hk, 2 * t + c);
+      if (!r.live) continue;
+      float* out = p.part + (part * rows + r.at) * p.Dv;
+#pragma unroll
+      for (int n = 0; n < NB; ++n)
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const int d = n * 32 + 8 * (g / 2) + 2 * w + g % 2;
+          if (d < p.Dv) out[d] = acc[n * 2 + w / 2][2 * (w % 2) + c];
+        }
+    }
+    return;
+  }
+  T* out = row_of<T>(p.out, p.so, b, own.h, own.i);
+  T* rest = p.rest ? static_cast<T*>(p.rest) + own.at * p.Dv : nullptr;
+#pragma unroll
+  for (int n = 0; n < NB; ++n) {
+    const int d = n * 32 + t * 8;
+    uint32_t w[4], x[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float a0 = acc[n * 2 + i / 2][2 * (i % 2)] * inv[0];
+      const float a1 = acc[n * 2 + i / 2][2 * (i % 2) + 1] * inv[1];
+      const uint32_t pr = pack_pair<T>(a0, a1);
+      w[i] = turn(pr);
+      const float2 f = pair<T>(pr);
+      x[i] = turn(pack_pair<T>(a0 - f.x, a1 - f.y));
+    }
+    if (!own.live || d >= p.Dv) continue;
+    *reinterpret_cast<uint4*>(out + d) = make_uint4(w[0], w[1], w[2], w[3]);
+    if (rest)
+      *reinterpret_cast<uint4*>(rest + d) = make_uint4(x[0], x[1], x[2], x[3]);
+  }
+}
+
 // The turned q and e of dk and dv, [warp][q or e][block][row group and word]:
 // in shared memory for widths whose registers they would take.
 template <int NB>
@@ -716,7 +916,10 @@ cudaError_t run_cross_rows_forward(const CrossProblem& problem, Workspace& ws,
     using T = std::remove_pointer_t<decltype(t)>;
     constexpr int NB = decltype(nb)::value;
     constexpr int bytes = Ring<T, NB, kForwardStages<NB>>::BYTES;
-    auto kern = rows_forward_kernel<T, NB, decltype(nr)::value>;
+    auto kern = rows_forward_kernel<T, NB, 2>;
+    if (decltype(nr)::value == 1)
+      kern = p.lse ? few_rows_forward_kernel<T, NB, true>
+                   : few_rows_forward_kernel<T, NB, false>;
     const cudaError_t st = cudaFuncSetAttribute(
         kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
     if (st != cudaSuccess) return st;

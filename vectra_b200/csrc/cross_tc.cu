@@ -237,20 +237,20 @@ __device__ __forceinline__ void store8f(float* out, const float* v, int live) {
     if (i < live) out[i] = v[i];
 }
 
+// One pass' work of one block: rows `block`, part `part` of the columns.
 template <typename T, int W, int PASS, bool KEEP>
-__global__ void __launch_bounds__(kThreads, 1)
-    cross_tc_kernel(const __grid_constant__ CUtensorMap tr,
-                    const __grid_constant__ CUtensorMap tr2,
-                    const __grid_constant__ CUtensorMap tcol,
-                    const __grid_constant__ CUtensorMap tcol2,
-                    const __grid_constant__ TcArgs a) {
+__device__ __forceinline__ void cross_pass(const CUtensorMap& tr,
+                                           const CUtensorMap& tr2,
+                                           const CUtensorMap& tcol,
+                                           const CUtensorMap& tcol2,
+                                           const TcArgs& a, uint32_t block,
+                                           int part, uint8_t* smem_raw) {
   using C = Cfg<W, PASS>;
   constexpr bool kBack = C::kBack;
   constexpr bool kRowsAreQueries = PASS != kKeys;
   constexpr int CN = C::CN, NS = C::NS;
   constexpr int FMT = std::is_same<T, __nv_bfloat16>::value ? 1 : 0;
   const CrossProblem& p = a.p;
-  extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const uint32_t sbase = smem_addr(smem);
@@ -268,14 +268,11 @@ __global__ void __launch_bounds__(kThreads, 1)
   float* term = reinterpret_cast<float*>(smem + C::OFF_TERM);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t plane = blockIdx.x / p.row_blocks;
-  const int tile = int(blockIdx.x - plane * p.row_blocks);
+  const int64_t plane = block / p.row_blocks;
+  const int tile = int(block - plane * p.row_blocks);
   const int b = int(plane / p.Hk), hk = int(plane - int64_t(b) * p.Hk);
   const int G = int(p.G);
-  const int part = blockIdx.y;
 
-  allow_dependents();
-  grid_dependency_wait();
   const int len = cross_length(p, b);
   const int nq = int(p.Nq);
   const int row0 = tile * a.rows_i;    // first query, or first key
@@ -924,77 +921,168 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
+template <typename T, int W, bool KEEP>
+__global__ void __launch_bounds__(kThreads, 1)
+    cross_tc_forward_kernel(const __grid_constant__ CUtensorMap q,
+                            const __grid_constant__ CUtensorMap k,
+                            const __grid_constant__ CUtensorMap v,
+                            const __grid_constant__ TcArgs a) {
+  extern __shared__ uint8_t smem_raw[];
+  allow_dependents();
+  grid_dependency_wait();
+  cross_pass<T, W, kForward, KEEP>(q, q, k, v, a, blockIdx.x, blockIdx.y,
+                                   smem_raw);
+}
+
+// Both backward passes in one grid: the keys' blocks, which are longer, first,
+// and the queries' behind them fill the SMs that they leave. All gradients of 2048
+// queries x 16 heads over 4500 keys x 4 heads, width 128, batch 4: 726 us, as
+// two launches 838.
+struct BackwardArgs {
+  CUtensorMap keys[4];     // k, v, q, e
+  CUtensorMap queries[4];  // q, e, k, v
+  TcArgs a[2];             // of the keys' and the queries' pass
+  uint32_t blocks[2];      // of a part of each
+  uint32_t key_blocks;     // of all parts
+};
+template <typename T, int W>
+__global__ void __launch_bounds__(kThreads, 1)
+    cross_tc_backward_kernel(const __grid_constant__ BackwardArgs x) {
+  extern __shared__ uint8_t smem_raw[];
+  allow_dependents();
+  grid_dependency_wait();
+  if (blockIdx.x < x.key_blocks) {
+    const uint32_t part = blockIdx.x / x.blocks[0];
+    cross_pass<T, W, kKeys, false>(x.keys[0], x.keys[1], x.keys[2], x.keys[3],
+                                   x.a[0], blockIdx.x - part * x.blocks[0],
+                                   int(part), smem_raw);
+  } else {
+    const uint32_t at = blockIdx.x - x.key_blocks;
+    const uint32_t part = at / x.blocks[1];
+    cross_pass<T, W, kQueries, false>(
+        x.queries[0], x.queries[1], x.queries[2], x.queries[3], x.a[1],
+        at - part * x.blocks[1], int(part), smem_raw);
+  }
+}
+
 // ---------------------------------------------------------------------------
 // Host side.
 // ---------------------------------------------------------------------------
-template <typename T, int W, int PASS, bool KEEP>
-cudaError_t launch(const CrossProblem& problem, cudaStream_t stream) {
+// A pass' tiles and blocks; false: too many blocks.
+template <int W, int PASS>
+bool describe_pass(const CrossProblem& problem, TcArgs* a) {
   using C = Cfg<W, PASS>;
-  TcArgs a{};
-  a.p = problem;
-  CrossProblem& p = a.p;
+  a->p = problem;
+  CrossProblem& p = a->p;
   const int G = int(p.G);
   const bool rows_q = PASS != kKeys;
-  a.rows_i = rows_q ? kRows / G : kRows;
-  a.cols_i = rows_q ? C::CN : C::CN / G;
-  a.row_bytes = 128 * a.rows_i * (rows_q ? G : 1);
-  a.col_bytes = 128 * a.cols_i * (rows_q ? 1 : G);
-  const int64_t rows = rows_q ? p.Nq : p.Nk;
-  p.row_blocks = (rows + a.rows_i - 1) / a.rows_i;
-  const int64_t blocks = p.row_blocks * p.B * p.Hk;
-  if (blocks > 0x7fffffff) return cudaErrorInvalidValue;
+  a->rows_i = rows_q ? kRows / G : kRows;
+  a->cols_i = rows_q ? C::CN : C::CN / G;
+  a->row_bytes = 128 * a->rows_i * (rows_q ? G : 1);
+  a->col_bytes = 128 * a->cols_i * (rows_q ? 1 : G);
+  p.row_blocks = ((rows_q ? p.Nq : p.Nk) + a->rows_i - 1) / a->rows_i;
+  return p.row_blocks * p.B * p.Hk * p.splits <= 0x7fffffff;
+}
+uint32_t blocks_of(const TcArgs& a) {
+  return uint32_t(a.p.row_blocks * a.p.B * a.p.Hk);
+}
 
-  if (!tensor_maps_available()) return cudaErrorNotSupported;
-  CUtensorMap q, e, k, v;
-  const int qi = rows_q ? a.rows_i : a.cols_i;
-  const int ki = rows_q ? a.cols_i : a.rows_i;
-  bool made = make_group_map(&q, p.q, p.dtype, p.B, p.Hk, G, p.Nq, p.D, p.sq,
-                             qi) &&
-              make_tile_map(&k, p.k, p.dtype, p.B, p.Hk, p.Nk, p.D, p.sk,
-                            ki) &&
-              make_tile_map(&v, p.v, p.dtype, p.B, p.Hk, p.Nk, p.Dv, p.sv, ki);
-  e = q;
-  if (made && C::kBack)
-    made = make_group_map(&e, p.dout, p.dtype, p.B, p.Hk, G, p.Nq, p.Dv, p.se,
-                          qi);
-  if (!made) return cudaErrorInvalidValue;
+// Maps of q, e (backward), k and v with boxes of `queries` and `keys` rows.
+bool make_maps(const CrossProblem& p, int queries, int keys, CUtensorMap* q,
+               CUtensorMap* e, CUtensorMap* k, CUtensorMap* v) {
+  return make_group_map(q, p.q, p.dtype, p.B, p.Hk, p.G, p.Nq, p.D, p.sq,
+                        queries) &&
+         (e == nullptr ||
+          make_group_map(e, p.dout, p.dtype, p.B, p.Hk, p.G, p.Nq, p.Dv, p.se,
+                         queries)) &&
+         make_tile_map(k, p.k, p.dtype, p.B, p.Hk, p.Nk, p.D, p.sk, keys) &&
+         make_tile_map(v, p.v, p.dtype, p.B, p.Hk, p.Nk, p.Dv, p.sv, keys);
+}
 
-  auto kern = cross_tc_kernel<T, W, PASS, KEEP>;
-  static std::atomic<int> configured[64];
+// Once a kernel and device: its shared memory, and that the setmaxnreg split
+// fits in the registers the block is launched with; a deficit would leave
+// setmaxnreg.inc waiting forever.
+template <typename K>
+cudaError_t configure(K kern, int bytes, std::atomic<int>* configured) {
   int dev = 0;
   cudaError_t err = cudaGetDevice(&dev);
   if (err != cudaSuccess) return err;
-  if (dev < 0 || dev >= 64 || !configured[dev].load()) {
-    // The setmaxnreg split must fit in the registers the block is launched
-    // with; a deficit would leave setmaxnreg.inc waiting forever.
-    cudaFuncAttributes attr;
-    err = cudaFuncGetAttributes(&attr, kern);
-    if (err != cudaSuccess) return err;
-    if (int64_t(attr.numRegs) * kThreads <
-        int64_t(256) * (kRowRegs + kOtherRegs))
-      return cudaErrorInvalidConfiguration;
-    err = cudaFuncSetAttribute(
-        kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM_ALLOC);
-    if (err != cudaSuccess) return err;
-    if (dev >= 0 && dev < 64) configured[dev].store(1);
-  }
-  count_launches(1);
-  const dim3 grid(unsigned(blocks), unsigned(p.splits));
-  if (PASS == kKeys)
-    return launch_pdl(kern, grid, dim3(kThreads), C::SMEM_ALLOC, stream, k, v,
-                      q, e, a);
-  return launch_pdl(kern, grid, dim3(kThreads), C::SMEM_ALLOC, stream, q, e, k,
-                    v, a);
+  if (dev >= 0 && dev < 64 && configured[dev].load()) return cudaSuccess;
+  cudaFuncAttributes attr;
+  err = cudaFuncGetAttributes(&attr, kern);
+  if (err != cudaSuccess) return err;
+  if (int64_t(attr.numRegs) * kThreads <
+      int64_t(256) * (kRowRegs + kOtherRegs))
+    return cudaErrorInvalidConfiguration;
+  err = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             bytes);
+  if (err == cudaSuccess && dev >= 0 && dev < 64) configured[dev].store(1);
+  return err;
 }
 
-template <int PASS, bool KEEP = false>
-cudaError_t launch_pass(const CrossProblem& p, cudaStream_t stream) {
+template <typename T, int W, bool KEEP>
+cudaError_t launch_forward(const CrossProblem& p, cudaStream_t stream) {
+  TcArgs a{};
+  if (!describe_pass<W, kForward>(p, &a)) return cudaErrorInvalidValue;
+  CUtensorMap q, k, v;
+  if (!tensor_maps_available()) return cudaErrorNotSupported;
+  if (!make_maps(p, a.rows_i, a.cols_i, &q, nullptr, &k, &v))
+    return cudaErrorInvalidValue;
+  constexpr int bytes = Cfg<W, kForward>::SMEM_ALLOC;
+  auto kern = cross_tc_forward_kernel<T, W, KEEP>;
+  static std::atomic<int> configured[64];
+  const cudaError_t err = configure(kern, bytes, configured);
+  if (err != cudaSuccess) return err;
+  count_launches(1);
+  return launch_pdl(kern, dim3(blocks_of(a), unsigned(p.splits)),
+                    dim3(kThreads), bytes, stream, q, k, v, a);
+}
+
+// The keys' pass where it has dk, the queries' where `want_q`.
+template <typename T, int W>
+cudaError_t launch_backward(const CrossProblem& keys,
+                            const CrossProblem& queries, bool want_q,
+                            cudaStream_t stream) {
+  BackwardArgs x{};
+  if (!describe_pass<W, kKeys>(keys, &x.a[0]) ||
+      !describe_pass<W, kQueries>(queries, &x.a[1]))
+    return cudaErrorInvalidValue;
+  if (!tensor_maps_available()) return cudaErrorNotSupported;
+  if (!make_maps(keys, x.a[0].cols_i, x.a[0].rows_i, &x.keys[2], &x.keys[3],
+                 &x.keys[0], &x.keys[1]) ||
+      !make_maps(queries, x.a[1].rows_i, x.a[1].cols_i, &x.queries[0],
+                 &x.queries[1], &x.queries[2], &x.queries[3]))
+    return cudaErrorInvalidValue;
+  for (int i = 0; i < 2; ++i) x.blocks[i] = blocks_of(x.a[i]);
+  const int64_t key_blocks =
+      keys.dk ? int64_t(x.blocks[0]) * keys.splits : 0;
+  const int64_t all =
+      key_blocks + (want_q ? int64_t(x.blocks[1]) * queries.splits : 0);
+  if (all > 0x7fffffff) return cudaErrorInvalidValue;
+  if (all == 0) return cudaSuccess;
+  x.key_blocks = uint32_t(key_blocks);
+  constexpr int k_bytes = Cfg<W, kKeys>::SMEM_ALLOC;
+  constexpr int q_bytes = Cfg<W, kQueries>::SMEM_ALLOC;
+  constexpr int bytes = k_bytes > q_bytes ? k_bytes : q_bytes;
+  auto kern = cross_tc_backward_kernel<T, W>;
+  static std::atomic<int> configured[64];
+  const cudaError_t err = configure(kern, bytes, configured);
+  if (err != cudaSuccess) return err;
+  count_launches(1);
+  return launch_pdl(kern, dim3(unsigned(all)), dim3(kThreads), bytes, stream,
+                    x);
+}
+
+// Calls f with the type and the padded width.
+template <typename F>
+cudaError_t with_width(const CrossProblem& p, F&& f) {
   const bool wide = p.D > 64 || p.Dv > 64;
-  if (p.dtype == VECTRA_BF16)
-    return wide ? launch<__nv_bfloat16, 128, PASS, KEEP>(p, stream)
-                : launch<__nv_bfloat16, 64, PASS, KEEP>(p, stream);
-  return wide ? launch<__half, 128, PASS, KEEP>(p, stream)
-              : launch<__half, 64, PASS, KEEP>(p, stream);
+  const auto typed = [&](auto* t) {
+    return wide ? f(t, std::integral_constant<int, 128>{})
+                : f(t, std::integral_constant<int, 64>{});
+  };
+  return p.dtype == VECTRA_BF16 ? typed(static_cast<__nv_bfloat16*>(nullptr))
+                                : typed(static_cast<__half*>(nullptr));
 }
 
 // Parts of the axis that a block walks, where the rows alone leave SMs
@@ -1058,8 +1146,12 @@ cudaError_t run_cross_tc_forward(const CrossProblem& problem, Workspace& ws,
     const cudaError_t st = launch_cross_squares(p, squares, stream);
     if (st != cudaSuccess) return st;
   }
-  const cudaError_t e = p.lse ? launch_pass<kForward, true>(p, stream)
-                              : launch_pass<kForward>(p, stream);
+  const cudaError_t e = with_width(p, [&](auto* t, auto width) {
+    using T = std::remove_pointer_t<decltype(t)>;
+    constexpr int W = decltype(width)::value;
+    return p.lse ? launch_forward<T, W, true>(p, stream)
+                 : launch_forward<T, W, false>(p, stream);
+  });
   return e != cudaSuccess || p.splits == 1 ? e : launch_cross_join(p, stream);
 }
 
@@ -1092,23 +1184,22 @@ cudaError_t run_cross_tc_backward(const CrossProblem& problem, Workspace& ws,
   cudaError_t e = launch_cross_delta(p, delta, stream);
   if (e == cudaSuccess && squares)
     e = launch_cross_squares(p, squares, stream);
-  if (e == cudaSuccess && want_q && rows > 0) {
-    e = launch_pass<kQueries>(pq, stream);
-    if (e == cudaSuccess && pq.part)
-      e = launch_cross_sum(p.dtype, pq.part, pq.splits, p.B, p.H, p.Nq, p.D,
-                           p.dq, p.sdq, stream);
-  }
+  if (e == cudaSuccess)
+    e = with_width(p, [&](auto* t, auto width) {
+      return launch_backward<std::remove_pointer_t<decltype(t)>,
+                             decltype(width)::value>(pk, pq, want_q, stream);
+    });
+  if (e == cudaSuccess && pq.part)
+    e = launch_cross_sum(p.dtype, pq.part, pq.splits, p.B, p.H, p.Nq, p.D,
+                         p.dq, p.sdq, stream);
   if (e == cudaSuccess && p.dscale)
     e = launch_cross_dscale(pq, pq.splits, stream);
-  if (e == cudaSuccess && p.dk && keys > 0) {
-    e = launch_pass<kKeys>(pk, stream);
-    if (e == cudaSuccess && pk.part)
-      e = launch_cross_sum(p.dtype, pk.part, pk.splits, p.B, p.Hk, p.Nk, p.D,
-                           p.dk, p.sdk, stream);
-    if (e == cudaSuccess && pk.part)
-      e = launch_cross_sum(p.dtype, pk.part_v, pk.splits, p.B, p.Hk, p.Nk,
-                           p.Dv, p.dv, p.sdv, stream);
-  }
+  if (e == cudaSuccess && pk.part)
+    e = launch_cross_sum(p.dtype, pk.part, pk.splits, p.B, p.Hk, p.Nk, p.D,
+                         p.dk, p.sdk, stream);
+  if (e == cudaSuccess && pk.part)
+    e = launch_cross_sum(p.dtype, pk.part_v, pk.splits, p.B, p.Hk, p.Nk, p.Dv,
+                         p.dv, p.sdv, stream);
   return e;
 }
 

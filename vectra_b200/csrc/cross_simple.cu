@@ -205,6 +205,7 @@ __global__ void __launch_bounds__(kThreads)
     }
   }
 
+  const bool works = first + threadIdx.x / 32 * 2 * RT < rows;
   for (int t = t0; t < t1; ++t) {
     const int64_t c0 = int64_t(t) * CN;
     __syncthreads();  // the tile before is no longer read
@@ -243,6 +244,9 @@ __global__ void __launch_bounds__(kThreads)
       }
       __syncthreads();
     }
+
+    // A warp none of whose rows lives only stages the others' operands.
+    if (!works) continue;
 
     float s[RT][CT], u[RT][CT];
 #pragma unroll
@@ -355,7 +359,7 @@ __global__ void __launch_bounds__(kThreads)
         }
       }
     }
-    __syncthreads();
+    __syncwarp();  // a row's P and z are its own warp's
 
     // acc += z c, acc' += P c', four columns of the tile at a time.
 #pragma unroll 1

@@ -109,13 +109,14 @@ __device__ __forceinline__ float logit(float g, float distance) {
   return __fmul_rn(-g * kLog2e, distance);
 }
 
+// One pass' work of one block: rows `block`, part `part` of the columns.
 template <typename T, int W, int R, int CN, int PASS>
-__global__ void __launch_bounds__(kThreads)
-    cross_simple_kernel(const __grid_constant__ CrossProblem p) {
+__device__ __forceinline__ void cross_pass(const CrossProblem& p,
+                                           uint32_t block, int part,
+                                           float* smem) {
   using S = Shape<W, R, CN, PASS>;
   constexpr int RT = S::RT, CT = S::CT, WT = S::WT;
   constexpr bool kRowsAreQueries = PASS != kKeys;
-  extern __shared__ __align__(16) float smem[];
   float* sr = smem + S::OFF_R;
   float* sr2 = smem + S::OFF_R2;
   float* sc = smem + S::OFF_C;
@@ -125,14 +126,11 @@ __global__ void __launch_bounds__(kThreads)
   float* col_lse = smem + S::OFF_COL;
   float* col_delta = col_lse + CN;
   float* col_g = col_delta + CN;
-  allow_dependents();
-  grid_dependency_wait();
 
   const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
-  const int64_t plane = blockIdx.x / p.row_blocks;
+  const int64_t plane = block / p.row_blocks;
   const int64_t b = plane / p.Hk, hk = plane - b * p.Hk, h0 = hk * p.G;
-  const int part = blockIdx.y;
-  const int64_t first = (blockIdx.x - plane * p.row_blocks) * R;
+  const int64_t first = (block - plane * p.row_blocks) * R;
   const int len = cross_length(p, b);
   const int64_t n_q = p.Nq * p.G;
   const int64_t rows = kRowsAreQueries ? n_q : int64_t(len);
@@ -506,18 +504,74 @@ __global__ void __launch_bounds__(kThreads)
 }
 
 template <typename T, int W, int R, int CN, int PASS>
-cudaError_t launch(CrossProblem p, int64_t rows, cudaStream_t stream) {
-  using S = Shape<W, R, CN, PASS>;
-  auto kern = cross_simple_kernel<T, W, R, CN, PASS>;
+__global__ void __launch_bounds__(kThreads)
+    cross_simple_kernel(const __grid_constant__ CrossProblem p) {
+  extern __shared__ __align__(16) float smem[];
+  allow_dependents();
+  grid_dependency_wait();
+  cross_pass<T, W, R, CN, PASS>(p, blockIdx.x, blockIdx.y, smem);
+}
+
+// Both backward passes in one grid, the keys' blocks, which are longer, first:
+// the last wave of blocks, of two an SM and more, is left half empty once.
+template <typename T, int W, int R, int CN>
+__global__ void __launch_bounds__(kThreads)
+    cross_backward_kernel(const __grid_constant__ CrossProblem keys,
+                          const __grid_constant__ CrossProblem queries,
+                          uint32_t key_part, uint32_t key_blocks,
+                          uint32_t query_part) {
+  extern __shared__ __align__(16) float smem[];
+  allow_dependents();
+  grid_dependency_wait();
+  if (blockIdx.x < key_blocks) {
+    const uint32_t part = blockIdx.x / key_part;
+    cross_pass<T, W, R, CN, kKeys>(keys, blockIdx.x - part * key_part,
+                                   int(part), smem);
+  } else {
+    const uint32_t at = blockIdx.x - key_blocks, part = at / query_part;
+    cross_pass<T, W, R, CN, kQueries>(queries, at - part * query_part,
+                                      int(part), smem);
+  }
+}
+
+template <typename K, typename... A>
+cudaError_t start(K kern, dim3 grid, int bytes, cudaStream_t stream,
+                  const A&... args) {
   const cudaError_t e = cudaFuncSetAttribute(
-      kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::BYTES);
+      kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
   if (e != cudaSuccess) return e;
-  p.row_blocks = (rows + R - 1) / R;
-  const int64_t blocks = p.row_blocks * p.B * p.Hk;
-  if (blocks > 0x7fffffff) return cudaErrorInvalidValue;
   count_launches(1);
-  return launch_pdl(kern, dim3(unsigned(blocks), unsigned(p.splits)),
-                    dim3(kThreads), S::BYTES, stream, p);
+  return launch_pdl(kern, grid, dim3(kThreads), bytes, stream, args...);
+}
+
+// Blocks of a part of a pass.
+int64_t set_blocks(CrossProblem* p, int64_t rows, int R) {
+  p->row_blocks = (rows + R - 1) / R;
+  return p->row_blocks * p->B * p->Hk;
+}
+
+template <typename T, int W, int R, int CN, int PASS>
+cudaError_t launch(CrossProblem p, int64_t rows, cudaStream_t stream) {
+  const int64_t blocks = set_blocks(&p, rows, R);
+  if (blocks > 0x7fffffff) return cudaErrorInvalidValue;
+  return start(cross_simple_kernel<T, W, R, CN, PASS>,
+               dim3(unsigned(blocks), unsigned(p.splits)),
+               Shape<W, R, CN, PASS>::BYTES, stream, p);
+}
+
+template <typename T, int W, int R, int CN>
+cudaError_t launch_both(CrossProblem keys, CrossProblem queries, bool want_k,
+                        bool want_q, cudaStream_t stream) {
+  const int64_t k = set_blocks(&keys, keys.Nk, R);
+  const int64_t q = set_blocks(&queries, queries.Nq * queries.G, R);
+  const int64_t k_all = want_k ? k * keys.splits : 0;
+  const int64_t all = k_all + (want_q ? q * queries.splits : 0);
+  if (all > 0x7fffffff) return cudaErrorInvalidValue;
+  constexpr int k_bytes = Shape<W, R, CN, kKeys>::BYTES;
+  constexpr int q_bytes = Shape<W, R, CN, kQueries>::BYTES;
+  return start(cross_backward_kernel<T, W, R, CN>, dim3(unsigned(all)),
+               k_bytes > q_bytes ? k_bytes : q_bytes, stream, keys, queries,
+               uint32_t(k), uint32_t(k_all), uint32_t(q));
 }
 
 int width_of(const CrossProblem& p) {
@@ -533,30 +587,52 @@ void tile_of(const CrossProblem& p, int64_t rows, int* r, int* c) {
   *c = wide ? 32 : 64;
 }
 
-template <typename T, int W, int PASS>
-cudaError_t with_rows(const CrossProblem& p, int64_t rows,
-                      cudaStream_t stream) {
-  constexpr int CN = W == 256 ? 32 : 64;
-  return rows <= 16 ? launch<T, W, 16, CN, PASS>(p, rows, stream)
-                    : launch<T, W, W == 256 ? 32 : 64, CN, PASS>(p, rows,
-                                                                 stream);
-}
-
-template <int PASS>
-cudaError_t launch_pass(const CrossProblem& p, cudaStream_t stream) {
-  const int64_t rows = PASS == kKeys ? p.Nk : p.Nq * p.G;
+// f(the type, the padded width, and a tile's columns, as tile_of has them).
+template <typename F>
+cudaError_t with_shape(const CrossProblem& p, F&& f) {
   return with_dtype(p.dtype, [&](auto* t) {
-    using T = std::remove_pointer_t<decltype(t)>;
+    using C32 = std::integral_constant<int, 32>;
+    using C64 = std::integral_constant<int, 64>;
     switch (width_of(p)) {
       case 32:
-        return with_rows<T, 32, PASS>(p, rows, stream);
+        return f(t, C32{}, C64{});
       case 64:
-        return with_rows<T, 64, PASS>(p, rows, stream);
+        return f(t, C64{}, C64{});
       case 128:
-        return with_rows<T, 128, PASS>(p, rows, stream);
+        return f(t, std::integral_constant<int, 128>{}, C64{});
       default:
-        return with_rows<T, 256, PASS>(p, rows, stream);
+        return f(t, std::integral_constant<int, 256>{}, C32{});
     }
+  });
+}
+
+cudaError_t launch_forward(const CrossProblem& p, cudaStream_t stream) {
+  const int64_t rows = p.Nq * p.G;
+  return with_shape(p, [&](auto* t, auto width, auto cols) {
+    using T = std::remove_pointer_t<decltype(t)>;
+    constexpr int W = decltype(width)::value, CN = decltype(cols)::value;
+    return rows <= 16 ? launch<T, W, 16, CN, kForward>(p, rows, stream)
+                      : launch<T, W, CN, CN, kForward>(p, rows, stream);
+  });
+}
+
+// The passes over 16 rows or fewer by themselves, the others in one grid.
+cudaError_t launch_backward(const CrossProblem& keys,
+                            const CrossProblem& queries, bool want_k,
+                            bool want_q, cudaStream_t stream) {
+  const int64_t n_k = keys.Nk, n_q = queries.Nq * queries.G;
+  return with_shape(keys, [&](auto* t, auto width, auto cols) {
+    using T = std::remove_pointer_t<decltype(t)>;
+    constexpr int W = decltype(width)::value, CN = decltype(cols)::value;
+    cudaError_t e = cudaSuccess;
+    if (want_k && n_k <= 16)
+      e = launch<T, W, 16, CN, kKeys>(keys, n_k, stream);
+    if (e == cudaSuccess && want_q && n_q <= 16)
+      e = launch<T, W, 16, CN, kQueries>(queries, n_q, stream);
+    const bool k = want_k && n_k > 16, q = want_q && n_q > 16;
+    if (e == cudaSuccess && (k || q))
+      e = launch_both<T, W, CN, CN>(keys, queries, k, q, stream);
+    return e;
   });
 }
 
@@ -597,7 +673,7 @@ cudaError_t run_cross_simple_forward(const CrossProblem& problem,
     p.part_ml = take_floats(ws, p.splits * rows * 2);
   }
   if (ws.dry || ws.overflow || rows == 0) return cudaSuccess;
-  const cudaError_t e = launch_pass<kForward>(p, stream);
+  const cudaError_t e = launch_forward(p, stream);
   return e != cudaSuccess || p.splits == 1 ? e : launch_cross_join(p, stream);
 }
 
@@ -623,23 +699,19 @@ cudaError_t run_cross_simple_backward(const CrossProblem& problem,
   }
   if (ws.dry || ws.overflow) return cudaSuccess;
   cudaError_t e = launch_cross_delta(p, delta, stream);
-  if (e == cudaSuccess && want_q && rows > 0) {
-    e = launch_pass<kQueries>(pq, stream);
-    if (e == cudaSuccess && pq.part)
-      e = launch_cross_sum(p.dtype, pq.part, pq.splits, p.B, p.H, p.Nq, p.D,
-                           p.dq, p.sdq, stream);
-  }
+  if (e == cudaSuccess)
+    e = launch_backward(pk, pq, p.dk && keys > 0, want_q && rows > 0, stream);
+  if (e == cudaSuccess && pq.part && rows > 0)
+    e = launch_cross_sum(p.dtype, pq.part, pq.splits, p.B, p.H, p.Nq, p.D,
+                         p.dq, p.sdq, stream);
   if (e == cudaSuccess && p.dscale)
     e = launch_cross_dscale(pq, pq.splits, stream);
-  if (e == cudaSuccess && p.dk && keys > 0) {
-    e = launch_pass<kKeys>(pk, stream);
-    if (e == cudaSuccess && pk.part)
-      e = launch_cross_sum(p.dtype, pk.part, pk.splits, p.B, p.Hk, p.Nk, p.D,
-                           p.dk, p.sdk, stream);
-    if (e == cudaSuccess && pk.part)
-      e = launch_cross_sum(p.dtype, pk.part_v, pk.splits, p.B, p.Hk, p.Nk,
-                           p.Dv, p.dv, p.sdv, stream);
-  }
+  if (e == cudaSuccess && pk.part && keys > 0)
+    e = launch_cross_sum(p.dtype, pk.part, pk.splits, p.B, p.Hk, p.Nk, p.D,
+                         p.dk, p.sdk, stream);
+  if (e == cudaSuccess && pk.part && keys > 0)
+    e = launch_cross_sum(p.dtype, pk.part_v, pk.splits, p.B, p.Hk, p.Nk, p.Dv,
+                         p.dv, p.sdv, stream);
   return e;
 }
 

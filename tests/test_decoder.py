@@ -834,6 +834,24 @@ def test_cross_empty(device):
 
 
 @pytest.mark.parametrize('device', DEVICES)
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('nq', [1, 200])
+@pytest.mark.parametrize('dim', [64, 66])
+def test_cross_without_keys(device, dtype, nq, dim):
+    """Few and many queries, and widths of 16-byte pieces and not, over an
+    encoder without states."""
+    rand = Rand(59, device, dtype)
+    q, k, v, scale = (t.requires_grad_() for t in
+                      cross_inputs(rand, 2, 4, 2, nq, 0, dim))
+    with torch.no_grad():
+        assert (block.cross_attention(q, k, v, scale) == 0).all()
+    out = block.cross_attention(q, k, v, scale)
+    assert out.shape == q.shape and (out == 0).all()
+    for t in torch.autograd.grad(out.sum(), (q, k, v, scale)):
+        assert (t == 0).all()
+
+
+@pytest.mark.parametrize('device', DEVICES)
 @pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
 def test_cross_only_wanted_gradients(device, dtype):
     rand = Rand(55, device, dtype)

@@ -1123,6 +1123,8 @@ bool map_ok(const void* base, const int64_t* s, const int64_t* sizes) {
 bool cross_tc_supports(const CrossProblem& p, bool backward) {
   if (p.dtype != VECTRA_BF16 && p.dtype != VECTRA_F16) return false;
   if (p.D > 128 || p.Dv > 128 || p.G > 64 || p.G < 1) return false;
+  // A tensor map has no empty dimension.
+  if (p.B * p.H * p.Nq == 0 || p.Nk == 0) return false;
   const int64_t q[4] = {p.B, p.H, p.Nq, p.D}, e[4] = {p.B, p.H, p.Nq, p.Dv};
   const int64_t k[4] = {p.B, p.Hk, p.Nk, p.D}, v[4] = {p.B, p.Hk, p.Nk, p.Dv};
   return map_ok(p.q, p.sq, q) && map_ok(p.k, p.sk, k) &&

@@ -17,8 +17,11 @@
 // 16-byte multiples, and P and z as [row][column]: every product then reads
 // float4 pieces, for s and t along rows and columns, for acc along the summed
 // columns. A thread owns R / 16 by CN / 16 of a tile and R / 16 by width / 16
-// of a result. Bound by the FP32 pipe and shared-memory reads (64 x 64 tiles:
-// 2 reads of 16 bytes for 16 multiply-adds).
+// of a result. Bound by latency at the two blocks an SM that registers and
+// shared memory hold: issue 41 % of cycles, the FP32 pipe 30 %, and a last wave
+// of blocks. 257 queries on up to 700 keys, 8 heads of 64, batch 4, float32:
+// forward 81 us, all gradients 178. Loading the next tile's operands by
+// 4-byte asynchronous copies under the products: 77 and 187.
 #include <type_traits>
 
 #include "cross.cuh"

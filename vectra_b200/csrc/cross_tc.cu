@@ -16,8 +16,8 @@
 //
 // Warps: two warpgroups form P and z, one thread a row, each of one half of a
 // tile's columns, while the tensor cores work on the next tile's S and T (two
-// tiles are in TMEM); a TMA producer; an MMA issuer; a warpgroup for the columns' terms, which are
-// |k_j|^2, or a query's lse, c_i and scale. Where several blocks walk the same
+// tiles are in TMEM); a TMA producer; an MMA issuer; a warpgroup for the
+// columns' terms, which are |k_j|^2, or a query's lse, c_i and scale. Where several blocks walk the same
 // keys their |k_j|^2 are formed once beforehand; a lone block (a decoding step)
 // forms them from the tile in shared memory (two warps doing that in every
 // block set the pace: 627 us of 4,096 queries on 5,003 keys, 32 heads of 128,
@@ -32,10 +32,15 @@
 //
 // Rounding, beside each result's: P and z enter their products in 16 bits. For
 // a backward pass the forward one multiplies what P's rounding left as well
-// (KEEP): c_i of a
-// result that is off by 2^-9 of its weights would put 2^-9 of the distance
-// between q_i and the mean key into dq, as much as all other roundings of dq
-// together (bf16: 3.2e-3 of dq against 2.4e-3).
+// (KEEP): c_i of a result that is off by 2^-9 of its weights would put 2^-9 of
+// the distance between q_i and the mean key into dq, as much as all other
+// roundings of dq together (bf16: 3.2e-3 of dq against 2.4e-3).
+//
+// Measured: 4,096 queries of 32 heads on 5,003 keys of 8 heads of 128, f16:
+// 395 us, 850 TFLOP/s; bound by the row warpgroups' instructions (an exponential
+// and the terms of each logit). Training of 2,048 queries of 16 heads on up to
+// 4,500 keys of 4 heads of 128, batch 4, bf16: forward 249, and 284 with what
+// the backward pass takes; all gradients 730 to 750 us.
 #include <atomic>
 #include <type_traits>
 

@@ -21,6 +21,18 @@
 // registers. The next rows are on their way into shared memory meanwhile, by
 // asynchronous copies; a thread reads only what it copied itself, so they need
 // no barrier.
+//
+// Measured, bf16: 66,560 rows of 256, layer norm, one gate row, dropout:
+// forward 37 us (136 MB: 3.7 TB/s, half of it writes, whose own rate here is
+// 3.7), backward 62 us (205 MB: 3.3 TB/s, of which the joins of the column
+// sums 9). 8,193 rows of 5,120, norms on both sides, a gate row for each
+// 2,731: forward 76 us (336 MB, 4.4 TB/s); backward 208 us (503 MB, 2.4 TB/s),
+// bound by instructions (73 an element) and by the column sums, 64 of
+// which a thread keeps, in part in spilled registers. Of its 208 us no loads
+// would leave 188, no stores 195; one block of 640 threads an SM with half the
+// sums each took 313. With loads to registers in turn instead of copies ahead
+// it was 280. Dropout alone, 16,396 rows of 4,096: 56 us a pass (269 MB,
+// 4.8 TB/s).
 #pragma once
 
 #include <type_traits>

@@ -661,7 +661,6 @@ __global__ void __launch_bounds__(kWarps * 32, NB > 2 ? 2 : 3)
   for (int n = 0; n < NB * 4; ++n)
 #pragma unroll
     for (int i = 0; i < 4; ++i) dq[n][i] = 0.f;
-  float zsum[4] = {0.f, 0.f, 0.f, 0.f};  // of rounded z, by row
   float xs[NR], ys[NR], zx[NR];
 #pragma unroll
   for (int r = 0; r < NR; ++r) xs[r] = ys[r] = zx[r] = 0.f;
@@ -714,7 +713,9 @@ __global__ void __launch_bounds__(kWarps * 32, NB > 2 ? 2 : 3)
       nk[h] = squares<T, NB>(k[h], lane);
     }
     // P and z of the 16 keys; z for dk has its row's scale before rounding.
+    // What z's rounding leaves enters dq as well (cross_tc.cu).
     uint32_t pw[4] = {0, 0, 0, 0}, zw[4] = {0, 0, 0, 0}, zk[4] = {0, 0, 0, 0};
+    uint32_t zl[4] = {0, 0, 0, 0};
     const int first = step * kKeys + 2 * t;
 #pragma unroll
     for (int r = 0; r < NR; ++r)
@@ -735,15 +736,20 @@ __global__ void __launch_bounds__(kWarps * 32, NB > 2 ? 2 : 3)
         }
         pw[2 * h + r] = pack_pair<T>(w[0], w[1]);
         zw[2 * h + r] = pack_pair<T>(z[0], z[1]);
+        const float2 near = pair<T>(zw[2 * h + r]);
+        zl[2 * h + r] = pack_pair<T>(z[0] - near.x, z[1] - near.y);
         zk[2 * h + r] = pack_pair<T>(g2[r] * z[0], g2[r] * z[1]);
       }
     // dq += z k.
-    mma16816<T>(zsum, zw, ones<T>(), ones<T>());
 #pragma unroll
     for (int n = 0; n < NB; ++n)
 #pragma unroll
       for (int w = 0; w < 4; ++w)
-        mma16816<T>(dq[n * 4 + w], zw, turn(k[0][n][w]), turn(k[1][n][w]));
+      {
+        const uint32_t k0 = turn(k[0][n][w]), k1 = turn(k[1][n][w]);
+        mma16816<T>(dq[n * 4 + w], zw, k0, k1);
+        mma16816<T>(dq[n * 4 + w], zl, k0, k1);
+      }
     if (!p.dk) continue;
     // P^T and z^T: fragments of 16 keys by 16 rows.
     const uint32_t pt[4] = {turn(pw[0]), turn(pw[2]), turn(pw[1]),
@@ -828,9 +834,9 @@ __global__ void __launch_bounds__(kWarps * 32, NB > 2 ? 2 : 3)
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
         const float2 f = pair<T>(q[r][n][w]);
-        const float a0 = g2[r] * (dq[n * 4 + w][2 * r] - f.x * zsum[2 * r]);
+        const float a0 = g2[r] * (dq[n * 4 + w][2 * r] - f.x * zx[r]);
         const float a1 =
-            g2[r] * (dq[n * 4 + w][2 * r + 1] - f.y * zsum[2 * r]);
+            g2[r] * (dq[n * 4 + w][2 * r + 1] - f.y * zx[r]);
         if (p.splits > 1)
           *reinterpret_cast<float2*>(p.part + k_part * p.D + d + 2 * w) =
               make_float2(a0, a1);

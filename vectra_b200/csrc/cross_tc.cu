@@ -34,7 +34,8 @@
 // a backward pass the forward one multiplies what P's rounding left as well
 // (KEEP): c_i of a result that is off by 2^-9 of its weights would put 2^-9 of
 // the distance between q_i and the mean key into dq, as much as all other
-// roundings of dq together (bf16: 3.2e-3 of dq against 2.4e-3).
+// roundings of dq together (bf16: 3.2e-3 of dq against 2.4e-3). The queries'
+// pass does the same with z.
 //
 // Measured: 4,096 queries of 32 heads on 5,003 keys of 8 heads of 128, f16:
 // 395 us, 850 TFLOP/s; bound by the row warpgroups' instructions (an exponential
@@ -435,6 +436,8 @@ __device__ __forceinline__ void cross_pass(const CUtensorMap& tr,
                 sum(C::A0 + g * W, src + CN / 4, col2, idesc_a2, g, false);
             } else {
               sum(C::A0, C::T0 + x * CN, col, idesc_a, g, t == 0 && g == 0);
+              if (PASS == kQueries)
+                sum(C::A0, C::T0 + x * CN + CN / 4, col, idesc_a, g, false);
               if (PASS == kKeys)
                 sum(C::A0 + W, C::S0 + x * CN, col2, idesc_a2, g,
                     t == 0 && g == 0);
@@ -717,7 +720,9 @@ __device__ __forceinline__ void cross_pass(const CUtensorMap& tr,
         nkr = -row_square<T, 8 * C::KB>(smem + C::OFF_R, C::RBLOCK, r, 0);
       const uint64_t nkr2 = both(nkr), gl2 = both(gl), lse2 = both(-lse),
                      ci2 = both(-ci);
-      uint64_t zs = 0, zx = 0, xs = 0, ys = 0;  // of rounded z; for dscale
+      // Sums of z, rounded where its product takes no more; for dscale.
+      uint64_t zs = 0, xs = 0, ys = 0;
+      static_assert(!kBack || HALF == 32, "a tile is read before z is written");
       const bool want_scale = PASS == kQueries && p.dscale_rows != nullptr;
       for (int t = 0; t < n && ok; ++t) {
         const int s = t % NS, buf = t & 1;
@@ -735,7 +740,7 @@ __device__ __forceinline__ void cross_pass(const CUtensorMap& tr,
           for (int c = 0; c < HALF; c += 32) {
             uint32_t sv[32], tv[32];
             tmem_load32x2(s_col + c, sv, t_col + c, tv);
-            uint32_t pw[16], zw[16];
+            uint32_t pw[16], zw[16];  // pw of queries: z's rest
 #pragma unroll
             for (int j = 0; j < 32; j += 4) {
               uint64_t lg[2], zc[2], u2[2];
@@ -782,18 +787,24 @@ __device__ __forceinline__ void cross_pass(const CUtensorMap& tr,
                 }
                 const uint32_t zp = pack2<T>(z.x, z.y);
                 zw[j / 2 + q] = zp;
-                zs = fadd2(zs, unpack2<T>(zp));
+                const uint64_t zr = unpack2<T>(zp);
                 if constexpr (PASS == kKeys) {
+                  zs = fadd2(zs, zr);
                   pw[j / 2 + q] = pack2<T>(w0, w1);
-                } else if (want_scale) {
-                  xs = ffma2(f2pk(z.x, z.y), u2[q], xs);
-                  ys = ffma2(f2pk(w0, w1), u2[q], ys);
-                  zx = fadd2(zx, f2pk(z.x, z.y));
+                } else {
+                  const uint64_t z2 = f2pk(z.x, z.y);
+                  const float2 rest = f2upk(ffma2(zr, both(-1.f), z2));
+                  pw[j / 2 + q] = pack2<T>(rest.x, rest.y);
+                  zs = fadd2(zs, z2);
+                  if (want_scale) {
+                    xs = ffma2(z2, u2[q], xs);
+                    ys = ffma2(f2pk(w0, w1), u2[q], ys);
+                  }
                 }
               }
             }
             tmem_st16(t_col + c / 2, zw);
-            if constexpr (PASS == kKeys) tmem_st16(s_col + c / 2, pw);
+            tmem_st16(PASS == kKeys ? s_col + c / 2 : t_col + HALF / 2, pw);
           }
           tmem_wait_st();
         }
@@ -806,7 +817,7 @@ __device__ __forceinline__ void cross_pass(const CUtensorMap& tr,
       tc_fence_after();
       float4* join = reinterpret_cast<float4*>(smem + C::OFF_JOIN);
       join[x * kRows + r] =
-          make_float4(halves(zs), halves(xs), halves(ys), halves(zx));
+          make_float4(halves(zs), halves(xs), halves(ys), 0.f);
       sync_rows();
       const float4 j0 = join[r], j1 = join[kRows + r];
       const float z_sum = j0.x + j1.x;
@@ -817,7 +828,7 @@ __device__ __forceinline__ void cross_pass(const CUtensorMap& tr,
           float* w = p.dscale_rows + (part * all_rows + at) * 3;
           w[0] = -(j0.y + j1.y);
           w[1] = -(j0.z + j1.z);
-          w[2] = j0.w + j1.w;
+          w[2] = z_sum;
         }
         // acc less the row's own vector times its sum: dq by columns between
         // the warpgroups; of the keys' two results one each.

@@ -38,8 +38,8 @@
 // pass does the same with z.
 //
 // Measured: 4,096 queries of 32 heads on 5,003 keys of 8 heads of 128, f16:
-// 395 us, 850 TFLOP/s; bound by the row warpgroups' instructions (an exponential
-// and the terms of each logit). Training of 2,048 queries of 16 heads on up to
+// 395 us, 850 TFLOP/s; bound by the latency of the row warps, two a scheduler
+// (tensor pipe 41 %, issue 35 %). Training of 2,048 queries of 16 heads on up to
 // 4,500 keys of 4 heads of 128, batch 4, bf16: forward 249, and 284 with what
 // the backward pass takes; all gradients 730 to 750 us.
 #include <atomic>

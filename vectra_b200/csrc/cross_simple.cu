@@ -17,17 +17,26 @@
 // 16-byte multiples, and P and z as [row][column]: every product then reads
 // float4 pieces, for s and t along rows and columns, for acc along the summed
 // columns. A thread owns R / 16 by CN / 16 of a tile and R / 16 by width / 16
-// of a result. Bound by latency at the two blocks an SM that registers and
-// shared memory hold: issue 41 % of cycles, the FP32 pipe 30 %, and a last wave
-// of blocks. 257 queries on up to 700 keys, 8 heads of 64, batch 4, float32:
-// forward 81 us, all gradients 178. Loading the next tile's operands by
-// 4-byte asynchronous copies under the products: 77 and 187.
+// of a result. s and t take two columns an instruction (packed floats: 81 and
+// 178 us of the figures below without).
+//
+// Bound by latency at the two blocks an SM that registers and shared memory
+// hold (issue about 40 % of cycles, the FP32 pipe 30 %), and by a last wave of
+// blocks. 257 queries on up to 700 keys, 8 heads of 64, batch 4, float32:
+// forward 78 us, all gradients 168. Loading the next tile's operands by 4-byte
+// asynchronous copies under the products changed 81 and 178 to 77 and 187.
 #include <type_traits>
 
 #include "cross.cuh"
+#include "tcgen05.cuh"
 
 namespace vectra {
 namespace {
+
+using tc::f2pk;
+using tc::f2upk;
+using tc::fadd2;
+using tc::ffma2;
 
 enum Pass { kForward = 0, kQueries = 1, kKeys = 2 };
 
@@ -110,6 +119,20 @@ constexpr bool kLeaveOut = !std::is_same<T, float>::value;
 // Rounded once, in all passes alike: a single key weighs exactly 1.
 __device__ __forceinline__ float logit(float g, float distance) {
   return __fmul_rn(-g * kLog2e, distance);
+}
+
+// RT rows' components, each twice, and CT columns' in pairs.
+template <int RT, int CT>
+__device__ __forceinline__ void load_pairs(const float* rows,
+                                           const float* columns, uint64_t* r,
+                                           uint64_t* c) {
+#pragma unroll
+  for (int i = 0; i < RT; ++i) r[i] = f2pk(rows[i], rows[i]);
+#pragma unroll
+  for (int j = 0; j < CT; j += 2) {
+    const float2 x = *reinterpret_cast<const float2*>(columns + j);
+    c[j / 2] = f2pk(x.x, x.y);
+  }
 }
 
 // One pass' work of one block: rows `block`, part `part` of the columns.
@@ -249,54 +272,63 @@ __device__ __forceinline__ void cross_pass(const CrossProblem& p,
     // A warp none of whose rows lives only stages the others' operands.
     if (!works) continue;
 
-    float s[RT][CT], u[RT][CT];
+    // Sums of eight components at a time: a sum of D terms one by one would
+    // be off by twice as much, and the weights' exponents with it. Two columns
+    // in one instruction.
+    uint64_t s2[RT][CT / 2], u2[RT][CT / 2];
 #pragma unroll
     for (int i = 0; i < RT; ++i)
 #pragma unroll
-      for (int j = 0; j < CT; ++j) s[i][j] = u[i][j] = 0.f;
-    // Sums of eight components at a time: a sum of D terms one by one would
-    // be off by twice as much, and the weights' exponents with it.
+      for (int j = 0; j < CT / 2; ++j) s2[i][j] = u2[i][j] = 0;
+    const uint64_t minus = f2pk(-1.f, -1.f);
 #pragma unroll 1
     for (int d0 = 0; d0 < p.D; d0 += 8) {
-      float eight[RT][CT];
+      uint64_t eight[RT][CT / 2];
 #pragma unroll
       for (int i = 0; i < RT; ++i)
 #pragma unroll
-        for (int j = 0; j < CT; ++j) eight[i][j] = 0.f;
+        for (int j = 0; j < CT / 2; ++j) eight[i][j] = 0;
 #pragma unroll
       for (int d = d0; d < d0 + 8; ++d) {  // zeros past the width
-        float r[RT], c[CT];
-#pragma unroll
-        for (int i = 0; i < RT; ++i) r[i] = sr[d * S::LR + ty * RT + i];
-#pragma unroll
-        for (int j = 0; j < CT; ++j) c[j] = sc[d * S::LC + tx * CT + j];
+        uint64_t r[RT], c[CT / 2];
+        load_pairs<RT, CT>(sr + d * S::LR + ty * RT, sc + d * S::LC + tx * CT,
+                           r, c);
 #pragma unroll
         for (int i = 0; i < RT; ++i)
 #pragma unroll
-          for (int j = 0; j < CT; ++j) {
-            const float x = r[i] - c[j];
-            eight[i][j] = fmaf(x, x, eight[i][j]);
+          for (int j = 0; j < CT / 2; ++j) {
+            const uint64_t x = ffma2(c[j], minus, r[i]);
+            eight[i][j] = ffma2(x, x, eight[i][j]);
           }
       }
 #pragma unroll
       for (int i = 0; i < RT; ++i)
 #pragma unroll
-        for (int j = 0; j < CT; ++j) s[i][j] += eight[i][j];
+        for (int j = 0; j < CT / 2; ++j)
+          s2[i][j] = fadd2(s2[i][j], eight[i][j]);
     }
     if constexpr (S::kBack) {
 #pragma unroll 4
       for (int d = 0; d < p.Dv; ++d) {
-        float r[RT], c[CT];
-#pragma unroll
-        for (int i = 0; i < RT; ++i) r[i] = sr2[d * S::LR + ty * RT + i];
-#pragma unroll
-        for (int j = 0; j < CT; ++j) c[j] = sc2[d * S::LC + tx * CT + j];
+        uint64_t r[RT], c[CT / 2];
+        load_pairs<RT, CT>(sr2 + d * S::LR + ty * RT,
+                           sc2 + d * S::LC + tx * CT, r, c);
 #pragma unroll
         for (int i = 0; i < RT; ++i)
 #pragma unroll
-          for (int j = 0; j < CT; ++j) u[i][j] = fmaf(r[i], c[j], u[i][j]);
+          for (int j = 0; j < CT / 2; ++j)
+            u2[i][j] = ffma2(r[i], c[j], u2[i][j]);
       }
     }
+    float s[RT][CT], u[RT][CT];
+#pragma unroll
+    for (int i = 0; i < RT; ++i)
+#pragma unroll
+      for (int j = 0; j < CT; j += 2) {
+        const float2 x = f2upk(s2[i][j / 2]), y = f2upk(u2[i][j / 2]);
+        s[i][j] = x.x, s[i][j + 1] = x.y;
+        u[i][j] = y.x, u[i][j + 1] = y.y;
+      }
 
     if constexpr (PASS == kForward) {
 #pragma unroll

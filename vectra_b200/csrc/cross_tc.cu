@@ -17,13 +17,13 @@
 // Warps: two warpgroups form P and z, one thread a row, each of one half of a
 // tile's columns, while the tensor cores work on the next tile's S and T (two
 // tiles are in TMEM); a TMA producer; an MMA issuer; a warpgroup for the
-// columns' terms, which are |k_j|^2, or a query's lse, c_i and scale. Where several blocks walk the same
-// keys their |k_j|^2 are formed once beforehand; a lone block (a decoding step)
-// forms them from the tile in shared memory (two warps doing that in every
-// block set the pace: 627 us of 4,096 queries on 5,003 keys, 32 heads of 128,
-// against 432 without). In the forward pass every warpgroup has its own
-// accumulator, maximum and sum, joined once at the end: nothing is exchanged
-// on the way.
+// columns' terms, which are |k_j|^2, or a query's lse, c_i and scale. Where
+// several blocks walk the same keys their |k_j|^2 are formed once beforehand; a
+// lone block (a decoding step) forms them from the tile in shared memory (two
+// warps doing that in every block set the pace: 627 us of 4,096 queries on
+// 5,003 keys, 32 heads of 128, against 432 without). In the forward pass every
+// warpgroup has its own accumulator, maximum and sum, joined once at the end:
+// nothing is exchanged on the way.
 //
 // Lengths: tiles past a sequence's length are not walked. In the last tile the
 // unseen rows of the operand that a product sums over are overwritten with

@@ -1,0 +1,122 @@
+"""The decoder operators (vectra_b200.block) beside the ordinary: values that
+are not finite, small gradients, rows far from zero, long walks and split axes,
+and what a call has to refuse.
+
+A test that compares whole tensors does so by their norms: with `u` the unit
+roundoff (half a step, relative to the value), a result that is rounded once
+is off by at most u of its norm. The roundings spread evenly over the steps,
+so that it is off by 0.39 u where its mantissas spread evenly over a binade's
+logarithm (the error of m 2^e is uniform in u 2^e: mean squares u^2 / 3 against
+1.5 / ln 2 for m^2), and by no more than u / sqrt(3) = 0.58 u if all mantissas
+were 1. ONCE = 0.5 lies between: two roundings of a value, or of the values
+that it sums, are off by 0.39 sqrt(2) = 0.55 u.
+"""
+
+import math
+
+import pytest
+import torch
+
+from tests.test_decoder import DEVICES
+from tests.test_decoder import TYPES
+from tests.test_decoder import U
+from tests.test_decoder import Rand
+from tests.test_decoder import cross_inputs
+from tests.test_decoder import d
+from vectra_b200 import block
+
+HALVES = [torch.bfloat16, torch.float16]
+ONCE = 0.5
+
+
+def off(got, want, dtype):
+    """The error of a tensor as a share of its norm, in units of u."""
+    return float((d(got) - want).norm() / want.norm()) / U[dtype]
+
+
+def gradients(leaves, lengths, dout):
+    leaves = [t.detach().clone().requires_grad_() for t in leaves]
+    out = block.cross_attention(*leaves, lengths)
+    return out.detach(), torch.autograd.grad(out, leaves, dout)
+
+
+def exact_cross(q, k, v, scale, lengths, dout):
+    """out, dq, dk, dv in float64, by matrix products a sequence at a time."""
+    b, h, nq = q.shape[:3]
+    hk, nk = k.shape[1:3]
+    rep = h // hk
+    Q, K, V, G = d(q), d(k), d(v), d(dout)
+    S = d(scale).expand(b, h, 1, 1)
+    n = torch.full((b,), nk) if lengths is None else lengths.cpu()
+    out, dq = torch.zeros_like(G), torch.zeros_like(Q)
+    dk, dv = torch.zeros_like(K), torch.zeros_like(V)
+    for i in range(b):
+        m = int(n[i])
+        for j in range(h):
+            x, y, z = Q[i, j], K[i, j // rep, :m], V[i, j // rep, :m]
+            g, e = S[i, j], G[i, j]
+            dist = x.square().sum(-1, keepdim=True) + y.square().sum(-1) - \
+                2 * x @ y.mT
+            w = torch.softmax(-g * dist, -1)
+            out[i, j] = w @ z
+            t = w * (e @ z.mT - (e * out[i, j]).sum(-1, keepdim=True))
+            dq[i, j] = 2 * g * (t @ y - t.sum(-1, keepdim=True) * x)
+            dk[i, j // rep, :m] += 2 * g * (t.mT @ x -
+                                            t.sum(0)[:, None] * y)
+            dv[i, j // rep, :m] += w.mT @ e
+    return out, dq, dk, dv
+
+
+# ---------------------------------------------------------------------------
+# cross_attention: values that are not finite.
+# ---------------------------------------------------------------------------
+# b, h, hk, nq, nk, D, and a length whose last key is alone in its part where
+# the kernels split the keys (16 a step up to 16 packed queries, else tiles of
+# 128, and of 64 in float32 and for odd widths): up to 8, up to 16 and more
+# packed queries, split and not.
+NAN_SIZES = [(2, 2, 2, 1, 700, 64, 17), (2, 2, 2, 1, 24, 64, 17),
+             (2, 6, 2, 4, 700, 128, 17), (2, 6, 2, 4, 24, 32, 17),
+             (2, 4, 2, 20, 1100, 64, 129), (2, 4, 2, 20, 1100, 128, 129),
+             (2, 4, 2, 20, 140, 64, 129), (2, 4, 2, 20, 700, 33, 65)]
+
+
+@pytest.mark.parametrize('device', DEVICES)
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('size', NAN_SIZES)
+@pytest.mark.parametrize('where', ['key', 'value', 'far value'])
+def test_cross_nan_in_a_seen_key(device, dtype, size, where):
+    """It reaches every query of the key's heads (a value's: its component, of
+    a key that weighs nothing too), and nothing else."""
+    b, h, hk, nq, nk, dim, n = size
+    rand = Rand(nk + dim, device, dtype)
+    q, k, v, scale = cross_inputs(rand, b, h, hk, nq, nk, dim)
+    dout = rand(b, h, nq, dim)
+    lengths = torch.tensor([n, nk], device=device)
+    if where == 'far value':
+        k[0, 0, n - 1] = 60.0
+    clean, cleans = gradients((q, k, v, scale), lengths, dout)
+    (k if where == 'key' else v)[0, 0, n - 1, 3] = math.nan
+    out, (dq, dk, dv, dscale) = gradients((q, k, v, scale), lengths, dout)
+    own = h // hk
+    if where == 'key':
+        assert out[0, :own].isnan().all()
+        assert dv[0, 0, :n].isnan().all()
+    else:
+        assert out[0, :own, :, 3].isnan().all()
+        assert out[0, :own, :, :3].isfinite().all()
+        assert dv[0, 0].isfinite().all()
+    assert dq[0, :own].isnan().all()
+    assert dk[0, 0, :n].isnan().all()
+    assert dscale[0, :own].isnan().all()
+    with torch.no_grad():
+        served = block.cross_attention(q, k, v, scale, lengths)
+    assert torch.equal(served.isnan(), out.isnan())
+    for got, want in ((out, clean), (dq, cleans[0])):
+        assert got[0, own:].isfinite().all() and got[1].isfinite().all()
+        assert torch.equal(got[1], want[1])
+    for got, want in ((dk, cleans[1]), (dv, cleans[2])):
+        assert (got[0, :, n:] == 0).all()
+        assert torch.equal(got[0, 1:], want[0, 1:])
+        assert torch.equal(got[1], want[1])
+
+

@@ -121,15 +121,20 @@ __global__ void __launch_bounds__(256)
       const int s = lane + 32 * i;
       own[i] = s < p.splits ? ml[s * rows] : make_float2(kNegInf, 0.f);
     }
-    const bool nan = __any_sync(0xffffffffu, own[0].x != own[0].x ||
-                                                 own[1].x != own[1].x);
-    const float m = nan ? NAN : warp_max(fmaxf(own[0].x, own[1].x));
+    // A maximum leaves NaN out, a sum does not: either makes the row NaN.
+    bool odd = false;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      odd = odd || own[i].x != own[i].x || own[i].y != own[i].y;
+    const float m = __any_sync(0xffffffffu, odd)
+                        ? NAN
+                        : warp_max(fmaxf(own[0].x, own[1].x));
     float f[2], l = 0.f;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       // A part whose keys all weigh nothing (or that has none) adds nothing.
       f[i] = own[i].x == kNegInf ? 0.f : fast_exp2(own[i].x - m);
-      l += own[i].x == kNegInf ? 0.f : own[i].y * f[i];
+      l += own[i].y * f[i];
     }
     l = warp_sum(l);
     float acc[kMaxCrossWidth / 32];
@@ -152,7 +157,7 @@ __global__ void __launch_bounds__(256)
       for (int i = 0; i < 4; ++i)
 #pragma unroll
         for (int c = 0; c < kMaxCrossWidth / 32; ++c)
-          if (by[i] != 0.f) acc[c] = fmaf(v[i][c], by[i], acc[c]);
+          acc[c] = fmaf(v[i][c], by[i], acc[c]);  // 0 * NaN of a far part too
     }
     const bool any = cross_length(p, b) > 0;
     T* out = static_cast<T*>(p.out) + b * p.so[0] + h * p.so[1] + i * p.so[2];

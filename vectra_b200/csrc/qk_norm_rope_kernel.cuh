@@ -104,7 +104,7 @@ __device__ __forceinline__ void pair_elements(int j, int r2, int d,
   if (*e1 >= d) *e1 = -1;
 }
 
-template <typename T, bool BACKWARD>
+template <typename T, bool BACKWARD, bool MULTI>
 __global__ void __launch_bounds__(kWarps * 32)
     qk_general_kernel(const QkArgs a) {
   __shared__ float sums[kWarps][512];
@@ -134,7 +134,7 @@ __global__ void __launch_bounds__(kWarps * 32)
     const int64_t h = v - token * s.H, b = token / p.N, n = token - b * p.N;
     const T* x = static_cast<const T*>(s.x) + b * s.sx[0] + h * s.sx[1] +
                  n * s.sx[2];
-    const Rows<true> rows = load_rows<true>(p, b, n);
+    const Rows<MULTI> rows = load_rows<MULTI>(p, b, n);
     const bool known = rows.known;
     float x0[kMaxPairs], x1[kMaxPairs];
     float ss = 0.f;
@@ -845,7 +845,7 @@ cudaError_t forward_with(const QkProblem& p, cudaStream_t stream) {
     using T = std::remove_pointer_t<decltype(t)>;
     if (!vec_ok(p, false)) {
       const QkArgs a{p, nullptr};
-      return launch_pdl(qk_general_kernel<T, false>,
+      return launch_pdl(qk_general_kernel<T, false, MULTI>,
                         dim3(unsigned(general_blocks(p)), 2),
                         dim3(kWarps * 32), 0, stream, a);
     }
@@ -910,7 +910,7 @@ cudaError_t backward_with(const QkProblem& p, Workspace& ws,
     using T = std::remove_pointer_t<decltype(t)>;
     if (!vec) {
       const QkArgs ga{p, partial};
-      return launch_pdl(qk_general_kernel<T, true>,
+      return launch_pdl(qk_general_kernel<T, true, MULTI>,
                         dim3(unsigned(general), 2), dim3(kWarps * 32), 0,
                         stream, ga);
     }

@@ -218,8 +218,9 @@ typedef struct {
  *  with M a multiple of G: row r takes gate row r / (M / G).
  *  x_out, y [M,C]: contiguous. y's data NULL: no second norm (weight and bias
  *  NULL then). The norm is of x_out before its rounding.
- *  stats [M,4] F32, contiguous: mean and factor of the second norm, mean and
- *  factor of the first, for the backward pass; data NULL: not wanted.
+ *  stats [M,4] F32, contiguous, on a 16-byte boundary: mean and factor of the
+ *  second norm, mean and factor of the first, for the backward pass; data NULL:
+ *  not wanted.
  * C is at most 16384. */
 typedef enum { VECTRA_NORM_RMS = 0, VECTRA_NORM_LAYER = 1 } vectra_norm_kind;
 typedef struct {

@@ -12,6 +12,7 @@ were 1. ONCE = 0.5 lies between: two roundings of a value, or of the values
 that it sums, are off by 0.39 sqrt(2) = 0.55 u.
 """
 
+import ctypes
 import math
 
 import pytest
@@ -21,8 +22,12 @@ from tests.test_decoder import DEVICES
 from tests.test_decoder import TYPES
 from tests.test_decoder import U
 from tests.test_decoder import Rand
+from tests.test_decoder import _abi
+from tests.test_decoder import _Drop
+from tests.test_decoder import _NormArgs
 from tests.test_decoder import cross_inputs
 from tests.test_decoder import d
+from vectra_b200 import _lib
 from vectra_b200 import block
 
 HALVES = [torch.bfloat16, torch.float16]
@@ -118,5 +123,40 @@ def test_cross_nan_in_a_seen_key(device, dtype, size, where):
         assert (got[0, :, n:] == 0).all()
         assert torch.equal(got[0, 1:], want[0, 1:])
         assert torch.equal(got[1], want[1])
+
+
+# ---------------------------------------------------------------------------
+# The C ABI, without a device.
+# ---------------------------------------------------------------------------
+class _NormGradArgs(ctypes.Structure):
+    """vectra_residual_norm_grad_args."""
+    _fields_ = [('fwd', _NormArgs)] + [(n, _lib.Tensor) for n in (
+        'dx_out', 'dy', 'dx', 'dbranch', 'dweight', 'dbias', 'dbranch_weight',
+        'dgate')] + [('workspace', ctypes.c_void_p),
+                     ('workspace_bytes', ctypes.c_size_t)]
+
+
+def test_abi_statistics_start_on_16_bytes():
+    """The kernels move a row's four statistics at once."""
+    forward = _lib.LIB.vectra_residual_norm_forward
+    size = _lib.LIB.vectra_residual_norm_backward_workspace_bytes
+    size.restype = ctypes.c_int64
+    layout = -12  # VECTRA_ERR_LAYOUT
+
+    def args(addr, **over):
+        n = _NormArgs(x=_abi((6, 8)), branch=_abi((6, 8)), x_out=_abi((6, 8)),
+                      y=_abi((6, 8)), stats=_abi((6, 4), _lib.F32, addr=addr),
+                      drop=_Drop(0.0, None, 0), residual_scale=1.0, eps=1e-6)
+        for name, value in over.items():
+            setattr(n, name, value)
+        return n
+
+    for addr in (0x10004, 0x10008):
+        assert forward(ctypes.byref(args(addr)), None) == layout
+    for addr, status in ((0x10004, layout), (0x10008, layout),
+                         (0x10010, _lib.OK)):
+        g = _NormGradArgs(fwd=args(addr), dy=_abi((6, 8)), dx=_abi((6, 8)))
+        got = size(ctypes.byref(g))
+        assert (got if status else min(got, 0)) == status
 
 

@@ -549,7 +549,7 @@ const char* vectra_block_strerror(int status) {
              "or a size above 2^29 - 256";
     case VECTRA_ERR_LAYOUT:
       return "results and rotation tables need a unit inner stride and rows "
-             "that do not overlap";
+             "that do not overlap, a norm's statistics 16-byte alignment";
     case VECTRA_ERR_WORKSPACE:
       return "the workspace is too small or not 256-byte aligned";
     default:

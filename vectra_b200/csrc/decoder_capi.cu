@@ -26,6 +26,13 @@ int check_contiguous(const vectra_tensor& t, int32_t dtype, int64_t n) {
   return VECTRA_OK;
 }
 
+// [rows, 4] float32, which the kernels move a row at a time.
+int check_stats(const vectra_tensor& t, int64_t rows) {
+  VECTRA_TRY(check_contiguous(t, VECTRA_F32, rows, 4));
+  return reinterpret_cast<uintptr_t>(t.data) & 15 ? VECTRA_ERR_LAYOUT
+                                                  : VECTRA_OK;
+}
+
 RowView view(const vectra_tensor& t) {  // [rows, columns]
   return {t.data, t.stride[0], t.size[1] > 1 ? t.stride[1] : 1};
 }
@@ -109,7 +116,7 @@ int norm_forward(const vectra_residual_norm_args& a, cudaStream_t stream) {
   if (present(a.y)) VECTRA_TRY(check_contiguous(a.y, p.dtype, p.M, p.C));
   p.y = const_cast<void*>(a.y.data);
   if (present(a.stats)) {
-    VECTRA_TRY(check_contiguous(a.stats, VECTRA_F32, p.M, 4));
+    VECTRA_TRY(check_stats(a.stats, p.M));
     p.stats = static_cast<float*>(const_cast<void*>(a.stats.data));
   }
   return launch_norm_forward(p, stream) == cudaSuccess ? VECTRA_OK
@@ -134,7 +141,7 @@ int norm_backward(const vectra_residual_norm_grad_args& a, Workspace& ws,
     p.f = view(a.dy);
   }
   if (norm1 || present(a.fwd.branch_weight)) {
-    VECTRA_TRY(check_contiguous(a.fwd.stats, VECTRA_F32, m, 4));
+    VECTRA_TRY(check_stats(a.fwd.stats, m));
     p.stats = static_cast<float*>(const_cast<void*>(a.fwd.stats.data));
   }
   // The branch itself is read for its norm and for the gate's gradient only.

@@ -231,6 +231,15 @@ typedef struct {
   int32_t kind; /* vectra_norm_kind */
 } vectra_residual_norm_args;
 
+/* The same for a backward pass to come. rest [M,C], of 16-bit tensors with a
+ * branch and y only, contiguous, their type: what x_out's rounding left, itself
+ * rounded. The second norm's gradient takes x_out less its mean, whose rounding
+ * a mean of many deviations would multiply. Data NULL: not wanted. */
+typedef struct {
+  vectra_residual_norm_args fwd;
+  vectra_tensor rest;
+} vectra_residual_norm_train_args;
+
 /* Gradients of the above for dx_out and dy [M,C] (any strides; dx_out's data
  * NULL: zero; dy's: y had none, its norm is left out). Of fwd, x_out and
  * stats are read as the forward wrote them (x_out is x, strides and all, where
@@ -246,6 +255,13 @@ typedef struct {
   void* workspace;
   size_t workspace_bytes;
 } vectra_residual_norm_grad_args;
+
+/* The same with the forward's rest (data NULL where it wrote none, or without
+ * dy); vectra_residual_norm_backward takes x_out as it was rounded. */
+typedef struct {
+  vectra_residual_norm_grad_args grad;
+  vectra_tensor rest;
+} vectra_residual_norm_train_grad_args;
 
 /* out[b,h,i] = sum over j < len_b of softmax_j(-scale |q_i - k_j|^2) v_j, with
  * q of head h and k, v of head h / (H / Hk).
@@ -296,7 +312,9 @@ VECTRA_API int vectra_qk_norm_rope_axes_forward(const vectra_qk_axes_args* args,
 VECTRA_API int vectra_qk_norm_rope_axes_backward(const vectra_qk_axes_grad_args* args, void* stream);
 VECTRA_API int vectra_dropout(const vectra_dropout_args* args, void* stream);
 VECTRA_API int vectra_residual_norm_forward(const vectra_residual_norm_args* args, void* stream);
+VECTRA_API int vectra_residual_norm_forward_train(const vectra_residual_norm_train_args* args, void* stream);
 VECTRA_API int vectra_residual_norm_backward(const vectra_residual_norm_grad_args* args, void* stream);
+VECTRA_API int vectra_residual_norm_backward_train(const vectra_residual_norm_train_grad_args* args, void* stream);
 VECTRA_API int vectra_cross_attention_forward(const vectra_cross_args* args, void* stream);
 VECTRA_API int vectra_cross_attention_backward(const vectra_cross_grad_args* args, void* stream);
 
@@ -309,6 +327,7 @@ VECTRA_API int64_t vectra_gated_linear_backward_workspace_bytes(const vectra_gat
 VECTRA_API int64_t vectra_qk_norm_rope_backward_workspace_bytes(const vectra_qk_grad_args* args);
 VECTRA_API int64_t vectra_qk_norm_rope_axes_backward_workspace_bytes(const vectra_qk_axes_grad_args* args);
 VECTRA_API int64_t vectra_residual_norm_backward_workspace_bytes(const vectra_residual_norm_grad_args* args);
+VECTRA_API int64_t vectra_residual_norm_backward_train_workspace_bytes(const vectra_residual_norm_train_grad_args* args);
 VECTRA_API int64_t vectra_cross_attention_forward_workspace_bytes(const vectra_cross_args* args);
 VECTRA_API int64_t vectra_cross_attention_backward_workspace_bytes(const vectra_cross_grad_args* args);
 

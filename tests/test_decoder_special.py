@@ -126,6 +126,61 @@ def test_cross_nan_in_a_seen_key(device, dtype, size, where):
 
 
 # ---------------------------------------------------------------------------
+# residual_norm: rows far from zero.
+# ---------------------------------------------------------------------------
+def exact_norm(x, branch, weight, bias, dx_out, dy, kind, eps):
+    """Gradients of x, branch, weight and bias in float64."""
+    leaves = [d(t).requires_grad_() for t in (x, branch, weight, bias)]
+    v = leaves[0] + leaves[1]
+    c = v - v.mean(-1, keepdim=True) if kind == 'layer' else v
+    y = c * (c.square().mean(-1, keepdim=True) + eps).rsqrt() * leaves[2] + \
+        leaves[3]
+    return torch.autograd.grad((v, y), leaves, (d(dx_out), d(dy)))
+
+
+@pytest.mark.parametrize('device', DEVICES)
+@pytest.mark.parametrize('dtype', HALVES)
+@pytest.mark.parametrize('kind', ['rms', 'layer'])
+@pytest.mark.parametrize('mean', [0.0, 16.0])
+@pytest.mark.parametrize('size', [(2, 40, 256), (3, 30, 1000), (1, 7, 4096)])
+def test_norm_gradients_of_rows_far_from_zero(device, dtype, kind, mean,
+                                              size):
+    """The stream's rounding does not enter the gradients of its norm, which a
+    mean of many deviations would multiply: gradients are rounded once."""
+    b, n, c = size
+    rand = Rand(c, device, dtype)
+    x, branch = rand(b, n, c) + mean, rand(b, n, c)
+    weight, bias = 1 + rand(c, scale=0.2), rand(c)
+    dx_out, dy = rand(b, n, c), rand(b, n, c)
+    leaves = [t.requires_grad_() for t in (x, branch, weight, bias)]
+    out = block.residual_norm(*leaves, kind=kind)
+    got = torch.autograd.grad(out, leaves, (dx_out, dy))
+    want = exact_norm(x, branch, weight, bias, dx_out, dy, kind, 1e-6)
+    for a, y, name in zip(got, want, ('dx', 'dbranch', 'dweight', 'dbias')):
+        # Of c roundings the share in a norm varies by sqrt(0.2 / c) of itself.
+        assert off(a, y, dtype) <= ONCE * (1 + 3 * math.sqrt(
+            0.2 / a.numel())), name
+
+
+@pytest.mark.parametrize('device', DEVICES)
+def test_norm_keeps_what_a_rounding_left_only_where_it_is_read(device):
+    """Nothing is kept beside x_out for float32, without a branch, or where no
+    norm follows."""
+    op = torch.ops.vectra_b200.residual_norm_with_stats
+
+    def rest(dtype, branch, norm, want=True):
+        x = torch.ones(3, 16, device=device, dtype=dtype)
+        return op(x, x if branch else None, None, None, None, None, 1.0, 0.0,
+                  None, 0, 1e-6, 'rms', norm, want)[3]
+
+    assert rest(torch.bfloat16, True, True).shape == (3, 16)
+    for call in ((torch.float32, True, True), (torch.bfloat16, False, True),
+                 (torch.float16, True, False),
+                 (torch.float16, True, True, False)):
+        assert rest(*call).numel() == 0
+
+
+# ---------------------------------------------------------------------------
 # The C ABI, without a device.
 # ---------------------------------------------------------------------------
 class _NormGradArgs(ctypes.Structure):

@@ -68,6 +68,9 @@ EXPORTED = (
     'vectra_qk_norm_rope_axes_backward',
     'vectra_dropout',
     'vectra_residual_norm_forward',
+    'vectra_residual_norm_forward_train',
+    'vectra_residual_norm_backward_train',
+    'vectra_residual_norm_backward_train_workspace_bytes',
     'vectra_residual_norm_backward',
     'vectra_cross_attention_forward',
     'vectra_cross_attention_backward',
@@ -404,14 +407,17 @@ def _norm_with_stats_fake(x, branch, weight, bias, branch_weight, gate,
     rows = math.prod(x.shape[:-1]) if want_stats and x.shape[-1] else 0
     return (x.new_empty(x.shape if branch is not None else (0,)),
             x.new_empty(x.shape if norm else (0,)),
-            x.new_empty((rows, 4), dtype=torch.float32))
+            x.new_empty((rows, 4), dtype=torch.float32),
+            x.new_empty(x.shape if want_stats and norm and
+                        branch is not None and x.dtype != torch.float32
+                        else (0,)))
 
 
 @torch.library.register_fake('vectra_b200::residual_norm_backward')
-def _norm_backward_fake(dx_out, dy, x_out, stats, branch, weight,
+def _norm_backward_fake(dx_out, dy, x_out, rest, stats, branch, weight,
                         branch_weight, gate, residual_scale, p, rng, stream,
                         eps, kind, need):
-    del x_out, stats, branch, weight, branch_weight, residual_scale, p, rng
+    del x_out, rest, stats, branch, weight, branch_weight, residual_scale, p, rng
     del stream, eps, kind
     g = dx_out if dy is None else dy
     c = g.shape[-1:]

@@ -105,7 +105,16 @@ int build_norm(const vectra_residual_norm_args& a, const vectra_tensor& rows,
   return VECTRA_OK;
 }
 
-int norm_forward(const vectra_residual_norm_args& a, cudaStream_t stream) {
+// What x_out's rounding left; 16-bit tensors with a branch and a norm.
+int check_rest(const vectra_tensor& rest, const NormProblem& p,
+               bool rounded) {
+  if (p.dtype == VECTRA_F32) return VECTRA_ERR_DTYPE;
+  if (!rounded) return VECTRA_ERR_NULL;
+  return check_contiguous(rest, p.dtype, p.M, p.C);
+}
+
+int norm_forward(const vectra_residual_norm_args& a, const vectra_tensor& rest,
+                 cudaStream_t stream) {
   NormProblem p;
   VECTRA_TRY(build_norm(a, a.x, present(a.y), false, &p));
   VECTRA_TRY(check(a.x, p.dtype, {p.M, p.C}));
@@ -119,12 +128,17 @@ int norm_forward(const vectra_residual_norm_args& a, cudaStream_t stream) {
     VECTRA_TRY(check_stats(a.stats, p.M));
     p.stats = static_cast<float*>(const_cast<void*>(a.stats.data));
   }
+  if (present(rest)) {
+    VECTRA_TRY(check_rest(rest, p, present(a.branch) && present(a.y)));
+    p.rest = const_cast<void*>(rest.data);
+  }
   return launch_norm_forward(p, stream) == cudaSuccess ? VECTRA_OK
                                                        : VECTRA_ERR_CUDA;
 }
 
-int norm_backward(const vectra_residual_norm_grad_args& a, Workspace& ws,
-                  cudaStream_t stream) {
+int norm_backward_with(const vectra_residual_norm_grad_args& a,
+                       const vectra_tensor& rest, Workspace& ws,
+                       cudaStream_t stream) {
   NormProblem p;
   const bool norm1 = present(a.dy);
   const vectra_tensor& rows = norm1 ? a.dy : a.dx_out;
@@ -139,6 +153,10 @@ int norm_backward(const vectra_residual_norm_grad_args& a, Workspace& ws,
     VECTRA_TRY(check(a.fwd.x_out, p.dtype, {m, c}));
     p.x = view(a.fwd.x_out);
     p.f = view(a.dy);
+  }
+  if (present(rest)) {
+    VECTRA_TRY(check_rest(rest, p, norm1));
+    p.rest = const_cast<void*>(rest.data);
   }
   if (norm1 || present(a.fwd.branch_weight)) {
     VECTRA_TRY(check_stats(a.fwd.stats, m));
@@ -170,6 +188,17 @@ int norm_backward(const vectra_residual_norm_grad_args& a, Workspace& ws,
     p.dgate = const_cast<void*>(a.dgate.data);
   }
   return to_status(run_norm_backward(p, ws, stream), ws);
+}
+int norm_backward(const vectra_residual_norm_grad_args& a, Workspace& ws,
+                  cudaStream_t stream) {
+  return norm_backward_with(a, vectra_tensor{}, ws, stream);
+}
+// The workspace of the call with `rest` is its other part's.
+auto norm_backward_train(const vectra_tensor& rest) {
+  return [&rest](const vectra_residual_norm_grad_args& a, Workspace& ws,
+                 cudaStream_t stream) {
+    return norm_backward_with(a, rest, ws, stream);
+  };
 }
 
 void strides_of(const vectra_tensor& t, int64_t* s) {
@@ -320,11 +349,26 @@ int vectra_dropout(const vectra_dropout_args* a, void* stream) {
 int vectra_residual_norm_forward(const vectra_residual_norm_args* a,
                                  void* stream) {
   if (a == nullptr) return VECTRA_ERR_NULL;
-  return norm_forward(*a, static_cast<cudaStream_t>(stream));
+  return norm_forward(*a, vectra_tensor{}, static_cast<cudaStream_t>(stream));
+}
+int vectra_residual_norm_forward_train(const vectra_residual_norm_train_args* a,
+                                       void* stream) {
+  if (a == nullptr) return VECTRA_ERR_NULL;
+  return norm_forward(a->fwd, a->rest, static_cast<cudaStream_t>(stream));
 }
 int vectra_residual_norm_backward(const vectra_residual_norm_grad_args* a,
                                   void* stream) {
   return run_with_workspace(a, stream, norm_backward);
+}
+int vectra_residual_norm_backward_train(
+    const vectra_residual_norm_train_grad_args* a, void* stream) {
+  if (a == nullptr) return VECTRA_ERR_NULL;
+  return run_with_workspace(&a->grad, stream, norm_backward_train(a->rest));
+}
+int64_t vectra_residual_norm_backward_train_workspace_bytes(
+    const vectra_residual_norm_train_grad_args* a) {
+  if (a == nullptr) return VECTRA_ERR_NULL;
+  return workspace_of(&a->grad, norm_backward_train(a->rest));
 }
 int vectra_cross_attention_forward(const vectra_cross_args* a, void* stream) {
   return run_with_workspace(a, stream, cross_forward);

@@ -202,9 +202,17 @@ vectra_residual_norm_args describe_norm(const NormCall& call) {
 }
 
 using Three = std::tuple<Tensor, Tensor, Tensor>;
+using Four = std::tuple<Tensor, Tensor, Tensor, Tensor>;
 using Six = std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor>;
 
-Three norm_cuda(const Tensor& x, const OptTensor& branch,
+// What x_out's rounding leaves, for the backward pass of the norm behind.
+Tensor rest_of_sum(const Tensor& x, bool branched, bool norm, bool want) {
+  const bool kept =
+      want && branched && norm && x.scalar_type() != at::kFloat;
+  return kept ? at::empty(x.sizes(), x.options()) : at::empty({0}, x.options());
+}
+
+Four norm_cuda(const Tensor& x, const OptTensor& branch,
                 const OptTensor& weight, const OptTensor& bias,
                 const OptTensor& branch_weight, const OptTensor& gate,
                 const NormCall& call, bool norm, bool want_stats) {
@@ -216,8 +224,12 @@ Three norm_cuda(const Tensor& x, const OptTensor& branch,
   Tensor y = norm ? at::empty(x.sizes(), x.options()) : none();
   Tensor stats = at::empty({want_stats ? rows : 0, 4},
                            x.options().dtype(at::kFloat));
-  if (x.numel() == 0) return {x_out, y, stats};
-  vectra_residual_norm_args a = describe_norm(call);
+  Tensor rest = rest_of_sum(x, has(branch), norm, want_stats);
+  if (x.numel() == 0) return {x_out, y, stats, rest};
+  vectra_residual_norm_train_args train{};
+  train.fwd = describe_norm(call);
+  if (rest.numel()) train.rest = describe_rows(rest, nullptr);
+  vectra_residual_norm_args& a = train.fwd;
   Tensor x_copy, branch_copy, gate_copy;
   a.x = describe_rows(x, &x_copy);
   if (has(branch)) {
@@ -233,10 +245,10 @@ Three norm_cuda(const Tensor& x, const OptTensor& branch,
   }
   if (norm) a.y = describe_rows(y, nullptr);
   if (want_stats) a.stats = describe(stats);
-  const int st = vectra_residual_norm_forward(
-      &a, at::cuda::getCurrentCUDAStream(x.device().index()).stream());
+  const int st = vectra_residual_norm_forward_train(
+      &train, at::cuda::getCurrentCUDAStream(x.device().index()).stream());
   if (st != VECTRA_OK) raise_status("residual_norm", st);
-  return {x_out, y, stats};
+  return {x_out, y, stats, rest};
 }
 
 // The gradients that a backward pass is to form, as bits.
@@ -251,7 +263,8 @@ const Tensor& upstream(const OptTensor& dx_out, const OptTensor& dy) {
 }
 
 void check_norm_grad(const OptTensor& dx_out, const OptTensor& dy,
-                     const Tensor& x_out, const Tensor& stats,
+                     const Tensor& x_out, const Tensor& rest,
+                     const Tensor& stats,
                      const OptTensor& branch, const OptTensor& weight,
                      const OptTensor& branch_weight, const OptTensor& gate,
                      const NormCall& call, int64_t need) {
@@ -265,6 +278,12 @@ void check_norm_grad(const OptTensor& dx_out, const OptTensor& dy,
   if (has(dy)) {
     check_like(x_out, "x_out", g);
     check_sizes(x_out, "x_out", g.sizes());
+    if (rest.numel()) {
+      check_like(rest, "rest", g);
+      check_sizes(rest, "rest", g.sizes());
+      TORCH_CHECK_VALUE(rest.is_contiguous() && g.scalar_type() != at::kFloat,
+                        "rest must be the forward's");
+    }
   }
   if (has(dy) || has(branch_weight)) {
     const int64_t c = g.size(-1);
@@ -287,12 +306,13 @@ void check_norm_grad(const OptTensor& dx_out, const OptTensor& dy,
 }
 
 Six norm_backward_cuda(const OptTensor& dx_out, const OptTensor& dy,
-                       const Tensor& x_out, const Tensor& stats,
+                       const Tensor& x_out, const Tensor& rest,
+                       const Tensor& stats,
                        const OptTensor& branch, const OptTensor& weight,
                        const OptTensor& branch_weight, const OptTensor& gate,
                        const NormCall& call, int64_t need) {
-  check_norm_grad(dx_out, dy, x_out, stats, branch, weight, branch_weight,
-                  gate, call, need);
+  check_norm_grad(dx_out, dy, x_out, rest, stats, branch, weight,
+                  branch_weight, gate, call, need);
   const Tensor& g = upstream(dx_out, dy);
   c10::cuda::CUDAGuard guard(g.device());
   const int64_t c = g.size(-1);
@@ -309,13 +329,19 @@ Six norm_backward_cuda(const OptTensor& dx_out, const OptTensor& dy,
     for (Tensor* t : {&dweight, &dbias, &dbw, &dgate}) t->zero_();
     return {dx, dbranch, dweight, dbias, dbw, dgate};
   }
-  vectra_residual_norm_grad_args a{};
+  // The workspace is the grad part's.
+  struct Args : vectra_residual_norm_train_grad_args {
+    void*& workspace = grad.workspace;
+    size_t& workspace_bytes = grad.workspace_bytes;
+  } train{};
+  vectra_residual_norm_grad_args& a = train.grad;
   a.fwd = describe_norm(call);
   Tensor copies[5], gate_copy;
   if (has(dx_out)) a.dx_out = describe_rows(*dx_out, &copies[0]);
   if (has(dy)) {
     a.dy = describe_rows(*dy, &copies[1]);
     a.fwd.x_out = describe_rows(x_out, &copies[2]);
+    if (rest.numel()) train.rest = describe_rows(rest, nullptr);
     a.fwd.weight = describe(weight);
   }
   if (has(branch)) a.fwd.branch = describe_rows(*branch, &copies[3]);
@@ -336,9 +362,9 @@ Six norm_backward_cuda(const OptTensor& dx_out, const OptTensor& dy,
     a.dgate.stride[0] = c;
     a.dgate.stride[1] = 1;
   }
-  call_with_workspace("residual_norm_backward", a, g,
-                      vectra_residual_norm_backward_workspace_bytes,
-                      vectra_residual_norm_backward);
+  call_with_workspace("residual_norm_backward", train, g,
+                      vectra_residual_norm_backward_train_workspace_bytes,
+                      vectra_residual_norm_backward_train);
   return {dx, dbranch, dweight, dbias, dbw, dgate};
 }
 
@@ -351,7 +377,7 @@ std::pair<Tensor, Tensor> cpu_row_norm(const Tensor& v, const NormCall& call) {
   return {mean.expand(r.sizes()), r};
 }
 
-Three norm_cpu(const Tensor& x, const OptTensor& branch,
+Four norm_cpu(const Tensor& x, const OptTensor& branch,
                const OptTensor& weight, const OptTensor& bias,
                const OptTensor& branch_weight, const OptTensor& gate,
                const NormCall& call, bool norm, bool want_stats) {
@@ -360,6 +386,7 @@ Three norm_cpu(const Tensor& x, const OptTensor& branch,
   const auto none = [&] { return at::empty({0}, x.options()); };
   Tensor stats = at::zeros({want_stats ? rows : 0, 4}, at::kFloat);
   Tensor v = f32(x), x_out = none(), y = none();
+  Tensor rest = rest_of_sum(x, has(branch), norm, want_stats);
   const auto keep = [&](int64_t at, const std::pair<Tensor, Tensor>& n) {
     if (!want_stats) return;
     stats.select(1, at).copy_(n.first.reshape({rows}));
@@ -376,6 +403,7 @@ Three norm_cpu(const Tensor& x, const OptTensor& branch,
     if (has(gate)) u = u * f32(*gate);
     v = v * call.residual_scale + u;
     x_out = at::empty(x.sizes(), x.options()).copy_(v);
+    if (rest.numel()) rest.copy_(v - f32(x_out));
   }
   if (norm) {
     const auto n = cpu_row_norm(v, call);
@@ -385,16 +413,17 @@ Three norm_cpu(const Tensor& x, const OptTensor& branch,
     if (has(bias)) v = v + f32(*bias);
     y = at::empty(x.sizes(), x.options()).copy_(v);
   }
-  return {x_out, y, stats};
+  return {x_out, y, stats, rest};
 }
 
 Six norm_backward_cpu(const OptTensor& dx_out, const OptTensor& dy,
-                      const Tensor& x_out, const Tensor& stats,
+                      const Tensor& x_out, const Tensor& rest,
+                      const Tensor& stats,
                       const OptTensor& branch, const OptTensor& weight,
                       const OptTensor& branch_weight, const OptTensor& gate,
                       const NormCall& call, int64_t need) {
-  check_norm_grad(dx_out, dy, x_out, stats, branch, weight, branch_weight,
-                  gate, call, need);
+  check_norm_grad(dx_out, dy, x_out, rest, stats, branch, weight,
+                  branch_weight, gate, call, need);
   const Tensor& like = upstream(dx_out, dy);
   const int64_t c = like.size(-1), rows = c > 0 ? like.numel() / c : 0;
   const at::ScalarType dt = like.scalar_type();
@@ -415,7 +444,9 @@ Six norm_backward_cpu(const OptTensor& dx_out, const OptTensor& dy,
   Tensor dweight = none(), dbias = none(), dbw = none(), dgate = none();
   if (has(dy)) {
     const Tensor f = flat(*dy), r = column(1);
-    const Tensor n = (flat(x_out) - column(0)) * r;
+    Tensor v = flat(x_out);
+    if (rest.numel()) v = v + flat(rest);
+    const Tensor n = (v - column(0)) * r;
     if (need & kDweight) dweight = (f * n).sum(0).to(dt);
     if (need & kDbias) dbias = f.sum(0).to(dt);
     g = g + back(has(weight) ? f * f32(*weight) : f, n, r);
@@ -561,8 +592,6 @@ Three cross_cuda(const Tensor& q, const Tensor& k, const Tensor& v,
                       vectra_cross_attention_forward);
   return {out, lse, rest};
 }
-
-using Four = std::tuple<Tensor, Tensor, Tensor, Tensor>;
 
 void check_cross_grad(const Tensor& dout, const Tensor& q, const Tensor& v,
                       const Tensor& out, const Tensor& lse,
@@ -806,15 +835,15 @@ Tensor dropout_autograd(const Tensor& x, double p, const OptTensor& rng,
   return call_dropout(x, p, rng, stream);
 }
 
-using NormOp = Three(const Tensor&, const OptTensor&, const OptTensor&,
+using NormOp = Four(const Tensor&, const OptTensor&, const OptTensor&,
                      const OptTensor&, const OptTensor&, const OptTensor&,
                      double, double, const OptTensor&, int64_t, double,
                      c10::string_view, bool, bool);
 using NormBackwardOp = Six(const OptTensor&, const OptTensor&, const Tensor&,
-                           const Tensor&, const OptTensor&, const OptTensor&,
-                           const OptTensor&, const OptTensor&, double, double,
-                           const OptTensor&, int64_t, double,
-                           c10::string_view, int64_t);
+                           const Tensor&, const Tensor&, const OptTensor&,
+                           const OptTensor&, const OptTensor&,
+                           const OptTensor&, double, double, const OptTensor&,
+                           int64_t, double, c10::string_view, int64_t);
 
 struct NormFunction : public Function<NormFunction> {
   static variable_list forward(
@@ -826,14 +855,14 @@ struct NormFunction : public Function<NormFunction> {
     at::AutoDispatchBelowADInplaceOrView below;
     static const auto op =
         find_op<NormOp>("vectra_b200::residual_norm_with_stats");
-    auto [x_out, y, stats] =
+    auto [x_out, y, stats, rest] =
         op.call(x, branch, weight, bias, branch_weight, gate, residual_scale,
                 p, rng, stream, eps, kind, norm, true);
     const bool branched = has(branch);
     // The branch is read again for its norm and for the gate's gradient.
     const bool keep = has(branch_weight) || wants_grad(gate);
     ctx->save_for_backward(
-        {norm ? (branched ? x_out : x) : shape_of(x), stats,
+        {norm ? (branched ? x_out : x) : shape_of(x), rest, stats,
          branched && keep ? *branch : Tensor(), or_undefined(weight),
          or_undefined(branch_weight), or_undefined(gate), or_undefined(rng)});
     ctx->saved_data["residual_scale"] = residual_scale;
@@ -869,10 +898,10 @@ struct NormFunction : public Function<NormFunction> {
     static const auto op =
         find_op<NormBackwardOp>("vectra_b200::residual_norm_backward");
     auto [dx, dbranch, dweight, dbias, dbw, dgate] = op.call(
-        optional(dx_out), optional(dy), s[0], s[1], optional(s[2]),
-        optional(s[3]), optional(s[4]), optional(s[5]),
+        optional(dx_out), optional(dy), s[0], s[1], s[2], optional(s[3]),
+        optional(s[4]), optional(s[5]), optional(s[6]),
         ctx->saved_data["residual_scale"].toDouble(),
-        ctx->saved_data["p"].toDouble(), optional(s[6]),
+        ctx->saved_data["p"].toDouble(), optional(s[7]),
         ctx->saved_data["stream"].toInt(), ctx->saved_data["eps"].toDouble(),
         ctx->saved_data["kind"].toStringRef(), need);
     const Tensor results[6] = {dx, dbranch, dweight, dbias, dbw, dgate};
@@ -904,10 +933,9 @@ std::tuple<Tensor, Tensor> norm_autograd(
   at::AutoDispatchBelowADInplaceOrView below;
   static const auto op =
       find_op<NormOp>("vectra_b200::residual_norm_with_stats");
-  auto [x_out, y, stats] =
-      op.call(x, branch, weight, bias, branch_weight, gate, residual_scale, p,
-              rng, stream, eps, kind, norm, false);
-  return {x_out, y};
+  auto out = op.call(x, branch, weight, bias, branch_weight, gate,
+                     residual_scale, p, rng, stream, eps, kind, norm, false);
+  return {std::get<0>(out), std::get<1>(out)};
 }
 
 using CrossOp = Three(const Tensor&, const Tensor&, const Tensor&,
@@ -969,7 +997,7 @@ Tensor cross_autograd(const Tensor& q, const Tensor& k, const Tensor& v,
 
 // The implementations with the schemas' types.
 template <auto F>
-Three norm_impl(const Tensor& x, const OptTensor& branch,
+Four norm_impl(const Tensor& x, const OptTensor& branch,
                 const OptTensor& weight, const OptTensor& bias,
                 const OptTensor& branch_weight, const OptTensor& gate,
                 double residual_scale, double p, const OptTensor& rng,
@@ -986,20 +1014,21 @@ std::tuple<Tensor, Tensor> norm_only_impl(
     const OptTensor& gate, double residual_scale, double p,
     const OptTensor& rng, int64_t stream, double eps, c10::string_view kind,
     bool norm) {
-  auto [x_out, y, stats] =
-      norm_impl<F>(x, branch, weight, bias, branch_weight, gate,
-                   residual_scale, p, rng, stream, eps, kind, norm, false);
-  return {x_out, y};
+  auto out = norm_impl<F>(x, branch, weight, bias, branch_weight, gate,
+                          residual_scale, p, rng, stream, eps, kind, norm,
+                          false);
+  return {std::get<0>(out), std::get<1>(out)};
 }
 template <auto F>
 Six norm_backward_impl(const OptTensor& dx_out, const OptTensor& dy,
-                       const Tensor& x_out, const Tensor& stats,
+                       const Tensor& x_out, const Tensor& rest,
+                       const Tensor& stats,
                        const OptTensor& branch, const OptTensor& weight,
                        const OptTensor& branch_weight, const OptTensor& gate,
                        double residual_scale, double p, const OptTensor& rng,
                        int64_t stream, double eps, c10::string_view kind,
                        int64_t need) {
-  return F(dx_out, dy, x_out, stats, branch, weight, branch_weight, gate,
+  return F(dx_out, dy, x_out, rest, stats, branch, weight, branch_weight, gate,
            NormCall{residual_scale, p, rng, stream, eps, kind_of(kind)},
            need);
 }
@@ -1024,10 +1053,11 @@ TORCH_LIBRARY_FRAGMENT(vectra_b200, m) {
       "residual_norm_with_stats(Tensor x, Tensor? branch, Tensor? weight, "
       "Tensor? bias, Tensor? branch_weight, Tensor? gate, "
       "float residual_scale, float p, Tensor? rng, int stream, float eps, "
-      "str kind, bool norm, bool want_stats) -> (Tensor, Tensor, Tensor)");
+      "str kind, bool norm, bool want_stats) "
+      "-> (Tensor, Tensor, Tensor, Tensor)");
   m.def(
       "residual_norm_backward(Tensor? dx_out, Tensor? dy, Tensor x_out, "
-      "Tensor stats, Tensor? branch, Tensor? weight, Tensor? branch_weight, "
+      "Tensor rest, Tensor stats, Tensor? branch, Tensor? weight, Tensor? branch_weight, "
       "Tensor? gate, float residual_scale, float p, Tensor? rng, int stream, "
       "float eps, str kind, int need) "
       "-> (Tensor, Tensor, Tensor, Tensor, Tensor, Tensor)");

@@ -24,7 +24,7 @@ bool all_vec(const NormProblem& p) {
          rows_vec(p.gate, p.gate_count, es) && rows_vec(p.e, p.M, es) &&
          rows_vec(p.f, p.M, es) && ptr_vec(p.x_out) && ptr_vec(p.y) &&
          ptr_vec(p.dx) && ptr_vec(p.dbranch) && ptr_vec(p.dgate) &&
-         ptr_vec(p.stats);
+         ptr_vec(p.stats) && ptr_vec(p.rest);
 }
 
 // A row's team: chunks a thread, threads, teams a block. A warp up to 512
@@ -169,7 +169,7 @@ cudaError_t run_norm_backward(const NormProblem& problem, Workspace& ws,
     if (st != cudaSuccess) return st;
   }
   size_t bytes = 0;
-  p.tensors = gate && p.gate_rows == 1 ? 5 : 4;
+  p.tensors = 4 + (gate && p.gate_rows == 1) + (p.rest != nullptr);
   p.stages = stages_of(p, team, resident, 3, &bytes);
   const bool vec = all_vec(p) && p.stages > 0;
   if (!vec) bytes = 0;

@@ -171,6 +171,16 @@ __device__ __forceinline__ void store8(void* row, int col, int cols,
   }
 }
 
+// What rounding v to T leaves.
+template <typename T>
+__device__ __forceinline__ void left_over(const uint64_t* v, uint64_t* rest) {
+  uint64_t rounded[kPairs];
+  unpack<T>(pack<T>(v), rounded);
+  const uint64_t minus = both(-1.f);
+#pragma unroll
+  for (int i = 0; i < kPairs; ++i) rest[i] = ffma2(rounded[i], minus, v[i]);
+}
+
 // Kept elements times `scale`, 0 for the others.
 __device__ __forceinline__ void drop8(uint32_t keep, float scale,
                                       uint64_t* v) {
@@ -551,6 +561,12 @@ __global__ void __launch_bounds__(1024)
 #pragma unroll
         for (int i = 0; i < kPairs; ++i) v[c][i] = ffma2(scale, x[i], v[c][i]);
         store8<T, VEC>(static_cast<T*>(p.x_out) + at, col[c], C, v[c]);
+        if constexpr (!std::is_same<T, float>::value) {
+          if (p.rest) {
+            left_over<T>(v[c], x);
+            store8<T, VEC>(static_cast<T*>(p.rest) + at, col[c], C, x);
+          }
+        }
       }
     }
     if (p.y) {
@@ -614,6 +630,10 @@ __global__ void __launch_bounds__(THREADS, THREADS <= 320 ? 2 : 1)
   if constexpr (NORM0) rows.keep(kBranchWeight, p.branch_weight, 0, 1.f);
   // A gate that differs from row to row comes as the rows do.
   const bool gate_moves = GATE && p.gate_rows == 1;
+  // What x_out's rounding left, of 16-bit types.
+  const bool has_rest = !std::is_same<T, float>::value && p.rest != nullptr;
+  const RowView rest{p.rest, C, 1};
+  const int rest_at = gate_moves ? 5 : 4;
   int gate_row = -1;
   const uint32_t end = rows.stage * p.stages;
   const int team = int(blockIdx.x * blockDim.y + threadIdx.y);
@@ -649,6 +669,7 @@ __global__ void __launch_bounds__(THREADS, THREADS <= 320 ? 2 : 1)
       rows.fetch(stage, 2, p.e, later.row);
       rows.fetch(stage, 3, p.f, later.row);
       if (gate_moves) rows.fetch(stage, 4, p.gate, later.row);
+      if (has_rest) rows.fetch(stage, rest_at, rest, later.row);
       rows.fetch_stats(stage, p.stats, later.row);
       step(&later);
     }
@@ -683,6 +704,11 @@ __global__ void __launch_bounds__(THREADS, THREADS <= 320 ? 2 : 1)
         uint64_t w[kPairs];
         rows.vector(kWeight, p.weight, 0, 1.f, c, w);
         rows.get(stage, 0, p.x, row, c, n);
+        if (has_rest) {
+          rows.get(stage, rest_at, rest, row, c, f);
+#pragma unroll
+          for (int i = 0; i < kPairs; ++i) n[i] = fadd2(n[i], f[i]);
+        }
         rows.get(stage, 3, p.f, row, c, f);
 #pragma unroll
         for (int i = 0; i < kPairs; ++i) {

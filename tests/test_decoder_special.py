@@ -19,6 +19,7 @@ import pytest
 import torch
 
 from tests.test_decoder import DEVICES
+from tests.test_decoder import TINY
 from tests.test_decoder import TYPES
 from tests.test_decoder import U
 from tests.test_decoder import Rand
@@ -27,6 +28,7 @@ from tests.test_decoder import _Drop
 from tests.test_decoder import _NormArgs
 from tests.test_decoder import cross_inputs
 from tests.test_decoder import d
+from tests.test_decoder import sums
 from vectra_b200 import _lib
 from vectra_b200 import block
 
@@ -123,6 +125,101 @@ def test_cross_nan_in_a_seen_key(device, dtype, size, where):
         assert (got[0, :, n:] == 0).all()
         assert torch.equal(got[0, 1:], want[0, 1:])
         assert torch.equal(got[1], want[1])
+
+
+# ---------------------------------------------------------------------------
+# cross_attention: the range of 16-bit operands.
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize('device', DEVICES)
+@pytest.mark.parametrize('dtype', HALVES)
+@pytest.mark.parametrize('size', [(1, 2, 2, 3, 4500, 64),
+                                  (1, 6, 1, 2, 4500, 128),
+                                  (1, 2, 1, 250, 4500, 128),
+                                  (2, 2, 2, 130, 2000, 48)])
+@pytest.mark.parametrize('up', [1.0, 1e-2, 1e-3, 1e-4])
+def test_cross_small_gradients(device, dtype, size, up):
+    """Many keys and a small upstream gradient: the gradients are within twice
+    their own rounding (float16's spacing, 2^-24, counted once a result)."""
+    b, h, hk, nq, nk, dim = size
+    rand = Rand(nk + dim, device, dtype)
+    a = cross_inputs(rand, *size)
+    dout = rand(b, h, nq, dim, scale=up)
+    lengths = torch.tensor([nk, nk - 9][:b], device=device)
+    got = gradients(a, lengths, dout)
+    want = exact_cross(*a, lengths, dout)
+    for x, y, name in zip((got[0], *got[1][:3]), want,
+                          ('out', 'dq', 'dk', 'dv')):
+        bound = 2 * (U[dtype] * y.norm() + TINY[dtype] / 2 *
+                     math.sqrt(y.numel()))
+        assert (d(x) - y).norm() <= bound, name
+
+
+@pytest.mark.parametrize('device', DEVICES)
+@pytest.mark.parametrize('nq', [1, 5, 24])
+def test_cross_gradients_of_unequal_rows(device, nq):
+    """Rows whose upstream gradients lie far apart: each row of dq is within
+    twice its own rounding."""
+    rand = Rand(nq, device, torch.float16)
+    b, h, hk, nk, dim = 2, 4, 2, 3000, 64
+    a = cross_inputs(rand, b, h, hk, nq, nk, dim)
+    size = torch.tensor([4.0, 0.25, 2.0**-6, 2.0**-10], device=device)
+    dout = rand(b, h, nq, dim) * size.view(1, 4, 1, 1).half()
+    got = gradients(a, None, dout)[1][0]
+    want = exact_cross(*a, None, dout)[1]
+    err = (d(got) - want).norm(dim=-1)
+    bound = 2 * (U[torch.float16] * want.norm(dim=-1) + 2.0**-25 *
+                 math.sqrt(dim))
+    assert (err <= bound).all()
+
+
+@pytest.mark.parametrize('device', DEVICES)
+@pytest.mark.parametrize('nq', [2, 10, 24])
+def test_cross_large_gradients(device, nq):
+    """Upstream gradients whose products with the values pass float16's
+    largest number, though no gradient does: within twice their rounding."""
+    rand = Rand(nq, device, torch.float16)
+    b, h, hk, nk, dim = 2, 2, 2, 6, 64
+    q, k, v, _ = cross_inputs(rand, b, h, hk, nq, nk, dim)
+    scale = torch.full((1, h, 1, 1), 0.01, device=device)
+    dout = rand(b, h, nq, dim, scale=10000.0)
+    got = gradients((q, k, 2 * v, scale), None, dout)
+    want = exact_cross(q, k, 2 * v, scale, None, dout)
+    for x, y, name in zip((got[0], *got[1][:3]), want,
+                          ('out', 'dq', 'dk', 'dv')):
+        assert y.abs().max() < 65504, name
+        assert off(x, y, torch.float16) <= 2, name
+
+
+@pytest.mark.parametrize('device', DEVICES)
+@pytest.mark.parametrize('nq', [3, 10, 40])
+def test_cross_float16_weights_far_below_one(device, nq):
+    """120,000 keys. Each weighs 2^-17: values' gradients are within twice
+    their rounding. And with one key beside the queries, the others weigh 2^-25
+    of it and still 0.36 % together."""
+    rand = Rand(nq, device, torch.float16)
+    b, h, hk, nk, dim = 1, 1, 1, 120000, 32
+    q = rand(b, h, 1, dim, scale=0.1).expand(b, h, nq, dim).contiguous()
+    k = q[:, :, :1] + rand(b, hk, nk, dim, scale=0.05)
+    v = 1 + rand(b, hk, nk, dim)
+    scale = torch.full((1, h, 1, 1), 0.5, device=device)
+    dout = rand(b, h, nq, dim, scale=32.0)
+    got = gradients((q, k, v, scale), None, dout)[1][2]
+    want = exact_cross(q, k, v, scale, None, dout)[3]
+    assert off(got, want, torch.float16) <= 2 + 2.0**-24 * math.sqrt(
+        want.numel()) / (U[torch.float16] * float(want.norm()))
+    # All but the first at a distance of 4 from the queries.
+    q = torch.zeros_like(q)
+    k = rand(b, hk, nk, dim)
+    k = (4 * k.float() / k.float().norm(dim=-1, keepdim=True)).half()
+    k[:, :, 0] = 0.0
+    v[:, :, 0] = 0.0
+    scale = torch.full((1, h, 1, 1), 25 * math.log(2) / 16, device=device)
+    out = block.cross_attention(q, k, v, scale)
+    want = exact_cross(q, k, v, scale, None, dout)[0]
+    # A distance is off by its products' rounding, 16 sums(32) at most.
+    slack = 2 * float(scale.max()) * 32 * sums(dim)
+    assert ((d(out) - want).abs() <= (2 * U[torch.float16] + slack) *
+            want.abs()).all()
 
 
 # ---------------------------------------------------------------------------

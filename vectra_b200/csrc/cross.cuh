@@ -14,6 +14,10 @@
 // Query heads that share a key head are rows of one problem: packed row
 // i G + g is query i of the g-th of the G heads. Their keys and values are
 // read once, and the gradients of shared heads are sums inside a block.
+// float16 operands: a product takes P and z as 16-bit numbers, and with
+// thousands of keys both lie below 2^-14, where float16 loses bits, while the
+// results, sums over keys or queries, do not. They are multiplied by powers of
+// two first, exactly, and the sums in float32 divided by them again.
 // Whatever a kernel does not finish itself (a long axis split over blocks) it
 // leaves in the workspace in float32, and the finish kernels join it in order.
 #pragma once
@@ -49,6 +53,9 @@ struct CrossProblem {
   const float* delta = nullptr;   // [B, H, Nq]: c_i
   float* dscale_rows = nullptr;   // [splits][B, H, Nq][3]
   const float* key_squares = nullptr;  // [B, Hk, Nk]: |k_j|^2, or not formed
+  // [B, Hk][2], float16 on the tensor cores: the largest 2 |g| |e_i| of a key
+  // head's queries and the largest |v_j| of its seen keys.
+  const float* bounds = nullptr;
   // A split axis: parts of it, and their float32 results.
   int32_t splits = 1;
   int64_t row_blocks = 1;    // blocks of one sequence's key head
@@ -78,6 +85,21 @@ __device__ __forceinline__ void store_with_rest(T* out, T* rest, float x) {
 __device__ __forceinline__ float cross_scale(const CrossProblem& p, int64_t b,
                                              int64_t h) {
   return load_any(p.scale, p.scale_dtype, b * p.ss[0] + h * p.ss[1]);
+}
+
+// What weights of float16 are multiplied by before a product with them, if
+// they are 1 at most (and a little more by rounding).
+constexpr float kLift = 0x1p14f;
+
+// A power of two that brings x >= 0 to [2^to, 2^(to + 1)), and 2^60 for what
+// is smaller than that could; its inverse is exact too.
+__device__ __forceinline__ float scale_up_to(float x, int to) {
+  const int exponent = int(__float_as_uint(x) >> 23 & 0xff) - 127;
+  const int k = min(to - exponent, 60);
+  return __uint_as_float(uint32_t(k + 127) << 23);
+}
+__device__ __forceinline__ float inverse_of(float power_of_two) {
+  return __uint_as_float((254u << 23) - __float_as_uint(power_of_two));
 }
 
 // Tiles [first, last) of `tiles` that part s of `splits` takes.
@@ -115,6 +137,9 @@ cudaError_t launch_cross_delta(const CrossProblem& p, float* delta,
 // cross_tc_supports allows).
 cudaError_t launch_cross_squares(const CrossProblem& p, float* squares,
                                  cudaStream_t stream);
+// p.bounds (16-byte pieces too): zeros, then the maxima.
+cudaError_t launch_cross_bounds(const CrossProblem& p, float* bounds,
+                                cudaStream_t stream);
 // out and lse from the parts.
 cudaError_t launch_cross_join(const CrossProblem& p, cudaStream_t stream);
 // `out` [B, H, N, width] from [splits][B, H, N][width].

@@ -57,7 +57,38 @@ __global__ void __launch_bounds__(256)
   }
 }
 
-// Sixteen lanes a key, 16-byte pieces (bf16 and f16).
+// The sum of squares of a vector, by sixteen neighbouring lanes of a warp, all
+// of which call it; `live`: there is one. 16-byte pieces.
+template <typename T>
+__device__ __forceinline__ float vector_square(const T* x, bool live,
+                                               int width) {
+  float t = 0.f;
+  if (live) {
+    for (int d = threadIdx.x % 16 * 8; d < width; d += 128) {
+      union {
+        uint4 u;
+        T e[8];
+      } y;
+      if (d + 8 <= width) {
+        y.u = __ldg(reinterpret_cast<const uint4*>(x + d));
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          y.e[j] = d + j < width ? x[d + j] : from_f32<T>(0.f);
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float v = to_f32(y.e[j]);
+        t = fmaf(v, v, t);
+      }
+    }
+  }
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+  return t;
+}
+
+// Sixteen lanes a key (bf16 and f16).
 template <typename T>
 __global__ void __launch_bounds__(256)
     squares_kernel(const __grid_constant__ CrossProblem p, float* squares) {
@@ -68,34 +99,62 @@ __global__ void __launch_bounds__(256)
   for (int64_t r0 = (int64_t(blockIdx.x) * 8 + threadIdx.x / 32) * 2; r0 < rows;
        r0 += int64_t(gridDim.x) * 16) {
     const int64_t r = r0 + threadIdx.x % 32 / 16;
+    const bool live = r < rows;
+    const int64_t bh = live ? r / p.Nk : 0, i = live ? r - bh * p.Nk : 0;
+    const int64_t b = bh / p.Hk, h = bh - b * p.Hk;
+    const float t = vector_square<T>(static_cast<const T*>(p.k) + b * p.sk[0] +
+                                         h * p.sk[1] + i * p.sk[2],
+                                     live, p.D);
+    if (lane == 0 && live) squares[r] = t;
+  }
+}
+
+// `parts` blocks a key head of a sequence, which take its seen values and then
+// its packed queries' gradients in turn. Maxima do not depend on the order.
+__global__ void __launch_bounds__(256)
+    bounds_kernel(const __grid_constant__ CrossProblem p, float* bounds,
+                  int parts) {
+  using T = __half;
+  __shared__ float tops[8][2];
+  allow_dependents();
+  grid_dependency_wait();
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int64_t plane = blockIdx.x / parts;
+  const int part = int(blockIdx.x - plane * parts);
+  const int64_t b = plane / p.Hk, hk = plane - b * p.Hk;
+  const int64_t len = cross_length(p, b), rows = len > 0 ? p.Nq * p.G : 0;
+  const int64_t first = (int64_t(part) * 8 + warp) * 2 + lane / 16;
+  const int64_t step = int64_t(parts) * 16;
+  float top[2] = {0.f, 0.f};
+  // The loops run to the warp's last row: the sums need every lane.
+  for (int64_t r = first; r - lane / 16 < len; r += step) {
+    const bool live = r < len;
+    const T* v = static_cast<const T*>(p.v) + b * p.sv[0] + hk * p.sv[1] +
+                 (live ? r : 0) * p.sv[2];
+    top[1] = fmaxf(top[1], sqrtf(vector_square<T>(v, live, p.Dv)));
+  }
+  for (int64_t r = first; r - lane / 16 < rows; r += step) {
+    const bool live = r < rows;
+    const int64_t i = live ? r / p.G : 0;
+    const int64_t h = hk * p.G + (live ? r - i * p.G : 0);
+    const T* e = static_cast<const T*>(p.dout) + b * p.se[0] + h * p.se[1] +
+                 i * p.se[2];
+    const float size = sqrtf(vector_square<T>(e, live, p.Dv));
+    top[0] = fmaxf(top[0], 2.f * fabsf(cross_scale(p, b, h)) * size);
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    top[i] = warp_max(top[i]);
+    if (lane == 0) tops[warp][i] = top[i];
+  }
+  __syncthreads();
+  if (threadIdx.x < 2) {
     float t = 0.f;
-    if (r < rows) {
-      const int64_t bh = r / p.Nk, i = r - bh * p.Nk;
-      const int64_t b = bh / p.Hk, h = bh - b * p.Hk;
-      const T* k = static_cast<const T*>(p.k) + b * p.sk[0] + h * p.sk[1] +
-                   i * p.sk[2];
-      for (int d = lane * 8; d < p.D; d += 128) {
-        union {
-          uint4 u;
-          T e[8];
-        } x;
-        if (d + 8 <= p.D) {
-          x.u = __ldg(reinterpret_cast<const uint4*>(k + d));
-        } else {
-#pragma unroll
-          for (int j = 0; j < 8; ++j)
-            x.e[j] = d + j < p.D ? k[d + j] : from_f32<T>(0.f);
-        }
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const float v = to_f32(x.e[j]);
-          t = fmaf(v, v, t);
-        }
-      }
-    }
-#pragma unroll
-    for (int o = 8; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
-    if (lane == 0 && r < rows) squares[r] = t;
+    for (int w = 0; w < 8; ++w) t = fmaxf(t, tops[w][threadIdx.x]);
+    // Floats that are not negative are ordered as their bits are.
+    atomicMax(reinterpret_cast<unsigned int*>(bounds + plane * 2) +
+                  threadIdx.x,
+              __float_as_uint(t));
   }
 }
 
@@ -280,6 +339,23 @@ cudaError_t launch_cross_squares(const CrossProblem& p, float* squares,
                       stream, p, squares);
   return launch_pdl(squares_kernel<__half>, grid, dim3(256), 0, stream, p,
                     squares);
+}
+
+cudaError_t launch_cross_bounds(const CrossProblem& p, float* bounds,
+                                cudaStream_t stream) {
+  const int64_t planes = p.B * p.Hk;
+  const cudaError_t e =
+      cudaMemsetAsync(bounds, 0, size_t(planes) * 2 * sizeof(float), stream);
+  if (e != cudaSuccess) return e;
+  // A block takes 64 rows or more of each kind.
+  const int64_t most = p.Nk > p.Nq * p.G ? p.Nk : p.Nq * p.G;
+  int64_t parts = int64_t(device_sm_count()) * 8 / planes;
+  if (parts > most / 64) parts = most / 64;
+  if (parts < 1) parts = 1;
+  if (planes * parts > 0x7fffffff) return cudaErrorInvalidValue;
+  count_launches(1);
+  return launch_pdl(bounds_kernel, dim3(unsigned(planes * parts)), dim3(256),
+                    0, stream, p, bounds, int(parts));
 }
 
 cudaError_t launch_cross_join(const CrossProblem& p, cudaStream_t stream) {

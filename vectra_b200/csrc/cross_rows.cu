@@ -22,6 +22,9 @@
 //   S = q k^T, T = e v^T            operands as loaded
 //   out += P v, dq += z k           v and k turned
 //   dv = P^T e, dk = z^T q          P, z (and, once, e and q) turned
+// float16 (cross.cuh): forward weights are multiplied by 2^14, P of dv too; z
+// of dk by what its step's largest needs, z of dq by what its row's largest so
+// far does, and dq's sums are brought along when that grows.
 // Sums of z over keys and rows are products with ones, of the rounded values
 // that the other products take. What P's rounding leaves is multiplied as well
 // in the forward pass, as on the tensor cores (cross_tc.cu, KEEP): the time
@@ -59,6 +62,12 @@ __device__ __forceinline__ float2 pair(uint32_t w) {
     return __half22float2(*reinterpret_cast<const __half2*>(&w));
   }
 }
+
+// log2 of what forward weights, 1 at most, are multiplied by, and that of P.
+template <typename T>
+constexpr float kLog2Lift = std::is_same<T, __half>::value ? 14.f : 0.f;
+template <typename T>
+constexpr float kLiftOf = std::is_same<T, __half>::value ? kLift : 1.f;
 
 // One of T in both halves.
 template <typename T>
@@ -300,7 +309,7 @@ __global__ void __launch_bounds__(kWarps * 32)
           acc[n][2 * r + 1] *= f;
         }
       }
-      const float ref = m[r] == kNegInf ? 0.f : m[r];
+      const float ref = m[r] == kNegInf ? 0.f : m[r] - kLog2Lift<T>;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         x[i] = fast_exp2(x[i] - ref);
@@ -330,6 +339,7 @@ __global__ void __launch_bounds__(kWarps * 32)
 #pragma unroll
   for (int r = 0; r < NR; ++r) {
     l[r] = quad_sum(l[r]);
+    m[r] -= kLog2Lift<T>;
     if (!row[r].live) continue;
     const int64_t k_part = part * rows + row[r].at;
     const bool whole = p.splits == 1;
@@ -484,8 +494,8 @@ __global__ void __launch_bounds__(kWarps * 32)
     for (int h = 0; h < 2; ++h)
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        x[2 * h + c] =
-            fast_exp2(x[2 * h + c] - (m[c] == kNegInf ? 0.f : m[c]));
+        const float ref = m[c] == kNegInf ? 0.f : m[c] - kLog2Lift<T>;
+        x[2 * h + c] = fast_exp2(x[2 * h + c] - ref);
         l[c] += x[2 * h + c];
       }
     uint32_t hi[2], lo[2];
@@ -521,6 +531,7 @@ __global__ void __launch_bounds__(kWarps * 32)
     for (int o = 4; o < 32; o *= 2)
       l[c] += __shfl_xor_sync(0xffffffffu, l[c], o);
     inv[c] = whole ? (len > 0 ? 1.f / l[c] : 0.f) : 1.f;
+    m[c] -= kLog2Lift<T>;
     const Row r = packed_row(p, b, hk, 2 * t + c);
     if (g != 0 || !r.live) continue;
     if (!whole) {
@@ -580,6 +591,7 @@ template <typename T, int NB, int NR>
 __global__ void __launch_bounds__(kWarps * 32, NB > 2 ? 2 : 3)
     rows_backward_kernel(const __grid_constant__ CrossProblem p) {
   constexpr bool kShared = kTurnedInShared<NB>;
+  constexpr bool kScaled = std::is_same<T, __half>::value;
   constexpr int STAGES = kBackwardStages<NB>;
   extern __shared__ uint4 ring_memory[];
   // Behind the ring.
@@ -662,8 +674,12 @@ __global__ void __launch_bounds__(kWarps * 32, NB > 2 ? 2 : 3)
 #pragma unroll
     for (int i = 0; i < 4; ++i) dq[n][i] = 0.f;
   float xs[NR], ys[NR], zx[NR];
+  float up[NR];  // float16: what z of dq is multiplied by
 #pragma unroll
-  for (int r = 0; r < NR; ++r) xs[r] = ys[r] = zx[r] = 0.f;
+  for (int r = 0; r < NR; ++r) {
+    xs[r] = ys[r] = zx[r] = 0.f;
+    up[r] = kScaled ? scale_up_to(0.f, 0) : 1.f;
+  }
 
   Ring<T, NB, STAGES> ring{ring_memory + threadIdx.x};
   const int t_seen = min(t1, (len + kKeys - 1) / kKeys);
@@ -717,28 +733,65 @@ __global__ void __launch_bounds__(kWarps * 32, NB > 2 ? 2 : 3)
     uint32_t pw[4] = {0, 0, 0, 0}, zw[4] = {0, 0, 0, 0}, zk[4] = {0, 0, 0, 0};
     uint32_t zl[4] = {0, 0, 0, 0};
     const int first = step * kKeys + 2 * t;
+    float z[NR][2][2];
 #pragma unroll
     for (int r = 0; r < NR; ++r)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        float w[2], z[2];
+        float w[2];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           const float a = fmaf(2.f, s[h][2 * r + i], i ? -nk[h].y : -nk[h].x);
           const bool in = first + 8 * h + i < len;
           w[i] = in ? fast_exp2(fmaf(gl[r], a, -lse[r])) : 0.f;
-          z[i] = in ? w[i] * (u[h][2 * r + i] - ci[r]) : 0.f;
+          z[r][h][i] = in ? w[i] * (u[h][2 * r + i] - ci[r]) : 0.f;
           if (in) {
-            xs[r] = fmaf(z[i], a, xs[r]);
+            xs[r] = fmaf(z[r][h][i], a, xs[r]);
             ys[r] = fmaf(w[i], a, ys[r]);
-            zx[r] += z[i];
+            zx[r] += z[r][h][i];
           }
         }
-        pw[2 * h + r] = pack_pair<T>(w[0], w[1]);
-        zw[2 * h + r] = pack_pair<T>(z[0], z[1]);
+        pw[2 * h + r] =
+            pack_pair<T>(w[0] * kLiftOf<T>, w[1] * kLiftOf<T>);
+      }
+    float up_k = 1.f;  // what z of dk is multiplied by
+    if constexpr (kScaled) {
+      float all = 0.f;
+#pragma unroll
+      for (int r = 0; r < NR; ++r) {
+        const float top = quad_max(
+            fmaxf(fmaxf(fabsf(z[r][0][0]), fabsf(z[r][0][1])),
+                  fmaxf(fabsf(z[r][1][0]), fabsf(z[r][1][1]))));
+        all = fmaxf(all, fabsf(g2[r]) * top);
+        // To 2^10, until one reaches 2^14.
+        const bool grows = top * up[r] > 0x1p14f;
+        if (__any_sync(0xffffffffu, grows)) {
+          const float next = grows ? scale_up_to(top, 10) : up[r];
+          const float f = next * inverse_of(up[r]);
+          up[r] = next;
+#pragma unroll
+          for (int n = 0; n < NB * 4; ++n) {
+            dq[n][2 * r] *= f;
+            dq[n][2 * r + 1] *= f;
+          }
+        }
+      }
+#pragma unroll
+      for (int o = 4; o < 32; o *= 2)
+        all = fmaxf(all, __shfl_xor_sync(0xffffffffu, all, o));
+      up_k = scale_up_to(all, 13);
+    }
+    const float down_k = inverse_of(up_k);
+#pragma unroll
+    for (int r = 0; r < NR; ++r)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const float z0 = z[r][h][0] * up[r], z1 = z[r][h][1] * up[r];
+        zw[2 * h + r] = pack_pair<T>(z0, z1);
         const float2 near = pair<T>(zw[2 * h + r]);
-        zl[2 * h + r] = pack_pair<T>(z[0] - near.x, z[1] - near.y);
-        zk[2 * h + r] = pack_pair<T>(g2[r] * z[0], g2[r] * z[1]);
+        zl[2 * h + r] = pack_pair<T>(z0 - near.x, z1 - near.y);
+        zk[2 * h + r] = pack_pair<T>(g2[r] * z[r][h][0] * up_k,
+                                     g2[r] * z[r][h][1] * up_k);
       }
     // dq += z k.
 #pragma unroll
@@ -796,9 +849,10 @@ __global__ void __launch_bounds__(kWarps * 32, NB > 2 ? 2 : 3)
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
           const float2 f = pair<T>(k[h][n][w]);  // 0 where not seen
-          x[w] = pack_pair<T>(a[w][2 * h] - f.x * ksum[2 * h],
-                              a[w][2 * h + 1] - f.y * ksum[2 * h]);
-          y[w] = pack_pair<T>(c[w][2 * h], c[w][2 * h + 1]);
+          x[w] = pack_pair<T>((a[w][2 * h] - f.x * ksum[2 * h]) * down_k,
+                              (a[w][2 * h + 1] - f.y * ksum[2 * h]) * down_k);
+          y[w] = pack_pair<T>(c[w][2 * h] * (1.f / kLiftOf<T>),
+                              c[w][2 * h + 1] * (1.f / kLiftOf<T>));
         }
         if (d < p.D)
           *reinterpret_cast<uint4*>(dk[h] + d) =
@@ -826,6 +880,7 @@ __global__ void __launch_bounds__(kWarps * 32, NB > 2 ? 2 : 3)
     }
     if (!p.dq) continue;
     T* out = row_of<T>(p.dq, p.sdq, b, row[r].h, row[r].i);
+    const float down = inverse_of(up[r]);
 #pragma unroll
     for (int n = 0; n < NB; ++n) {
       const int d = n * 32 + t * 8;
@@ -834,9 +889,9 @@ __global__ void __launch_bounds__(kWarps * 32, NB > 2 ? 2 : 3)
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
         const float2 f = pair<T>(q[r][n][w]);
-        const float a0 = g2[r] * (dq[n * 4 + w][2 * r] - f.x * zx[r]);
+        const float a0 = g2[r] * (dq[n * 4 + w][2 * r] * down - f.x * zx[r]);
         const float a1 =
-            g2[r] * (dq[n * 4 + w][2 * r + 1] - f.y * zx[r]);
+            g2[r] * (dq[n * 4 + w][2 * r + 1] * down - f.y * zx[r]);
         if (p.splits > 1)
           *reinterpret_cast<float2*>(p.part + k_part * p.D + d + 2 * w) =
               make_float2(a0, a1);

@@ -37,6 +37,11 @@
 // the same with z, whose errors meet the same distances. bf16, of dq: 3.2e-3
 // without both, 2.8e-3 without the second, 1.7e-3 (its own rounding) with them.
 //
+// float16 (cross.cuh): forward weights, at most 2^8, are multiplied by 2^7, P
+// of dv by 2^14, z of dq by what a bound of its row needs and z of dk by what
+// that of its key head does: |z_ij| <= P_ij |e_i| (|v_j| + |out_i|), at most
+// 2 |e_i| max |v_j|.
+//
 // Measured: 4,096 queries of 32 heads on 5,003 keys of 8 heads of 128, f16:
 // 395 us, 850 TFLOP/s; bound by the latency of the row warps, two a scheduler
 // (tensor pipe 41 %, issue 35 %). Training of 2,048 queries of 16 heads on up to
@@ -62,6 +67,9 @@ constexpr int kMmaWarp = 9;
 constexpr int kTermWarp = 12;
 constexpr int kTermThreads = 128;
 constexpr float kRescaleThreshold = 8.f;  // log2 of the lazy-rescale factor
+// log2 of what forward weights, at most 2^8, are multiplied by.
+template <typename T>
+constexpr float kLog2Lift = std::is_same<T, __half>::value ? 7.f : 0.f;
 // Registers after the launch's equal share: the warpgroups that hold a row of
 // a tile, and the others (checked against the launch's total on the host).
 constexpr int kRowRegs = 200;
@@ -253,6 +261,7 @@ __device__ __forceinline__ void cross_pass(const CUtensorMap& tr,
                                            int part, uint8_t* smem_raw) {
   using C = Cfg<W, PASS>;
   constexpr bool kBack = C::kBack;
+  constexpr bool kScaled = std::is_same<T, __half>::value;
   constexpr bool kRowsAreQueries = PASS != kKeys;
   constexpr int CN = C::CN, NS = C::NS;
   constexpr int FMT = std::is_same<T, __nv_bfloat16>::value ? 1 : 0;
@@ -290,6 +299,12 @@ __device__ __forceinline__ void cross_pass(const CUtensorMap& tr,
     split_range(tiles, part, p.splits, &t0, &t1);
   }
   const int n = t1 - t0;
+  // What z of dk is multiplied by.
+  float up_k = 1.f;
+  if (kScaled && PASS == kKeys && n > 0)
+    up_k = scale_up_to(
+        __ldg(p.bounds + 2 * plane) * (2.f * __ldg(p.bounds + 2 * plane + 1)),
+        13);
 
   // This thread's row, and its place among the results' rows.
   const int r = threadIdx.x & 127;
@@ -508,10 +523,11 @@ __device__ __forceinline__ void cross_pass(const CUtensorMap& tr,
               ci = __ldg(p.delta + q);
               g = cross_scale(p, b, h);
             }
-            out[th] = -lse;
+            // P is formed times kLift, z times up_k.
+            out[th] = kScaled ? 14.f - lse : -lse;
             out[CN + th] = -ci;
             out[2 * CN + th] = g * kLog2e;
-            out[3 * CN + th] = 2.f * g;
+            out[3 * CN + th] = kScaled ? 2.f * g * (up_k / kLift) : 2.f * g;
           }
         }
         __syncwarp();
@@ -615,7 +631,7 @@ __device__ __forceinline__ void cross_pass(const CUtensorMap& tr,
               tmem_st32(o_col + c * 32, f);
             }
           }
-          const float ref = m_used == kNegInf ? 0.f : m_used;
+          const float ref = m_used == kNegInf ? 0.f : m_used - kLog2Lift<T>;
           const uint64_t neg = both(-ref);
           const uint64_t minus = both(-1.f);
           uint64_t sa = 0, sb = 0;
@@ -658,7 +674,7 @@ __device__ __forceinline__ void cross_pass(const CUtensorMap& tr,
       // The warpgroups' maxima and sums, through the row operand's memory
       // (every product has read it by now).
       float2* join = reinterpret_cast<float2*>(smem + C::OFF_R);
-      join[x * kRows + r] = make_float2(m_used, l);
+      join[x * kRows + r] = make_float2(m_used - kLog2Lift<T>, l);
       sync_rows();
       const float2 j0 = join[r], j1 = join[kRows + r];
       const float m = fmaxf(j0.x, j1.x);
@@ -718,8 +734,16 @@ __device__ __forceinline__ void cross_pass(const CUtensorMap& tr,
       ok = __all_sync(0xffffffffu, ok);
       if (!kRowsAreQueries && ok)
         nkr = -row_square<T, 8 * C::KB>(smem + C::OFF_R, C::RBLOCK, r, 0);
+      // What z of dq is multiplied by.
+      float up = 1.f;
+      if (kScaled && kRowsAreQueries && ok)
+        up = scale_up_to(
+            sqrtf(row_square<T, 8 * C::KB>(smem + C::OFF_R + C::RTILE,
+                                           C::RBLOCK, r, 0)) *
+                (2.f * __ldg(p.bounds + 2 * plane + 1)),
+            13);
       const uint64_t nkr2 = both(nkr), gl2 = both(gl), lse2 = both(-lse),
-                     ci2 = both(-ci);
+                     ci2 = both(-ci * up), up2 = both(up);
       // Sums of z, rounded where its product takes no more; for dscale.
       uint64_t zs = 0, xs = 0, ys = 0;
       static_assert(!kBack || HALF == 32, "a tile is read before z is written");
@@ -751,8 +775,10 @@ __device__ __forceinline__ void cross_pass(const CUtensorMap& tr,
                 u2[1] = ffma2(two, bits2(sv + j + 2), f2pk(n4.z, n4.w));
                 lg[0] = ffma2(gl2, u2[0], lse2);
                 lg[1] = ffma2(gl2, u2[1], lse2);
-                zc[0] = fadd2(bits2(tv + j), ci2);
-                zc[1] = fadd2(bits2(tv + j + 2), ci2);
+                zc[0] = kScaled ? ffma2(bits2(tv + j), up2, ci2)
+                                : fadd2(bits2(tv + j), ci2);
+                zc[1] = kScaled ? ffma2(bits2(tv + j + 2), up2, ci2)
+                                : fadd2(bits2(tv + j + 2), ci2);
               } else {
                 const float4 l4 =
                     *reinterpret_cast<const float4*>(col + c + j);
@@ -821,18 +847,19 @@ __device__ __forceinline__ void cross_pass(const CUtensorMap& tr,
       sync_rows();
       const float4 j0 = join[r], j1 = join[kRows + r];
       const float z_sum = j0.x + j1.x;
+      const float down = inverse_of(PASS == kKeys ? up_k : up);
       if (ok && warp_live) {
         if (want_scale && row_live && x == 0) {
           // Minus: the finish kernel takes sums of distances, and u is
           // |q|^2 less one.
           float* w = p.dscale_rows + (part * all_rows + at) * 3;
-          w[0] = -(j0.y + j1.y);
+          w[0] = -(j0.y + j1.y) * down;
           w[1] = -(j0.z + j1.z);
-          w[2] = z_sum;
+          w[2] = z_sum * down;
         }
         // acc less the row's own vector times its sum: dq by columns between
         // the warpgroups; of the keys' two results one each.
-        const float g = kRowsAreQueries ? 2.f * scale : 1.f;
+        const float g = (kRowsAreQueries ? 2.f * scale : 1.f) * down;
         const bool live = kRowsAreQueries ? row_live : key < len;
         const bool second = PASS == kKeys && x == 1;
         const int width = second ? p.Dv : p.D;
@@ -871,6 +898,10 @@ __device__ __forceinline__ void cross_pass(const CUtensorMap& tr,
                   v[2 * i] = g * (v[2 * i] - f.x * z_sum);
                   v[2 * i + 1] = g * (v[2 * i + 1] - f.y * z_sum);
                 }
+              }
+              if (kScaled && second) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[i] *= 1.f / kLift;
               }
               if (!live) {
 #pragma unroll
@@ -1183,6 +1214,9 @@ cudaError_t run_cross_tc_backward(const CrossProblem& problem, Workspace& ws,
                        ? take_floats(ws, p.B * p.Hk * p.Nk)
                        : nullptr;
   p.key_squares = squares;
+  float* bounds =
+      p.dtype == VECTRA_F16 ? take_floats(ws, p.B * p.Hk * 2) : nullptr;
+  p.bounds = bounds;
   CrossProblem pq = p, pk = p;
   const bool want_q = p.dq || p.dscale;
   if (want_q) {
@@ -1202,6 +1236,7 @@ cudaError_t run_cross_tc_backward(const CrossProblem& problem, Workspace& ws,
   cudaError_t e = launch_cross_delta(p, delta, stream);
   if (e == cudaSuccess && squares)
     e = launch_cross_squares(p, squares, stream);
+  if (e == cudaSuccess && bounds) e = launch_cross_bounds(p, bounds, stream);
   if (e == cudaSuccess)
     e = with_width(p, [&](auto* t, auto width) {
       return launch_backward<std::remove_pointer_t<decltype(t)>,

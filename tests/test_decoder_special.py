@@ -26,6 +26,7 @@ from tests.test_decoder import Rand
 from tests.test_decoder import _abi
 from tests.test_decoder import _Drop
 from tests.test_decoder import _NormArgs
+from tests.test_decoder import check_cross
 from tests.test_decoder import cross_inputs
 from tests.test_decoder import d
 from tests.test_decoder import sums
@@ -220,6 +221,121 @@ def test_cross_float16_weights_far_below_one(device, nq):
     slack = 2 * float(scale.max()) * 32 * sums(dim)
     assert ((d(out) - want).abs() <= (2 * U[torch.float16] + slack) *
             want.abs()).all()
+
+
+# ---------------------------------------------------------------------------
+# cross_attention: one rounding a result.
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize('device', DEVICES)
+@pytest.mark.parametrize('dtype', HALVES)
+@pytest.mark.parametrize('size', [(4, 4, 4, 1, 300, 64),
+                                  (2, 8, 2, 3, 300, 128),
+                                  (1, 4, 2, 150, 500, 128),
+                                  (2, 2, 2, 200, 300, 32)])
+def test_cross_results_are_rounded_once(device, dtype, size):
+    """Weights and their gradients enter the products with what their
+    rounding left: results and gradients are off by their own rounding, and a
+    call that will have no backward pass gives the same bits."""
+    b, h, hk, nq, nk, dim = size
+    rand = Rand(nk + dim, device, dtype)
+    a = cross_inputs(rand, *size)
+    dout = rand(b, h, nq, dim)
+    out, grads = gradients(a, None, dout)
+    assert torch.equal(out, block.cross_attention(*a))
+    want = exact_cross(*a, None, dout)
+    for got, y, name in zip((out, *grads[:3]), want,
+                            ('out', 'dq', 'dk', 'dv')):
+        assert off(got, y, dtype) <= ONCE, name
+
+
+# ---------------------------------------------------------------------------
+# cross_attention: long walks, split axes, few keys.
+# ---------------------------------------------------------------------------
+def check_long(a, lengths, dout):
+    """check_cross for sizes whose differences of all queries and keys would
+    not fit: |q - k| is at most |q| + |k| where it weighs an error. Training
+    keeps what the rounding of weights left."""
+    q, k, v, scale = a
+    dtype, dim, dv_ = q.dtype, q.shape[3], v.shape[3]
+    b, h, nq = q.shape[:3]
+    hk, nk = k.shape[1:3]
+    rep, u, tiny = h // hk, U[dtype], TINY[dtype]
+    out, (dq, dk, dv, _) = gradients(a, lengths, dout)
+    want = exact_cross(*a, lengths, dout)
+    n = torch.full((b,), nk) if lengths is None else lengths.cpu()
+    bounds = [torch.zeros_like(t) for t in want]
+    for i in range(b):
+        m = int(n[i])
+        for j in range(h):
+            x, y, z = d(q[i, j]), d(k[i, j // rep, :m]), d(v[i, j // rep, :m])
+            e, g = d(dout[i, j]), float(d(scale).expand(b, h, 1, 1)[i, j])
+            size = x.square().sum(-1, keepdim=True) + y.square().sum(-1) + \
+                2 * x.abs() @ y.abs().mT
+            dist = x.square().sum(-1, keepdim=True) + y.square().sum(-1) - \
+                2 * x @ y.mT
+            w = torch.softmax(-g * dist, -1)
+            ew = torch.expm1(2 * (abs(g) * (sums(dim) + 2.0**-21) *
+                                  size).amax(-1, keepdim=True) + sums(m))
+            keep = 3 * u * u + sums(max(m, nq * rep))
+            eo = (w * (ew + keep)) @ z.abs()
+            bounds[0][i, j] = eo
+            o = want[0][i, j]
+            ec = (e.abs() * (eo + 3 * u * u * o.abs() + tiny)).sum(
+                -1, keepdim=True) + sums(dv_) * (e * o).abs().sum(
+                    -1, keepdim=True)
+            t = (e @ z.mT - (e * o).sum(-1, keepdim=True)).abs()
+            et = sums(dv_) * (e.abs() @ z.abs().mT)
+            ez = 2 * abs(g) * w * ((ew + keep) * (t + et + ec) + et + ec)
+            bounds[1][i, j] = ez.sum(-1, keepdim=True) * x.abs() + \
+                ez @ y.abs()
+            bounds[2][i, j // rep, :m] += ez.mT @ x.abs() + \
+                ez.sum(0)[:, None] * y.abs()
+            bounds[3][i, j // rep, :m] += (w * (ew + keep)).mT @ e.abs()
+    for got, y, bound, name in zip((out, dq, dk, dv), want, bounds,
+                                   ('out', 'dq', 'dk', 'dv')):
+        err = (d(got) - y).abs()
+        limit = bound * (1 + u) + u * y.abs() + tiny
+        assert (err <= limit).all(), (name, float((err / limit).max()))
+
+
+# By the 16-bit kernels' rules for more than 16 packed queries: keys that are
+# split in the forward and the queries' pass (8 tiles of 128 and of 64 or
+# more); queries that are split in the keys' pass; and enough blocks that
+# nothing splits, with rings of up to four tiles that wrap twice, of keys and of
+# queries.
+LONG = [(1, 2, 1, 40, 1100, 64), (1, 2, 1, 40, 1030, 128),
+        (1, 2, 1, 300, 200, 64), (1, 2, 1, 300, 190, 128),
+        (3, 6, 2, 170, 1000, 64),
+        (5, 16, 16, 20, 1290, 64), (5, 16, 16, 20, 1290, 128),
+        (5, 16, 16, 600, 70, 64), (5, 16, 16, 600, 70, 128)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', HALVES)
+@pytest.mark.parametrize('size', LONG)
+@pytest.mark.parametrize('ragged', [False, True])
+def test_cross_long_walks(dtype, size, ragged):
+    b, h, hk, nq, nk, dim = size
+    rand = Rand(nk + dim, 'cuda', dtype)
+    a = cross_inputs(rand, *size)
+    lengths = None
+    if ragged:
+        some = [nk - 1, nk // 2 + 1, nk, 1, 64]
+        lengths = torch.tensor(some[:b], device='cuda')
+    check_long(a, lengths, rand(b, h, nq, dim))
+
+
+@pytest.mark.parametrize('device', DEVICES)
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('size', [(2, 4, 2, 3, 64), (1, 6, 1, 2, 128),
+                                  (2, 2, 1, 30, 64), (1, 1, 1, 150, 128),
+                                  (1, 2, 2, 40, 33), (1, 2, 1, 20, 160)])
+@pytest.mark.parametrize('nk', [2, 3])
+def test_cross_two_and_three_keys(device, dtype, size, nk):
+    b, h, hk, nq, dim = size
+    rand = Rand(nk + dim, device, dtype)
+    check_cross(*cross_inputs(rand, b, h, hk, nq, nk, dim),
+                dout=rand(b, h, nq, dim))
 
 
 # ---------------------------------------------------------------------------

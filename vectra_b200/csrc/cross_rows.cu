@@ -25,10 +25,9 @@
 // float16 (cross.cuh): forward weights are multiplied by 2^14, P of dv too; z
 // of dk by what its step's largest needs, z of dq by what its row's largest so
 // far does, and dq's sums are brought along when that grows.
-// Sums of z over keys and rows are products with ones, of the rounded values
-// that the other products take. What P's rounding leaves is multiplied as well
-// in the forward pass, as on the tensor cores (cross_tc.cu, KEEP): the time
-// goes to memory.
+// What the rounding of P and z to an operand leaves is multiplied as well, as on
+// the tensor cores (cross_tc.cu): the time goes to memory. z's sums over rows
+// are products with ones.
 //
 // Measured against tcgen05 tiles, which are 128 rows high: one query of 32
 // heads on up to 4,001 keys of 8 heads of 128, 32 sequences: 67 us (61 of them
@@ -73,6 +72,15 @@ constexpr float kLiftOf = std::is_same<T, __half>::value ? kLift : 1.f;
 template <typename T>
 __device__ __forceinline__ uint32_t ones() {
   return pack_pair<T>(1.f, 1.f);
+}
+
+// Two values as a pair of T, and what rounding left.
+template <typename T>
+__device__ __forceinline__ void split_pair(float x, float y, uint32_t* near,
+                                           uint32_t* rest) {
+  *near = pack_pair<T>(x, y);
+  const float2 f = pair<T>(*near);
+  *rest = pack_pair<T>(x - f.x, y - f.y);
 }
 
 // Sum over the four threads of a quad.
@@ -385,10 +393,9 @@ __global__ void __launch_bounds__(kWarps * 32)
 // components of out, their 16 rows, which takes half as many instructions on
 // the tensor cores (whose warp-level form set the pace of a decoding step: 48 a
 // step of 16 keys of 128 with the rows as rows, 79 us for 32 sequences over up
-// to 4,001 keys; REST false, without a backward pass to come, leaves out the
-// products with what P's rounding left).
+// to 4,001 keys).
 //   S^T = k q^T, out^T += v^T P^T
-template <typename T, int NB, bool REST>
+template <typename T, int NB>
 __global__ void __launch_bounds__(kWarps * 32)
     few_rows_forward_kernel(const __grid_constant__ CrossProblem p) {
   allow_dependents();
@@ -503,10 +510,8 @@ __global__ void __launch_bounds__(kWarps * 32)
     for (int h = 0; h < 2; ++h) {
       const uint32_t w = pack_pair<T>(x[2 * h], x[2 * h + 1]);
       hi[h] = turn(w);
-      if constexpr (REST) {
-        const float2 f = pair<T>(w);
-        lo[h] = turn(pack_pair<T>(x[2 * h] - f.x, x[2 * h + 1] - f.y));
-      }
+      const float2 f = pair<T>(w);
+      lo[h] = turn(pack_pair<T>(x[2 * h] - f.x, x[2 * h + 1] - f.y));
     }
     uint32_t v[2][NB][4];
     ring.read(step, 1, 0, v[0]);
@@ -518,7 +523,7 @@ __global__ void __launch_bounds__(kWarps * 32)
         const uint32_t f[4] = {turn(v[0][n][w]), turn(v[0][n][w + 1]),
                                turn(v[1][n][w]), turn(v[1][n][w + 1])};
         mma16816<T>(acc[n * 2 + w / 2], f, hi[0], hi[1]);
-        if constexpr (REST) mma16816<T>(acc[n * 2 + w / 2], f, lo[0], lo[1]);
+        mma16816<T>(acc[n * 2 + w / 2], f, lo[0], lo[1]);
       }
   }
 
@@ -728,10 +733,10 @@ __global__ void __launch_bounds__(kWarps * 32, NB > 2 ? 2 : 3)
       inner<T, NB, NR>(u[h], e, v);
       nk[h] = squares<T, NB>(k[h], lane);
     }
-    // P and z of the 16 keys; z for dk has its row's scale before rounding.
-    // What z's rounding leaves enters dq as well (cross_tc.cu).
+    // P and z of the 16 keys, and what rounding left of them; z for dk has its
+    // row's scale before rounding.
     uint32_t pw[4] = {0, 0, 0, 0}, zw[4] = {0, 0, 0, 0}, zk[4] = {0, 0, 0, 0};
-    uint32_t zl[4] = {0, 0, 0, 0};
+    uint32_t pl[4] = {0, 0, 0, 0}, zl[4] = {0, 0, 0, 0}, kl[4] = {0, 0, 0, 0};
     const int first = step * kKeys + 2 * t;
     float z[NR][2][2];
 #pragma unroll
@@ -751,8 +756,8 @@ __global__ void __launch_bounds__(kWarps * 32, NB > 2 ? 2 : 3)
             zx[r] += z[r][h][i];
           }
         }
-        pw[2 * h + r] =
-            pack_pair<T>(w[0] * kLiftOf<T>, w[1] * kLiftOf<T>);
+        split_pair<T>(w[0] * kLiftOf<T>, w[1] * kLiftOf<T>, &pw[2 * h + r],
+                      &pl[2 * h + r]);
       }
     float up_k = 1.f;  // what z of dk is multiplied by
     if constexpr (kScaled) {
@@ -786,12 +791,10 @@ __global__ void __launch_bounds__(kWarps * 32, NB > 2 ? 2 : 3)
     for (int r = 0; r < NR; ++r)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const float z0 = z[r][h][0] * up[r], z1 = z[r][h][1] * up[r];
-        zw[2 * h + r] = pack_pair<T>(z0, z1);
-        const float2 near = pair<T>(zw[2 * h + r]);
-        zl[2 * h + r] = pack_pair<T>(z0 - near.x, z1 - near.y);
-        zk[2 * h + r] = pack_pair<T>(g2[r] * z[r][h][0] * up_k,
-                                     g2[r] * z[r][h][1] * up_k);
+        split_pair<T>(z[r][h][0] * up[r], z[r][h][1] * up[r], &zw[2 * h + r],
+                      &zl[2 * h + r]);
+        split_pair<T>(g2[r] * z[r][h][0] * up_k, g2[r] * z[r][h][1] * up_k,
+                      &zk[2 * h + r], &kl[2 * h + r]);
       }
     // dq += z k.
 #pragma unroll
@@ -809,8 +812,13 @@ __global__ void __launch_bounds__(kWarps * 32, NB > 2 ? 2 : 3)
                             turn(pw[3])};
     const uint32_t zt[4] = {turn(zk[0]), turn(zk[2]), turn(zk[1]),
                             turn(zk[3])};
+    const uint32_t ptl[4] = {turn(pl[0]), turn(pl[2]), turn(pl[1]),
+                             turn(pl[3])};
+    const uint32_t ztl[4] = {turn(kl[0]), turn(kl[2]), turn(kl[1]),
+                             turn(kl[3])};
     float ksum[4] = {0.f, 0.f, 0.f, 0.f};
     mma16816<T>(ksum, zt, ones<T>(), ones<T>());
+    mma16816<T>(ksum, ztl, ones<T>(), ones<T>());
 #pragma unroll
     for (int n = 0; n < NB; ++n) {
       uint32_t qb[2][4], eb[2][4];
@@ -839,7 +847,9 @@ __global__ void __launch_bounds__(kWarps * 32, NB > 2 ? 2 : 3)
 #pragma unroll
         for (int i = 0; i < 4; ++i) a[w][i] = c[w][i] = 0.f;
         mma16816<T>(a[w], zt, qb[0][w], qb[1][w]);
+        mma16816<T>(a[w], ztl, qb[0][w], qb[1][w]);
         mma16816<T>(c[w], pt, eb[0][w], eb[1][w]);
+        mma16816<T>(c[w], ptl, eb[0][w], eb[1][w]);
       }
       const int d = n * 32 + t * 8;
 #pragma unroll
@@ -985,8 +995,7 @@ cudaError_t run_cross_rows_forward(const CrossProblem& problem, Workspace& ws,
     constexpr int bytes = Ring<T, NB, kForwardStages<NB>>::BYTES;
     auto kern = rows_forward_kernel<T, NB, 2>;
     if (decltype(nr)::value == 1)
-      kern = p.lse ? few_rows_forward_kernel<T, NB, true>
-                   : few_rows_forward_kernel<T, NB, false>;
+      kern = few_rows_forward_kernel<T, NB>;
     const cudaError_t st = cudaFuncSetAttribute(
         kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
     if (st != cudaSuccess) return st;

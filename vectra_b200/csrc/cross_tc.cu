@@ -30,12 +30,11 @@
 // zeros in shared memory, so that what they held (NaN included) meets no
 // weight.
 //
-// Rounding, beside each result's: P and z enter their products in 16 bits. For
-// a backward pass the forward one multiplies what P's rounding left as well
-// (KEEP): c_i of a result that is off by 2^-9 of its weights would put 2^-9 of
-// the distance between q_i and the mean key into dq. The queries' pass does
-// the same with z, whose errors meet the same distances. bf16, of dq: 3.2e-3
-// without both, 2.8e-3 without the second, 1.7e-3 (its own rounding) with them.
+// P and z enter their products as two 16-bit numbers, the second what the
+// first's rounding left, so that each result is off by its own rounding (bf16
+// 1.7e-3) alone. With the first numbers only it were 1.8e-3 of out, 2.35e-3 of
+// dk and dv, and 3.2e-3 of dq, whose errors meet the distances between q_i and
+// the keys, c_i's too.
 //
 // float16 (cross.cuh): forward weights, at most 2^8, are multiplied by 2^7, P
 // of dv by 2^14, z of dq by what a bound of its row needs and z of dk by what
@@ -185,6 +184,13 @@ __device__ __forceinline__ uint64_t unpack2(uint32_t w) {
   }
 }
 
+// What rounding the pair v to `rounded` left, rounded itself.
+template <typename T>
+__device__ __forceinline__ uint32_t rest_of(uint32_t rounded, uint64_t v) {
+  const float2 f = f2upk(ffma2(unpack2<T>(rounded), both(-1.f), v));
+  return pack2<T>(f.x, f.y);
+}
+
 // Row r's vector in a 128-byte swizzled tile whose pieces are `block` bytes
 // apart: 16-byte chunk c of piece kb.
 __device__ __forceinline__ uint32_t chunk_at(int block, int r, int kb, int c) {
@@ -252,7 +258,7 @@ __device__ __forceinline__ void store8f(float* out, const float* v, int live) {
 }
 
 // One pass' work of one block: rows `block`, part `part` of the columns.
-template <typename T, int W, int PASS, bool KEEP>
+template <typename T, int W, int PASS>
 __device__ __forceinline__ void cross_pass(const CUtensorMap& tr,
                                            const CUtensorMap& tr2,
                                            const CUtensorMap& tcol,
@@ -447,15 +453,15 @@ __device__ __forceinline__ void cross_pass(const CUtensorMap& tr,
             if (PASS == kForward) {
               const uint32_t src = C::S0 + x * CN;
               sum(C::A0 + g * W, src, col2, idesc_a2, g, t == 0);
-              if (KEEP)
-                sum(C::A0 + g * W, src + CN / 4, col2, idesc_a2, g, false);
+              sum(C::A0 + g * W, src + CN / 4, col2, idesc_a2, g, false);
             } else {
-              sum(C::A0, C::T0 + x * CN, col, idesc_a, g, t == 0 && g == 0);
-              if (PASS == kQueries)
-                sum(C::A0, C::T0 + x * CN + CN / 4, col, idesc_a, g, false);
-              if (PASS == kKeys)
-                sum(C::A0 + W, C::S0 + x * CN, col2, idesc_a2, g,
-                    t == 0 && g == 0);
+              const uint32_t z = C::T0 + x * CN, w = C::S0 + x * CN;
+              sum(C::A0, z, col, idesc_a, g, t == 0 && g == 0);
+              sum(C::A0, z + CN / 4, col, idesc_a, g, false);
+              if (PASS == kKeys) {
+                sum(C::A0 + W, w, col2, idesc_a2, g, t == 0 && g == 0);
+                sum(C::A0 + W, w + CN / 4, col2, idesc_a2, g, false);
+              }
             }
           }
           tc_commit(bar_free(s));
@@ -633,7 +639,6 @@ __device__ __forceinline__ void cross_pass(const CUtensorMap& tr,
           }
           const float ref = m_used == kNegInf ? 0.f : m_used - kLog2Lift<T>;
           const uint64_t neg = both(-ref);
-          const uint64_t minus = both(-1.f);
           uint64_t sa = 0, sb = 0;
 #pragma unroll
           for (int c = 0; c < HALF / 32; ++c) {
@@ -649,17 +654,11 @@ __device__ __forceinline__ void cross_pass(const CUtensorMap& tr,
               w[j + 1] = pack2<T>(f2upk(p1).x, f2upk(p1).y);
               sa = fadd2(sa, p0);
               sb = fadd2(sb, p1);
-              if constexpr (KEEP) {
-                const uint64_t r0 = unpack2<T>(w[j]),
-                               r1 = unpack2<T>(w[j + 1]);
-                const float2 d0 = f2upk(ffma2(r0, minus, p0));
-                const float2 d1 = f2upk(ffma2(r1, minus, p1));
-                rest[j] = pack2<T>(d0.x, d0.y);
-                rest[j + 1] = pack2<T>(d1.x, d1.y);
-              }
+              rest[j] = rest_of<T>(w[j], p0);
+              rest[j + 1] = rest_of<T>(w[j + 1], p1);
             }
             tmem_st16(s_col + c * 16, w);
-            if constexpr (KEEP) tmem_st16(s_col + HALF / 2 + c * 16, rest);
+            tmem_st16(s_col + HALF / 2 + c * 16, rest);
           }
           l += halves(fadd2(sa, sb));
           tmem_wait_st();
@@ -744,8 +743,7 @@ __device__ __forceinline__ void cross_pass(const CUtensorMap& tr,
             13);
       const uint64_t nkr2 = both(nkr), gl2 = both(gl), lse2 = both(-lse),
                      ci2 = both(-ci * up), up2 = both(up);
-      // Sums of z, rounded where its product takes no more; for dscale.
-      uint64_t zs = 0, xs = 0, ys = 0;
+      uint64_t zs = 0, xs = 0, ys = 0;  // sums of z; for dscale
       static_assert(!kBack || HALF == 32, "a tile is read before z is written");
       const bool want_scale = PASS == kQueries && p.dscale_rows != nullptr;
       for (int t = 0; t < n && ok; ++t) {
@@ -764,7 +762,8 @@ __device__ __forceinline__ void cross_pass(const CUtensorMap& tr,
           for (int c = 0; c < HALF; c += 32) {
             uint32_t sv[32], tv[32];
             tmem_load32x2(s_col + c, sv, t_col + c, tv);
-            uint32_t pw[16], zw[16];  // pw of queries: z's rest
+            uint32_t zw[16], zl[16];  // z and what its rounding left
+            uint32_t pw[16], pl[16];  // keys: P
 #pragma unroll
             for (int j = 0; j < 32; j += 4) {
               uint64_t lg[2], zc[2], u2[2];
@@ -812,25 +811,26 @@ __device__ __forceinline__ void cross_pass(const CUtensorMap& tr,
                   u2[q] = f2pk(f.x, f.y);
                 }
                 const uint32_t zp = pack2<T>(z.x, z.y);
+                const uint64_t z2 = f2pk(z.x, z.y);
                 zw[j / 2 + q] = zp;
-                const uint64_t zr = unpack2<T>(zp);
+                zl[j / 2 + q] = rest_of<T>(zp, z2);
+                zs = fadd2(zs, z2);
                 if constexpr (PASS == kKeys) {
-                  zs = fadd2(zs, zr);
-                  pw[j / 2 + q] = pack2<T>(w0, w1);
-                } else {
-                  const uint64_t z2 = f2pk(z.x, z.y);
-                  const float2 rest = f2upk(ffma2(zr, both(-1.f), z2));
-                  pw[j / 2 + q] = pack2<T>(rest.x, rest.y);
-                  zs = fadd2(zs, z2);
-                  if (want_scale) {
-                    xs = ffma2(z2, u2[q], xs);
-                    ys = ffma2(f2pk(w0, w1), u2[q], ys);
-                  }
+                  const uint32_t pp = pack2<T>(w0, w1);
+                  pw[j / 2 + q] = pp;
+                  pl[j / 2 + q] = rest_of<T>(pp, f2pk(w0, w1));
+                } else if (want_scale) {
+                  xs = ffma2(z2, u2[q], xs);
+                  ys = ffma2(f2pk(w0, w1), u2[q], ys);
                 }
               }
             }
             tmem_st16(t_col + c / 2, zw);
-            tmem_st16(PASS == kKeys ? s_col + c / 2 : t_col + HALF / 2, pw);
+            tmem_st16(t_col + HALF / 2, zl);
+            if constexpr (PASS == kKeys) {
+              tmem_st16(s_col + c / 2, pw);
+              tmem_st16(s_col + HALF / 2, pl);
+            }
           }
           tmem_wait_st();
         }
@@ -968,7 +968,7 @@ __device__ __forceinline__ void cross_pass(const CUtensorMap& tr,
   }
 }
 
-template <typename T, int W, bool KEEP>
+template <typename T, int W>
 __global__ void __launch_bounds__(kThreads, 1)
     cross_tc_forward_kernel(const __grid_constant__ CUtensorMap q,
                             const __grid_constant__ CUtensorMap k,
@@ -977,8 +977,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   extern __shared__ uint8_t smem_raw[];
   allow_dependents();
   grid_dependency_wait();
-  cross_pass<T, W, kForward, KEEP>(q, q, k, v, a, blockIdx.x, blockIdx.y,
-                                   smem_raw);
+  cross_pass<T, W, kForward>(q, q, k, v, a, blockIdx.x, blockIdx.y, smem_raw);
 }
 
 // Both backward passes in one grid: the keys' blocks, which are longer, first,
@@ -1000,15 +999,15 @@ __global__ void __launch_bounds__(kThreads, 1)
   grid_dependency_wait();
   if (blockIdx.x < x.key_blocks) {
     const uint32_t part = blockIdx.x / x.blocks[0];
-    cross_pass<T, W, kKeys, false>(x.keys[0], x.keys[1], x.keys[2], x.keys[3],
-                                   x.a[0], blockIdx.x - part * x.blocks[0],
-                                   int(part), smem_raw);
+    cross_pass<T, W, kKeys>(x.keys[0], x.keys[1], x.keys[2], x.keys[3], x.a[0],
+                            blockIdx.x - part * x.blocks[0], int(part),
+                            smem_raw);
   } else {
     const uint32_t at = blockIdx.x - x.key_blocks;
     const uint32_t part = at / x.blocks[1];
-    cross_pass<T, W, kQueries, false>(
-        x.queries[0], x.queries[1], x.queries[2], x.queries[3], x.a[1],
-        at - part * x.blocks[1], int(part), smem_raw);
+    cross_pass<T, W, kQueries>(x.queries[0], x.queries[1], x.queries[2],
+                               x.queries[3], x.a[1], at - part * x.blocks[1],
+                               int(part), smem_raw);
   }
 }
 
@@ -1067,7 +1066,7 @@ cudaError_t configure(K kern, int bytes, std::atomic<int>* configured) {
   return err;
 }
 
-template <typename T, int W, bool KEEP>
+template <typename T, int W>
 cudaError_t launch_forward(const CrossProblem& p, cudaStream_t stream) {
   TcArgs a{};
   if (!describe_pass<W, kForward>(p, &a)) return cudaErrorInvalidValue;
@@ -1076,7 +1075,7 @@ cudaError_t launch_forward(const CrossProblem& p, cudaStream_t stream) {
   if (!make_maps(p, a.rows_i, a.cols_i, &q, nullptr, &k, &v))
     return cudaErrorInvalidValue;
   constexpr int bytes = Cfg<W, kForward>::SMEM_ALLOC;
-  auto kern = cross_tc_forward_kernel<T, W, KEEP>;
+  auto kern = cross_tc_forward_kernel<T, W>;
   static std::atomic<int> configured[64];
   const cudaError_t err = configure(kern, bytes, configured);
   if (err != cudaSuccess) return err;
@@ -1197,9 +1196,7 @@ cudaError_t run_cross_tc_forward(const CrossProblem& problem, Workspace& ws,
   }
   const cudaError_t e = with_width(p, [&](auto* t, auto width) {
     using T = std::remove_pointer_t<decltype(t)>;
-    constexpr int W = decltype(width)::value;
-    return p.lse ? launch_forward<T, W, true>(p, stream)
-                 : launch_forward<T, W, false>(p, stream);
+    return launch_forward<T, decltype(width)::value>(p, stream);
   });
   return e != cudaSuccess || p.splits == 1 ? e : launch_cross_join(p, stream);
 }

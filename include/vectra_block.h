@@ -233,8 +233,9 @@ typedef struct {
 
 /* The same for a backward pass to come. rest [M,C], of 16-bit tensors with a
  * branch and y only, contiguous, their type: what x_out's rounding left, itself
- * rounded. The second norm's gradient takes x_out less its mean, whose rounding
- * a mean of many deviations would multiply. Data NULL: not wanted. */
+ * rounded (of F16 2^11 times that, which stays in its range). The second norm's
+ * gradient takes x_out less its mean, and a mean of many deviations would
+ * multiply that rounding. Data NULL: not wanted. */
 typedef struct {
   vectra_residual_norm_args fwd;
   vectra_tensor rest;
@@ -277,9 +278,9 @@ typedef struct {
  *  division (in 16-bit types without their common factor exp(-scale |q|^2)),
  *  infinity for a sequence of length 0.
  *  rest [B,H,Nq,Dv], of 16-bit tensors only, contiguous, their type: what out's
- *  rounding left, itself rounded. The backward pass subtracts numbers that are
- *  nearly equal where a row has one large weight, and out alone would decide
- *  their difference. */
+ *  rounding left, itself rounded (of F16 2^11 times that). The backward pass
+ *  subtracts numbers that are nearly equal where a row has one large weight,
+ *  and out alone would decide their difference. */
 typedef struct {
   vectra_tensor q, k, v, scale;
   const void* key_lengths;

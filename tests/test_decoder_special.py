@@ -223,6 +223,24 @@ def test_cross_float16_weights_far_below_one(device, nq):
             want.abs()).all()
 
 
+@pytest.mark.parametrize('device', DEVICES)
+@pytest.mark.parametrize('nq', [2, 6, 20])
+@pytest.mark.parametrize('dim', [64, 33])
+def test_cross_small_values(device, nq, dim):
+    """Small values under large upstream gradients, and one large weight: what
+    out's rounding left is in float16's range as well."""
+    rand = Rand(nq, device, torch.float16)
+    b, h, hk, nk = 2, 4, 2, 100
+    q, k, v, _ = cross_inputs(rand, b, h, hk, nq, nk, dim)
+    v = v * 1e-4
+    scale = torch.full((1, h, 1, 1), 0.3, device=device)
+    dout = rand(b, h, nq, dim, scale=4000.0)
+    got = gradients((q, k, v, scale), None, dout)
+    want = exact_cross(q, k, v, scale, None, dout)
+    for x, y, name in zip(got[1][:2], want[1:3], ('dq', 'dk')):
+        assert off(x, y, torch.float16) <= 1, name
+
+
 # ---------------------------------------------------------------------------
 # cross_attention: one rounding a result.
 # ---------------------------------------------------------------------------
@@ -391,6 +409,33 @@ def test_norm_keeps_what_a_rounding_left_only_where_it_is_read(device):
                  (torch.float16, True, False),
                  (torch.float16, True, True, False)):
         assert rest(*call).numel() == 0
+
+
+@pytest.mark.parametrize('device', DEVICES)
+@pytest.mark.parametrize('kind', ['rms', 'layer'])
+@pytest.mark.parametrize('c', [256, 1000])
+def test_norm_gradients_of_small_rows(device, kind, c):
+    """What the stream's rounding left is in float16's range as well: rows of
+    2e-5, whose own spacing is 6e-8."""
+    rand = Rand(c, device, torch.float16)
+    x, branch = rand(2, 30, c, scale=2e-5), rand(2, 30, c, scale=2e-5)
+    # The sum with a scale is rounded where a plain one would be exact.
+    weight, dy = 1 + rand(c, scale=0.2), rand(2, 30, c, scale=1e-4)
+    x, branch, weight = leaves = [t.requires_grad_() for t in
+                                  (x, branch, weight)]
+    y = block.residual_norm(x, branch, weight, residual_scale=0.7, kind=kind,
+                            eps=1e-12)[1]
+    got = torch.autograd.grad(y, leaves, dy)
+    X, R, W = (d(t).requires_grad_() for t in leaves)
+    v = 0.7 * X + R
+    t = v - v.mean(-1, keepdim=True) if kind == 'layer' else v
+    t = t * (t.square().mean(-1, keepdim=True) + 1e-12).rsqrt() * W
+    want = torch.autograd.grad(t, (X, R, W), d(dy))
+    for a, b, name in zip(got, want, ('dx', 'dbranch', 'dweight')):
+        # (dweight's own spacing: 30 gradients of 1e-4 have sums of 8e-4.)
+        assert off(a, b, torch.float16) <= ONCE * (1 + 3 * math.sqrt(
+            0.2 / a.numel())) + 2.0**-24 / 3 / (
+                U[torch.float16] * float(b.square().mean().sqrt())), name
 
 
 # ---------------------------------------------------------------------------

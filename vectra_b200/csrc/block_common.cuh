@@ -301,6 +301,12 @@ cudaError_t launch_qk_forward_axes(const QkProblem& p, cudaStream_t stream);
 cudaError_t run_qk_backward_axes(const QkProblem& p, Workspace& ws,
                                  cudaStream_t stream);
 
+// What a value's rounding left, kept in another number of its type for a
+// backward pass, is multiplied by this: in float16 it is 2^-11 of the value at
+// most, and would lie below the type's range for values below 2^-3.
+template <typename T>
+constexpr float kRestLift = std::is_same<T, __half>::value ? 2048.f : 1.f;
+
 // Largest size of one dimension: tensor-map coordinates are 32-bit, and
 // float32 operands keep three planes of lines in one map.
 constexpr int64_t kMaxSize = (int64_t(1) << 29) - 256;

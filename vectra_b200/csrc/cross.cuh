@@ -42,7 +42,7 @@ struct CrossProblem {
   void* out = nullptr;
   int64_t so[4];
   float* lse = nullptr;  // [B, H, Nq]
-  void* rest = nullptr;  // [B, H, Nq, Dv]: out less its rounding
+  void* rest = nullptr;  // [B, H, Nq, Dv]: what out's rounding left
   // Backward.
   const void* dout = nullptr;
   void* dq = nullptr;
@@ -79,7 +79,7 @@ template <typename T>
 __device__ __forceinline__ void store_with_rest(T* out, T* rest, float x) {
   const T r = from_f32<T>(x);
   *out = r;
-  if (rest) *rest = from_f32<T>(x - to_f32(r));
+  if (rest) *rest = from_f32<T>((x - to_f32(r)) * kRestLift<T>);
 }
 
 __device__ __forceinline__ float cross_scale(const CrossProblem& p, int64_t b,

@@ -46,7 +46,7 @@ __global__ void __launch_bounds__(256)
 #pragma unroll
         for (int j = 0; j < N; ++j) {
           float v = to_f32(x.e[j]);
-          if (rest) v += to_f32(z.e[j]);
+          if (rest) v = fmaf(to_f32(z.e[j]), 1.f / kRestLift<T>, v);
           t = fmaf(v, to_f32(y.e[j]), t);
         }
       }

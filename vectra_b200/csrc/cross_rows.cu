@@ -378,7 +378,8 @@ __global__ void __launch_bounds__(kWarps * 32)
         }
         w[i] = pack_pair<T>(a0, a1);
         const float2 f = pair<T>(w[i]);
-        x[i] = pack_pair<T>(a0 - f.x, a1 - f.y);
+        x[i] = pack_pair<T>((a0 - f.x) * kRestLift<T>,
+                            (a1 - f.y) * kRestLift<T>);
       }
       if (!whole) continue;
       *reinterpret_cast<uint4*>(out + d) = make_uint4(w[0], w[1], w[2], w[3]);
@@ -578,7 +579,8 @@ __global__ void __launch_bounds__(kWarps * 32)
       const uint32_t pr = pack_pair<T>(a0, a1);
       w[i] = turn(pr);
       const float2 f = pair<T>(pr);
-      x[i] = turn(pack_pair<T>(a0 - f.x, a1 - f.y));
+      x[i] = turn(pack_pair<T>((a0 - f.x) * kRestLift<T>,
+                               (a1 - f.y) * kRestLift<T>));
     }
     if (!own.live || d >= p.Dv) continue;
     *reinterpret_cast<uint4*>(out + d) = make_uint4(w[0], w[1], w[2], w[3]);
@@ -644,8 +646,8 @@ __global__ void __launch_bounds__(kWarps * 32, NB > 2 ? 2 : 3)
       for (int w = 0; w < 4; ++w) {
         const float2 a = pair<T>(o[n][w]), d = pair<T>(x[n][w]),
                      f = pair<T>(e[r][n][w]);
-        c = fmaf(a.x + d.x, f.x, c);
-        c = fmaf(a.y + d.y, f.y, c);
+        c = fmaf(fmaf(d.x, 1.f / kRestLift<T>, a.x), f.x, c);
+        c = fmaf(fmaf(d.y, 1.f / kRestLift<T>, a.y), f.y, c);
       }
     ci[r] = quad_sum(c);
   }

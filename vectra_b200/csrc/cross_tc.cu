@@ -231,7 +231,7 @@ __device__ __forceinline__ void store8(T* out, T* rest, const float* v,
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     a.e[i] = from_f32<T>(v[i]);
-    b.e[i] = from_f32<T>(v[i] - to_f32(a.e[i]));
+    b.e[i] = from_f32<T>((v[i] - to_f32(a.e[i])) * kRestLift<T>);
   }
   const bool whole =
       live >= 8 && (reinterpret_cast<uintptr_t>(out) & 15) == 0;

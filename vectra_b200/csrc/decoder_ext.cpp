@@ -205,6 +205,11 @@ using Three = std::tuple<Tensor, Tensor, Tensor>;
 using Four = std::tuple<Tensor, Tensor, Tensor, Tensor>;
 using Six = std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor>;
 
+// What a 16-bit value's rounding left is kept times this (block_common.cuh).
+double rest_lift(const Tensor& t) {
+  return t.scalar_type() == at::kHalf ? 2048.0 : 1.0;
+}
+
 // What x_out's rounding leaves, for the backward pass of the norm behind.
 Tensor rest_of_sum(const Tensor& x, bool branched, bool norm, bool want) {
   const bool kept =
@@ -403,7 +408,7 @@ Four norm_cpu(const Tensor& x, const OptTensor& branch,
     if (has(gate)) u = u * f32(*gate);
     v = v * call.residual_scale + u;
     x_out = at::empty(x.sizes(), x.options()).copy_(v);
-    if (rest.numel()) rest.copy_(v - f32(x_out));
+    if (rest.numel()) rest.copy_((v - f32(x_out)) * rest_lift(x));
   }
   if (norm) {
     const auto n = cpu_row_norm(v, call);
@@ -445,7 +450,7 @@ Six norm_backward_cpu(const OptTensor& dx_out, const OptTensor& dy,
   if (has(dy)) {
     const Tensor f = flat(*dy), r = column(1);
     Tensor v = flat(x_out);
-    if (rest.numel()) v = v + flat(rest);
+    if (rest.numel()) v = v + flat(rest) / rest_lift(rest);
     const Tensor n = (v - column(0)) * r;
     if (need & kDweight) dweight = (f * n).sum(0).to(dt);
     if (need & kDbias) dbias = f.sum(0).to(dt);
@@ -720,7 +725,7 @@ Three cross_cpu(const Tensor& q, const Tensor& k, const Tensor& v,
       at::where(any, at::matmul(at::softmax(s, -1), t.v), zero)
           .reshape(out.sizes());
   out.copy_(o);
-  if (rest.numel()) rest.copy_(o - f32(out));
+  if (rest.numel()) rest.copy_((o - f32(out)) * rest_lift(q));
   if (want_lse)
     lse.copy_(at::where(any,
                         at::logsumexp(s, {-1}, true) * 1.4426950408889634 +
@@ -752,7 +757,7 @@ Four cross_backward_cpu(const Tensor& dout, const Tensor& q, const Tensor& k,
                 nq = t.q.size(3);
   const Tensor e = f32(dout).reshape({b, hk, g, nq, v.size(3)});
   Tensor o = f32(out);
-  if (q.scalar_type() != at::kFloat) o = o + f32(rest);
+  if (q.scalar_type() != at::kFloat) o = o + f32(rest) / rest_lift(q);
   o = o.reshape(e.sizes());
   const Tensor zero = at::zeros({}, at::kFloat);
   const Tensor from =

@@ -33,7 +33,7 @@ struct NormProblem {
   void* x_out = nullptr;
   void* y = nullptr;
   float* stats = nullptr;  // [M][4]
-  void* rest = nullptr;    // [M][C]: x_out less its rounding
+  void* rest = nullptr;    // [M][C]: what x_out's rounding left
   // Backward's results.
   void* dx = nullptr;
   void* dbranch = nullptr;

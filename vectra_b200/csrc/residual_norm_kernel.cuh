@@ -171,14 +171,15 @@ __device__ __forceinline__ void store8(void* row, int col, int cols,
   }
 }
 
-// What rounding v to T leaves.
+// What rounding v to T leaves, as it is kept.
 template <typename T>
 __device__ __forceinline__ void left_over(const uint64_t* v, uint64_t* rest) {
   uint64_t rounded[kPairs];
   unpack<T>(pack<T>(v), rounded);
   const uint64_t minus = both(-1.f);
 #pragma unroll
-  for (int i = 0; i < kPairs; ++i) rest[i] = ffma2(rounded[i], minus, v[i]);
+  for (int i = 0; i < kPairs; ++i)
+    rest[i] = mul2(ffma2(rounded[i], minus, v[i]), both(kRestLift<T>));
 }
 
 // Kept elements times `scale`, 0 for the others.
@@ -707,7 +708,8 @@ __global__ void __launch_bounds__(THREADS, THREADS <= 320 ? 2 : 1)
         if (has_rest) {
           rows.get(stage, rest_at, rest, row, c, f);
 #pragma unroll
-          for (int i = 0; i < kPairs; ++i) n[i] = fadd2(n[i], f[i]);
+          for (int i = 0; i < kPairs; ++i)
+            n[i] = ffma2(f[i], both(1.f / kRestLift<T>), n[i]);
         }
         rows.get(stage, 3, p.f, row, c, f);
 #pragma unroll

@@ -17,6 +17,7 @@ import math
 
 import pytest
 import torch
+from torch.utils.checkpoint import checkpoint
 
 from tests.test_decoder import DEVICES
 from tests.test_decoder import TINY
@@ -436,6 +437,50 @@ def test_norm_gradients_of_small_rows(device, kind, c):
         assert off(a, b, torch.float16) <= ONCE * (1 + 3 * math.sqrt(
             0.2 / a.numel())) + 2.0**-24 / 3 / (
                 U[torch.float16] * float(b.square().mean().sqrt())), name
+
+
+# ---------------------------------------------------------------------------
+# All of them.
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize('device', DEVICES)
+@pytest.mark.parametrize('dtype', TYPES)
+def test_checkpointed_block(device, dtype):
+    """A block whose forward pass runs without gradients and again with them:
+    the same bits, results and gradients, as one that keeps everything."""
+    torch.manual_seed(1)
+    blk = block.RbfCrossBlock(64, 48, 4, 2, 96, dropout=0.1).to(device, dtype)
+    rand = Rand(101, device, dtype)
+    x, states = rand(3, 40, 64).requires_grad_(), rand(3, 70, 48)
+    lengths = torch.tensor([70, 0, 33], device=device)
+    rng = torch.tensor([5, 6], device=device)
+    dy = rand(3, 40, 64)
+    leaves = [x, *blk.parameters()]
+    y = blk(x, states, lengths, rng)
+    want = torch.autograd.grad(y, leaves, dy)
+    z = checkpoint(blk, x, states, lengths, rng, use_reentrant=False)
+    got = torch.autograd.grad(z, leaves, dy)
+    assert torch.equal(y, z)
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+    with torch.no_grad():
+        assert torch.equal(y, blk(x, states, lengths, rng))
+
+
+@pytest.mark.parametrize('device', DEVICES)
+@pytest.mark.parametrize('dtype', HALVES)
+def test_opcheck_of_16_bit_norms(device, dtype):
+    rand = Rand(102, device, dtype)
+    leaves = [rand(*s).requires_grad_() for s in (
+        (2, 3, 8), (2, 3, 8), (8,), (8,), (8,), (2, 1, 8))]
+    torch.library.opcheck(
+        torch.ops.vectra_b200.residual_norm.default,
+        (*leaves, 0.5, 0.0, None, 0, 1e-6, 'layer'),
+        test_utils=('test_schema', 'test_faketensor',
+                    'test_aot_dispatch_static', 'test_aot_dispatch_dynamic'))
+    torch.library.opcheck(
+        torch.ops.vectra_b200.residual_norm_with_stats.default,
+        (*(t.detach() for t in leaves), 0.5, 0.0, None, 0, 1e-6, 'layer',
+         True, True), test_utils=('test_schema', 'test_faketensor'))
 
 
 # ---------------------------------------------------------------------------

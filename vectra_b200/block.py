@@ -28,8 +28,10 @@ call. CUDA tensors run this library's sm_100a kernels on the current stream
 in float32. Sums, norms and activations are in float32 and each result is
 rounded once; with 16-bit tensors a gradient is also rounded before its
 products with the weight and the input, and `linear` keeps act's argument for
-the backward pass in its type. `cross_attention` rounds weights and their
-gradients to 16 bits before the products that take them, with 16-bit tensors.
+the backward pass in its type. `cross_attention` takes weights and their
+gradients into its products as two 16-bit numbers each, with 16-bit tensors: its
+results are off by their own rounding. Like `residual_norm` it keeps what a
+result's rounding left beside it for the backward pass.
 All differentiate (once, in reverse, `dropout` again and again;
 forward mode raises NotImplementedError); under torch.no_grad(), or when no
 argument needs a gradient, nothing is kept for a backward pass.
@@ -241,8 +243,8 @@ def residual_norm(x, branch=None, weight=None, bias=None, gate=None,
       norm: False: no norm behind; y is None.
 
     Returns:
-      (x_out, y), contiguous. y is formed from x_out before its rounding.
-      Without a branch x_out is x itself.
+      (x_out, y), contiguous. y is formed from x_out before its rounding, and
+      so are the gradients of its norm. Without a branch x_out is x itself.
 
     Raises:
       ValueError: shapes, dtypes or devices that do not agree, arguments of a
@@ -273,7 +275,9 @@ def cross_attention(q, k, v, scale, key_lengths=None) -> torch.Tensor:
         has zero results.
 
     Returns:
-      [B, H, Nq, Dv], laid out as `custom_ops.output_strides` says.
+      [B, H, Nq, Dv], laid out as `custom_ops.output_strides` says; the same
+      bits with and without gradients. A NaN in a seen key or value reaches
+      every query of its heads.
 
     Raises:
       ValueError: shapes, dtypes or devices that do not agree.

@@ -32,7 +32,8 @@
 // Measured against tcgen05 tiles, which are 128 rows high: one query of 32
 // heads on up to 4,001 keys of 8 heads of 128, 32 sequences: 67 us (61 of them
 // the keys, at 5.3 TB/s), with tiles 81; training of 1,024 subjects of 8 heads
-// on 64 keys of 32: forward 17 and backward 43 us, with tiles 1,050 together.
+// on 64 keys of 32: forward 18 and backward 45 us (41.5 without the second
+// products of dk and dv), with tiles 1,050 together.
 // Above 16 packed rows a fragment would no longer hold them.
 #include <type_traits>
 

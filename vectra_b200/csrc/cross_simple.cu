@@ -23,7 +23,7 @@
 // Bound by latency at the two blocks an SM that registers and shared memory
 // hold (issue about 40 % of cycles, the FP32 pipe 30 %), and by a last wave of
 // blocks. 257 queries on up to 700 keys, 8 heads of 64, batch 4, float32:
-// forward 78 us, all gradients 168. Loading the next tile's operands by 4-byte
+// forward 80 us, all gradients 172. Loading the next tile's operands by 4-byte
 // asynchronous copies under the products changed 81 and 178 to 77 and 187.
 #include <type_traits>
 

@@ -39,13 +39,17 @@
 // float16 (cross.cuh): forward weights, at most 2^8, are multiplied by 2^7, P
 // of dv by 2^14, z of dq by what a bound of its row needs and z of dk by what
 // that of its key head does: |z_ij| <= P_ij |e_i| (|v_j| + |out_i|), at most
-// 2 |e_i| max |v_j|.
+// 2 |e_i| max |v_j|. (A query's share of dk loses bits where its weight times its
+// gradient over the largest of its key head is below 2^-23.) The bounds' kernel
+// takes 27 us of all gradients of the training below in f16, their use 50.
 //
 // Measured: 4,096 queries of 32 heads on 5,003 keys of 8 heads of 128, f16:
-// 395 us, 850 TFLOP/s; bound by the latency of the row warps, two a scheduler
-// (tensor pipe 41 %, issue 35 %). Training of 2,048 queries of 16 heads on up to
-// 4,500 keys of 4 heads of 128, batch 4, bf16: forward 249, and 284 with what
-// the backward pass takes; all gradients 730 to 750 us.
+// 452 us by itself and 524 call after call, 640 TFLOP/s of the formula's; bound
+// by the latency of the row warps, two a scheduler (tensor pipe 51 %, issue
+// 43 %). (396 and 441 us without the second products.) Training of 2,048 queries
+// of 16 heads on up to 4,500 keys of 4 heads of 128, batch 4, bf16: forward 305,
+// all gradients 855 us (775 without the second products of dk and dv; tensor
+// pipe 54 %, issue 43 %).
 #include <atomic>
 #include <type_traits>
 

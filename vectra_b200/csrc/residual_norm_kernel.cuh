@@ -13,7 +13,10 @@
 //   dx = a g, dgate = sum g d, h = dropout'(g gate)
 //   dbw = sum h n0, dbranch = r0 (h bw - n0 c(h bw n0) [- c(h bw)])
 // Rows are held in float32 registers between their reading and writing; sums
-// over rows are joined in a fixed order, without atomics.
+// over rows are joined in a fixed order, without atomics. 16-bit tensors keep
+// what x_out's rounding left as well, for n1: without it dw of a bf16 row of
+// mean 0 was 0.60 of a unit roundoff off instead of 0.41, and with the layer
+// norm by the ratio of mean to deviation more.
 //
 // Memory-bound. A team of threads (a warp up to 512 columns, else a block)
 // owns a row: each thread holds one or two chunks of 8 neighbouring columns,
@@ -23,16 +26,19 @@
 // no barrier.
 //
 // Measured, bf16: 66,560 rows of 256, layer norm, one gate row, dropout:
-// forward 37 us (136 MB: 3.7 TB/s, half of it writes, whose own rate here is
-// 3.7), backward 62 us (205 MB: 3.3 TB/s, of which the joins of the column
-// sums 9). 8,193 rows of 5,120, norms on both sides, a gate row for each
-// 2,731: forward 76 us (336 MB, 4.4 TB/s); backward 208 us (503 MB, 2.4 TB/s),
-// bound by instructions (73 an element) and by the column sums, 64 of
-// which a thread keeps, in part in spilled registers. Of its 208 us no loads
-// would leave 188, no stores 195; one block of 640 threads an SM with half the
-// sums each took 313. With loads to registers in turn instead of copies ahead
-// it was 280. Dropout alone, 16,396 rows of 4,096: 56 us a pass (269 MB,
-// 4.8 TB/s).
+// forward for training 40 us (170 MB: 4.3 TB/s; 37 without the rest), bound by
+// instructions (issue 68 %, DRAM 33 %); backward 69 us (239 MB: 3.5 TB/s, of
+// which the joins of the column sums 9), the same (issue 63 % with two blocks
+// an SM). 8,193 rows of 5,120, norms on both sides, a gate row for each
+// 2,731: forward for training 85 us (420 MB, 4.9 TB/s; 77 without the rest);
+// backward 230 us (587 MB, 2.6 TB/s; 207 without the rest), bound by
+// instructions (issue 49 %) and by the column sums, 64 of which a thread keeps,
+// in part in spilled registers. Of 207 us no loads would have left 188, no
+// stores 195; one block of 640 threads an SM with half the sums each took 313.
+// With loads to registers in turn instead of copies ahead it was 280. Dropout
+// alone, 16,396 rows of 4,096: 55 us a pass (269 MB, 4.8 TB/s), bound by the
+// numbers' integer products (issue 57 %, half of the stalls on that pipe) and by
+// a thread's one load under way.
 #pragma once
 
 #include <type_traits>

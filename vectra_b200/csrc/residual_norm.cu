@@ -40,14 +40,14 @@ Team team_of(int C) {
 }
 
 // Rows that are under way: up to `most`, as many as let `blocks` blocks of
-// this team have their copies on an SM beside their vectors, else one; 0: not
-// one fits.
+// this team have their copies on an SM beside their `kept` vectors, else one; 0:
+// not one fits.
 int stages_of(const NormProblem& p, const Team& team, int blocks, int most,
-              size_t* bytes) {
+              int kept, size_t* bytes) {
   const size_t es = p.dtype == VECTRA_F32 ? 4 : 2;
   const size_t threads = size_t(team.block.x) * team.block.y;
   const size_t chunks = threads * team.nc * kChunk * es;
-  const size_t one = threads * 16 + chunks * p.tensors, vectors = chunks * 4;
+  const size_t one = threads * 16 + chunks * p.tensors, vectors = chunks * kept;
   const auto fit = [&](int n) {
     const size_t all = size_t(224 * 1024) / n;
     return all < vectors ? 0 : int((all - vectors) / one);
@@ -101,7 +101,7 @@ cudaError_t launch_norm_forward(const NormProblem& problem,
   if (blocks > most) blocks = most;
   size_t bytes = 0;
   p.tensors = p.gate.p && p.gate_rows == 1 ? 3 : 2;
-  p.stages = stages_of(p, team, resident, depth, &bytes);
+  p.stages = stages_of(p, team, resident, depth, kNormVectors, &bytes);
   const bool vec = all_vec(p) && p.stages > 0;
   if (!vec) bytes = 0;
   const NormLaunch how{team.nc, team.block, unsigned(blocks), vec, false, bytes};
@@ -170,7 +170,8 @@ cudaError_t run_norm_backward(const NormProblem& problem, Workspace& ws,
   }
   size_t bytes = 0;
   p.tensors = 4 + (gate && p.gate_rows == 1) + (p.rest != nullptr);
-  p.stages = stages_of(p, team, resident, 3, &bytes);
+  // The bias, the last vector, is not read backward.
+  p.stages = stages_of(p, team, resident, 3, kNormVectors - 1, &bytes);
   const bool vec = all_vec(p) && p.stages > 0;
   if (!vec) bytes = 0;
   // Teams of a warp join their sums in this memory.

@@ -53,6 +53,7 @@ struct NormProblem {
 constexpr int kMaxNormCols = 16384;
 
 constexpr int kChunk = 8;  // columns a thread reads at once
+constexpr int kNormVectors = 4;  // over the columns, the bias last
 
 struct DropArgs {
   const void* x;

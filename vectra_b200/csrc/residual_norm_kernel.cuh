@@ -363,6 +363,7 @@ struct Rows {
 
 // The vectors' places.
 enum { kWeight = 0, kBranchWeight = 1, kGate = 2, kBias = 3 };
+static_assert(kBias == kNormVectors - 1, "a backward pass keeps no bias");
 
 // ---------------------------------------------------------------------------
 // Dropout.

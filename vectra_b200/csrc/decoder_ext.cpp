@@ -217,23 +217,27 @@ Tensor rest_of_sum(const Tensor& x, bool branched, bool norm, bool want) {
   return kept ? at::empty(x.sizes(), x.options()) : at::empty({0}, x.options());
 }
 
+// `only`: x_out and y alone; the others stay undefined.
 Four norm_cuda(const Tensor& x, const OptTensor& branch,
-                const OptTensor& weight, const OptTensor& bias,
-                const OptTensor& branch_weight, const OptTensor& gate,
-                const NormCall& call, bool norm, bool want_stats) {
+               const OptTensor& weight, const OptTensor& bias,
+               const OptTensor& branch_weight, const OptTensor& gate,
+               const NormCall& call, bool norm, bool want_stats, bool only) {
   check_norm(x, branch, weight, bias, branch_weight, gate, call, norm);
   c10::cuda::CUDAGuard guard(x.device());
   const auto none = [&] { return at::empty({0}, x.options()); };
   const int64_t c = x.size(-1), rows = c > 0 ? x.numel() / c : 0;
   Tensor x_out = has(branch) ? at::empty(x.sizes(), x.options()) : none();
   Tensor y = norm ? at::empty(x.sizes(), x.options()) : none();
-  Tensor stats = at::empty({want_stats ? rows : 0, 4},
-                           x.options().dtype(at::kFloat));
-  Tensor rest = rest_of_sum(x, has(branch), norm, want_stats);
+  Tensor stats, rest;
+  if (!only) {
+    stats = at::empty({want_stats ? rows : 0, 4},
+                      x.options().dtype(at::kFloat));
+    rest = rest_of_sum(x, has(branch), norm, want_stats);
+  }
   if (x.numel() == 0) return {x_out, y, stats, rest};
   vectra_residual_norm_train_args train{};
   train.fwd = describe_norm(call);
-  if (rest.numel()) train.rest = describe_rows(rest, nullptr);
+  if (!only && rest.numel()) train.rest = describe_rows(rest, nullptr);
   vectra_residual_norm_args& a = train.fwd;
   Tensor x_copy, branch_copy, gate_copy;
   a.x = describe_rows(x, &x_copy);
@@ -383,9 +387,9 @@ std::pair<Tensor, Tensor> cpu_row_norm(const Tensor& v, const NormCall& call) {
 }
 
 Four norm_cpu(const Tensor& x, const OptTensor& branch,
-               const OptTensor& weight, const OptTensor& bias,
-               const OptTensor& branch_weight, const OptTensor& gate,
-               const NormCall& call, bool norm, bool want_stats) {
+              const OptTensor& weight, const OptTensor& bias,
+              const OptTensor& branch_weight, const OptTensor& gate,
+              const NormCall& call, bool norm, bool want_stats, bool /*only*/) {
   check_norm(x, branch, weight, bias, branch_weight, gate, call, norm);
   const int64_t c = x.size(-1), rows = c > 0 ? x.numel() / c : 0;
   const auto none = [&] { return at::empty({0}, x.options()); };
@@ -840,6 +844,10 @@ Tensor dropout_autograd(const Tensor& x, double p, const OptTensor& rng,
   return call_dropout(x, p, rng, stream);
 }
 
+using NormOnlyOp = std::tuple<Tensor, Tensor>(
+    const Tensor&, const OptTensor&, const OptTensor&, const OptTensor&,
+    const OptTensor&, const OptTensor&, double, double, const OptTensor&,
+    int64_t, double, c10::string_view, bool);
 using NormOp = Four(const Tensor&, const OptTensor&, const OptTensor&,
                      const OptTensor&, const OptTensor&, const OptTensor&,
                      double, double, const OptTensor&, int64_t, double,
@@ -936,11 +944,9 @@ std::tuple<Tensor, Tensor> norm_autograd(
             norm ? out[branched ? 1 : 0] : none()};
   }
   at::AutoDispatchBelowADInplaceOrView below;
-  static const auto op =
-      find_op<NormOp>("vectra_b200::residual_norm_with_stats");
-  auto out = op.call(x, branch, weight, bias, branch_weight, gate,
-                     residual_scale, p, rng, stream, eps, kind, norm, false);
-  return {std::get<0>(out), std::get<1>(out)};
+  static const auto op = find_op<NormOnlyOp>("vectra_b200::residual_norm");
+  return op.call(x, branch, weight, bias, branch_weight, gate, residual_scale,
+                 p, rng, stream, eps, kind, norm);
 }
 
 using CrossOp = Three(const Tensor&, const Tensor&, const Tensor&,
@@ -1010,7 +1016,7 @@ Four norm_impl(const Tensor& x, const OptTensor& branch,
                 bool want_stats) {
   return F(x, branch, weight, bias, branch_weight, gate,
            NormCall{residual_scale, p, rng, stream, eps, kind_of(kind)}, norm,
-           want_stats);
+           want_stats, false);
 }
 template <auto F>
 std::tuple<Tensor, Tensor> norm_only_impl(
@@ -1019,9 +1025,9 @@ std::tuple<Tensor, Tensor> norm_only_impl(
     const OptTensor& gate, double residual_scale, double p,
     const OptTensor& rng, int64_t stream, double eps, c10::string_view kind,
     bool norm) {
-  auto out = norm_impl<F>(x, branch, weight, bias, branch_weight, gate,
-                          residual_scale, p, rng, stream, eps, kind, norm,
-                          false);
+  auto out = F(x, branch, weight, bias, branch_weight, gate,
+               NormCall{residual_scale, p, rng, stream, eps, kind_of(kind)},
+               norm, false, true);
   return {std::get<0>(out), std::get<1>(out)};
 }
 template <auto F>

@@ -518,3 +518,52 @@ def test_abi_statistics_start_on_16_bytes():
         assert (got if status else min(got, 0)) == status
 
 
+
+
+class _NormTrainArgs(ctypes.Structure):
+    """vectra_residual_norm_train_args."""
+    _fields_ = [('fwd', _NormArgs), ('rest', _lib.Tensor)]
+
+
+class _NormTrainGradArgs(ctypes.Structure):
+    """vectra_residual_norm_train_grad_args."""
+    _fields_ = [('grad', _NormGradArgs), ('rest', _lib.Tensor)]
+
+
+def test_abi_statuses_of_a_kept_rest():
+    forward = _lib.LIB.vectra_residual_norm_forward_train
+    size = _lib.LIB.vectra_residual_norm_backward_train_workspace_bytes
+    size.restype = ctypes.c_int64
+    backward = _lib.LIB.vectra_residual_norm_backward_train
+
+    def norm(dtype, **over):
+        n = _NormArgs(x=_abi((6, 8), dtype), branch=_abi((6, 8), dtype),
+                      x_out=_abi((6, 8), dtype), y=_abi((6, 8), dtype),
+                      stats=_abi((6, 4), _lib.F32),
+                      drop=_Drop(0.0, None, 0), residual_scale=1.0, eps=1e-6)
+        for name, value in over.items():
+            setattr(n, name, value)
+        return n
+
+    def there(rest, dtype=_lib.BF16, **over):
+        a = _NormTrainArgs(norm(dtype, **over), rest)
+        return forward(ctypes.byref(a), None)
+
+    def back(rest, dtype=_lib.BF16, **over):
+        g = _NormGradArgs(fwd=norm(dtype), dy=_abi((6, 8), dtype),
+                          dx=_abi((6, 8), dtype))
+        for name, value in over.items():
+            setattr(g, name, value)
+        return size(ctypes.byref(_NormTrainGradArgs(g, rest)))
+
+    for call in (there, back):
+        assert call(_abi((6, 8), _lib.F32), _lib.F32) == _lib.ERR_DTYPE
+        assert call(_abi((6, 8), _lib.F16)) == _lib.ERR_DTYPE
+        assert call(_abi((6, 9))) == _lib.ERR_SHAPE
+        assert call(_abi((6, 8), strides=(16, 1))) == -12
+    assert there(_abi((6, 8)), y=_lib.Tensor()) == _lib.ERR_NULL
+    assert back(_abi((6, 8)), dy=_lib.Tensor(),
+                dx_out=_abi((6, 8))) == _lib.ERR_NULL
+    assert back(_lib.Tensor()) >= 0 and back(_abi((6, 8))) >= 0
+    assert forward(None, None) == backward(None, None) == size(None) == \
+        _lib.ERR_NULL

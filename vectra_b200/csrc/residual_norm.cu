@@ -123,7 +123,11 @@ cudaError_t run_norm_backward(const NormProblem& problem, Workspace& ws,
   const bool gate = p.gate.p != nullptr;
   const bool norm0 = p.branch_weight.p != nullptr;
   // Two resident blocks an SM (one of the widest rows), teams that each get a
-  // unit at least.
+  // unit at least. The limit, in us of two blocks an SM and of one, 8,193 bf16
+  // rows, norms on both sides: 5,120 columns (320 threads) with a gate 232 and
+  // 485, without 169 and 152; 5,632 (352 threads) 299 and 500, 207 and 156. Two
+  // blocks of 352 threads have fewer registers: with that limit 5,120 columns
+  // take 278 and 195.
   const int resident = team.block.x > 320 ? 1 : 2;
   int64_t blocks = int64_t(device_sm_count()) * resident;
   const int64_t groups = gate ? p.gate_count : 1;

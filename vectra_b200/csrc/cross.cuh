@@ -8,8 +8,11 @@
 //   dq_i = 2 g sum_j z_ij (k_j - q_i),  dk_j = sum_i 2 g z_ij (q_i - k_j)
 //   dg = -sum_ij z_ij |q_i - k_j|^2
 // A row of z sums to zero, but for the rounding of c_i and of z: the sums keep
-// their q_i and k_j terms, so that what rounding leaves is weighed by
-// distances and not by positions, and dg takes distances from their mean.
+// their q_i and k_j terms, so that what that rounding leaves is weighed by
+// distances and not by positions, and dg takes distances from their mean. (The
+// sums' own rounding, 2^-24 of a term, is weighed by positions: float32 tensors
+// 1,000 deviations from the origin have dq 2.4e-4 off, dk 1.2e-4; 16-bit ones
+// show it below their own rounding.)
 //
 // Query heads that share a key head are rows of one problem: packed row
 // i G + g is query i of the g-th of the G heads. Their keys and values are
